@@ -285,14 +285,66 @@ int cb_decode_plan(int bits, int64_t B, int64_t V, int64_t K, int64_t split_k, i
  * 0 = no problem; 0 < k < 1000 = in a decode kernel a shared-memory copy of pass k-1 did not arrive
  * within the wait limit and the affected outputs were not written; 1000 + r (2000 + r for the
  * weights-in-TMEM kernel) = in the tensor-core GEMM role r (1 activation producer, 2 MMA issuer,
- * 3 dequantiser, 4 epilogue, 5 packed-word producer) gave up a bounded wait.  No counterpart in the
- * reference. */
+ * 3 dequantiser, 4 epilogue, 5 packed-word producer) gave up a bounded wait; 3001 = a kernel of the 4-bit cache met a position
+ * outside its page table or a page number outside the cache and left it out, 3002 = a copy of the cache's attention did not
+ * arrive in time and outputs were not written.  No counterpart in the reference. */
 int cb_decode_status(int* status);
 
 /* Introspection used by the Split-K policy (packed_gemv.cu:339-347; bindings.cpp:37-39). */
 int cb_sm_count(void);                 /* SMs of the current device, or -1 on error     */
 int cb_tile_n(void);                   /* virtual output rows per decode work tile       */
 int cb_max_rho(int bits, int mode);    /* occupancy-limited resident CTAs per SM, -1 on error */
+
+/* ---- attention next to the packed linears (no counterpart in the reference, which leaves attention to its host) ---- */
+
+/* A key/value cache held in 4 bits, one layer of a model.  pages: [n_pages][kv_heads][page_size / 16] blocks of
+ * cb_kv4_block_bytes() bytes, 16-byte aligned; a block holds the keys and values of 16 tokens of one head.  head_dim 64 or
+ * 128, group_size 32, 64 or 128 (at most head_dim), page_size a multiple of 16, dtype CB_F16 or CB_BF16 (of the
+ * keys, values and queries, and of the groups' scales and smallest values).
+ * A group of group_size values x of one token and head is kept as lo = min(x), scale = (max(x) - lo) / 15 rounded to dtype, and
+ * 4-bit codes round_half_even((x - lo) / scale), at most 15; it stands for code * scale + lo.  A group with an infinity or a NaN reads
+ * back as NaN; a scale below 2^-126 is kept as 0 and the group reads back as lo.
+ * The bytes need no initialisation: what no token was appended to is never used. */
+typedef struct cb_kv4_cache {
+    void* pages;
+    int64_t n_pages;
+    int64_t kv_heads;
+    int head_dim;
+    int group_size;
+    int page_size;
+    int dtype;
+} cb_kv4_cache;
+
+/* Bytes of a block of 16 tokens of one head, or 0 for a head_dim / group_size that has no kernel. */
+size_t cb_kv4_block_bytes(int head_dim, int group_size);
+
+/* Quantise the keys and values of n_tokens new tokens into the cache.  k, v: [n_tokens, kv_heads, head_dim], values of a head
+ * contiguous, rows 16-byte aligned; strides4 = {k token, k head, v token, v head} in elements, multiples of 8.
+ * Token i belongs to sequence s with cu_seqlens[s] <= i < cu_seqlens[s + 1] (cu_seqlens NULL: n_tokens / n_seqs tokens each; a
+ * token of no sequence is left out) and goes to position p = starts[s] + i - cu_seqlens[s], that is to row p % page_size of page
+ * page_table[s * table_stride + p / page_size].  No position may be written twice in one call.  Positions outside the
+ * table and page numbers outside the cache are left out and set the status word (cb_decode_status: 3001). */
+int cb_kv4_append(const cb_kv4_cache* cache, const void* k, const void* v, const int64_t* strides4, int64_t n_tokens,
+                  const int32_t* page_table, int64_t table_stride, int64_t n_seqs, const int32_t* starts,
+                  const int32_t* cu_seqlens, void* stream);
+
+/* The values of cached tokens in dtype (those beyond its largest finite number are that number): k, v [n_tokens, kv_heads, head_dim] contiguous, 16-byte aligned; tokens named as in
+ * cb_kv4_append.  Rows of tokens that are left out there are left as they were. */
+int cb_kv4_read(const cb_kv4_cache* cache, void* k, void* v, int64_t n_tokens, const int32_t* page_table,
+                int64_t table_stride, int64_t n_seqs, const int32_t* starts, const int32_t* cu_seqlens, void* stream);
+
+/* Attention of the newest T tokens of each of B sequences over the cache: out[b, j] = softmax(scale * q[b, j] K^T) V over the first
+ * lengths[b] - T + 1 + j cached tokens of sequence b; head h reads key head h / (H / kv_heads).  A row that sees
+ * nothing is 0.  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
+ * strides3 = {b, t, h} in elements, multiples of 8; out [B, T, H, head_dim] contiguous.  Tokens on a page whose number
+ * lies outside the cache are left out and set the status word (3001).  counters: cb_kv4_attention_counters() int32, zeroed ONCE,
+ * left zero by every call; partial: cb_kv4_attention_partial_bytes() bytes, 16-byte aligned, of any content.  Calls that may overlap on
+ * the GPU need their own counters and partial. */
+int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* strides3, void* out, int64_t B, int64_t T,
+                     int64_t H, const int32_t* page_table, int64_t table_stride, const int32_t* lengths, float scale,
+                     void* counters, size_t counter_bytes, void* partial, size_t partial_bytes, void* stream);
+int64_t cb_kv4_attention_counters(int64_t B, int64_t T, int64_t H, int64_t kv_heads);
+size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, int head_dim);
 
 #ifdef __cplusplus
 }

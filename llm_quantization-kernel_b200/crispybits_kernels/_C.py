@@ -622,3 +622,175 @@ def decode_status() -> int:
 
 def version() -> str:
     return _lib.cb_version().decode()
+
+
+# ------------------------------------------------------------------ attention and the 4-bit cache (no reference counterpart)
+class _KV4Cache(ctypes.Structure):
+    """struct cb_kv4_cache of include/crispybits_b200.h"""
+    _fields_ = [("pages", _vp), ("n_pages", _i64), ("kv_heads", _i64), ("head_dim", _int), ("group_size", _int),
+                ("page_size", _int), ("dtype", _int)]
+
+
+_KP = ctypes.POINTER(_KV4Cache)
+_lib.cb_kv4_block_bytes.argtypes = [_int, _int]
+_lib.cb_kv4_block_bytes.restype = _sz
+_lib.cb_kv4_append.argtypes = [_KP, _vp, _vp, ctypes.POINTER(_i64), _i64, _vp, _i64, _i64, _vp, _vp, _vp]
+_lib.cb_kv4_read.argtypes = [_KP, _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp]
+_lib.cb_kv4_attention.argtypes = [_KP, _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _vp, _i64, _vp, ctypes.c_float,
+                                  _vp, _sz, _vp, _sz, _vp]
+_lib.cb_kv4_attention_counters.argtypes = [_i64, _i64, _i64, _i64]
+_lib.cb_kv4_attention_counters.restype = _i64
+_lib.cb_kv4_attention_partial_bytes.argtypes = [_i64, _i64, _i64, _int]
+_lib.cb_kv4_attention_partial_bytes.restype = _sz
+for _f in ("cb_kv4_append", "cb_kv4_read", "cb_kv4_attention"):
+    getattr(_lib, _f).restype = _int
+
+
+def kv4_block_bytes(head_dim: int, group_size: int) -> int:
+    """Bytes that 16 tokens of one head take in the 4-bit cache; 0: no kernel for this head_dim and group_size."""
+    return int(_lib.cb_kv4_block_bytes(int(head_dim), int(group_size)))
+
+
+def _kv4_record(cache, who: str) -> _KV4Cache:
+    pages = cache.pages
+    if not pages.is_cuda or pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous():
+        _fail(f"{who}: the cache's pages must be a contiguous 3-D CUDA uint8 tensor")
+    if cache.dtype not in (torch.float16, torch.bfloat16):
+        _fail(f"{who}: the cache's dtype must be float16 or bfloat16")
+    if pages.shape[2] * 16 != cache.page_size * kv4_block_bytes(cache.head_dim, cache.group_size):
+        _fail(f"{who}: pages do not fit the cache's head_dim, group_size and page_size")
+    if pages.numel() == 0:
+        _fail(f"{who}: the cache has no pages")
+    return _KV4Cache(pages.data_ptr(), pages.shape[0], pages.shape[1], cache.head_dim, cache.group_size, cache.page_size,
+                     _DTYPE[cache.dtype])
+
+
+def _check_index(t, device, shape, name: str, who: str):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device:
+        _fail(f"{who}: {name} must be an int32 tensor on the cache's device")
+    if tuple(t.shape) != shape or not t.is_contiguous():
+        _fail(f"{who}: {name} must be contiguous of shape {list(shape)}")
+
+
+def _check_table(page_table, device, who: str):
+    if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or page_table.device != device:
+        _fail(f"{who}: page_table must be an int32 tensor on the cache's device")
+    if page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        _fail(f"{who}: page_table must be [sequences, pages] with contiguous rows")
+    if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
+        _fail(f"{who}: page_table must be contiguous")
+
+
+def _vector_rows(t: torch.Tensor) -> torch.Tensor:
+    """`t` itself where every row of its last dimension is contiguous and 16-byte aligned, else a contiguous copy."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def kv4_append(cache, k, v, page_table, starts, cu_seqlens):
+    """k, v [tokens, kv_heads, head_dim] -> the cache's pages (struct cb_kv4_cache; cb_kv4_append)."""
+    rec, dev = _kv4_record(cache, "kv4_append"), cache.pages.device
+    for t, name in ((k, "k"), (v, "v")):
+        if t.device != dev or t.dtype != cache.dtype:
+            _fail(f"kv4_append: {name} must be of the cache's dtype, on its device")
+        if t.dim() != 3 or t.shape[1] != rec.kv_heads or t.shape[2] != rec.head_dim:
+            _fail(f"kv4_append: {name} must be [tokens, {rec.kv_heads}, {rec.head_dim}]")
+    if k.shape != v.shape:
+        _fail("kv4_append: k and v must have the same shape")
+    _check_table(page_table, dev, "kv4_append")
+    n, seqs = k.shape[0], page_table.shape[0]
+    _check_index(starts, dev, (seqs,), "starts", "kv4_append")
+    if cu_seqlens is not None:
+        _check_index(cu_seqlens, dev, (seqs + 1,), "cu_seqlens", "kv4_append")
+    if n == 0:
+        return
+    k, v = _vector_rows(k), _vector_rows(v)
+    strides = (_i64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
+    with _on_device(dev):
+        _rc(_lib.cb_kv4_append(ctypes.byref(rec), k.data_ptr(), v.data_ptr(), strides, n, page_table.data_ptr(),
+                               page_table.shape[1], seqs, starts.data_ptr(),
+                               0 if cu_seqlens is None else cu_seqlens.data_ptr(), _stream(k)))
+
+
+def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
+    """(k, v) [tokens, kv_heads, head_dim]: the values that the cache holds for the named tokens (cb_kv4_read)."""
+    rec, dev = _kv4_record(cache, "kv4_read"), cache.pages.device
+    _check_table(page_table, dev, "kv4_read")
+    n, seqs = int(n_tokens), page_table.shape[0]
+    if n < 0:
+        _fail("kv4_read: n_tokens must not be negative")
+    _check_index(starts, dev, (seqs,), "starts", "kv4_read")
+    if cu_seqlens is not None:
+        _check_index(cu_seqlens, dev, (seqs + 1,), "cu_seqlens", "kv4_read")
+    k = torch.empty((n, rec.kv_heads, rec.head_dim), dtype=cache.dtype, device=dev)
+    v = torch.empty_like(k)
+    if n:
+        with _on_device(dev):
+            _rc(_lib.cb_kv4_read(ctypes.byref(rec), k.data_ptr(), v.data_ptr(), n, page_table.data_ptr(),
+                                 page_table.shape[1], seqs, starts.data_ptr(),
+                                 0 if cu_seqlens is None else cu_seqlens.data_ptr(), _stream(k)))
+    return k, v
+
+
+# Scratch of the cache's attention.  Eager calls: counters (zeroed when made; every call leaves them zero) and partial
+# sums of one (device, stream), where calls run one after another.  Captured calls: partial sums from the graph's own
+# pool, and counters that no other call ever gets, cut from a slab zeroed beforehand -- two graphs may then run at the
+# same time.  A capture that finds no slab, or an empty one, zeroes its counters inside the graph.
+_kv4_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
+_kv4_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
+_KV4_SLAB = 1 << 18
+
+
+def kv4_prepare_device(device: torch.device):
+    """Make the slab of zeroed counters that captured calls on this device draw from (not inside a capture)."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    if index not in _kv4_slab and not torch.cuda.is_current_stream_capturing():
+        with _on_device(torch.device("cuda", index)):
+            slab = torch.zeros(_KV4_SLAB, dtype=torch.int32, device=torch.device("cuda", index))
+            torch.cuda.current_stream(index).synchronize()       # visible to whatever stream a graph will run on
+        _kv4_slab[index] = [slab, 0]
+
+
+def _kv4_scratch(dev, stream: int, counters: int, nbytes: int):
+    if torch.cuda.is_current_stream_capturing():
+        partial = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        slab, need = _kv4_slab.get(dev.index), -(-counters // 32) * 32
+        if slab is None or slab[1] + need > _KV4_SLAB:
+            return torch.zeros(counters, dtype=torch.int32, device=dev), partial
+        slab[1] += need
+        return slab[0][slab[1] - need:slab[1]], partial
+    have = _kv4_eager.get((dev.index, stream))
+    if have is None or have[0].numel() < counters or have[1].numel() < nbytes:
+        have = (torch.zeros(max(counters, 4096), dtype=torch.int32, device=dev),
+                torch.empty(nbytes, dtype=torch.uint8, device=dev))
+        _kv4_eager[(dev.index, stream)] = have
+    return have
+
+
+def kv4_attention(q, cache, page_table, lengths, scale: float):
+    """q [B, T, H, head_dim] -> [B, T, H, head_dim] (cb_kv4_attention)."""
+    rec, dev = _kv4_record(cache, "kv4_attention"), cache.pages.device
+    if q.device != dev or q.dtype != cache.dtype:
+        _fail("kv4_attention: q must be of the cache's dtype, on its device")
+    if q.dim() != 4 or q.shape[3] != rec.head_dim:
+        _fail(f"kv4_attention: q must be [B, T, H, {rec.head_dim}]")
+    B, T, H, D = q.shape
+    if H % rec.kv_heads:
+        _fail("kv4_attention: q's heads must be a multiple of the cache's")
+    _check_table(page_table, dev, "kv4_attention")
+    if page_table.shape[0] != B:
+        _fail("kv4_attention: page_table needs one row for each sequence of q")
+    _check_index(lengths, dev, (B,), "lengths", "kv4_attention")
+    out = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    q = _vector_rows(q)
+    with _on_device(dev):
+        st = _stream(q)
+        counters, partial = _kv4_scratch(dev, st, _lib.cb_kv4_attention_counters(B, T, H, rec.kv_heads),
+                                         _lib.cb_kv4_attention_partial_bytes(T, H, rec.kv_heads, D))
+        _rc(_lib.cb_kv4_attention(ctypes.byref(rec), q.data_ptr(), (_i64 * 3)(*q.stride()[:3]), out.data_ptr(), B, T, H,
+                                  page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), scale,
+                                  counters.data_ptr(), counters.numel() * 4, partial.data_ptr(), partial.numel(), st))
+    return out

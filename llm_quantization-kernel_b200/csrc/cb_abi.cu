@@ -45,6 +45,8 @@ int launch_peer_wait(const GemvParams& P, cudaStream_t stream);
 int launch_peer_signal(const GemvParams& P, cudaStream_t stream);
 int gemm_status_read_and_clear(int* out);
 int gemm_ws_status_read_and_clear(int* out);
+int kv4_status_read_and_clear(int* out);
+int kv4_attn_status_read_and_clear(int* out);
 int launch_gemm_ws_gate_up(int dtype, const void* x, int64_t M, const cb_weight* gate, const cb_weight* up, void* out,
                            int64_t K, int bits, int64_t gs, cudaStream_t stream);
 int launch_gemm_ws_qkv(int dtype, const void* x, int64_t M, const cb_weight* q, const cb_weight* k, const cb_weight* v,
@@ -92,14 +94,6 @@ inline int64_t effective_split(int64_t B, int64_t V, int64_t split_k) {
     if (split_k <= 1) return 1;
     return ceil_div(B, kMaxBatchBlock) * ceil_div(V, kTileN) > kMaxCounters ? 1 : split_k;
 }
-
-#define CB_REQUIRE(cond, ...)                 \
-    do {                                      \
-        if (!(cond)) {                        \
-            cb::set_error(__VA_ARGS__);       \
-            return CB_ERR_INVALID;            \
-        }                                     \
-    } while (0)
 
 int check_common(const char* who, const void* x, int64_t B, int64_t K, int bits, int64_t gs, int dtype) {
     CB_REQUIRE(B >= 0, "%s: negative batch", who);
@@ -214,7 +208,10 @@ int cb_decode_status(int* status) {
     int c = 0;
     rc = gemm_ws_status_read_and_clear(&c);
     if (rc != CB_OK) return rc;
-    *status = a != 0 ? a : (b != 0 ? 1000 + b : (c != 0 ? 2000 + c : 0));
+    int d = 0, e = 0;
+    if ((rc = kv4_status_read_and_clear(&d)) != CB_OK) return rc;
+    if ((rc = kv4_attn_status_read_and_clear(&e)) != CB_OK) return rc;
+    *status = a != 0 ? a : (b != 0 ? 1000 + b : (c != 0 ? 2000 + c : (d != 0 ? d : e)));
     return CB_OK;
 }
 int cb_tile_n(void) { return kTileN; }

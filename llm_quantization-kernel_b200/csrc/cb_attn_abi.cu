@@ -1,0 +1,114 @@
+// extern "C" entry points of the attention operators: argument checks and kernel choice.
+#include "cb_common.cuh"
+#include "cb_kv4.cuh"
+
+namespace cb {
+
+int launch_kv4_rows(bool append, const cb_kv4_cache* c, const void* k_in, const void* v_in, const int64_t* strides, void* k_out,
+                    void* v_out, int64_t n_tokens, const int32_t* table, int64_t table_stride, int64_t n_seqs,
+                    const int32_t* starts, const int32_t* cu, cudaStream_t stream);
+int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_strides, void* out, int64_t B, int64_t T, int64_t H,
+                         const int32_t* table, int64_t table_stride, const int32_t* lengths, float scale, int* counters,
+                         float* partial, cudaStream_t stream);
+int64_t kv4_attention_segments(int64_t B, int64_t rows, int64_t kv_heads);
+size_t kv4_attention_partial_bytes(int64_t rows, int head_dim);
+
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+int64_t block_bytes(int head_dim, int group_size) {
+    if ((head_dim != 64 && head_dim != 128) || (group_size != 32 && group_size != 64 && group_size != 128) || group_size > head_dim) return 0;
+    return 2 * kKvBlock * (head_dim / 2 + 4 * (head_dim / group_size));
+}
+
+int check_cache(const char* who, const cb_kv4_cache* c) {
+    CB_REQUIRE(c != nullptr, "%s: cache record is NULL", who);
+    CB_REQUIRE(c->dtype == CB_F16 || c->dtype == CB_BF16, "%s: the cache's dtype must be fp16 or bf16", who);
+    CB_REQUIRE(block_bytes(c->head_dim, c->group_size) != 0,
+               "%s: head_dim must be 64 or 128 and group_size 32, 64 or 128, at most head_dim (got %d, %d)", who, c->head_dim, c->group_size);
+    CB_REQUIRE(c->page_size >= kKvBlock && c->page_size % kKvBlock == 0 && c->page_size <= (1 << 20),
+               "%s: page_size must be a multiple of 16", who);
+    CB_REQUIRE(c->kv_heads > 0 && c->kv_heads < (1 << 20), "%s: kv_heads out of range", who);
+    CB_REQUIRE(c->n_pages >= 0 && c->n_pages < (1ll << 31), "%s: n_pages out of range", who);
+    CB_REQUIRE(c->pages != nullptr && aligned16(c->pages), "%s: pages must be a 16-byte aligned pointer", who);
+    return CB_OK;
+}
+
+int check_rows(const char* who, const cb_kv4_cache* c, const void* k, const void* v, int64_t n_tokens, const int32_t* table,
+               int64_t table_stride, int64_t n_seqs, const int32_t* starts, const int32_t* cu) {
+    const int rc = check_cache(who, c);
+    if (rc != CB_OK) return rc;
+    CB_REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 31), "%s: n_tokens out of range", who);
+    CB_REQUIRE(n_seqs >= 0 && n_seqs < (1ll << 31) && table_stride >= 0 && table_stride < (1ll << 31), "%s: page table out of range", who);
+    if (n_tokens == 0) return CB_OK;
+    CB_REQUIRE(n_seqs > 0, "%s: tokens without a sequence", who);
+    CB_REQUIRE(cu != nullptr || n_tokens % n_seqs == 0, "%s: without cu_seqlens every sequence has as many tokens", who);
+    CB_REQUIRE(k && v && starts && (table || table_stride == 0), "%s: NULL pointer", who);
+    CB_REQUIRE(aligned16(k) && aligned16(v), "%s: k and v must be 16-byte aligned", who);
+    return CB_OK;
+}
+
+}  // namespace
+}  // namespace cb
+
+using namespace cb;
+
+extern "C" {
+
+size_t cb_kv4_block_bytes(int head_dim, int group_size) { return (size_t)block_bytes(head_dim, group_size); }
+
+int cb_kv4_append(const cb_kv4_cache* cache, const void* k, const void* v, const int64_t* strides4, int64_t n_tokens,
+                  const int32_t* page_table, int64_t table_stride, int64_t n_seqs, const int32_t* starts,
+                  const int32_t* cu_seqlens, void* stream) {
+    const int rc = check_rows("kv4_append", cache, k, v, n_tokens, page_table, table_stride, n_seqs, starts, cu_seqlens);
+    if (rc != CB_OK || n_tokens == 0) return rc;
+    CB_REQUIRE(strides4 != nullptr, "kv4_append: strides are NULL");
+    for (int i = 0; i < 4; ++i) CB_REQUIRE(strides4[i] % 8 == 0, "kv4_append: strides must be multiples of 8 elements");
+    return launch_kv4_rows(true, cache, k, v, strides4, nullptr, nullptr, n_tokens, page_table, table_stride, n_seqs, starts,
+                           cu_seqlens, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int cb_kv4_read(const cb_kv4_cache* cache, void* k, void* v, int64_t n_tokens, const int32_t* page_table, int64_t table_stride,
+                int64_t n_seqs, const int32_t* starts, const int32_t* cu_seqlens, void* stream) {
+    const int rc = check_rows("kv4_read", cache, k, v, n_tokens, page_table, table_stride, n_seqs, starts, cu_seqlens);
+    if (rc != CB_OK || n_tokens == 0) return rc;
+    return launch_kv4_rows(false, cache, nullptr, nullptr, nullptr, k, v, n_tokens, page_table, table_stride, n_seqs, starts,
+                           cu_seqlens, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int64_t cb_kv4_attention_counters(int64_t B, int64_t T, int64_t H, int64_t kv_heads) {
+    if (B <= 0 || T <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads != 0) return 0;
+    return kv4_attention_segments(B, T * (H / kv_heads), kv_heads);
+}
+
+size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, int head_dim) {
+    if (T <= 0 || H <= 0 || kv_heads <= 0 || H % kv_heads != 0) return 0;
+    return kv4_attention_partial_bytes(T * (H / kv_heads), head_dim);
+}
+
+int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* strides3, void* out, int64_t B, int64_t T, int64_t H,
+                     const int32_t* page_table, int64_t table_stride, const int32_t* lengths, float scale, void* counters,
+                     size_t counter_bytes, void* partial, size_t partial_bytes, void* stream) {
+    const char* who = "kv4_attention";
+    const int rc = check_cache(who, cache);
+    if (rc != CB_OK) return rc;
+    CB_REQUIRE(B >= 0 && B < (1ll << 31) && T >= 0 && H >= 0, "%s: negative or too large batch, T or H", who);
+    CB_REQUIRE(table_stride >= 0 && table_stride < (1ll << 31), "%s: page table out of range", who);
+    if (B == 0 || T == 0 || H == 0) return CB_OK;
+    CB_REQUIRE(H % cache->kv_heads == 0, "%s: H must be a multiple of kv_heads", who);
+    CB_REQUIRE(T < (1 << 24) && H < (1 << 20) && T * H * cache->head_dim < (1ll << 31), "%s: T * H out of range", who);
+    const int64_t segs = cb_kv4_attention_counters(B, T, H, cache->kv_heads);
+    CB_REQUIRE(segs < (1ll << 31), "%s: too many rows", who);
+    CB_REQUIRE(q && out && lengths && strides3 && (page_table || table_stride == 0), "%s: NULL pointer", who);
+    CB_REQUIRE(aligned16(q) && aligned16(out), "%s: q and out must be 16-byte aligned", who);
+    for (int i = 0; i < 3; ++i) CB_REQUIRE(strides3[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    CB_REQUIRE(counters != nullptr && counter_bytes >= (size_t)segs * sizeof(int), "%s: needs %lld zeroed counters", who, (long long)segs);
+    const size_t need = cb_kv4_attention_partial_bytes(T, H, cache->kv_heads, cache->head_dim);
+    CB_REQUIRE(partial != nullptr && partial_bytes >= need && aligned16(partial), "%s: needs %zu bytes of 16-byte aligned scratch", who, need);
+    return launch_kv4_attention(cache, q, strides3, out, B, T, H, page_table, table_stride, lengths, scale,
+                                reinterpret_cast<int*>(counters), reinterpret_cast<float*>(partial),
+                                reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

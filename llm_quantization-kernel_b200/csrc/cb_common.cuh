@@ -211,4 +211,12 @@ bool pdl_enabled();   // programmatic dependent launches are in use (on unless s
         }                                                                                  \
     } while (0)
 
+#define CB_REQUIRE(cond, ...)                 \
+    do {                                      \
+        if (!(cond)) {                        \
+            cb::set_error(__VA_ARGS__);       \
+            return CB_ERR_INVALID;            \
+        }                                     \
+    } while (0)
+
 }  // namespace cb

@@ -1,0 +1,593 @@
+"""The 4-bit key/value cache: append, read and attention against their definition in 64 bits.
+
+    lo = min(x), scale = round_T((max(x) - lo) / 15), code = round_half_even((x - lo) / scale) <= 15, value = code * scale + lo
+    out = softmax(scale * q K^T) V over the cached tokens that a row sees
+
+What the bytes of a page mean is restated here (`Layout`), apart from the kernels' own arithmetic.
+"""
+import ctypes
+import math
+
+import pytest
+import torch
+
+DEV = "cuda"
+FORMATS = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)]
+
+
+# ------------------------------------------------------------------------------------------------ restatement
+def quantise64(x, gs):
+    """codes, scale, lo (double) of x [..., D], scale and lo as the cache's type holds them."""
+    g = x.double().unflatten(-1, (-1, gs))
+    lo = g.amin(-1)
+    scale = ((g.amax(-1) - lo) / 15).to(x.dtype).double()
+    safe = torch.where(scale == 0, torch.ones_like(scale), scale)
+    codes = torch.round((g - lo[..., None]) / safe[..., None]).clamp(0, 15)
+    return torch.where(scale[..., None] == 0, torch.zeros_like(codes), codes).flatten(-2), scale, lo
+
+
+def values64(codes, scale, lo):
+    gs = codes.shape[-1] // scale.shape[-1]
+    return codes * scale.repeat_interleave(gs, -1) + lo.repeat_interleave(gs, -1)
+
+
+class Layout:
+    """Byte positions inside a page of one head: blocks of 16 tokens [K codes | K (scale, lo) | V codes | V (scale, lo)]."""
+
+    def __init__(self, d, gs):
+        self.d, self.gs, self.ng = d, gs, d // gs
+        self.row, self.meta = d // 2, 4 * self.ng
+        self.half = 16 * (self.row + self.meta)
+        self.block = 2 * self.half
+
+    def nibble(self, which, d, tok):
+        j, w = divmod(d, self.gs)
+        lanes = 4 if which == "k" else 8              # lanes that share a row: each holds gs / lanes values of every group
+        lane, i = divmod(w, self.gs // lanes)
+        n = lane * (self.d // lanes) + j * (self.gs // lanes) + i
+        return n ^ 64 if which == "v" and self.d == 128 and tok & 2 else n
+
+    def put(self, page, which, off, codes, scale, lo, dtype):
+        """Write one row (token `off` of the page) into page [bytes] (a CPU uint8 tensor)."""
+        base = off // 16 * self.block + (self.half if which == "v" else 0)
+        tok = off % 16
+        row = [0] * self.row
+        for d in range(self.d):
+            n = self.nibble(which, d, tok)
+            row[n // 2] |= int(codes[d]) << (4 * (n % 2))
+        page[base + tok * self.row:base + (tok + 1) * self.row] = torch.tensor(row, dtype=torch.uint8)
+        at = base + 16 * self.row + tok * self.meta
+        pair = torch.stack((scale, lo), -1).to(dtype).contiguous().view(torch.uint8).flatten()
+        page[at:at + self.meta] = pair
+
+
+def test_layout_is_a_permutation_and_fills_a_block():
+    from crispybits_kernels import _C
+    for d, gs in FORMATS:
+        lay = Layout(d, gs)
+        for which in "kv":
+            for tok in range(16):
+                assert sorted(lay.nibble(which, i, tok) for i in range(d)) == list(range(d))
+        assert _C.kv4_block_bytes(d, gs) == lay.block and lay.block % 128 == 0
+    for d, gs in ((64, 128), (96, 32), (128, 16), (0, 0), (256, 64), (128, 256)):
+        assert _C.kv4_block_bytes(d, gs) == 0
+
+
+# ------------------------------------------------------------------------------------------------ refusals, no GPU needed
+def test_c_entry_points_refuse_bad_arguments():
+    from crispybits_kernels import _C
+    lib = _C._lib
+    strides, s3 = (ctypes.c_int64 * 4)(8, 8, 8, 8), (ctypes.c_int64 * 3)(8, 8, 8)
+
+    def cache(**kw):
+        f = dict(pages=256, n_pages=4, kv_heads=2, head_dim=128, group_size=64, page_size=64, dtype=1)
+        f.update(kw)
+        return _C._KV4Cache(*(f[n] for n, _ in _C._KV4Cache._fields_))
+
+    def append(c, k=256, v=256, st=strides, n=4, table=256, stride=2, seqs=2, starts=256, cu=256):
+        return lib.cb_kv4_append(ctypes.byref(c) if c is not None else None, k, v, st, n, table, stride, seqs, starts, cu, 0)
+
+    for bad in (dict(pages=0), dict(pages=8), dict(head_dim=96), dict(group_size=16), dict(head_dim=64, group_size=128),
+                dict(page_size=24), dict(page_size=0), dict(dtype=0), dict(kv_heads=0), dict(n_pages=-1), dict(n_pages=1 << 31)):
+        assert append(cache(**bad)) == 1 and lib.cb_last_error(), bad
+    good = cache()
+    assert append(None) == 1
+    for bad in (dict(n=-1), dict(seqs=0), dict(n=5, cu=0), dict(k=0), dict(v=8), dict(starts=0), dict(table=0), dict(st=None),
+                dict(st=(ctypes.c_int64 * 4)(8, 8, 4, 8)), dict(stride=-1)):
+        assert append(good, **bad) == 1, bad
+    assert append(good, n=0, k=0, v=0) == 0                    # nothing to do
+    assert lib.cb_kv4_read(ctypes.byref(good), 0, 256, 4, 256, 2, 2, 256, 256, 0) == 1
+    assert lib.cb_kv4_read(ctypes.byref(good), 256, 8, 4, 256, 2, 2, 256, 256, 0) == 1
+
+    def attend(c=good, q=256, st=s3, out=256, B=2, T=1, H=4, table=256, stride=2, lengths=256, cnt=256, nc=1 << 20, part=256,
+               np_=1 << 30):
+        return lib.cb_kv4_attention(ctypes.byref(c), q, st, out, B, T, H, table, stride, lengths, 1.0, cnt, nc, part, np_, 0)
+
+    for bad in (dict(H=3), dict(B=-1), dict(T=-1), dict(q=0), dict(out=4), dict(lengths=0), dict(st=None), dict(cnt=0), dict(nc=12),
+                dict(st=(ctypes.c_int64 * 3)(8, 3, 8)), dict(part=0), dict(part=8), dict(c=cache(dtype=7)), dict(T=1 << 24)):
+        assert attend(**bad) == 1, bad
+    assert attend(B=0) == 0 and attend(T=0) == 0
+    assert lib.cb_kv4_attention_counters(3, 4, 32, 8) == 3 * 8 and lib.cb_kv4_attention_counters(3, 5, 32, 8) == 3 * 8 * 2
+    assert lib.cb_kv4_attention_counters(1, 1, 5, 2) == 0
+
+
+def test_python_entry_points_refuse_cpu_tensors_and_bad_formats():
+    import crispybits_kernels as ck
+    for kw in (dict(head_dim=96), dict(head_dim=64, group_size=128), dict(head_dim=128, page_size=20), dict(head_dim=128, page_size=0),
+               dict(head_dim=128, dtype=torch.float32)):
+        with pytest.raises(ValueError):
+            ck.KV4Cache.empty(2, 2, device="cpu", **kw)
+    with pytest.raises(ValueError):
+        ck.KV4Cache.empty(0, 2, 64, device="cpu")
+    c = ck.KV4Cache.empty(2, 2, 64, device="cpu")
+    assert (c.n_pages, c.kv_heads, c.pages.shape[2]) == (2, 2, 4 * Layout(64, 64).block)
+    i32 = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        ck.kv4_append(c, torch.zeros(1, 2, 64).half(), torch.zeros(1, 2, 64).half(), i32[None], i32)
+    with pytest.raises(RuntimeError):
+        ck.kv4_attention(torch.zeros(1, 2, 64).half(), c, i32[None], i32)
+    with pytest.raises(RuntimeError):
+        ck.kv4_read(c, i32[None], i32, None, 1)
+
+
+def test_python_struct_mirror_matches_the_c_header(tmp_path):
+    import os
+    import subprocess
+
+    from conftest import ROOT
+    from crispybits_kernels import _C
+    lines = ['printf("%zu\\n", sizeof(cb_kv4_cache));'] + [f'printf("%zu\\n", offsetof(cb_kv4_cache, {f}));' for f, _ in _C._KV4Cache._fields_]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "crispybits_b200.h"\nint main(void) {\n' + "\n".join(lines) + "\nreturn 0; }\n")
+    subprocess.run(["gcc", "-std=c99", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "layout")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [ctypes.sizeof(_C._KV4Cache)] + [getattr(_C._KV4Cache, f).offset for f, _ in _C._KV4Cache._fields_]
+
+
+# ------------------------------------------------------------------------------------------------ GPU: append and read
+def i32(values, device=DEV):
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def rand_kv(n, heads, d, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(n, heads, d, generator=g) * (0.5 + 3.0 * (torch.rand(heads, d, generator=g) > 0.95))
+    return x.to(dtype).to(DEV)
+
+
+def table_for(need, n_pages, seed):
+    """Rows of distinct pages in random order; the rest of each row holds page numbers that do not exist."""
+    ids = torch.randperm(n_pages, generator=torch.Generator().manual_seed(seed)).tolist()
+    rows, at = [], 0
+    for n in need:
+        rows.append(ids[at:at + n] + [-1] * (max(need) - n))
+        at += n
+    return rows
+
+
+def offsets(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,gs", FORMATS)
+@pytest.mark.parametrize("page", [16, 48, 64])
+def test_append_writes_exactly_the_defined_bytes(dtype, d, gs, page):
+    """Every byte of the pool: the rows of the new tokens as defined, everything else as it was."""
+    import crispybits_kernels as ck
+    heads, lens, starts = 3, [1, 17, 0, 70, 5], [0, 15, 9, 31, 63]
+    need = [max(1, -(-(s + n) // page)) for s, n in zip(starts, lens)]
+    cache = ck.KV4Cache.empty(sum(need) + 1, heads, d, page, gs, dtype, DEV)
+    pool = torch.randint(0, 256, cache.pages.shape, generator=torch.Generator().manual_seed(7), dtype=torch.uint8)
+    cache.pages.copy_(pool)
+    rows = table_for(need, sum(need) + 1, 3)
+    k, v = rand_kv(sum(lens), heads, d, dtype, 1), rand_kv(sum(lens), heads, d, dtype, 2)
+    ck.kv4_append(cache, k, v, i32(rows), i32(starts), i32(offsets(lens)))
+    lay = Layout(d, gs)
+    for name, x in (("k", k), ("v", v)):
+        codes, scale, lo = (t.cpu() for t in quantise64(x, gs))
+        i = 0
+        for s, n in enumerate(lens):
+            for p in range(starts[s], starts[s] + n):
+                for h in range(heads):
+                    lay.put(pool[rows[s][p // page], h], name, p % page, codes[i, h], scale[i, h], lo[i, h], dtype)
+                i += 1
+    got = cache.pages.cpu()
+    assert torch.equal(got, pool), f"{int((got != pool).sum())} bytes differ"
+    # and back: one rounding of code * scale + lo in fp32 (2^-24 of its larger part), one to the type
+    gk, gv = ck.kv4_read(cache, i32(rows), i32(starts), i32(offsets(lens)), sum(lens))
+    for got_x, x in ((gk, k), (gv, v)):
+        codes, scale, lo = quantise64(x, gs)
+        want = values64(codes, scale, lo)
+        size = (15 * scale + lo.abs()).repeat_interleave(gs, -1)
+        tol = torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2 ** -20) + 2.0 ** -24 * size + 2.0 ** -25
+        assert ((got_x.double() - want).abs() <= tol).all()
+        # each value is within half a step of what was appended (and the rounding of scale: 15 eps / 2 of a step)
+        step = scale.repeat_interleave(gs, -1)
+        assert ((want - x.double()).abs() <= step * (0.5 + 15 * torch.finfo(dtype).eps)).all()
+
+
+@pytest.mark.gpu
+def test_append_forms_and_strides_agree():
+    """[B, H, D], [B, T, H, D], packed, column slices of a fused projection and misaligned rows: the same bytes."""
+    import crispybits_kernels as ck
+    B, T, heads, d = 3, 4, 2, 64
+    fused = rand_kv(B * T, 3 * heads + 1, d, torch.float16, 5).flatten(1)
+    k, v = fused[:, heads * d:2 * heads * d].view(-1, heads, d), fused[:, 2 * heads * d:3 * heads * d].view(-1, heads, d)
+    odd = torch.empty(k.numel() + 1, dtype=torch.float16, device=DEV)[1:].view(k.shape).copy_(k)
+    assert odd.data_ptr() % 16 and not k.is_contiguous()
+    rows, starts = i32(table_for([1] * B, B, 1)), i32([3, 0, 60 - T])
+
+    def bytes_of(*args):
+        c = ck.KV4Cache.empty(B, heads, d)
+        c.pages.zero_()
+        ck.kv4_append(c, *args)
+        return c.pages
+
+    want = bytes_of(k.contiguous(), v.contiguous(), rows, starts, i32([0, T, 2 * T, 3 * T]))
+    assert want.any()
+    assert torch.equal(want, bytes_of(k, v, rows, starts, i32([0, T, 2 * T, 3 * T])))
+    assert torch.equal(want, bytes_of(odd, v, rows, starts))
+    assert torch.equal(want, bytes_of(k.view(B, T, heads, d), v.reshape(B, T, heads, d), rows, starts))
+    heads_first = k.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(want, bytes_of(heads_first, v, rows, starts))
+    # token by token, as decode steps do
+    c = ck.KV4Cache.empty(B, heads, d)
+    c.pages.zero_()
+    for j in range(T):
+        ck.kv4_append(c, k.view(B, T, heads, d)[:, j], v.view(B, T, heads, d)[:, j], rows, starts + j)
+    assert torch.equal(want, c.pages)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_append_edge_values(dtype):
+    """Constant groups, zeros, negative zero, ties, the type's largest values, subnormal ranges, infinities and NaN."""
+    import crispybits_kernels as ck
+    d, gs, big = 64, 32, torch.finfo(dtype).max
+    if dtype == torch.bfloat16:
+        big = 2.0 ** 126            # the range of a group has to be a float
+    rows = [torch.full((d,), 3.0), torch.zeros(d), torch.linspace(-1, 1, d), torch.arange(d) * 0.5 - 7.5,
+            torch.cat((torch.full((16,), -big), torch.full((48,), big))), torch.full((d,), -big),
+            torch.arange(d) * torch.finfo(dtype).tiny / 64, torch.arange(d) % 16 * 1.0, torch.arange(d) % 31 * 0.5,
+            torch.cat((torch.full((31,), 1.0), torch.full((33,), 1.0 + torch.finfo(dtype).eps)))]
+    x = torch.stack(rows).to(dtype).to(DEV)[:, None]                     # [n, 1, d]
+    n = x.shape[0]
+    c = ck.KV4Cache.empty(1, 1, d, 64, gs, dtype)
+    ck.kv4_append(c, x, -x, i32([[0]]), i32([0]), i32([0, n]))
+    gk, gv = ck.kv4_read(c, i32([[0]]), i32([0]), i32([0, n]), n)
+    for got, src in ((gk, x), (gv, -x)):
+        codes, scale, lo = quantise64(src, gs)
+        if dtype == torch.bfloat16:
+            small = scale < 2.0 ** -126
+            scale = torch.where(small, 0.0, scale)
+            codes = torch.where(small.repeat_interleave(gs, -1), 0.0, codes)
+        # scale is rounded: 65504 of a range of 131008 stands for 15 * 8736 - 65504 = 65536, which fp16 does not have
+        want = values64(codes, scale, lo).clamp(-torch.finfo(dtype).max, torch.finfo(dtype).max)
+        size = (15 * scale + lo.abs()).repeat_interleave(gs, -1)
+        tol = torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2 ** -20) + 2.0 ** -24 * size + torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+        over = ((got.double() - want).abs() - tol).amax(-1).flatten().tolist()
+        assert max(over) <= 0, over
+    y = x.clone()
+    y[2, 0, 5], y[3, 0, 40], y[7, 0, 0] = math.nan, math.inf, -math.inf
+    ck.kv4_append(c, y, y, i32([[0]]), i32([0]), i32([0, n]))
+    gk, gv = ck.kv4_read(c, i32([[0]]), i32([0]), i32([0, n]), n)
+    bad = torch.zeros(n, 1, d, dtype=torch.bool, device=DEV)
+    bad[2, 0, :32] = bad[3, 0, 32:] = bad[7, 0, :32] = True
+    assert torch.equal(gk.isnan(), bad) and torch.equal(gv.isnan(), bad)
+
+
+@pytest.mark.gpu
+def test_tokens_without_a_place_are_left_out():
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    d, heads, page = 64, 2, 16
+    k, v = rand_kv(40, heads, d, torch.float16, 1), rand_kv(40, heads, d, torch.float16, 2)
+    _C.decode_status()
+    # sequence 0: its second page does not exist (-1, then one past the end); sequence 1 runs over the table's end; starts below 0
+    for wrong in (-1, 3, -(1 << 31), (1 << 31) - 1):
+        c = ck.KV4Cache.empty(3, heads, d, page)
+        c.pages.fill_(0xAB)
+        table = i32([[0, wrong], [1, 2]])
+        ck.kv4_append(c, k, v, table, i32([10, 25]), i32([0, 20, 40]))
+        assert _C.decode_status() == 3001 and _C.decode_status() == 0
+        good = ck.KV4Cache.empty(3, heads, d, page)
+        good.pages.fill_(0xAB)
+        ck.kv4_append(good, torch.cat((k[:6], k[20:27])), torch.cat((v[:6], v[20:27])), i32([[0, 0], [1, 2]]), i32([10, 25]), i32([0, 6, 13]))
+        assert torch.equal(c.pages, good.pages) and _C.decode_status() == 0
+        gk, _ = ck.kv4_read(c, table, i32([10, 25]), i32([0, 20, 40]), 40)
+        assert torch.equal(gk[:6], ck.kv4_read(good, i32([[0, 0], [1, 2]]), i32([10, 25]), i32([0, 6, 13]), 13)[0][:6])
+        assert _C.decode_status() == 3001
+    c.pages.fill_(0xAB)
+    ck.kv4_append(c, k, v, i32([[0, 1]]), i32([-50]), i32([0, 40]))
+    assert (c.pages == 0xAB).all() and _C.decode_status() == 3001
+    # tokens before the first and behind the last sequence belong to none: no error
+    ck.kv4_append(c, k, v, i32([[0, 1]]), i32([0]), i32([3, 5]))
+    assert _C.decode_status() == 0
+    gk, _ = ck.kv4_read(c, i32([[0, 1]]), i32([0]), i32([0, 2]), 2)
+    codes, scale, lo = quantise64(k[3:5], 64)
+    assert (gk.double() - values64(codes, scale, lo)).abs().max() < 2e-2
+    assert (c.pages[2] == 0xAB).all()
+
+
+# ------------------------------------------------------------------------------------------------ GPU: attention
+class Filled:
+    """A cache with sequences of the given lengths, and the values it holds in 64 bits."""
+
+    def __init__(self, lens, heads, d, gs, page, dtype, seed=0, spare=2, k_gain=1.0):
+        import crispybits_kernels as ck
+        need = [max(1, -(-n // page)) for n in lens]
+        self.lens, self.rows = lens, table_for(need, sum(need) + spare, seed + 3)
+        self.cache = ck.KV4Cache.empty(sum(need) + spare, heads, d, page, gs, dtype)
+        self.cache.pages.fill_(0xFF)                       # what was never appended: NaN scales, codes 15
+        self.k, self.v = rand_kv(sum(lens), heads, d, dtype, seed) * k_gain, rand_kv(sum(lens), heads, d, dtype, seed + 1)
+        self.table, self.lengths = i32(self.rows), i32(lens)
+        ck.kv4_append(self.cache, self.k, self.v, self.table, i32([0] * len(lens)), i32(offsets(lens)))
+        self.gs = gs
+
+    def reference(self, q, scale=None, drop=None):
+        """(out, tolerance) for q [B, T, H, D]; drop[b]: positions left out.
+
+        Tolerance, for each output: the final rounding; the weights' rounding to fp16, 2^-11 of the code part (v - lo)
+        that they multiply; the scores' error -- fp32 sums of 2 D products, and of D code products each cut to the
+        accumulator's width, 2^-20 of their absolute sum is ample -- which moves every weight and their sum by exp of it."""
+        B, T, H, D = q.shape
+        scale = D ** -0.5 if scale is None else scale
+        heads = self.cache.kv_heads
+        out, tol = torch.zeros(B, T, H, D, dtype=torch.double, device=DEV), torch.zeros(B, T, H, D, dtype=torch.double, device=DEV)
+        parts = [quantise64(x, self.gs) for x in (self.k, self.v)]
+        at = offsets(self.lens)
+        for b, n in enumerate(self.lens):
+            (kc, ks, kl), (vc, vs, vl) = ([t[at[b]:at[b + 1]] for t in part] for part in parts)
+            kv, vv = values64(kc, ks, kl), values64(vc, vs, vl)
+            vcode = values64(vc, vs, torch.zeros_like(vl))
+            kabs = values64(kc, ks, kl.abs())
+            pos = torch.arange(n, device=DEV)
+            for j in range(T):
+                seen = pos < n - T + 1 + j
+                if drop is not None:
+                    for p in drop[b]:
+                        seen &= pos != p
+                if not seen.any():
+                    continue
+                for h in range(H):
+                    g = h // (H // heads)
+                    qq = q[b, j, h].double()
+                    w = torch.softmax((kv[seen, g] @ qq) * scale, 0)
+                    err = 2.0 ** -20 * ((kabs[seen, g] @ qq.abs()) * abs(scale)).max()
+                    out[b, j, h] = w @ vv[seen, g]
+                    tol[b, j, h] = (torch.finfo(q.dtype).eps / 2 * out[b, j, h].abs() * 1.01 + 2.0 ** -11 * 1.01 * (w @ vcode[seen, g])
+                                    + 2 * (err + 2.0 ** -21) * (w @ (vcode[seen, g] + vl.abs().repeat_interleave(self.gs, -1)[seen, g])) + 1e-7)
+        return out, tol
+
+
+def check(got, want):
+    out, tol = want
+    over = (got.double() - out).abs() - tol
+    assert torch.isfinite(got).all() and (over <= 0).all(), f"{over.max():.2e} over, at tolerance {tol[over == over.max()][0]:.2e}"
+
+
+def rand_q(B, T, H, D, dtype, seed=9):
+    return torch.randn(B, T, H, D, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,gs", FORMATS)
+@pytest.mark.parametrize("T,group,page", [(1, 1, 64), (1, 8, 16), (3, 4, 32), (5, 2, 80)])
+def test_attention_matches_the_definition(dtype, d, gs, T, group, page):
+    import crispybits_kernels as ck
+    heads, lens = 3, [1, 0, 2, 15, 16, 17, 333, 64, 700]
+    f = Filled(lens, heads, d, gs, page, dtype, seed=d + gs)
+    q = rand_q(len(lens), T, heads * group, d, dtype)
+    got = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    check(got, f.reference(q))
+    for b, n in enumerate(lens):
+        for j in range(T):
+            if n - T + 1 + j <= 0:
+                assert (got[b, j] == 0).all()
+    if T == 1:
+        assert torch.equal(got[:, 0], ck.kv4_attention(q[:, 0], f.cache, f.table, f.lengths))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,heads,group,n", [(1, 1, 1, 1), (1, 1, 1, 5000), (1, 2, 16, 2500), (2, 1, 71, 400), (40, 5, 1, 33), (300, 1, 2, 20)])
+def test_attention_over_shapes(B, heads, group, n):
+    """One head and one long sequence, many query heads, many short sequences (more of them than a warp scans at once)."""
+    import crispybits_kernels as ck
+    lens = [max(0, n - 7 * (b % 4)) for b in range(B)]
+    f = Filled(lens, heads, 64, 32, 32, torch.float16, seed=n)
+    q = rand_q(B, 1, heads * group, 64, torch.float16)
+    check(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
+
+
+@pytest.mark.gpu
+def test_attention_scale_strides_and_sharp_scores():
+    import crispybits_kernels as ck
+    f = Filled([200, 77], 2, 128, 128, 64, torch.bfloat16, k_gain=8.0)
+    wide = rand_q(2, 2, 11, 128, torch.bfloat16) * 4
+    q = wide[:, :, 3:7]                                            # a slice of a fused projection
+    want = f.reference(q, 0.5)
+    got = ck.kv4_attention(q, f.cache, f.table, f.lengths, scale=0.5)
+    check(got, want)
+    assert torch.equal(got, ck.kv4_attention(q.contiguous(), f.cache, f.table, f.lengths, 0.5))
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape).copy_(q)
+    assert torch.equal(got, ck.kv4_attention(odd, f.cache, f.table, f.lengths, 0.5))
+    t = q.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(got, ck.kv4_attention(t, f.cache, f.table, f.lengths, 0.5))
+
+
+@pytest.mark.gpu
+def test_attention_value_scales_of_very_different_size():
+    """Values of most tokens 2^-9 of a few tokens': the weights are rounded against the largest scale met."""
+    import crispybits_kernels as ck
+    f = Filled([600], 1, 64, 32, 16, torch.float16)
+    f.v[::3] *= 2.0 ** -9
+    f.v[5] *= 64.0
+    ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0]), i32([0, 600]))
+    q = rand_q(1, 2, 4, 64, torch.float16)
+    check(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
+
+
+@pytest.mark.gpu
+def test_attention_ignores_what_a_row_does_not_see():
+    """Infinities and NaN in tokens behind the length, and in the newest token for the rows before it."""
+    import crispybits_kernels as ck
+    f = Filled([100, 50], 2, 128, 64, 64, torch.float16)
+    q = rand_q(2, 3, 4, 128, torch.float16)
+    want = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    bad = torch.full((2, 2, 128), math.nan, dtype=torch.float16, device=DEV)
+    bad[1] = math.inf
+    ck.kv4_append(f.cache, bad, bad, f.table, f.lengths)           # one token more, not counted by lengths
+    assert torch.equal(want, ck.kv4_attention(q, f.cache, f.table, f.lengths))
+    got = ck.kv4_attention(q, f.cache, f.table, f.lengths + 1)     # now the last row of each sequence sees it
+    assert got[:, 2].isnan().all() and torch.isfinite(got[:, :2]).all()
+    # rows 0 and 1 see what rows 1 and 2 saw before
+    out, tol = f.reference(torch.cat((q[:, :1], q[:, :2]), 1))
+    check(got[:, :2], (out[:, 1:], tol[:, 1:]))
+
+
+@pytest.mark.gpu
+def test_attention_leaves_out_pages_that_do_not_exist():
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    f = Filled([100, 90], 1, 64, 64, 16, torch.float16)
+    q = rand_q(2, 1, 2, 64, torch.float16)
+    _C.decode_status()
+    table = f.table.clone()
+    table[0, 2], table[1, 0], table[1, 5] = -1, f.cache.n_pages, (1 << 31) - 1
+    got = ck.kv4_attention(q, f.cache, table, f.lengths)
+    assert _C.decode_status() == 3001 and _C.decode_status() == 0
+    check(got, f.reference(q, drop=[range(32, 48), [*range(16), *range(80, 96)]]))
+    none = torch.full_like(table, -5)
+    assert (ck.kv4_attention(q, f.cache, none, f.lengths) == 0).all() and _C.decode_status() == 3001
+    # lengths below zero see nothing, beyond the table everything there is (all six pages full)
+    full = Filled([96, 96], 1, 64, 64, 16, torch.float16)
+    got = ck.kv4_attention(q, full.cache, full.table, i32([-3, 1 << 30]))
+    assert (got[0] == 0).all() and torch.equal(got[1], ck.kv4_attention(q, full.cache, full.table, full.lengths)[1])
+    assert torch.isfinite(got).all() and _C.decode_status() == 0
+
+
+@pytest.mark.gpu
+def test_attention_is_the_same_every_time_on_any_stream_and_captured():
+    import crispybits_kernels as ck
+    f = Filled([3000, 10, 1500], 2, 128, 64, 64, torch.bfloat16)
+    q = rand_q(3, 1, 8, 128, torch.bfloat16)
+    want = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    check(want, f.reference(q))
+    for _ in range(5):
+        assert torch.equal(want, ck.kv4_attention(q, f.cache, f.table, f.lengths))
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams * 4:
+        with torch.cuda.stream(s):
+            outs.append(ck.kv4_attention(q, f.cache, f.table, f.lengths))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, o) for o in outs)
+    graphs = []
+    for _ in range(2):                                             # two graphs that run at the same time
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = [ck.kv4_attention(q, f.cache, f.table, f.lengths) for _ in range(3)]
+        graphs.append((g, outs))
+    for _ in range(10):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, o) for _, outs in graphs for o in outs)
+    # a replay reads what the index tensors hold then
+    f.lengths.copy_(i32([2999, 0, 1]))
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1][0], ck.kv4_attention(q, f.cache, f.table, f.lengths)) and (graphs[0][1][0][1] == 0).all()
+
+
+@pytest.mark.gpu
+def test_a_captured_decode_step_appends_and_attends():
+    """One step's append and attention captured, replayed for several tokens: as eager steps."""
+    import crispybits_kernels as ck
+    B, heads, d, steps, dt = 3, 2, 64, 20, torch.float16
+    k, v = rand_kv(B * steps, heads, d, dt, 1).view(steps, B, heads, d), rand_kv(B * steps, heads, d, dt, 2).view(steps, B, heads, d)
+    q = torch.stack([rand_q(B, 1, 4, d, dt, s)[:, 0] for s in range(steps)])
+    table = i32(table_for([2] * B, 2 * B, 4))
+
+    def fresh():
+        c = ck.KV4Cache.empty(2 * B, heads, d, 16)
+        return c, i32([0, 3, 11])
+
+    c, n = fresh()
+    ck.kv4_append(c, v[0].repeat(11, 1, 1)[:14], k[0].repeat(11, 1, 1)[:14], table, i32([0, 0, 0]), i32([0, 0, 3, 14]))
+    start = c.pages.clone()
+    eager = []
+    for s in range(steps):
+        ck.kv4_append(c, k[s], v[s], table, n)
+        n = n + 1
+        eager.append(ck.kv4_attention(q[s], c, table, n))
+    pages = c.pages.clone()
+    c.pages.copy_(start)
+    n = i32([0, 3, 11])
+    sk, sv, sq = k[0].clone(), v[0].clone(), q[0].clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ck.kv4_append(c, sk, sv, table, n)
+        n += 1
+        out = ck.kv4_attention(sq, c, table, n)
+    for s in range(steps):
+        sk.copy_(k[s]); sv.copy_(v[s]); sq.copy_(q[s])
+        g.replay()
+        assert torch.equal(out, eager[s]), s
+    assert torch.equal(c.pages, pages)
+
+
+@pytest.mark.gpu
+def test_pages_beyond_32_bit_offsets():
+    import crispybits_kernels as ck
+    heads, d, page = 64, 128, 64
+    per_page = heads * 4 * Layout(d, 64).block
+    n_pages = (1 << 32) // per_page + 40
+    c = ck.KV4Cache.empty(n_pages, heads, d, page)
+    lens = [130, 64]
+    table = i32([[n_pages - 1, n_pages - 20, 7], [n_pages - 3, 0, 0]])
+    k, v = rand_kv(194, heads, d, torch.float16, 1), rand_kv(194, heads, d, torch.float16, 2)
+    small = ck.KV4Cache.empty(5, heads, d, page)
+    table_small = i32([[0, 1, 2], [3, 0, 0]])
+    q = rand_q(2, 1, heads, d, torch.float16)
+    res = []
+    for cache, tab in ((c, table), (small, table_small)):
+        ck.kv4_append(cache, k, v, tab, i32([0, 0]), i32([0, 130, 194]))
+        res.append((*ck.kv4_read(cache, tab, i32([0, 0]), i32([0, 130, 194]), 194), ck.kv4_attention(q, cache, tab, i32(lens))))
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_shapes_and_devices_that_do_not_fit_are_refused():
+    import crispybits_kernels as ck
+    f = Filled([20], 2, 64, 32, 16, torch.float16)
+    q = rand_q(1, 1, 4, 64, torch.float16)
+    k = f.k[:1]
+    ok = (f.table, f.lengths)
+    for args in ((q.bfloat16(), f.cache, *ok), (q[..., :32], f.cache, *ok), (q[:, :, :3], f.cache, *ok), (q.cpu(), f.cache, *ok),
+                 (q, f.cache, f.table.long(), f.lengths), (q, f.cache, f.table, f.lengths.long()), (q, f.cache, f.table.cpu(), f.lengths),
+                 (q, f.cache, f.table, i32([1, 2])), (q.repeat(2, 1, 1, 1), f.cache, *ok), (q, f.cache, f.table[0], f.lengths),
+                 (q, f.cache, f.table.repeat(1, 2)[:, ::2], f.lengths)):
+        with pytest.raises(RuntimeError):
+            ck.kv4_attention(*args)
+    for args in ((k.float(), k, *ok), (k, k[:, :1], *ok), (k[..., :32], k[..., :32], *ok), (k, k.cpu(), *ok),
+                 (k, k, f.table, f.lengths.cpu()), (k, k, *ok, i32([0, 1, 1])), (k, k, *ok, torch.tensor([0, 1], device=DEV))):
+        with pytest.raises(RuntimeError):
+            ck.kv4_append(f.cache, *args)
+    with pytest.raises(ValueError):
+        ck.kv4_append(f.cache, f.k[:3], f.k[:3], f.table.repeat(2, 1), i32([0, 0]))
+    with pytest.raises(RuntimeError):
+        ck.kv4_read(f.cache, *ok, None, -1)
+    wrong = ck.KV4Cache(f.cache.pages, 128, 16, 32, torch.float16)
+    with pytest.raises(RuntimeError):
+        ck.kv4_attention(rand_q(1, 1, 4, 128, torch.float16), wrong, *ok)
+    assert ck.kv4_attention(q[:, :0], f.cache, *ok).shape == (1, 0, 4, 64)
+    ck.kv4_append(f.cache, k[:0], k[:0], *ok, i32([0, 0]))
