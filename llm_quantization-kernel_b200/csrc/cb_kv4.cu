@@ -176,13 +176,8 @@ kv4_append_kernel(const RowParams P) {
                     *reinterpret_cast<uint32_t*>(blk + in_block * L::kRow + L::k_nibble(d) / 2) = word;
                     if (lead) *reinterpret_cast<uint32_t*>(blk + L::kKMeta + in_block * L::kMeta + (d / GS) * 4) = meta;
                 } else {
-                    unsigned char* row = blk + L::kVCodes + in_block * L::kRow;
-                    if constexpr (GS >= 64) {
-                        *reinterpret_cast<uint32_t*>(row + L::v_nibble(d, in_block) / 2) = word;
-                    } else {                                              // four values to a lane and group
-                        *reinterpret_cast<uint16_t*>(row + L::v_nibble(d, in_block) / 2) = (uint16_t)word;
-                        *reinterpret_cast<uint16_t*>(row + L::v_nibble(d + 4, in_block) / 2) = (uint16_t)(word >> 16);
-                    }
+                    *reinterpret_cast<uint16_t*>(blk + L::kVCodes + L::v_byte(d, in_block)) = (uint16_t)word;
+                    *reinterpret_cast<uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, in_block)) = (uint16_t)(word >> 16);
                     if (lead) *reinterpret_cast<uint32_t*>(blk + L::kVMeta + in_block * L::kMeta + (d / GS) * 4) = meta;
                 }
             }
@@ -225,10 +220,8 @@ kv4_read_kernel(const RowParams P) {
                     word[i] = *reinterpret_cast<const uint32_t*>(blk + in_block * L::kRow + L::k_nibble(d) / 2);
                     meta[i] = *reinterpret_cast<const uint32_t*>(blk + L::kKMeta + in_block * L::kMeta + (d / GS) * 4);
                 } else {
-                    const unsigned char* row = blk + L::kVCodes + in_block * L::kRow;
-                    if constexpr (GS >= 64) word[i] = *reinterpret_cast<const uint32_t*>(row + L::v_nibble(d, in_block) / 2);
-                    else word[i] = *reinterpret_cast<const uint16_t*>(row + L::v_nibble(d, in_block) / 2) |
-                                   ((uint32_t)*reinterpret_cast<const uint16_t*>(row + L::v_nibble(d + 4, in_block) / 2) << 16);
+                    word[i] = *reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d, in_block)) |
+                              ((uint32_t)*reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, in_block)) << 16);
                     meta[i] = *reinterpret_cast<const uint32_t*>(blk + L::kVMeta + in_block * L::kMeta + (d / GS) * 4);
                 }
             }

@@ -4,17 +4,17 @@
 // value = code * scale + lo.  lo and scale are of the cache's 16-bit type.
 //
 // The unit of storage is a BLOCK of 16 tokens of one head, contiguous:
-//     K codes [16][D/2 bytes] | K meta [16][D/GS] (scale, lo) | V codes [16][D/2 bytes] | V meta [16][D/GS] (scale, lo)
+//     K codes 16 x D/2 bytes | K meta [16][D/GS] (scale, lo) | V codes 16 x D/2 bytes | V meta [16][D/GS] (scale, lo)
 // so that one bulk copy brings everything the attention of 16 tokens needs.  A page of a head is page_size / 16
 // consecutive blocks, and pages are [n_pages][kv_heads][page].
 //
-// Inside a token's D/2 code bytes the values stand in the order in which the lanes of mma.sync fragments want them
-// (a lane's codes are contiguous, one wide shared-memory load each):
-//   * K is the A operand of S^T = K q^T.  Lane (r, t) of a fragment (r = lane / 4, t = lane % 4) takes the values
-//     t * GS/4 .. t * GS/4 + GS/4 - 1 of every group, group after group.
-//   * V is the A operand of O^T = V^T P^T.  Lane (r, t) takes the values r * GS/8 .. r * GS/8 + GS/8 - 1 of every
-//     group.  At D = 128 the two 32-byte halves of a token whose number has bit 1 set are exchanged: the four tokens
-//     that the lanes t = 0..3 read together then lie in different banks.
+// The codes stand in the order in which the lanes of mma.sync fragments want them (lane = 4 r + t):
+//   * K is the 16-row operand of S^T = K q^T.  A token's D/2 bytes are contiguous; lane (r, t) takes the values
+//     t * GS/4 .. t * GS/4 + GS/4 - 1 of every group, and they lie side by side: one wide shared-memory load.
+//   * V is the 16-row operand of O^T = V^T P^T, whose registers hold the same value of two tokens: tokens t and 7 - t (t = 0..3),
+//     and t + 8 and 15 - t.  Such a pair shares D bytes, in which lane r's D/8 bytes are the values
+//     r * GS/8 .. r * GS/8 + GS/8 - 1 of every group, four at a time: 16 bits of the one token, 16 of the other.  The order of
+//     the lanes' pieces depends on the pair such that lanes which read together meet different banks.
 #pragma once
 #include "cb_common.cuh"
 
@@ -37,11 +37,15 @@ struct KvLayout {
         const int j = d / GS, w = d % GS;
         return (w / (GS / 4)) * (D / 4) + j * (GS / 4) + w % (GS / 4);
     }
-    // The same for value d (a multiple of min(8, GS / 8)) of token `tok` (0..15) of V; the next min(8, GS / 8) follow.
-    __host__ __device__ static constexpr int v_nibble(int d, int tok) {
-        const int j = d / GS, w = d % GS;
-        const int n = (w / (GS / 8)) * (D / 8) + j * (GS / 8) + w % (GS / 8);
-        return D == 128 ? n ^ (((tok >> 1) & 1) << 6) : n;
+    // Byte, inside V's codes, of values d .. d + 3 (d a multiple of 4) of token `tok` (0..15): two bytes.
+    __host__ __device__ static constexpr int v_byte(int d, int tok) {
+        const int pair = ((tok & 4) ? 7 - (tok & 7) : (tok & 3)) + 4 * (tok >> 3);
+        const int w = d % GS, lane = w / (GS / 8), unit = (d / GS * (GS / 8) + w % (GS / 8)) / 4;
+        return pair * D + v_piece(lane, pair) + unit * 4 + ((tok & 4) ? 2 : 0);
+    }
+    // Where lane r's piece of a pair begins in the pair's D bytes.
+    __host__ __device__ static constexpr int v_piece(int lane, int pair) {
+        return D == 128 ? (lane ^ (2 * (pair & 3))) * 16 : (lane ^ (4 * ((pair >> 1) & 1))) * 8;
     }
 };
 

@@ -44,7 +44,10 @@ struct AttnParams {
     const int32_t* lengths;
     int64_t B;
     int T, H, G, R, row_tiles;
-    float scale_log2;                                 // softmax scale * log2(e)
+    bool aligned;                                     // no CTA's part crosses a segment's end
+    float scale_log2;                                 // |softmax scale| * log2(e), above 0
+    float q_sign;                                     // 1, or -1 where the scale is negative
+    uint32_t zero;                                    // 0, unknown to the compiler
     int* counters;                                    // [B * kv_heads * row_tiles], zero between calls
     float* partial;                                   // [grid][2][rows of a tile * (D + 2)]
 };
@@ -55,17 +58,17 @@ struct AttnCfg {
     static constexpr int kRows = 8 * NT;
     static constexpr int kSlotBytes = kStageBlocks * L::kBytes;
     static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
-    // the ring fills what an SM has; the slots of a warp are at most 8
-    static constexpr int kRingBudget = (NT == 1 ? 108 : 216) * 1024;
+    static constexpr int kMerge = kWarps * kRows * D * 4;             // the warps' outputs; then the weights of a cut segment's parts
+    // the ring fills what an SM has left; the slots of a warp are at most 8
+    static constexpr int kRingBudget = (NT == 1 ? 110 : 222) * 1024 - kMerge;
     static constexpr int kSlots = kRingBudget / (kWarps * kSlotBytes) > 8 ? 8 : kRingBudget / (kWarps * kSlotBytes);
-    static constexpr int kRing = kWarps * kSlots * kSlotBytes;
-    static constexpr int kMerge = kWarps * kRows * D * 4;             // reuses the ring's space
-    static_assert(kMerge <= kRing, "the merge buffer lies over the ring");
-    static constexpr int kStatsOff = kRing;                           // [2][kWarps][kRows] floats: max, sum
+    static_assert(kSlots >= 1, "a ring has a slot");
+    static constexpr int kMergeOff = kWarps * kSlots * kSlotBytes;
+    static constexpr int kStatsOff = kMergeOff + kMerge;              // [2][kWarps][kRows] floats: max, sum
     static constexpr int kBarOff = kStatsOff + 2 * kWarps * kRows * 4;
     static constexpr int kOkOff = kBarOff + kWarps * kSlots * 8;      // [kWarps][kSlots] blocks whose page is good
     static constexpr int kMiscOff = kOkOff + kWarps * kSlots * 4;
-    static constexpr int kSmem = kMiscOff + 64 + kWarps * 8;
+    static constexpr int kSmem = kMiscOff + 16;
     static_assert(kSmem <= (227 * 1024) / kCtasPerSm - 1024, "shared memory of an SM");
     static constexpr int kPartFloats = kRows * (D + 2);
 };
@@ -87,12 +90,16 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -104,17 +111,32 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { retu
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
 }
+// Larger of each half; NaN loses.
+template <typename T> __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <> __device__ __forceinline__ uint32_t max2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
 template <int N> __device__ __forceinline__ void lds_words(const unsigned char* p, uint32_t (&w)[N]) {
     if constexpr (N == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
     else if constexpr (N == 2) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
     else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
-__device__ __forceinline__ int64_t seq_len(const AttnParams& P, int64_t b) {
+// Cached tokens and blocks of a sequence.  The caller has checked that the table's capacity in blocks, times the segments
+// of a sequence, fits 31 bits.
+__device__ __forceinline__ int seq_len(const AttnParams& P, int64_t b) {
     const int64_t cap = P.c.table_stride * P.c.blocks_per_page * kKvBlock;
-    return min(max((int64_t)P.lengths[b], (int64_t)0), cap);
+    return (int)min((int64_t)max(P.lengths[b], 0), cap);
 }
-__device__ __forceinline__ int64_t seq_blocks(const AttnParams& P, int64_t b) { return (seq_len(P, b) + kKvBlock - 1) / kKvBlock; }
+__device__ __forceinline__ int blocks_of(int len) { return (int)(((unsigned)len + kKvBlock - 1) / kKvBlock); }
+
+constexpr int kOpen = 12;
+__device__ __forceinline__ int units_open(int nblk) { return nblk == 0 ? 0 : nblk + kOpen; }
 
 template <typename T, int D, int GS, int NT>
 __global__ void __launch_bounds__(kThreads, (AttnCfg<D, GS, NT>::kCtasPerSm))
@@ -123,13 +145,11 @@ kv4_attention_kernel(const AttnParams P) {
     using L = typename C::L;
     constexpr int NG = L::NG, kSlots = C::kSlots, kRows = C::kRows;
     constexpr int KW = D / 32, KWG = GS / 32;          // code words of a lane and key row, of one group
-    constexpr int VW = D / 64;                         // code words of a lane and value row
     extern __shared__ __align__(128) unsigned char smem[];
-    float* merge = reinterpret_cast<float*>(smem);
+    float* merge = reinterpret_cast<float*>(smem + C::kMergeOff);
     float* st_max = reinterpret_cast<float*>(smem + C::kStatsOff);
     float* st_sum = st_max + kWarps * kRows;
     volatile int* misc = reinterpret_cast<volatile int*>(smem + C::kMiscOff);           // [0] abort, [1] last arrival
-    int64_t* red = reinterpret_cast<int64_t*>(smem + C::kMiscOff + 64);                 // [kWarps]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t bars = smem_u32(smem + C::kBarOff) + warp * kSlots * 8;
     volatile uint32_t* slot_ok = reinterpret_cast<volatile uint32_t*>(smem + C::kOkOff) + warp * kSlots;
@@ -143,29 +163,38 @@ kv4_attention_kernel(const AttnParams P) {
     }
     if (tid == 0) misc[0] = 0;
 
-    // ---- the whole line's length, and sequences without keys: their rows are zero
-    int64_t blocks = 0;
-    for (int64_t b = tid; b < P.B; b += kThreads) blocks += seq_blocks(P, b);
+    // ---- the line's length (every warp for itself), and sequences without keys: their rows are zero
+    int64_t U = 0;
+    {
+        int64_t units = 0;
+        for (int64_t b = lane; b < P.B; b += 32) units += P.aligned ? blocks_of(seq_len(P, b)) : units_open(blocks_of(seq_len(P, b)));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
-    if (lane == 0) red[warp] = blocks;
+        for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
+        U = units * segs;
+    }
     for (int64_t b = blockIdx.x; b < P.B; b += gridDim.x)
-        if (seq_blocks(P, b) == 0) {
+        if (seq_len(P, b) == 0) {
             uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(P.out) + b * P.T * P.H * D);
             for (int i = tid; i < P.T * P.H * D / 2; i += kThreads) o[i] = 0u;
         }
+    if (U == 0) return;
     __syncthreads();
-    int64_t U = 0;
-    for (int w = 0; w < kWarps; ++w) U += red[w];
-    U *= segs;
+    // ---- this CTA's part [u0, u1) of the line.  aligned: a segment of nb blocks is cut into ceil(nb / quota) parts, one to a CTA
+    // (quota such that there are CTAs enough), and u counts parts.  Otherwise the line is cut into equal parts, in which a segment
+    // counts kOpen units more than its blocks, ahead of them: what a CTA spends on a segment besides.
     const int64_t nc = min((int64_t)gridDim.x, U);
-    if (blockIdx.x >= nc) return;
-    const int64_t u0 = blockIdx.x * U / nc, u1 = (blockIdx.x + 1) * U / nc;
+    const int quota = P.aligned ? (int)((U + gridDim.x - 1 - P.B * segs) / (gridDim.x - P.B * segs)) : 1;
+    auto units_of = [&](int nblk) { return P.aligned ? (nblk + quota - 1) / quota : units_open(nblk); };     // of one segment
+    const int64_t u0 = P.aligned ? (int64_t)blockIdx.x : blockIdx.x * U / nc;
+    const int64_t u1 = P.aligned ? u0 + 1 : (blockIdx.x + 1) * U / nc;
+    if (u0 >= u1) return;
 
-    // ---- the sequence that holds unit u0 (every warp for itself)
-    int64_t b = 0, base = 0, nb = 0;
+    // ---- the sequence that holds unit u0
+    int64_t b = -1, base = 0;
+    int len = 0, nb = 0, per_seg = 0;
     for (int64_t b0 = 0; b0 < P.B; b0 += 32) {
-        const int64_t mine = b0 + lane < P.B ? seq_blocks(P, b0 + lane) * segs : 0;
+        const int my_len = b0 + lane < P.B ? seq_len(P, b0 + lane) : 0;
+        const int64_t mine = (int64_t)units_of(blocks_of(my_len)) * segs;
         int64_t cum = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -176,25 +205,75 @@ kv4_attention_kernel(const AttnParams P) {
         if (past != 0u) {
             const int l = __ffs(past) - 1;
             b = b0 + l;
-            nb = __shfl_sync(0xffffffffu, mine, l) / segs;
+            len = __shfl_sync(0xffffffffu, my_len, l);
             base += __shfl_sync(0xffffffffu, cum - mine, l);
             break;
         }
         base += __shfl_sync(0xffffffffu, cum, 31);
     }
+    if (b < 0) return;                                 // aligned: more CTAs than parts
+    nb = blocks_of(len);
+    per_seg = units_of(nb);
 
-    uint32_t it = 0;                                   // stages this warp has taken from its ring, ever
-    for (int64_t u = u0; u < u1;) {
-        while (u >= base + nb * segs) {
-            base += nb * segs;
-            if (++b >= P.B) return;                    // only if lengths changed while the kernel ran
-            nb = seq_blocks(P, b);
+    // ---- a piece: the blocks [blk0, blk1) of one segment
+    int64_t u = u0, seg0 = 0;                          // seg0: the segment's first unit
+    int seg = 0, blk0 = 0, blk1 = 0;
+    auto piece_at = [&](int64_t at) {
+        const unsigned local = (unsigned)(at - base);
+        seg = (int)(local / (unsigned)per_seg);
+        const int part = (int)(local - (unsigned)seg * (unsigned)per_seg);
+        seg0 = at - part;
+        if (P.aligned) {
+            blk0 = (int)((int64_t)part * nb / per_seg);
+            blk1 = (int)((int64_t)(part + 1) * nb / per_seg);
+        } else {
+            blk0 = max(part - kOpen, 0);
+            blk1 = (int)min((int64_t)nb, u1 - seg0 - kOpen);           // may be 0 or less: nothing but the opening
         }
-        const int seg = (int)((u - base) / nb);
-        const int64_t seg0 = base + seg * nb;          // first unit of the segment
-        const int64_t blk0 = u - seg0, blk1 = min(nb, u1 - seg0);
+    };
+    piece_at(u);
+    if (blk1 <= blk0) return;
+
+    // ---- this warp's stages of the piece: stage i holds `per` blocks from first(i) on; few blocks: one to a stage
+    uint32_t it = 0;                                   // stages this warp has taken from its ring, ever
+    int per = 1, mine = 0;
+    auto first_of = [&](int i) { return blk0 + (warp + i * kWarps) * per; };
+    auto issue = [&](int i, uint32_t at) {
+        const uint32_t s = at % kSlots;
+        const int blk = first_of(i) + lane;
+        int64_t page = -1;
+        int in_page = 0;
+        if (lane < per && blk < blk1) {
+            const int row = blk / P.c.blocks_per_page;
+            in_page = blk - row * P.c.blocks_per_page;
+            page = P.c.table[b * P.c.table_stride + row];
+            if (page < 0 || page >= P.c.n_pages) { page = -1; atomicExch(&g_kv4_attn_status, kKv4BadPage); }
+        }
+        const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
+        const uint32_t bar = bars + 8 * s;
+        if (lane == 0) {
+            slot_ok[s] = good;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(__popc(good) * L::kBytes)) : "memory");
+        }
+        __syncwarp();
+        if (page >= 0) {
+            const unsigned char* src = P.c.pages + ((page * kv_heads + seg % kv_heads) * P.c.blocks_per_page + in_page) * L::kBytes;
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(ring_u32 + s * C::kSlotBytes + lane * L::kBytes), "l"(src), "r"((uint32_t)L::kBytes), "r"(bar) : "memory");
+        }
+    };
+    auto begin_piece = [&]() {                         // the first stages of a piece are on their way before anything else
+        const int pieces = blk1 - blk0;
+        per = pieces > kWarps ? kStageBlocks : 1;
+        const int nstage = (pieces + per - 1) / per;
+        mine = warp < nstage ? (nstage - 1 - warp) / kWarps + 1 : 0;
+        for (int i = 0; i < kSlots && i < mine; ++i) issue(i, it + i);
+    };
+    begin_piece();
+
+    for (;;) {
         const int kvh = seg % kv_heads, row0 = (seg / kv_heads) * kRows;
-        const int len = (int)min(seq_len(P, b), (int64_t)0x7fffffff);
+        const bool whole = blk0 == 0 && blk1 == nb;
 
         // ---- query rows: fp16 fragments, their scales, sums and limits
         uint32_t qf[NT][KW * 4];
@@ -222,7 +301,7 @@ kv4_attention_kernel(const AttnParams P) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const int e = min(max((int)(__float_as_uint(mx) >> 23), 14), 254);
-            const float f = __uint_as_float((uint32_t)(267 - e) << 23);              // 2^(140 - e)
+            const float f = P.q_sign * __uint_as_float((uint32_t)(267 - e) << 23);   // 2^(140 - e)
             float sum[NG];
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
@@ -270,60 +349,17 @@ kv4_attention_kernel(const AttnParams P) {
         }
         int s_exp = 15;                                // exponent field of the power of two that p * scale is divided by
 
-        // ---- this warp's stages of the piece: stage i holds blocks first(i) .. + cnt; few blocks: one to a stage
-        const int pieces = (int)(blk1 - blk0);
-        const int per = pieces > kWarps ? kStageBlocks : 1;
-        const int nstage = (pieces + per - 1) / per;
-        const int mine = warp < nstage ? (nstage - 1 - warp) / kWarps + 1 : 0;
-        auto issue = [&](int i, uint32_t at) {
-            const uint32_t s = at % kSlots;
-            const int64_t first = blk0 + (int64_t)(warp + i * kWarps) * per;
-            const int64_t blk = first + lane;
-            int64_t page = -1;
-            const bool in = lane < per && blk < blk1;
-            if (in) {
-                page = P.c.table[b * P.c.table_stride + blk / P.c.blocks_per_page];
-                if (page < 0 || page >= P.c.n_pages) { page = -1; atomicExch(&g_kv4_attn_status, kKv4BadPage); }
-            }
-            const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
-            const uint32_t bar = bars + 8 * s;
-            if (lane == 0) {
-                slot_ok[s] = good;
-                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(__popc(good) * L::kBytes)) : "memory");
-            }
-            __syncwarp();
-            if (page >= 0) {
-                const unsigned char* src = P.c.pages + ((page * kv_heads + kvh) * P.c.blocks_per_page + blk % P.c.blocks_per_page) * L::kBytes;
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                             ::"r"(ring_u32 + s * C::kSlotBytes + lane * L::kBytes), "l"(src), "r"((uint32_t)L::kBytes), "r"(bar) : "memory");
-            }
-        };
-        for (int i = 0; i < kSlots && i < mine; ++i) issue(i, it + i);
-
         const int ra = g & 1 ? 7 - (g >> 1) : (g >> 1);            // token of accumulator row g; row g + 8 is token ra + 8
-        for (int i = 0; i < mine; ++i) {
-            const uint32_t at = it + i, s = at % kSlots;
-            if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * s, (at / kSlots) & 1))) {
-                if (lane == 0) { misc[0] = 1; atomicExch(&g_kv4_attn_status, kKv4Wait); }
-                for (int k = i + 1; k < mine && k < i + kSlots; ++k) mbar_wait(bars + 8 * ((it + k) % kSlots), ((it + k) / kSlots) & 1);
-                break;
-            }
-            const int64_t first = blk0 + (int64_t)(warp + i * kWarps) * per;
-            const unsigned good = slot_ok[s];
-            const unsigned char* stage = ring + s * C::kSlotBytes;
-            const int cnt = (int)min((int64_t)per, blk1 - first);
-            // every token of the stage seen by every row?
-            const bool plain = good == (1u << cnt) - 1u && cnt == kStageBlocks && (first + cnt) * kKvBlock <= lim_min;
+        const int va_off = L::kVCodes + t * D + L::v_piece(g, t);  // this lane's piece of token pair t; pair t + 4 is 4 D further
 
+        // One stage: scores, running maxima, weights, weighted values.  PLAIN: both blocks there, every token seen by every row.
+        auto take = [&](auto plain_tag, const unsigned char* stage, int first, unsigned good) -> uint32_t {
+            constexpr bool PLAIN = decltype(plain_tag)::value;
             float x[kStageBlocks][NT][4];
-            float mx[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mx[n][0] = mx[n][1] = -INFINITY;
-            float smax = 0.f;
+            uint32_t smax2 = 0u;                                   // largest (scale, lo) of the values, as a pair; only scale is used
 #pragma unroll
             for (int k = 0; k < kStageBlocks; ++k) {
-                const bool there = (good >> k) & 1u;
-                if (!there) {
+                if (!PLAIN && !((good >> k) & 1u)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n) x[k][n][0] = x[k][n][1] = x[k][n][2] = x[k][n][3] = -INFINITY;
                     continue;
@@ -334,58 +370,56 @@ kv4_attention_kernel(const AttnParams P) {
                 lds_words<KW>(blk + (ra + 8) * L::kRow + t * (D / 8), wb);
                 lds_words<NG>(blk + L::kKMeta + ra * L::kMeta, ma);
                 lds_words<NG>(blk + L::kKMeta + (ra + 8) * L::kMeta, mb);
+                float acc[NG][NT][4];
 #pragma unroll
-                for (int j = 0; j < NG; ++j) {
-                    float acc[NT][4];
+                for (int wg = 0; wg < KWG; ++wg)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-#pragma unroll
-                    for (int w = j * KWG; w < (j + 1) * KWG; ++w) {
+                    for (int j = 0; j < NG; ++j) {
+                        const int w = j * KWG + wg;
                         const uint32_t ya = wa[w] >> 8, yb = wb[w] >> 8;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma16816(acc[n], wa[w] & 0x000F000Fu, wb[w] & 0x000F000Fu, wa[w] & 0x00F000F0u, wb[w] & 0x00F000F0u,
-                                     qf[n][4 * w], qf[n][4 * w + 1]);
-                            mma16816(acc[n], ya & 0x000F000Fu, yb & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x00F000F0u,
+                            if (wg == 0) mma16816_first(acc[j][n], wa[w] & 0x000F000Fu, wb[w] & 0x000F000Fu, wa[w] & 0x00F000F0u, wb[w] & 0x00F000F0u,
+                                                        qf[n][4 * w], qf[n][4 * w + 1]);
+                            else mma16816(acc[j][n], wa[w] & 0x000F000Fu, wb[w] & 0x000F000Fu, wa[w] & 0x00F000F0u, wb[w] & 0x00F000F0u,
+                                          qf[n][4 * w], qf[n][4 * w + 1]);
+                            mma16816(acc[j][n], ya & 0x000F000Fu, yb & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x00F000F0u,
                                      qf[n][4 * w + 2], qf[n][4 * w + 3]);
                         }
                     }
+#pragma unroll
+                for (int j = 0; j < NG; ++j) {
                     const float2 sa = unpack2<T>(ma[j]), sb = unpack2<T>(mb[j]);     // (scale, lo)
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const float va = fmaf(acc[n][c], sa.x, sa.y * qsum[n][j][c]);
-                            const float vb = fmaf(acc[n][2 + c], sb.x, sb.y * qsum[n][j][c]);
-                            x[k][n][c] = j == 0 ? va : x[k][n][c] + va;
-                            x[k][n][2 + c] = j == 0 ? vb : x[k][n][2 + c] + vb;
+                            x[k][n][c] = fmaf(acc[j][n][c], sa.x, j == 0 ? sa.y * qsum[n][j][c] : fmaf(sa.y, qsum[n][j][c], x[k][n][c]));
+                            x[k][n][2 + c] = fmaf(acc[j][n][2 + c], sb.x, j == 0 ? sb.y * qsum[n][j][c] : fmaf(sb.y, qsum[n][j][c], x[k][n][2 + c]));
                         }
                 }
-                const int tok = (int)(first + k) * kKvBlock + ra;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        x[k][n][c] *= qmul[n][c];
-                        x[k][n][2 + c] *= qmul[n][c];
-                        if (!plain) {
-                            if (tok >= lim[n][c]) x[k][n][c] = -INFINITY;
-                            if (tok + 8 >= lim[n][c]) x[k][n][2 + c] = -INFINITY;
-                        }
-                        mx[n][c] = fmaxf(mx[n][c], fmaxf(x[k][n][c], x[k][n][2 + c]));
-                    }
                 uint32_t va[NG], vb[NG];
                 lds_words<NG>(blk + L::kVMeta + ra * L::kMeta, va);
                 lds_words<NG>(blk + L::kVMeta + (ra + 8) * L::kMeta, vb);
+                const int tok = (first + k) * kKvBlock + ra;
 #pragma unroll
-                for (int j = 0; j < NG; ++j) {                       // fmaxf drops NaN
-                    const float s0 = unpack2<T>(va[j]).x, s1 = unpack2<T>(vb[j]).x;
-                    smax = fmaxf(smax, plain || tok < len ? s0 : 0.f);
-                    smax = fmaxf(smax, plain || tok + 8 < len ? s1 : 0.f);
+                for (int j = 0; j < NG; ++j) {
+                    smax2 = max2<T>(smax2, PLAIN || tok < len ? va[j] : 0u);
+                    smax2 = max2<T>(smax2, PLAIN || tok + 8 < len ? vb[j] : 0u);
+                }
+                if constexpr (!PLAIN) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            if (tok >= lim[n][c]) x[k][n][c] = -INFINITY;
+                            if (tok + 8 >= lim[n][c]) x[k][n][2 + c] = -INFINITY;
+                        }
                 }
             }
-            // ---- running maximum and scale reference
+            // ---- running maximum (of the scaled scores) and scale reference
             float alpha[NT][2];
+            const float smax = fmaxf(unpack2<T>(smax2).x, 0.f);
             const int e_new = max(s_exp, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)) >> 23));
             bool moved = e_new != s_exp;
             const float rs = __uint_as_float((uint32_t)max(127 + s_exp - e_new, 0) << 23);
@@ -394,11 +428,13 @@ kv4_attention_kernel(const AttnParams P) {
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float m = mx[n][c];
+                    float m = fmaxf(x[0][n][c], x[0][n][2 + c]);
+#pragma unroll
+                    for (int k = 1; k < kStageBlocks; ++k) m = fmaxf(m, fmaxf(x[k][n][c], x[k][n][2 + c]));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    const float mn = fmaxf(m_run[n][c], m);
+                    const float mn = fmaxf(m_run[n][c], m * qmul[n][c]);
                     alpha[n][c] = mn == m_run[n][c] ? 1.f : ex2(m_run[n][c] - mn);
                     moved = moved || alpha[n][c] != 1.f;
                     m_run[n][c] = mn;
@@ -421,9 +457,10 @@ kv4_attention_kernel(const AttnParams P) {
                 }
             }
             const float cmul = __uint_as_float((uint32_t)(268 - s_exp) << 23);       // 2^14 / 2^(s_exp - 127)
+            uint32_t words = 0u;
 #pragma unroll
             for (int k = 0; k < kStageBlocks; ++k) {
-                if (!((good >> k) & 1u)) continue;
+                if (!PLAIN && !((good >> k) & 1u)) continue;
                 const unsigned char* blk = stage + k * L::kBytes;
                 uint32_t va[NG], vb[NG];
                 lds_words<NG>(blk + L::kVMeta + ra * L::kMeta, va);
@@ -433,9 +470,9 @@ kv4_attention_kernel(const AttnParams P) {
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const float m = m_run[n][c] == -INFINITY ? 0.f : m_run[n][c];
-                        p[n][c] = ex2(x[k][n][c] - m);
-                        p[n][2 + c] = ex2(x[k][n][2 + c] - m);
+                        const float m = !PLAIN && m_run[n][c] == -INFINITY ? 0.f : m_run[n][c];
+                        p[n][c] = ex2(fmaf(x[k][n][c], qmul[n][c], -m));
+                        p[n][2 + c] = ex2(fmaf(x[k][n][2 + c], qmul[n][c], -m));
                         l_run[n][c] += p[n][c] + p[n][2 + c];
                     }
                 uint32_t pb[NT][NG][2];
@@ -445,34 +482,34 @@ kv4_attention_kernel(const AttnParams P) {
                     const float fa = sa.x * cmul, fb = sb.x * cmul;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float h[4] = {p[n][0] * fa, p[n][1] * fa, p[n][2] * fb, p[n][3] * fb};
-                        float y[4] = {p[n][0] * sa.y, p[n][1] * sa.y, p[n][2] * sb.y, p[n][3] * sb.y};
-                        if (!plain) {
+                        if constexpr (PLAIN) {
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) z[n][j][c] = fmaf(p[n][c], sa.y, fmaf(p[n][2 + c], sb.y, z[n][j][c]));
+                            pb[n][j][0] = movmatrix_t(pack_h2(p[n][0] * fa, p[n][1] * fa));
+                            pb[n][j][1] = movmatrix_t(pack_h2(p[n][2] * fb, p[n][3] * fb));
+                        } else {
                             // what a row does not see adds nothing, whatever is stored there
+                            float h[4] = {p[n][0] * fa, p[n][1] * fa, p[n][2] * fb, p[n][3] * fb};
+                            float y[4] = {p[n][0] * sa.y, p[n][1] * sa.y, p[n][2] * sb.y, p[n][3] * sb.y};
 #pragma unroll
                             for (int c = 0; c < 4; ++c)
                                 if (p[n][c] == 0.f) h[c] = y[c] = 0.f;
+                            z[n][j][0] += y[0] + y[2];
+                            z[n][j][1] += y[1] + y[3];
+                            pb[n][j][0] = movmatrix_t(pack_h2(h[0], h[1]));
+                            pb[n][j][1] = movmatrix_t(pack_h2(h[2], h[3]));
                         }
-                        z[n][j][0] += y[0] + y[2];
-                        z[n][j][1] += y[1] + y[3];
-                        pb[n][j][0] = movmatrix_t(pack_h2(h[0], h[1]));
-                        pb[n][j][1] = movmatrix_t(pack_h2(h[2], h[3]));
+                        words |= pb[n][j][0] | pb[n][j][1];
                     }
                 }
-                // tokens t, 7 - t, t + 8, 15 - t: columns 2t, 2t + 1, 2t + 8, 2t + 9 of the operand
-                uint32_t v[4][VW];
+                uint32_t v0[D / 32], v1[D / 32];                                     // pairs t and t + 4
+                lds_words<D / 32>(blk + va_off, v0);
+                lds_words<D / 32>(blk + va_off + 4 * D, v1);
 #pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                    const int tk = (i4 & 1 ? 7 - t : t) + (i4 & 2 ? 8 : 0);
-                    const int at_byte = D == 128 ? (g * 8) ^ (((tk >> 1) & 1) << 5) : g * 4;
-                    lds_words<VW>(blk + L::kVCodes + tk * L::kRow + at_byte, v[i4]);
-                }
-#pragma unroll
-                for (int hw = 0; hw < 2 * VW; ++hw) {                                // four values of this lane
+                for (int hw = 0; hw < D / 32; ++hw) {                                // four values of this lane, two tokens each
                     const int j = hw * 4 / (GS / 8);
-                    const uint32_t x0 = __byte_perm(v[0][hw >> 1], v[1][hw >> 1], hw & 1 ? 0x7632 : 0x5410);
-                    const uint32_t x1 = __byte_perm(v[2][hw >> 1], v[3][hw >> 1], hw & 1 ? 0x7632 : 0x5410);
-                    const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+                    const uint32_t x0 = v0[hw], x1 = v1[hw], y0 = x0 >> 8, y1 = x1 >> 8;
+                    words |= x0 | x1;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma16816(o[n][2 * hw], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, pb[n][j][0], pb[n][j][1]);
@@ -480,13 +517,49 @@ kv4_attention_kernel(const AttnParams P) {
                     }
                 }
             }
-            __syncwarp();
-            if (i + kSlots < mine) issue(i + kSlots, at + kSlots);       // every code of this slot has gone into a product
+            return words;
+        };
+
+        for (int i = 0; i < mine; ++i) {
+            const uint32_t at = it + i, s = at % kSlots;
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * s, (at / kSlots) & 1))) {
+                if (lane == 0) { misc[0] = 1; atomicExch(&g_kv4_attn_status, kKv4Wait); }
+                for (int k = i + 1; k < mine && k < i + kSlots; ++k) mbar_wait(bars + 8 * ((it + k) % kSlots), ((it + k) / kSlots) & 1);
+                break;
+            }
+            const int first = first_of(i);
+            const unsigned good = slot_ok[s];
+            const unsigned char* stage = ring + s * C::kSlotBytes;
+            const int cnt = min(per, blk1 - first);
+            // A stage of whole blocks that every row sees needs no masks.
+            uint32_t seen_words;
+            if (good == 3u && cnt == kStageBlocks && (first + cnt) * kKvBlock <= lim_min) seen_words = take(std::true_type{}, stage, first, good);
+            else seen_words = take(std::false_type{}, stage, first, good);
+            // The slot may be overwritten once every lane has its codes in registers: the vote needs words that came last, and
+            // what was computed from the others (the bits are masked with a zero that the compiler does not know).
+            const unsigned held = __ballot_sync(0xffffffffu, (seen_words & P.zero) != 0u);
+            if (i + kSlots < mine) issue(i + kSlots, at + kSlots + held);
         }
         it += mine;
 
+        // ---- the next piece's copies start; it is finished with the values of this one kept aside
+        const int64_t this_b = b, this_u = u, this_seg0 = seg0, this_base_seg = b * segs + seg;
+        const int this_per = per_seg;
+        u = P.aligned ? u1 : seg0 + kOpen + blk1;
+        const bool more = u < u1;
+        bool begun = false;
+        if (more && misc[0] == 0) {
+            while (u >= base + (int64_t)per_seg * segs) {
+                base += (int64_t)per_seg * segs;
+                if (++b >= P.B) break;                 // only if lengths changed while the kernel ran
+                len = seq_len(P, b);
+                nb = blocks_of(len);
+                per_seg = units_of(nb);
+            }
+            if (b < P.B && u1 - u > kOpen) { piece_at(u); begin_piece(); begun = true; }
+        }
+
         // ---- the warps' results meet: value = o * 2^24 (2^20) / cmul + z
-        __syncthreads();                                                // nobody reads its ring any more
         {
             const float back = __uint_as_float((uint32_t)(s_exp - 14) << 23);        // 1 / cmul
 #pragma unroll
@@ -506,7 +579,7 @@ kv4_attention_kernel(const AttnParams P) {
                     if (g == 0) { st_max[warp * kRows + row] = m_run[n][c]; st_sum[warp * kRows + row] = l; }
                     float* dst = merge + ((size_t)warp * kRows + row) * D;
 #pragma unroll
-                    for (int hw = 0; hw < 2 * VW; ++hw) {
+                    for (int hw = 0; hw < D / 32; ++hw) {
                         const int j = hw * 4 / (GS / 8);
                         const int d = j * GS + g * (GS / 8) + (hw * 4) % (GS / 8);
                         float4 r4;
@@ -520,78 +593,95 @@ kv4_attention_kernel(const AttnParams P) {
             }
         }
         __syncthreads();
-        if (misc[0] != 0) return;
-        const bool whole = blk0 == 0 && blk1 == nb;
-        auto store = [&](int row, int d, float2 v, float l) {           // two neighbouring values of a finished row
+        if (misc[0] != 0) {                                             // a copy was not heard of: wait (bounded) for the others in flight
+            if (begun)
+                for (int i = 0; i < kSlots && i < mine; ++i) mbar_wait(bars + 8 * ((it + i) % kSlots), ((it + i) / kSlots) & 1);
+            return;
+        }
+        auto store = [&](int row, int d, float4 v, float l) {           // four neighbouring values of a finished row
             const int r = row0 + row;
             if (r >= P.R) return;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (l == 0.f) v = make_float2(0.f, 0.f);
-            T* dst = reinterpret_cast<T*>(P.out) + ((b * P.T + r / P.G) * P.H + kvh * P.G + r % P.G) * D + d;
-            dst[0] = from_f32<T>(v.x * inv);
-            dst[1] = from_f32<T>(v.y * inv);
+            if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+            T* dst = reinterpret_cast<T*>(P.out) + ((this_b * P.T + r / P.G) * P.H + kvh * P.G + r % P.G) * D + d;
+            const T y[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
+            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
         };
-        float* my_part = P.partial + ((int64_t)blockIdx.x * 2 + (u == u0 ? 0 : 1)) * C::kPartFloats;
-        for (int idx = tid; idx < kRows * D / 2; idx += kThreads) {
-            const int row = idx / (D / 2), d = idx % (D / 2) * 2;
-            float m = -INFINITY;
+        float* my_part = P.partial + ((int64_t)blockIdx.x * 2 + (this_u == u0 ? 0 : 1)) * C::kPartFloats;
+        for (int idx = tid; idx < kRows * D / 4; idx += kThreads) {
+            const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+            float mw[kWarps], m = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, st_max[w * kRows + row]);
-            float2 v = make_float2(0.f, 0.f);
+            for (int w = 0; w < kWarps; ++w) { mw[w] = st_max[w * kRows + row]; m = fmaxf(m, mw[w]); }
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             float l = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float f = st_max[w * kRows + row] == -INFINITY ? 0.f : ex2(st_max[w * kRows + row] - m);
-                if (f != 0.f) {
-                    const float2 a = *reinterpret_cast<const float2*>(merge + ((size_t)w * kRows + row) * D + d);
-                    v.x = fmaf(f, a.x, v.x); v.y = fmaf(f, a.y, v.y);
-                    l = fmaf(f, st_sum[w * kRows + row], l);
-                }
+                if (mw[w] == -INFINITY) continue;
+                const float f = ex2(mw[w] - m);
+                const float4 a = *reinterpret_cast<const float4*>(merge + ((size_t)w * kRows + row) * D + d);
+                v.x = fmaf(f, a.x, v.x); v.y = fmaf(f, a.y, v.y); v.z = fmaf(f, a.z, v.z); v.w = fmaf(f, a.w, v.w);
+                l = fmaf(f, st_sum[w * kRows + row], l);
             }
             if (whole) store(row, d, v, l);
             else {
-                *reinterpret_cast<float2*>(my_part + row * D + d) = v;
+                *reinterpret_cast<float4*>(my_part + row * D + d) = v;
                 if (d == 0) { my_part[kRows * D + row] = m; my_part[kRows * D + kRows + row] = l; }
             }
         }
         if (!whole) {
             __threadfence();
             __syncthreads();
-            const int64_t c0 = ((seg0 + 1) * nc - 1) / U, c1 = ((seg0 + nb) * nc - 1) / U;      // CTAs that hold its first and last unit
+            // CTAs that hold the segment's first and last unit
+            const int64_t c0 = P.aligned ? this_seg0 : ((this_seg0 + kOpen + 1) * nc - 1) / U;
+            const int n = P.aligned ? this_per : (int)(((this_seg0 + this_per) * nc - 1) / U - c0) + 1;
             if (tid == 0) {
-                int* counter = P.counters + b * segs + seg;
-                const bool last = atomicAdd(counter, 1) == (int)(c1 - c0);
+                int* counter = P.counters + this_base_seg;
+                const bool last = atomicAdd(counter, 1) == n - 1;
                 if (last) *counter = 0;
                 __threadfence();
                 misc[1] = last;
             }
             __syncthreads();
             if (misc[1] != 0) {
-                const float* first_part = P.partial + (c0 * 2 + (c0 * U / nc == seg0 ? 0 : 1)) * C::kPartFloats;
-                for (int idx = tid; idx < kRows * D / 2; idx += kThreads) {
-                    const int row = idx / (D / 2), d = idx % (D / 2) * 2;
-                    float m = -INFINITY;
-                    for (int64_t c = c0; c <= c1; ++c) {
-                        const float* part = c == c0 ? first_part : P.partial + c * 2 * C::kPartFloats;
-                        m = fmaxf(m, __ldcg(part + kRows * D + row));
+                // parts lie at c0 (its second one, if the segment does not begin with that CTA), c0 + 1, ...: their weights first
+                const int64_t off0 = (c0 * 2 + (P.aligned || c0 * U / nc >= this_seg0 ? 0 : 1)) * C::kPartFloats;
+                auto part = [&](int c) { return P.partial + (c == 0 ? off0 : (c0 + c) * 2 * C::kPartFloats); };
+                float* weight = merge;                                  // [kRows][n]
+                for (int row = warp; row < kRows; row += kWarps) {
+                    float m = -INFINITY, l = 0.f;
+                    for (int c = lane; c < n; c += 32) {
+                        const float pm = __ldcg(part(c) + kRows * D + row);
+                        weight[row * n + c] = pm;
+                        m = fmaxf(m, pm);
                     }
-                    float2 v = make_float2(0.f, 0.f);
-                    float l = 0.f;
-                    for (int64_t c = c0; c <= c1; ++c) {
-                        const float* part = c == c0 ? first_part : P.partial + c * 2 * C::kPartFloats;
-                        const float pm = __ldcg(part + kRows * D + row);
-                        const float f = pm == -INFINITY ? 0.f : ex2(pm - m);
-                        const float2 a = __ldcg(reinterpret_cast<const float2*>(part + row * D + d));
-                        v.x = fmaf(f, a.x, v.x); v.y = fmaf(f, a.y, v.y);
-                        l = fmaf(f, __ldcg(part + kRows * D + kRows + row), l);
+#pragma unroll
+                    for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
+                    for (int c = lane; c < n; c += 32) {
+                        const float pm = weight[row * n + c], f = pm == -INFINITY ? 0.f : ex2(pm - m);
+                        weight[row * n + c] = f;
+                        if (f != 0.f) l = fmaf(f, __ldcg(part(c) + kRows * D + kRows + row), l);
                     }
-                    store(row, d, v, l);
+#pragma unroll
+                    for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
+                    if (lane == 0) st_sum[row] = l;
+                }
+                __syncthreads();
+                for (int idx = tid; idx < kRows * D / 4; idx += kThreads) {
+                    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int c = 0; c < n; ++c) {
+                        const float f = weight[row * n + c];
+                        const float4 a = __ldcg(reinterpret_cast<const float4*>(part(c) + row * D + d));
+                        v.x = fmaf(f, a.x, v.x); v.y = fmaf(f, a.y, v.y); v.z = fmaf(f, a.z, v.z); v.w = fmaf(f, a.w, v.w);
+                    }
+                    store(row, d, v, st_sum[row]);
                 }
             }
         }
-        __syncthreads();                                                // the merge buffer becomes the ring again
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        u = seg0 + blk1;
+        if (!begun) return;
+        __syncthreads();                                                // merge, st_max and st_sum are free again
     }
 }
 
@@ -605,6 +695,8 @@ int launch_attn_t(const AttnParams& P, int sms, cudaStream_t stream) {
         CB_CUDA_TRY(cudaFuncSetAttribute(kv4_attention_kernel<T, D, GS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
+    // a cut segment has at most one part on each CTA: their weights share the merge buffer
+    if (sms * C::kCtasPerSm > kWarps * D) { set_error("kv4_attention: more SMs than this kernel was laid out for"); return CB_ERR_UNSUPPORTED; }
     kv4_attention_kernel<T, D, GS, NT><<<sms * C::kCtasPerSm, kThreads, C::kSmem, stream>>>(P);
     CB_CUDA_TRY(cudaGetLastError());
     return CB_OK;
@@ -638,10 +730,15 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     P.R = P.T * P.G;
     const int tile = attn_tile_rows(P.R);
     P.row_tiles = (P.R + tile - 1) / tile;
-    P.scale_log2 = scale * 1.4426950408889634f;
+    P.q_sign = scale < 0.f ? -1.f : 1.f;
+    P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
+    P.zero = 0u;
     P.counters = counters; P.partial = partial;
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
+    // Few segments: parts that end with their segment, so that each CTA goes through the chain of copy, product and join once; the parts are
+    // then up to a quarter longer.  Many: equal parts.
+    P.aligned = 4 * B * c->kv_heads * P.row_tiles <= (int64_t)sms * (tile == 8 ? 2 : 1);
     const bool bf = c->dtype == CB_BF16;
 #define CB_KV4_NT(d, gs, nt) (bf ? launch_attn_t<__nv_bfloat16, d, gs, nt>(P, sms, stream) : launch_attn_t<__half, d, gs, nt>(P, sms, stream))
 #define CB_KV4_CASE(d, gs) \

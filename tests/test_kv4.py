@@ -41,21 +41,26 @@ class Layout:
         self.block = 2 * self.half
 
     def nibble(self, which, d, tok):
+        """Number of the nibble, inside the 16 tokens' codes, of value d of token tok."""
         j, w = divmod(d, self.gs)
-        lanes = 4 if which == "k" else 8              # lanes that share a row: each holds gs / lanes values of every group
+        lanes = 4 if which == "k" else 8              # lanes that share a token: each holds gs / lanes values of every group
         lane, i = divmod(w, self.gs // lanes)
-        n = lane * (self.d // lanes) + j * (self.gs // lanes) + i
-        return n ^ 64 if which == "v" and self.d == 128 and tok & 2 else n
+        n = j * (self.gs // lanes) + i                # number of the value among the lane's
+        if which == "k":
+            return tok * self.d + lane * (self.d // 4) + n
+        second = tok % 8 > 3                          # tokens t and 7 - t (and t + 8, 15 - t) share the bytes of two
+        pair = (7 - tok % 8 if second else tok % 8) + 4 * (tok // 8)
+        lane ^= 2 * (pair % 4) if self.d == 128 else 4 * (pair // 2 % 2)
+        return pair * 2 * self.d + lane * (self.d // 4) + n // 4 * 8 + 4 * second + n % 4
 
     def put(self, page, which, off, codes, scale, lo, dtype):
         """Write one row (token `off` of the page) into page [bytes] (a CPU uint8 tensor)."""
         base = off // 16 * self.block + (self.half if which == "v" else 0)
         tok = off % 16
-        row = [0] * self.row
         for d in range(self.d):
             n = self.nibble(which, d, tok)
-            row[n // 2] |= int(codes[d]) << (4 * (n % 2))
-        page[base + tok * self.row:base + (tok + 1) * self.row] = torch.tensor(row, dtype=torch.uint8)
+            at, shift = base + n // 2, 4 * (n % 2)
+            page[at] = (int(page[at]) & ~(15 << shift) & 255) | int(codes[d]) << shift
         at = base + 16 * self.row + tok * self.meta
         pair = torch.stack((scale, lo), -1).to(dtype).contiguous().view(torch.uint8).flatten()
         page[at:at + self.meta] = pair
@@ -66,8 +71,7 @@ def test_layout_is_a_permutation_and_fills_a_block():
     for d, gs in FORMATS:
         lay = Layout(d, gs)
         for which in "kv":
-            for tok in range(16):
-                assert sorted(lay.nibble(which, i, tok) for i in range(d)) == list(range(d))
+            assert sorted(lay.nibble(which, i, tok) for i in range(d) for tok in range(16)) == list(range(16 * d))
         assert _C.kv4_block_bytes(d, gs) == lay.block and lay.block % 128 == 0
     for d, gs in ((64, 128), (96, 32), (128, 16), (0, 0), (256, 64), (128, 256)):
         assert _C.kv4_block_bytes(d, gs) == 0
