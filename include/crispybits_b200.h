@@ -287,7 +287,8 @@ int cb_decode_plan(int bits, int64_t B, int64_t V, int64_t K, int64_t split_k, i
  * weights-in-TMEM kernel) = in the tensor-core GEMM role r (1 activation producer, 2 MMA issuer,
  * 3 dequantiser, 4 epilogue, 5 packed-word producer) gave up a bounded wait; 3001 = a kernel of the 4-bit cache met a position
  * outside its page table or a page number outside the cache and left it out, 3002 = a copy of the cache's attention did not
- * arrive in time and outputs were not written.  No counterpart in the reference. */
+ * arrive in time and outputs were not written; 4000 + r = role r of the prompt attention (1 TMA, 2 MMA, 3 softmax, 4 epilogue) gave up a
+ * bounded wait.  No counterpart in the reference. */
 int cb_decode_status(int* status);
 
 /* Introspection used by the Split-K policy (packed_gemv.cu:339-347; bindings.cpp:37-39). */
@@ -345,6 +346,19 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
                      void* counters, size_t counter_bytes, void* partial, size_t partial_bytes, void* stream);
 int64_t cb_kv4_attention_counters(int64_t B, int64_t T, int64_t H, int64_t kv_heads);
 size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, int head_dim);
+
+/* Attention of whole prompts, packed: out[i] = softmax(scale * q[i] K^T) V over the keys of i's sequence, with causal != 0 over
+ * the first Lk - Lq + r + 1 of them for the sequence's query r of Lq (a prompt's keys, or a longer past and then its own).
+ * q [Tq, H, head_dim], k and v [Tk, Hkv, head_dim]: rows of contiguous values, 16-byte aligned; strides6 = {q token, q head,
+ * k token, k head, v token, v head} in elements, multiples of 8 and positive (that of a dimension of one entry is not used);
+ * out [Tq, H, head_dim] contiguous, 16-byte aligned.  Sequence s has queries cu_q[s] .. cu_q[s + 1] - 1 and keys cu_k[s] ..
+ * cu_k[s + 1] - 1 (device memory; bounds outside the tensors are cut to them).  Head h reads key head h / (H / Hkv).  head_dim 64 or 128,
+ * dtype CB_F16 or CB_BF16.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
+ * behind a query's last one are not used, except that an infinity or a NaN in v makes NaN of that value for
+ * queries up to 127 positions before it. */
+int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
+                        int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
+                        float scale, int causal, void* stream);
 
 #ifdef __cplusplus
 }

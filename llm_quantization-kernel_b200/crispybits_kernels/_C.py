@@ -794,3 +794,50 @@ def kv4_attention(q, cache, page_table, lengths, scale: float):
                                   page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), scale,
                                   counters.data_ptr(), counters.numel() * 4, partial.data_ptr(), partial.numel(), st))
     return out
+
+
+_lib.cb_prompt_attention.argtypes = [_vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _i64,
+                                     ctypes.c_float, _int, _vp]
+_lib.cb_prompt_attention.restype = _int
+
+
+def _tma_rows(t: torch.Tensor) -> torch.Tensor:
+    """As _vector_rows, and no dimension of several entries with a stride of 0 (an expanded tensor is copied)."""
+    if any(s <= 0 for s, n in zip(t.stride(), t.shape) if n > 1):
+        return t.clone(memory_format=torch.contiguous_format)
+    return _vector_rows(t)
+
+
+def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bool, out=None):
+    """q [Tq, H, D], k and v [Tk, Hkv, D] -> [Tq, H, D] (cb_prompt_attention)."""
+    who = "prompt_attention"
+    if not isinstance(q, torch.Tensor) or not q.is_cuda:
+        _fail(f"{who}: q must be a CUDA tensor (this build has no CPU path)")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        _fail(f"{who}: q must be float16 or bfloat16")
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        _fail(f"{who}: q must be [Tq, H, head_dim], k and v [Tk, Hkv, head_dim]")
+    if k.device != q.device or v.device != q.device or k.dtype != q.dtype or v.dtype != q.dtype:
+        _fail(f"{who}: q, k and v must be of one dtype, on one device")
+    (tq, h, d), (tk, hkv) = q.shape, k.shape[:2]
+    if k.shape != v.shape or k.shape[2] != d:
+        _fail(f"{who}: k and v must have the same shape, with q's head_dim")
+    if hkv == 0 or h % hkv:
+        _fail(f"{who}: q's heads must be a multiple of k's")
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        _fail(f"{who}: cu_seqlens must hold the first query of each sequence and their end")
+    _check_index(cu_seqlens, q.device, tuple(cu_seqlens.shape), "cu_seqlens", who)
+    _check_index(cu_seqlens_k, q.device, tuple(cu_seqlens.shape), "cu_seqlens_k", who)
+    if out is None:
+        out = torch.empty((tq, h, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
+        _fail(f"{who}: out must be contiguous and 16-byte aligned, of q's shape, dtype and device")
+    if out.numel() == 0 or cu_seqlens.numel() == 1:
+        return out
+    q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)
+    strides = (_i64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    with _on_device(q.device):
+        _rc(_lib.cb_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, out.data_ptr(), tq, tk, h, hkv, d,
+                                     _DTYPE[q.dtype], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), cu_seqlens.numel() - 1,
+                                     scale, 1 if causal else 0, _stream(q)))
+    return out

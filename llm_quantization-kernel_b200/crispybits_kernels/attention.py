@@ -1,7 +1,11 @@
-"""Attention next to the packed linears: a key/value cache held in 4 bits, and what writes, reads and attends to it.
+"""Attention next to the packed linears: of whole prompts, and over a key/value cache held in 4 bits.
 
-Between `fused_qkv` and the output projection a model needs attention.  With weights of 2 to 4 bits the keys and
-values of past tokens are the next largest thing that a decode step reads, so they are kept in 4 bits as well:
+Between `fused_qkv` and the output projection a model needs attention.  A prompt attends to itself:
+
+    out = prompt_attention(q, k, v, cu_seqlens)                    # packed prompts of any lengths, causal, grouped heads
+
+With weights of 2 to 4 bits the keys and values of past tokens are the next largest thing that a decode step reads, so
+they are kept in 4 bits as well:
 
     cache = KV4Cache.empty(n_pages, kv_heads, head_dim)            # one for each layer
     kv4_append(cache, k, v, page_table, starts, cu_seqlens)        # new tokens, at positions starts[s], starts[s] + 1, ...
@@ -105,3 +109,19 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
     out = _C().kv4_attention(q.unsqueeze(1) if one else q, cache, page_table, lengths,
                              cache.head_dim ** -0.5 if scale is None else float(scale))
     return out.squeeze(1) if one else out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     cu_seqlens_k: Optional[torch.Tensor] = None, scale: Optional[float] = None, causal: bool = True,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(scale * q K^T) V for packed prompts of different lengths.
+
+    q [Tq, H, head_dim], k and v [Tk, Hkv, head_dim], float16 or bfloat16, head_dim 64 or 128, H a multiple of Hkv (query head h
+    reads key head h // (H // Hkv)); any strides, rows that are not contiguous or not 16-byte aligned are copied first.
+    `cu_seqlens` int32 [B + 1]: the first query of each sequence and the end of the last; `cu_seqlens_k` the same for the keys where
+    they differ: a piece of a prompt attends to what came before it and to itself.  causal: query r of Lq sees the first
+    Lk - Lq + r + 1 keys.  A query that sees none gives 0.  Rows of no sequence are left as they are in `out` (and are
+    undefined without it).  scale: default head_dim ** -0.5.  Keys and values that a query does not see are not
+    used, except that an infinity or a NaN in v makes NaN of that value for queries up to 127 positions before it."""
+    return _C().prompt_attention(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k,
+                                 q.shape[-1] ** -0.5 if scale is None else float(scale), causal, out)

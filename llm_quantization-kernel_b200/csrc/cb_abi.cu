@@ -47,6 +47,7 @@ int gemm_status_read_and_clear(int* out);
 int gemm_ws_status_read_and_clear(int* out);
 int kv4_status_read_and_clear(int* out);
 int kv4_attn_status_read_and_clear(int* out);
+int prompt_status_read_and_clear(int* out);
 int launch_gemm_ws_gate_up(int dtype, const void* x, int64_t M, const cb_weight* gate, const cb_weight* up, void* out,
                            int64_t K, int bits, int64_t gs, cudaStream_t stream);
 int launch_gemm_ws_qkv(int dtype, const void* x, int64_t M, const cb_weight* q, const cb_weight* k, const cb_weight* v,
@@ -211,7 +212,9 @@ int cb_decode_status(int* status) {
     int d = 0, e = 0;
     if ((rc = kv4_status_read_and_clear(&d)) != CB_OK) return rc;
     if ((rc = kv4_attn_status_read_and_clear(&e)) != CB_OK) return rc;
-    *status = a != 0 ? a : (b != 0 ? 1000 + b : (c != 0 ? 2000 + c : (d != 0 ? d : e)));
+    int f = 0;
+    if ((rc = prompt_status_read_and_clear(&f)) != CB_OK) return rc;
+    *status = a != 0 ? a : (b != 0 ? 1000 + b : (c != 0 ? 2000 + c : (d != 0 ? d : (e != 0 ? e : (f != 0 ? 4000 + f : 0)))));
     return CB_OK;
 }
 int cb_tile_n(void) { return kTileN; }

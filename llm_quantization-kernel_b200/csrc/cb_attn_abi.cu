@@ -13,6 +13,10 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
 int64_t kv4_attention_segments(int64_t B, int64_t rows, int64_t kv_heads);
 size_t kv4_attention_partial_bytes(int64_t rows, int head_dim);
 
+int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
+                            int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
+                            float scale, int causal, cudaStream_t stream);
+
 namespace {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -110,6 +114,27 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
     return launch_kv4_attention(cache, q, strides3, out, B, T, H, page_table, table_stride, lengths, scale,
                                 reinterpret_cast<int*>(counters), reinterpret_cast<float*>(partial),
                                 reinterpret_cast<cudaStream_t>(stream));
+}
+
+int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
+                        int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
+                        float scale, int causal, void* stream) {
+    const char* who = "prompt_attention";
+    CB_REQUIRE(dtype == CB_F16 || dtype == CB_BF16, "%s: dtype must be fp16 or bf16", who);
+    CB_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128 (got %d)", who, head_dim);
+    CB_REQUIRE(Tq >= 0 && Tk >= 0 && Tq < (1ll << 30) && Tk < (1ll << 30), "%s: too many tokens", who);
+    CB_REQUIRE(H >= 0 && Hkv >= 0 && H < (1 << 20) && Hkv < (1 << 20) && B >= 0 && B < (1ll << 30), "%s: heads or sequences out of range", who);
+    if (Tq == 0 || H == 0 || B == 0) return CB_OK;
+    CB_REQUIRE(Hkv > 0 && H % Hkv == 0, "%s: H must be a multiple of Hkv", who);
+    CB_REQUIRE(q && out && cu_q && cu_k && strides6 && (Tk == 0 || (k && v)), "%s: NULL pointer", who);
+    CB_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "%s: q, k, v and out must be 16-byte aligned", who);
+    for (int i = 0; i < 6; ++i) {
+        const int64_t used = i == 0 ? Tq : i == 1 ? H : (i & 1) ? Hkv : Tk;
+        CB_REQUIRE(used <= 1 || (strides6[i] > 0 && strides6[i] % 8 == 0 && strides6[i] < (1ll << 38)),
+                   "%s: strides must be positive multiples of 8 elements", who);
+    }
+    return launch_prompt_attention(q, k, v, strides6, out, Tq, Tk, H, Hkv, head_dim, dtype, cu_q, cu_k, B, scale, causal,
+                                   reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

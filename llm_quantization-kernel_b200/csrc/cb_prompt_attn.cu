@@ -1,0 +1,546 @@
+// Attention of whole prompts on tcgen05: out_i = sum_{j <= i + Lk - Lq} softmax_j(scale * q_i . k_j) v_j for packed sequences of
+// different lengths, grouped heads, with or without the causal bound.
+//
+// One persistent CTA per SM takes tiles of 256 query rows of one head and sequence, as two sub-tiles of 128 rows, and walks over key
+// tiles of 128.  For each sub-tile and key tile
+//     S = Q K^T     128 x 128 x D, both operands in shared memory (K-major), fp32 in tensor memory
+//     p = exp2(c s - m), l += sum p, m a reference that follows the running maximum
+//     O += P V      128 x D x 128, P in 16 bits in tensor memory over S's columns, V as it lies in memory (N-major operand)
+// The two sub-tiles alternate: while the softmax warps of one work on its scores, the tensor cores run the other's products.
+// A thread of the softmax warps owns a row (a TMEM lane), so maxima and sums need no exchange.  The reference m is moved only
+// when the maximum has grown by more than 2^8 (then O and l are rescaled), which makes rescaling rare: p stays below 256, and its 16-bit
+// rounding is relative.  p is rounded to the inputs' type; the sum l takes the unrounded p.
+//
+// TMEM map (512 columns): S0/P0 [0, 128), S1/P1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D).
+// Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 and 11 none (they complete the
+// warpgroup that gives registers to the softmax warps, which hold a whole row of scores).
+//
+// V rows behind the last key of a sequence belong to another sequence (or to nothing): they are zeroed in shared memory, since 0 *
+// inf is not 0.  K rows there only make scores that are masked.
+//
+// What bounds it at D = 128: 4 * 128 * 128 * D operations of a sub-tile and key tile are 1024 clocks of the tensor cores, and
+// its 128 * 128 exponentials are 1024 clocks of the special-function units.
+//
+// Every wait is bounded; a wait that runs out raises a flag in shared memory and the status word, every role leaves its
+// loops, TMEM is released, and the kernel returns.
+#include <algorithm>
+
+#include "cb_common.cuh"
+
+namespace cb {
+namespace {
+
+constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kThreads = 384;
+// registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
+constexpr int kSoftRegs = 200, kOtherRegs = 104;
+constexpr long long kWaitCycles = 2000000000ll;       // about a second
+
+__device__ int g_prompt_status;
+
+struct PromptParams {
+    void* out;                                        // [Tq, H, D]
+    const int32_t* cu_q; const int32_t* cu_k;
+    int Tq, Tk, H, group, B;                          // group: query heads of a key head
+    float scale_log2;                                 // |scale| * log2(e), above 0
+    int negate;                                       // the scale is negative: the products with q are negated
+    int causal;
+};
+
+template <int D>
+struct PromptCfg {
+    static constexpr uint32_t kBox = 64 * 2 * kTileK;                       // 64 values x 128 rows
+    static constexpr uint32_t kTileBytes = kBox * (D / 64);
+    static constexpr int kSlots = D == 128 ? 4 : 8;                         // ring of K and V tiles
+    static constexpr uint32_t kQOff = 0, kRingOff = 2 * kTileBytes, kBarOff = kRingOff + kSlots * kTileBytes;
+    static constexpr uint32_t kSmem = kBarOff + 256 + 1024;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity))
+        if (*abort_flag != 0 || clock64() - t0 > kWaitCycles) return false;
+    return true;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+#define CB_R32(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7]), \
+    "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]), "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), \
+    "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]), "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), \
+    "=r"(v[o + 24]), "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]), "=r"(v[o + 31])
+#define CB_W32(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7]), \
+    "r"(v[o + 8]), "r"(v[o + 9]), "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]), "r"(v[o + 13]), "r"(v[o + 14]), "r"(v[o + 15]), \
+    "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]), "r"(v[o + 19]), "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), \
+    "r"(v[o + 24]), "r"(v[o + 25]), "r"(v[o + 26]), "r"(v[o + 27]), "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
+// 32 columns of this warp's lane quadrant, from column `addr` on, into v[O ..] / from v[O ..]
+template <int O, int N> __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[N]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : CB_R32(v, O) : "r"(addr));
+}
+template <int O, int N> __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[N]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(addr), CB_W32(v, O) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The work of a CTA, in order: every role walks through the same list by itself.  Tiles are ordered by their place in their
+// sequence, the last ones (with the causal bound: the longest) first, heads innermost; CTA i takes item i of the first
+// gridDim.x, then in turn the mirrored and the same place of the following ones.
+struct Work {
+    int head, row0, lq, lk, q_first, k_first;         // row0: the tile's first query row in its sequence
+    int n[2];                                         // key tiles of the sub-tiles
+};
+struct Walk {
+    const PromptParams& P;
+    int lane, level, round = 0, my_tiles = 0;
+    int64_t above = 0;                                // tiles of higher levels
+    __device__ __forceinline__ int lens(int b, int& first) const {
+        const int s = min(max(P.cu_q[b], 0), P.Tq), e = min(max(P.cu_q[b + 1], s), P.Tq);
+        first = s;
+        return e - s;
+    }
+    __device__ __forceinline__ int tiles_of(int b) const {
+        int first;
+        return b < P.B ? (int)(((int64_t)lens(b, first) + kTileQ - 1) / kTileQ) : 0;
+    }
+    __device__ Walk(const PromptParams& p, int l) : P(p), lane(l) {
+        int top = 0;
+        my_tiles = tiles_of(lane);                    // of sequence `lane`: all there are with up to 32 sequences
+        for (int b0 = 0; b0 < P.B; b0 += 32) top = max(top, tiles_of(b0 + lane));
+        level = __reduce_max_sync(0xffffffffu, top) - 1;
+    }
+    __device__ bool next(Work& w) {
+        const int64_t place = (round & 1) ? (int64_t)(gridDim.x - 1 - blockIdx.x) : (int64_t)blockIdx.x;
+        const int64_t item = (int64_t)round * gridDim.x + place;
+        ++round;
+        const int64_t rank = item / P.H;
+        w.head = (int)(item - rank * P.H);
+        for (; level >= 0; --level) {
+            int64_t seen = above;
+            for (int b0 = 0; b0 < P.B; b0 += 32) {
+                const int nt = P.B <= 32 ? my_tiles : tiles_of(b0 + lane);
+                const unsigned has = __ballot_sync(0xffffffffu, nt > level);
+                const int cnt = __popc(has);
+                if (rank < seen + cnt) {
+                    const int want = (int)(rank - seen);
+                    const bool me = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == want;
+                    const int b = b0 + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+                    w.lq = lens(b, w.q_first);
+                    const int s = min(max(P.cu_k[b], 0), P.Tk), e = min(max(P.cu_k[b + 1], s), P.Tk);
+                    w.k_first = s;
+                    w.lk = e - s;
+                    w.row0 = level * kTileQ;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int r0 = w.row0 + x * kSub, rows = min(w.lq - r0, kSub);
+                        int64_t keys = w.lk;
+                        if (P.causal) keys = min(keys, (int64_t)r0 + rows + (w.lk - w.lq));
+                        w.n[x] = rows <= 0 || keys <= 0 ? 0 : (int)((keys + kTileK - 1) / kTileK);
+                    }
+                    return true;
+                }
+                seen += cnt;
+            }
+            above = seen;
+        }
+        return false;
+    }
+};
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                        const __grid_constant__ CUtensorMap vmap, const PromptParams P) {
+    using C = PromptCfg<D>;
+    constexpr int kSlots = C::kSlots;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    unsigned char* smem = smem_raw + (base - raw);
+    const uint32_t bars = base + C::kBarOff;
+    auto q_full = [&](int x) { return bars + 8u * x; };
+    const uint32_t q_empty = bars + 16u;
+    auto s_full = [&](int x) { return bars + 24u + 8u * x; };
+    auto p_ready = [&](int x) { return bars + 40u + 8u * x; };
+    auto pv_done = [&](int x) { return bars + 56u + 8u * x; };
+    auto o_free = [&](int x) { return bars + 72u + 8u * x; };
+    auto kv_full = [&](int s) { return bars + 88u + 8u * s; };
+    auto kv_empty = [&](int s) { return bars + 88u + 8u * (kSlots + s); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 224);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 228);
+    static_assert(88 + 16 * kSlots <= 224, "barriers");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(q_full(x), 1); mbar_init(s_full(x), 1); mbar_init(p_ready(x), 4); mbar_init(pv_done(x), 1); mbar_init(o_free(x), 4);
+        }
+        mbar_init(q_empty, 1);
+        for (int s = 0; s < kSlots; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32((const void*)tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    int gave_up = 0;
+
+    Work w;
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    Walk walk(P, lane);
+    if (warp == kTmaWarp) {
+        // ================= TMA: Q once a tile, K and V tiles through the ring =================
+        uint32_t it = 0, tiles = 0;
+        while (!gave_up && walk.next(w)) {
+            const int n = max(w.n[0], w.n[1]);
+            if (n == 0) continue;
+            if (tiles > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (tiles - 1) & 1, abort_flag))) { gave_up = 1; break; }
+            ++tiles;
+            const int kv_head = w.head / P.group;
+            if (lane == 0)
+                for (int x = 0; x < 2; ++x) {
+                    mbar_expect_tx(q_full(x), C::kTileBytes);
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_load_3d(base + C::kQOff + x * C::kTileBytes + h * C::kBox, &qmap, h * 64, w.head, w.q_first + w.row0 + x * kSub, q_full(x));
+                }
+            for (int j = 0; j < 2 * n; ++j, ++it) {               // K tile, V tile, K tile, ...
+                const int s = it % kSlots;
+                if (it >= kSlots && !__all_sync(0xffffffffu, mbar_wait(kv_empty(s), (it / kSlots - 1) & 1, abort_flag))) { gave_up = 1; break; }
+                if (lane == 0) {
+                    mbar_expect_tx(kv_full(s), C::kTileBytes);
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_load_3d(base + C::kRingOff + s * C::kTileBytes + h * C::kBox, (j & 1) ? &vmap : &kmap, h * 64, kv_head,
+                                    w.k_first + (j >> 1) * kTileK, kv_full(s));
+                }
+            }
+        }
+        if (gave_up) {                                            // own copies in flight, again with a limit
+            const long long t0 = clock64();
+            for (uint32_t i = it > kSlots ? it - kSlots : 0; i < it; ++i)
+                while (!mbar_try_wait(kv_full(i % kSlots), (i / kSlots) & 1) && clock64() - t0 < kWaitCycles) {}
+            for (int x = 0; x < 2 && tiles > 0; ++x)
+                while (!mbar_try_wait(q_full(x), (tiles - 1) & 1) && clock64() - t0 < kWaitCycles) {}
+        }
+    } else if (warp == kMmaWarp) {
+        // ================= MMA issuer =================
+        constexpr uint32_t fmt = BF ? ((1u << 7) | (1u << 10)) : 0u;
+        const uint32_t idesc_s = (1u << 4) | fmt | ((uint32_t)P.negate << 13) | ((uint32_t)(kTileK >> 3) << 17) | ((uint32_t)(kSub >> 4) << 24);
+        constexpr uint32_t idesc_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kSub >> 4) << 24);
+        const uint64_t dk = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);                            // K-major, 128-byte swizzle, 8-row atoms 1024 bytes apart
+        const uint64_t dv = ((uint64_t)(C::kBox >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);        // N-major: 64-value boxes kBox apart, 8-key groups 1024 bytes apart
+        uint32_t it = 0, tiles = 0, pcount[2] = {0, 0}, ocount[2] = {0, 0};
+        // the ring place of K tile j of the present query tile is it + 2 j, of V tile j it + 2 j + 1
+        auto wait_kv = [&](uint32_t place) { return __all_sync(0xffffffffu, mbar_wait(kv_full(place % kSlots), (place / kSlots) & 1, abort_flag)); };
+        auto scores = [&](int x, int j, bool release) {
+            const uint32_t place = it + 2 * j;
+            if (!wait_kv(place)) { gave_up = 2; return; }
+            fence_after();
+            if (lane == 0) {
+                const uint32_t qa = base + C::kQOff + x * C::kTileBytes, ka = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k / 4) * C::kBox + (k % 4) * 32;
+                    const uint64_t ad = dk | (uint64_t)(((qa + off) >> 4) & 0x3FFF), bd = dk | (uint64_t)(((ka + off) >> 4) & 0x3FFF);
+                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
+                                 ::"r"(tmem + x * 128), "l"(ad), "l"(bd), "r"(idesc_s), "r"(k > 0 ? 1u : 0u), "r"(0u) : "memory");
+                }
+                commit(s_full(x));
+                if (release) commit(kv_empty(place % kSlots));
+            }
+            __syncwarp();
+        };
+        auto values = [&](int x, int j, bool release) {
+            const uint32_t place = it + 2 * j + 1;
+            if (!wait_kv(place)) { gave_up = 2; return; }
+            if (!__all_sync(0xffffffffu, mbar_wait(p_ready(x), pcount[x] & 1, abort_flag))) { gave_up = 2; return; }
+            ++pcount[x];
+            fence_after();
+            if (lane == 0) {
+                const uint32_t va = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+#pragma unroll
+                for (int k = 0; k < kTileK / 16; ++k) {
+                    const uint64_t bd = dv | (uint64_t)(((va + k * 2048) >> 4) & 0x3FFF);
+                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
+                                 ::"r"(tmem + 256 + x * 128), "r"(tmem + x * 128 + k * 8), "l"(bd), "r"(idesc_o), "r"(j > 0 || k > 0 ? 1u : 0u), "r"(0u) : "memory");
+                }
+                commit(pv_done(x));
+                if (release) commit(kv_empty(place % kSlots));
+            }
+            __syncwarp();
+        };
+        while (!gave_up && walk.next(w)) {
+            const int n = max(w.n[0], w.n[1]);
+            if (n == 0) continue;
+            for (int x = 0; x < 2; ++x)                           // both halves of Q are always loaded
+                if (!__all_sync(0xffffffffu, mbar_wait(q_full(x), tiles & 1, abort_flag))) gave_up = 2;
+            ++tiles;
+            for (int x = 0; x < 2 && !gave_up; ++x)
+                if (w.n[x] > 0) scores(x, 0, x == 1 || w.n[1] == 0);
+            for (int j = 0; j < n && !gave_up; ++j) {
+                const int valid = w.lk - j * kTileK;
+                if (valid < kTileK) {
+                    // rows behind the sequence's last key: zeros, before any product reads them
+                    const uint32_t place = it + 2 * j + 1;
+                    if (!wait_kv(place)) { gave_up = 2; break; }
+                    unsigned char* v = smem + C::kRingOff + (place % kSlots) * C::kTileBytes;
+                    for (int i = lane; i < (kTileK - valid) * 8; i += 32)
+                        for (int h = 0; h < D / 64; ++h) *reinterpret_cast<uint4*>(v + h * C::kBox + valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                for (int x = 0; x < 2 && !gave_up; ++x) {
+                    if (j < w.n[x]) {
+                        if (j == 0) {                             // the previous tile's O must have been read
+                            if (ocount[x] > 0 && !__all_sync(0xffffffffu, mbar_wait(o_free(x), (ocount[x] - 1) & 1, abort_flag))) { gave_up = 2; break; }
+                            ++ocount[x];
+                        }
+                        values(x, j, x == 1 || j >= w.n[1]);
+                    }
+                    if (!gave_up && j + 1 < w.n[x]) scores(x, j + 1, x == 1 || j + 1 >= w.n[1]);
+                }
+            }
+            it += 2 * n;
+            if (lane == 0 && !gave_up) commit(q_empty);
+            __syncwarp();
+        }
+    }
+    } else {
+        // ================= softmax and epilogue: a thread owns a row =================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
+        Walk walk(P, lane);
+        const int x = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), s_addr = lane_base + x * 128, o_addr = lane_base + 256 + x * 128;
+        uint32_t count = 0;                                       // score tiles of this sub-tile so far
+        while (!gave_up && walk.next(w)) {
+            const int n = w.n[x], r = w.row0 + x * kSub + row;    // query row in its sequence
+            const bool live = r < w.lq;
+            T* dst = reinterpret_cast<T*>(P.out) + ((int64_t)(w.q_first + r) * P.H + w.head) * D;
+            if (n == 0) {                                         // rows that see no key
+                if (live)
+                    for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0u, 0u, 0u, 0u);
+                continue;
+            }
+            const int limit = P.causal ? (int)min((int64_t)w.lk, max((int64_t)0, (int64_t)r + 1 + w.lk - w.lq)) : w.lk;      // keys this row sees
+            float m_ref = -INFINITY, l = 0.f;
+            for (int j = 0; j < n; ++j, ++count) {
+                if (!__all_sync(0xffffffffu, mbar_wait(s_full(x), count & 1, abort_flag))) { gave_up = 3; break; }
+                fence_after();
+                uint32_t s[128];
+                tmem_ld32<0>(s_addr, s); tmem_ld32<32>(s_addr + 32, s); tmem_ld32<64>(s_addr + 64, s); tmem_ld32<96>(s_addr + 96, s);
+                tmem_ld_wait();
+                const int seen = limit - j * kTileK;
+                if (__any_sync(0xffffffffu, seen < kTileK)) {
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (i >= seen) s[i] = 0xff800000u;
+                }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; i += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], fmaxf(__uint_as_float(s[i + c]), __uint_as_float(s[i + 4 + c])));
+                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * P.scale_log2;
+                const bool move = m > m_ref + 8.f;
+                if (__any_sync(0xffffffffu, move)) {
+                    const float a = move ? ex2(m_ref - m) : 1.f;
+                    if (move) m_ref = m;
+                    l *= a;
+                    if (j > 0) {
+                        if (!__all_sync(0xffffffffu, mbar_wait(pv_done(x), (count - 1) & 1, abort_flag))) { gave_up = 3; break; }
+                        fence_after();
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t v[32];
+                            tmem_ld32<0>(o_addr + c, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
+                            tmem_st32<0>(o_addr + c, v);
+                        }
+                        tmem_st_wait();
+                    }
+                }
+                const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+                float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 128; i += 4) {
+                    float p[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) { p[c] = ex2(fmaf(__uint_as_float(s[i + c]), P.scale_log2, neg)); l4[c] += p[c]; }
+                    s[i / 2] = pack2<T>(p[0], p[1]);
+                    s[i / 2 + 1] = pack2<T>(p[2], p[3]);
+                }
+                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                tmem_st32<0>(s_addr, s); tmem_st32<32>(s_addr + 32, s);
+                tmem_st_wait();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready(x));
+            }
+            if (gave_up) break;
+            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(x), (count - 1) & 1, abort_flag))) { gave_up = 4; break; }
+            fence_after();
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                uint32_t v[32];
+                tmem_ld32<0>(o_addr + c, v);
+                tmem_ld_wait();
+                if (c + 32 == D) {
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(o_free(x));
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint32_t y[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            y[k] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[i + 2 * k]) * inv, __uint_as_float(v[i + 2 * k + 1]) * inv);
+                        *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+            }
+        }
+    }
+    if (gave_up) {
+        *abort_flag = 1;
+        atomicExch(&g_prompt_status, gave_up);
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    if (fn == nullptr) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+    }
+    return fn;
+}
+
+template <typename T, int D>
+int launch_prompt_t(const CUtensorMap (&maps)[3], const PromptParams& P, int grid, cudaStream_t stream) {
+    using C = PromptCfg<D>;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    CB_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+        CB_CUDA_TRY(cudaFuncSetAttribute(prompt_attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
+        if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    }
+    prompt_attention_kernel<T, D><<<grid, kThreads, C::kSmem, stream>>>(maps[0], maps[1], maps[2], P);
+    CB_CUDA_TRY(cudaGetLastError());
+    return CB_OK;
+}
+
+}  // namespace
+
+// Arguments are checked by the caller.  strides: {q token, q head, k token, k head, v token, v head} in elements.
+int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
+                            int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
+                            float scale, int causal, cudaStream_t stream) {
+    const int sms = sm_count_current();
+    if (sms <= 0) return CB_ERR_CUDA;
+    EncodeTiledFn enc = encode_fn();
+    if (enc == nullptr) { set_error("prompt_attention: cuTensorMapEncodeTiled is not available"); return CB_ERR_CUDA; }
+    CUtensorMap maps[3];
+    for (int i = 0; i < 3; ++i) {
+        const bool none = i > 0 && Tk == 0;                       // no keys at all: a map that nothing is read through
+        const void* p = i == 0 || none ? q : i == 1 ? k : v;
+        const int64_t heads = i == 0 ? H : Hkv, rows = i == 0 ? Tq : none ? 1 : Tk;
+        const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)rows};
+        // the stride of a dimension of one entry is never used, but has to be a good one
+        const cuuint64_t bytes[2] = {heads == 1 || none ? (cuuint64_t)head_dim * 2 : (cuuint64_t)strides[2 * i + 1] * 2,
+                                     rows == 1 ? (cuuint64_t)head_dim * heads * 2 : (cuuint64_t)strides[2 * i] * 2};
+        const cuuint32_t box[3] = {64, 1, 128}, step[3] = {1, 1, 1};
+        const CUresult cr = enc(&maps[i], dtype == CB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                                const_cast<void*>(p), dims, bytes, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (cr != CUDA_SUCCESS) { set_error("prompt_attention: cuTensorMapEncodeTiled(%c) failed (%d)", "qkv"[i], (int)cr); return CB_ERR_CUDA; }
+    }
+    PromptParams P{};
+    P.out = out; P.cu_q = cu_q; P.cu_k = cu_k;
+    P.Tq = (int)Tq; P.Tk = (int)Tk; P.H = (int)H; P.group = (int)(H / Hkv); P.B = (int)B;
+    P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
+    P.negate = scale < 0.f ? 1 : 0;
+    P.causal = causal ? 1 : 0;
+    const int64_t most = (Tq / kTileQ + B) * H;                   // tiles there can be
+    const int grid = (int)std::min<int64_t>(sms, most);
+    const bool bf = dtype == CB_BF16;
+    if (head_dim == 128) return bf ? launch_prompt_t<__nv_bfloat16, 128>(maps, P, grid, stream) : launch_prompt_t<__half, 128>(maps, P, grid, stream);
+    return bf ? launch_prompt_t<__nv_bfloat16, 64>(maps, P, grid, stream) : launch_prompt_t<__half, 64>(maps, P, grid, stream);
+}
+
+int prompt_status_read_and_clear(int* out) {
+    int v = 0, zero = 0;
+    CB_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_prompt_status, sizeof(int)));
+    CB_CUDA_TRY(cudaMemcpyToSymbol(g_prompt_status, &zero, sizeof(int)));
+    *out = v;
+    return CB_OK;
+}
+
+}  // namespace cb

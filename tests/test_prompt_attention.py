@@ -1,0 +1,241 @@
+"""Attention of packed prompts against softmax(scale * q K^T) V in 64 bits."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+DEV = "cuda"
+
+
+# ------------------------------------------------------------------------------------------------ refusals, no GPU needed
+def test_c_entry_point_refuses_bad_arguments():
+    from crispybits_kernels import _C
+    lib, s6 = _C._lib, (ctypes.c_int64 * 6)(*[128] * 6)
+
+    def call(q=256, k=256, v=256, st=s6, out=256, tq=4, tk=4, h=2, hkv=2, d=64, dt=1, cq=256, ck=256, b=1):
+        return lib.cb_prompt_attention(q, k, v, st, out, tq, tk, h, hkv, d, dt, cq, ck, b, 1.0, 1, 0)
+
+    for bad in (dict(dt=0), dict(dt=3), dict(d=96), dict(d=256), dict(tq=-1), dict(tk=-1), dict(tq=1 << 30), dict(h=3), dict(hkv=0), dict(b=-1),
+                dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(cq=0), dict(ck=0), dict(st=None), dict(q=8), dict(k=8), dict(v=8),
+                dict(out=8), dict(st=(ctypes.c_int64 * 6)(128, 128, 128, 4, 128, 128)), dict(st=(ctypes.c_int64 * 6)(0, *[128] * 5)),
+                dict(st=(ctypes.c_int64 * 6)(128, 128, -128, 128, 128, 128))):
+        assert call(**bad) == 1 and lib.cb_last_error(), bad
+    assert call(tq=0) == 0 and call(b=0) == 0 and call(h=0) == 0
+
+
+def test_python_entry_point_refuses_cpu_tensors():
+    import crispybits_kernels as ck
+    x = torch.zeros(2, 2, 64).half()
+    with pytest.raises(RuntimeError):
+        ck.prompt_attention(x, x, x, torch.tensor([0, 2], dtype=torch.int32))
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device=DEV)
+
+
+def offsets(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def rand(n, heads, d, dtype, seed, gain=1.0):
+    return (torch.randn(n, heads, d, generator=torch.Generator().manual_seed(seed)) * gain).to(dtype).to(DEV)
+
+
+def reference(q, k, v, cu_q, cu_k, scale=None, causal=True):
+    """(out, tolerance) in 64 bits.
+
+    Tolerance: the output's rounding, eps / 2 of it; the weights' rounding to the inputs' type, eps / 2 of each, so eps / 2 of
+    sum w |v|; the scores' fp32 sums (2^-20 of sum |q| |k| is ample for 128 products) and the exponential (2^-21), which move
+    each weight and their sum."""
+    D, share = q.shape[2], q.shape[1] // k.shape[1]
+    scale = D ** -0.5 if scale is None else scale
+    out, tol = torch.zeros(q.shape, dtype=torch.double, device=DEV), torch.zeros(q.shape, dtype=torch.double, device=DEV)
+    half = torch.finfo(q.dtype).eps / 2
+    for b in range(len(cu_q) - 1):
+        (q0, q1), (k0, k1) = cu_q[b:b + 2], cu_k[b:b + 2]
+        if q1 <= q0 or k1 <= k0:
+            continue
+        qq = q[q0:q1].double().transpose(0, 1)
+        kk, vv = (x[k0:k1].double().transpose(0, 1).repeat_interleave(share, 0) for x in (k, v))
+        s = qq @ kk.transpose(1, 2) * scale
+        err = 2.0 ** -20 * (qq.abs() @ kk.abs().transpose(1, 2)) * abs(scale)
+        if causal:
+            hidden = torch.arange(k1 - k0, device=DEV)[None] > torch.arange(q1 - q0, device=DEV)[:, None] + (k1 - k0) - (q1 - q0)
+            s, err = s.masked_fill(hidden, -math.inf), err.masked_fill(hidden, 0)
+        w = torch.softmax(s, -1).nan_to_num(0.0)
+        o, size = w @ vv, w @ vv.abs()
+        e = err.amax(-1, keepdim=True) + 2.0 ** -21
+        out[q0:q1] = o.transpose(0, 1)
+        tol[q0:q1] = (half * o.abs() * 1.01 + (half * 1.01 + 2 * e) * size + 1e-7).transpose(0, 1)
+    return out, tol
+
+
+def check(got, want):
+    out, tol = want
+    over = (got.double() - out).abs() - tol
+    assert torch.isfinite(got).all() and (over <= 0).all(), f"{over.max():.2e} over, at tolerance {tol[over == over.max()][0]:.2e}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 127, 128, 129, 255, 256, 257, 300, 1000])
+def test_one_prompt(dtype, d, n):
+    import crispybits_kernels as ck
+    q, k, v = rand(n, 4, d, dtype, 1), rand(n, 2, d, dtype, 2), rand(n, 2, d, dtype, 3)
+    check(ck.prompt_attention(q, k, v, i32([0, n])), reference(q, k, v, [0, n], [0, n]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,heads,kv", [(128, 6, 2), (64, 5, 5), (64, 8, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_prompts_with_and_without_a_past(dtype, d, heads, kv, causal):
+    """Lengths from none to several tiles; keys more, as many, and fewer than queries (rows that see none), and none at all."""
+    import crispybits_kernels as ck
+    lens = [5, 0, 1, 300, 128, 513, 40, 7, 130]
+    keys = [5, 9, 700, 300, 385, 520, 33, 0, 2]
+    cq, ckv = offsets(lens), offsets(keys)
+    q, k, v = rand(cq[-1], heads, d, dtype, 1), rand(ckv[-1], kv, d, dtype, 2), rand(ckv[-1], kv, d, dtype, 3)
+    got = ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal)
+    check(got, reference(q, k, v, cq, ckv, causal=causal))
+    assert (got[cq[7]:cq[8]] == 0).all()                       # no keys
+    if causal:
+        assert (got[cq[6]:cq[6] + 7] == 0).all() and (got[cq[8]:cq[8] + 128] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [31, 32, 33, 200])
+def test_many_prompts(B):
+    """More sequences than a warp looks at together, more tiles than SMs."""
+    import crispybits_kernels as ck
+    lens = [(37 * b) % 90 + (500 if b % 17 == 3 else 0) for b in range(B)]
+    cu = offsets(lens)
+    q, k, v = rand(cu[-1], 2, 64, torch.float16, 1), rand(cu[-1], 1, 64, torch.float16, 2), rand(cu[-1], 1, 64, torch.float16, 3)
+    check(ck.prompt_attention(q, k, v, i32(cu)), reference(q, k, v, cu, cu))
+
+
+@pytest.mark.gpu
+def test_a_long_prompt_and_rising_scores():
+    """Keys that grow along the sequence, so that the running maximum moves at almost every tile."""
+    import crispybits_kernels as ck
+    n = 3000
+    for dtype in (torch.float16, torch.bfloat16):
+        q, k, v = rand(n, 2, 128, dtype, 1, 2.0), rand(n, 2, 128, dtype, 2), rand(n, 2, 128, dtype, 3)
+        k = (k.float() * torch.linspace(0.02, 3.0, n, device=DEV)[:, None, None]).to(dtype)
+        check(ck.prompt_attention(q, k, v, i32([0, n])), reference(q, k, v, [0, n], [0, n]))
+        k = k.flip(0).contiguous()
+        check(ck.prompt_attention(q, k, v, i32([0, n])), reference(q, k, v, [0, n], [0, n]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.25, -0.1, 0.0])
+def test_scale(scale):
+    import crispybits_kernels as ck
+    q, k, v = rand(200, 2, 64, torch.bfloat16, 1), rand(200, 2, 64, torch.bfloat16, 2), rand(200, 2, 64, torch.bfloat16, 3)
+    check(ck.prompt_attention(q, k, v, i32([0, 200]), scale=scale), reference(q, k, v, [0, 200], [0, 200], scale))
+
+
+@pytest.mark.gpu
+def test_strides_and_alignment():
+    import crispybits_kernels as ck
+    n, d = 150, 64
+    fused = rand(n, 8, d, torch.float16, 1).flatten(1)          # [q: 4 heads | k: 2 | v: 2]
+    q, k, v = fused[:, :4 * d].view(n, 4, d), fused[:, 4 * d:6 * d].view(n, 2, d), fused[:, 6 * d:].view(n, 2, d)
+    cu = i32([0, n])
+    want = ck.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu)
+    check(want, reference(q, k, v, [0, n], [0, n]))
+    assert torch.equal(want, ck.prompt_attention(q, k, v, cu))
+    heads_first = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    assert torch.equal(want, ck.prompt_attention(*heads_first, cu))
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape).copy_(q)
+    assert torch.equal(want, ck.prompt_attention(odd, k, v, cu))
+    one = k[:, :1].expand(n, 2, d)                              # a head shared by expanding it
+    assert torch.equal(ck.prompt_attention(q, one, one, cu), ck.prompt_attention(q, k[:, :1], k[:, :1], cu))
+    assert torch.equal(ck.prompt_attention(q[:1], k[:1], v[:1], i32([0, 1])), v[:1].repeat_interleave(2, 1))
+
+
+@pytest.mark.gpu
+def test_rows_of_no_sequence_and_values_of_others():
+    """Rows before the first and behind the last sequence stay; infinities and NaN of other rows do not reach a sequence."""
+    import crispybits_kernels as ck
+    n, d = 700, 128
+    q, k, v = rand(n, 2, d, torch.bfloat16, 1), rand(n, 1, d, torch.bfloat16, 2), rand(n, 1, d, torch.bfloat16, 3)
+    cu = [100, 233, 233, 600]
+    want = reference(q, k, v, cu, cu)
+    for x in (q, k, v):
+        x[:100] = math.nan
+        x[600:650] = math.inf
+        x[650:] = math.nan
+    out = torch.full((n, 2, d), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = ck.prompt_attention(q, k, v, i32(cu), out=out)
+    assert got is out and (out[:100] == 7).all() and (out[600:] == 7).all()
+    check(out[100:600], tuple(t[100:600] for t in want))
+    # keys of their own bounds, with NaN directly behind them
+    k[333:], v[333:] = math.nan, math.nan
+    got = ck.prompt_attention(q[100:300], k, v, i32([0, 200]), i32([150, 333]), causal=False)
+    check(got, reference(q[100:300], k, v, [0, 200], [150, 333], causal=False))
+    # bounds outside the tensors are cut to them
+    got = ck.prompt_attention(q[100:300], k[:333], v[:333], i32([-5, 10000]), i32([100, 1 << 30]), causal=False)
+    check(got, reference(q[100:300], k, v, [0, 200], [100, 333], causal=False))
+
+
+@pytest.mark.gpu
+def test_nan_in_a_sequence_reaches_only_that_sequence():
+    import crispybits_kernels as ck
+    cu = [0, 70, 140, 210]
+    q, k, v = (rand(210, 1, 64, torch.float16, s) for s in (1, 2, 3))
+    want = ck.prompt_attention(q, k, v, i32(cu))
+    k[100] = math.nan
+    got = ck.prompt_attention(q, k, v, i32(cu))
+    assert torch.equal(got[:100], want[:100]) and torch.equal(got[140:], want[140:]) and got[100:140].isnan().all()
+
+
+@pytest.mark.gpu
+def test_the_same_every_time_on_any_stream_and_captured():
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    cu = offsets([900, 30, 1400, 128])
+    q, k, v = rand(cu[-1], 8, 128, torch.bfloat16, 1), rand(cu[-1], 2, 128, torch.bfloat16, 2), rand(cu[-1], 2, 128, torch.bfloat16, 3)
+    c = i32(cu)
+    want = ck.prompt_attention(q, k, v, c)
+    check(want, reference(q, k, v, cu, cu))
+    torch.cuda.synchronize()
+    outs = []
+    for s in [torch.cuda.Stream() for _ in range(3)] * 3:
+        with torch.cuda.stream(s):
+            outs.append(ck.prompt_attention(q, k, v, c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(want, o) for o in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ck.prompt_attention(q, k, v, c)
+    for cu2 in ([0, 1, 2, 3, cu[-1]], cu):                       # a replay reads what the bounds hold then
+        c.copy_(i32(cu2))
+        g.replay()
+        check(out, reference(q, k, v, cu2, cu2))
+    assert torch.equal(out, want) and _C.decode_status() == 0
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    import crispybits_kernels as ck
+    q, k = rand(10, 4, 64, torch.float16, 1), rand(10, 2, 64, torch.float16, 2)
+    cu = i32([0, 10])
+    for args in ((q.float(), k.float(), k.float(), cu), (q, k.bfloat16(), k, cu), (q, k, k[:, :1], cu), (q[:, :3], k, k, cu), (q, k.cpu(), k, cu),
+                 (q[..., :32], k[..., :32], k[..., :32], cu), (q[0], k, k, cu), (q, k, k, cu.long()), (q, k, k, cu.cpu()), (q, k, k, cu[None]),
+                 (q, k, k, cu, i32([0, 5, 10]))):
+        with pytest.raises(RuntimeError):
+            ck.prompt_attention(*args)
+    for out in (torch.empty(10, 4, 64, device=DEV), torch.empty(10, 4, 128, device=DEV, dtype=q.dtype)[..., :64], torch.empty(9, 4, 64, device=DEV, dtype=q.dtype)):
+        with pytest.raises(RuntimeError):
+            ck.prompt_attention(q, k, k, cu, out=out)
+    assert ck.prompt_attention(q[:0], k, k, i32([0, 0])).shape == (0, 4, 64)
+    none = ck.prompt_attention(q, k[:0], k[:0], cu, i32([0, 0]))
+    assert (none == 0).all()
