@@ -33,7 +33,7 @@ int check_cache(const char* who, const cb_kv4_cache* c) {
                "%s: head_dim must be 64 or 128 and group_size 32, 64 or 128, at most head_dim (got %d, %d)", who, c->head_dim, c->group_size);
     CB_REQUIRE(c->page_size >= kKvBlock && c->page_size % kKvBlock == 0 && c->page_size <= (1 << 20),
                "%s: page_size must be a multiple of 16", who);
-    CB_REQUIRE(c->kv_heads > 0 && c->kv_heads < (1 << 20), "%s: kv_heads out of range", who);
+    CB_REQUIRE(c->kv_heads > 0 && c->kv_heads < (1 << 16), "%s: kv_heads out of range", who);
     CB_REQUIRE(c->n_pages >= 0 && c->n_pages < (1ll << 31), "%s: n_pages out of range", who);
     CB_REQUIRE(c->pages != nullptr && aligned16(c->pages), "%s: pages must be a 16-byte aligned pointer", who);
     return CB_OK;

@@ -5,10 +5,11 @@
 // over the GS values x of a group, T the cache's 16-bit type.  A group with an infinity or a NaN keeps NaN for both and
 // reads back as NaN; a scale below the smallest normal float is kept as 0, and the group reads back as lo.
 //
-// Both kernels are bound by memory: 2 bytes of a value on one side, 0.5 + 4 / GS on the other.  A thread owns 8
-// consecutive values of one row (token, head, K or V): one 16-byte access on the 16-bit side, one 4-byte word of codes on
-// the other.  A CTA takes 16 tokens and a few heads, the tokens along its threads, so that what it writes is contiguous
-// on both sides; it looks its 16 tokens' pages up once.
+// Both kernels are bound by memory: 2 bytes of a value on one side, 0.5 + 4 / GS on the other.  A CTA takes one block (16
+// positions) of one sequence and a few heads, so that it looks up one page and owns every byte of the heads' blocks that
+// tokens of this call fill; it turns them over in shared memory and moves whole blocks in 16-byte pieces.  A
+// block that the call fills in part (a decode step's token, the ends of a prompt) is written value by value.  A thread
+// owns 8 consecutive values of a row (token, head, K or V).
 #include <algorithm>
 
 #include "cb_kv4.cuh"
@@ -16,8 +17,8 @@
 namespace cb {
 namespace {
 
-constexpr int kTok = 16;              // tokens of a CTA
 constexpr int kThreads = 256;
+constexpr int kMaxHeads = 8;          // heads of a CTA, at most
 __device__ int g_kv4_status;
 
 struct RowParams {
@@ -31,30 +32,50 @@ struct RowParams {
     int heads_per_cta;
 };
 
-// Page and position inside it of packed token `tok`; page -1: no such place.
-__device__ __forceinline__ void find_slot(const RowParams& P, int64_t tok, int& page, int& off) {
-    page = -1; off = 0;
-    if (tok >= P.n_tokens) return;
-    int64_t b, first;
+// n tokens from position p on lie in at most (n + 30) / 16 blocks.  Items are numbered with gaps, so that an item's sequence can be
+// found without adding up the sequences' blocks: those of sequence b begin at cu[b] / 16 + 2 b (b * ((per_seq + 30) / 16)).
+__host__ __device__ inline int64_t items_of(int64_t n_tokens, int64_t n_seqs, int64_t per_seq, bool packed) {
+    return packed ? n_tokens / kKvBlock + 2 * n_seqs : n_seqs * ((per_seq + 30) / kKvBlock);
+}
+
+// What an item is: tokens [t0, t1) of the 16 positions of a block have their rows at packed token `token0` + position in the block.
+struct Item {
+    int64_t token0;
+    int t0, t1, page, block;          // page < 0: nothing to do;  block inside its page
+};
+__device__ __forceinline__ Item find_item(const RowParams& P, int64_t idx) {
+    Item it;
+    it.page = -1; it.t0 = it.t1 = 0; it.token0 = 0; it.block = 0;
+    int64_t b, k, first, n;
     if (P.cu != nullptr) {
-        int64_t lo = 0, hi = P.n_seqs;            // the last sequence that begins at or before tok
+        int64_t lo = 0, hi = P.n_seqs;            // the last sequence whose items begin at or before idx
         while (hi - lo > 1) {
             const int64_t mid = (lo + hi) >> 1;
-            if (P.cu[mid] <= tok) lo = mid; else hi = mid;
+            if (max((int64_t)P.cu[mid], (int64_t)0) / kKvBlock + 2 * mid <= idx) lo = mid; else hi = mid;
         }
         b = lo;
         first = P.cu[b];
-        if (tok < first || tok >= P.cu[b + 1]) return;
+        n = P.cu[b + 1] - first;
+        k = idx - (max(first, (int64_t)0) / kKvBlock + 2 * b);
     } else {
-        b = tok / P.per_seq;
+        const int64_t per = (P.per_seq + 30) / kKvBlock;
+        b = idx / per;
+        k = idx - b * per;
         first = b * P.per_seq;
+        n = P.per_seq;
     }
-    const int64_t pos = (int64_t)P.starts[b] + (tok - first), ps = (int64_t)P.c.blocks_per_page * kKvBlock;
-    if (pos < 0 || pos >= P.c.table_stride * ps) { atomicExch(&g_kv4_status, kKv4BadPage); return; }
-    const int64_t pg = P.c.table[b * P.c.table_stride + pos / ps];
-    if (pg < 0 || pg >= P.c.n_pages) { atomicExch(&g_kv4_status, kKv4BadPage); return; }
-    page = (int)pg;
-    off = (int)(pos % ps);
+    if (k < 0 || n <= 0 || first < 0 || first + n > P.n_tokens) return it;
+    const int64_t start = P.starts[b], pos0 = ((start - (start & 15)) / kKvBlock + k) * kKvBlock;
+    if (pos0 >= start + n) return it;
+    it.t0 = (int)max(start - pos0, (int64_t)0);
+    it.t1 = (int)min(start + n - pos0, (int64_t)kKvBlock);
+    it.token0 = first + pos0 - start;
+    const int64_t blk = pos0 / kKvBlock, row = blk / P.c.blocks_per_page;
+    it.block = (int)(blk - row * P.c.blocks_per_page);
+    const int64_t page = pos0 >= 0 && row < P.c.table_stride ? P.c.table[b * P.c.table_stride + row] : -1;
+    if (page < 0 || page >= P.c.n_pages) atomicExch(&g_kv4_status, kKv4BadPage);
+    else it.page = (int)page;
+    return it;
 }
 
 template <typename T> struct Pair;
@@ -100,35 +121,64 @@ __device__ __forceinline__ uint32_t group_meta(float lo, float hi) {
     return Pair<T>::pack(scale, lo);
 }
 
-// round_half_even((x - lo) / scale), at most 15.  x * inv may miss a tie or fall on the wrong side of one; the remainder
-// c * scale - (x - lo), which the fused multiply-add forms without rounding, puts that right.
-__device__ __forceinline__ uint32_t code_of(float x, float lo, float scale, float inv) {
-    const float a = x - lo, h = 0.5f * scale;
-    float c = rintf(a * inv);
-    const float d = fmaf(-c, scale, a);
-    const bool odd = ((int)c & 1) != 0;
-    if (d > h || (d == h && odd)) c += 1.f;
-    if (d < -h || (d == -h && odd)) c -= 1.f;
-    return (uint32_t)(int)fminf(c, 15.f);
+// round_half_even((x - lo) / scale), at most 15, for 8 values: the codes as 4-bit fields.  Adding 1.5 * 2^23 rounds and leaves
+// the code in the sum's low bits; the fields are gathered by multiply-adds of the sums' bits.  x * inv may miss a tie or fall on the wrong side of
+// one: then the remainder x - lo - code * scale, which the fused multiply-add forms without rounding, is half a step or more, and the
+// eight are done again with care.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale, float lo) {
+    constexpr float kMagic = 12582912.f;                          // bits 0x4B400000
+    if (!(scale > 0.f)) return 0u;
+    const float inv = __frcp_rn(scale), half = 0.5f * scale;
+    uint32_t word = 0u - 0x4B400000u * 0x11111111u;
+    bool near_tie = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float2 f = Pair<T>::f2(x[j >> 1]);
+        const float a = (j & 1 ? f.y : f.x) - lo;
+        const float t = fminf(fmaf(a, inv, kMagic), kMagic + 15.f);
+        const float rest = fmaf(-(t - kMagic), scale, a);
+        near_tie = near_tie || rest <= -half || (rest >= half && t < kMagic + 15.f);       // above 15 there is nothing to round up to
+        word += __float_as_uint(t) << (4 * j);
+    }
+    if (near_tie) {
+        word = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float2 f = Pair<T>::f2(x[j >> 1]);
+            const float a = (j & 1 ? f.y : f.x) - lo;
+            float c = rintf(a * inv);
+            const float d = fmaf(-c, scale, a);
+            const bool odd = ((int)c & 1) != 0;
+            if (d > half || (d == half && odd)) c += 1.f;
+            if (d < -half || (d == -half && odd)) c -= 1.f;
+            word |= (uint32_t)(int)fminf(c, 15.f) << (4 * j);
+        }
+    }
+    return word;
 }
+
+// Where thread `tid` stands: 8 values from `d` on, of block position `tok`, in every kPer-th row from `sub` on.
+template <int D> struct Place {
+    static constexpr int kTpr = D / 8;                                     // threads of a row
+    static constexpr int kPer = kThreads / (kTpr * kKvBlock);              // rows of a token side by side: 1 at D = 128, 2 at 64
+};
 
 template <typename T, int D, int GS>
 __global__ void __launch_bounds__(kThreads)
 kv4_append_kernel(const RowParams P) {
     using L = KvLayout<D, GS>;
-    constexpr int kTpr = D / 8;                        // threads of a row
-    constexpr int kPer = kThreads / (kTpr * kTok);     // rows of each token side by side: 1 at D = 128, 2 at 64
-    constexpr int kBatch = 4;                          // loads in flight
-    __shared__ int s_page[kTok], s_off[kTok];
+    constexpr int kTpr = Place<D>::kTpr, kPer = Place<D>::kPer, kBatch = 4;       // kBatch: loads in flight
+    __shared__ __align__(16) unsigned char image[kMaxHeads][L::kBytes];
+    const Item it = find_item(P, blockIdx.x);
+    if (it.page < 0) return;
     const int tid = threadIdx.x;
-    if (tid < kTok) find_slot(P, (int64_t)blockIdx.x * kTok + tid, s_page[tid], s_off[tid]);
-    const int part = tid % kTpr, tok = (tid / kTpr) % kTok, sub = tid / (kTpr * kTok);
-    const int h0 = blockIdx.y * P.heads_per_cta, h1 = min(h0 + P.heads_per_cta, P.c.kv_heads);
-    const int64_t token = (int64_t)blockIdx.x * kTok + tok;
-    const int rows = 2 * (h1 - h0);                    // (head, K or V)
-    __syncthreads();
-    const int page = s_page[tok], off = s_off[tok], in_block = off % kKvBlock;
-    const bool live = page >= 0;
+    const int d = tid % kTpr * 8, tok = (tid / kTpr) % kKvBlock, sub = tid / (kTpr * kKvBlock);
+    const int h0 = blockIdx.y * P.heads_per_cta, heads = min(P.heads_per_cta, P.c.kv_heads - h0), rows = 2 * heads;      // a row: (head, K or V)
+    const bool live = tok >= it.t0 && tok < it.t1, full = it.t1 - it.t0 == kKvBlock, lead = d % GS == 0;
+    const int64_t token = it.token0 + tok;
+    const int64_t stride = (int64_t)P.c.blocks_per_page * L::kBytes;              // from a head to the next
+    unsigned char* first = P.c.pages + (((int64_t)it.page * P.c.kv_heads + h0) * P.c.blocks_per_page + it.block) * L::kBytes;
     for (int r0 = sub; r0 < rows; r0 += kPer * kBatch) {
         uint4 x[kBatch];
 #pragma unroll
@@ -139,7 +189,7 @@ kv4_append_kernel(const RowParams P) {
                 const int h = h0 + (r >> 1);
                 const T* src = (r & 1) ? reinterpret_cast<const T*>(P.v_in) + token * P.v_tok + h * P.v_head
                                        : reinterpret_cast<const T*>(P.k_in) + token * P.k_tok + h * P.k_head;
-                x[i] = __ldg(reinterpret_cast<const uint4*>(src + part * 8));
+                x[i] = __ldg(reinterpret_cast<const uint4*>(src + d));
             }
         }
 #pragma unroll
@@ -156,32 +206,26 @@ kv4_append_kernel(const RowParams P) {
             const float2 mm = Pair<T>::f2(both);
             const uint32_t meta = group_meta<T>(mm.x, -mm.y);
             const float2 sl = Pair<T>::f2(meta);
-            const float inv = sl.x > 0.f ? __frcp_rn(sl.x) : 0.f;
-            uint32_t word = 0u;
             const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            if (sl.x > 0.f) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = Pair<T>::f2(xs[j]);
-                    word |= code_of(f.x, sl.y, sl.x, inv) << (8 * j);
-                    word |= code_of(f.y, sl.y, sl.x, inv) << (8 * j + 4);
-                }
-            }
-            if (live && r < rows) {
-                const int h = h0 + (r >> 1);
-                unsigned char* blk = P.c.pages + (((int64_t)page * P.c.kv_heads + h) * P.c.blocks_per_page + off / kKvBlock) * L::kBytes;
-                const int d = part * 8;
-                const bool lead = d % GS == 0;
-                if ((r & 1) == 0) {
-                    *reinterpret_cast<uint32_t*>(blk + in_block * L::kRow + L::k_nibble(d) / 2) = word;
-                    if (lead) *reinterpret_cast<uint32_t*>(blk + L::kKMeta + in_block * L::kMeta + (d / GS) * 4) = meta;
-                } else {
-                    *reinterpret_cast<uint16_t*>(blk + L::kVCodes + L::v_byte(d, in_block)) = (uint16_t)word;
-                    *reinterpret_cast<uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, in_block)) = (uint16_t)(word >> 16);
-                    if (lead) *reinterpret_cast<uint32_t*>(blk + L::kVMeta + in_block * L::kMeta + (d / GS) * 4) = meta;
-                }
+            const uint32_t word = codes_of<T>(xs, sl.x, sl.y);
+            if (!live || r >= rows) continue;
+            unsigned char* blk = full ? image[r >> 1] : first + (r >> 1) * stride;
+            if ((r & 1) == 0) {
+                *reinterpret_cast<uint32_t*>(blk + tok * L::kRow + L::k_nibble(d) / 2) = word;
+                if (lead) *reinterpret_cast<uint32_t*>(blk + L::kKMeta + tok * L::kMeta + (d / GS) * 4) = meta;
+            } else {
+                *reinterpret_cast<uint16_t*>(blk + L::kVCodes + L::v_byte(d, tok)) = (uint16_t)word;
+                *reinterpret_cast<uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, tok)) = (uint16_t)(word >> 16);
+                if (lead) *reinterpret_cast<uint32_t*>(blk + L::kVMeta + tok * L::kMeta + (d / GS) * 4) = meta;
             }
         }
+    }
+    if (!full) return;
+    __syncthreads();
+    constexpr int kPieces = L::kBytes / 16;
+    for (int i = tid; i < heads * kPieces; i += kThreads) {
+        const int h = i / kPieces, at = i % kPieces * 16;
+        *reinterpret_cast<uint4*>(first + h * stride + at) = *reinterpret_cast<const uint4*>(image[h] + at);
     }
 }
 
@@ -197,52 +241,45 @@ template <typename T, int D, int GS>
 __global__ void __launch_bounds__(kThreads)
 kv4_read_kernel(const RowParams P) {
     using L = KvLayout<D, GS>;
-    constexpr int kTpr = D / 8, kPer = kThreads / (kTpr * kTok), kBatch = 4;
-    __shared__ int s_page[kTok], s_off[kTok];
+    constexpr int kTpr = Place<D>::kTpr, kPer = Place<D>::kPer;
+    __shared__ __align__(16) unsigned char image[kMaxHeads][L::kBytes];
+    const Item it = find_item(P, blockIdx.x);
+    if (it.page < 0) return;
     const int tid = threadIdx.x;
-    if (tid < kTok) find_slot(P, (int64_t)blockIdx.x * kTok + tid, s_page[tid], s_off[tid]);
-    const int part = tid % kTpr, tok = (tid / kTpr) % kTok, sub = tid / (kTpr * kTok);
-    const int h0 = blockIdx.y * P.heads_per_cta, h1 = min(h0 + P.heads_per_cta, P.c.kv_heads);
-    const int64_t token = (int64_t)blockIdx.x * kTok + tok;
-    const int rows = 2 * (h1 - h0), d = part * 8;
+    const int d = tid % kTpr * 8, tok = (tid / kTpr) % kKvBlock, sub = tid / (kTpr * kKvBlock);
+    const int h0 = blockIdx.y * P.heads_per_cta, heads = min(P.heads_per_cta, P.c.kv_heads - h0);
+    const int64_t stride = (int64_t)P.c.blocks_per_page * L::kBytes;
+    const unsigned char* first = P.c.pages + (((int64_t)it.page * P.c.kv_heads + h0) * P.c.blocks_per_page + it.block) * L::kBytes;
+    constexpr int kPieces = L::kBytes / 16;
+    for (int i = tid; i < heads * kPieces; i += kThreads) {
+        const int h = i / kPieces, at = i % kPieces * 16;
+        *reinterpret_cast<uint4*>(image[h] + at) = __ldcs(reinterpret_cast<const uint4*>(first + h * stride + at));
+    }
     __syncthreads();
-    const int page = s_page[tok], off = s_off[tok], in_block = off % kKvBlock;
-    if (page < 0) return;
-    for (int r0 = sub; r0 < rows; r0 += kPer * kBatch) {
-        uint32_t word[kBatch], meta[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int r = r0 + i * kPer;
-            word[i] = meta[i] = 0u;
-            if (r < rows) {
-                const unsigned char* blk = P.c.pages + (((int64_t)page * P.c.kv_heads + h0 + (r >> 1)) * P.c.blocks_per_page + off / kKvBlock) * L::kBytes;
-                if ((r & 1) == 0) {
-                    word[i] = *reinterpret_cast<const uint32_t*>(blk + in_block * L::kRow + L::k_nibble(d) / 2);
-                    meta[i] = *reinterpret_cast<const uint32_t*>(blk + L::kKMeta + in_block * L::kMeta + (d / GS) * 4);
-                } else {
-                    word[i] = *reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d, in_block)) |
-                              ((uint32_t)*reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, in_block)) << 16);
-                    meta[i] = *reinterpret_cast<const uint32_t*>(blk + L::kVMeta + in_block * L::kMeta + (d / GS) * 4);
-                }
-            }
+    if (tok < it.t0 || tok >= it.t1) return;
+    const int64_t out = ((it.token0 + tok) * P.c.kv_heads + h0) * D + d;
+    for (int r = sub; r < 2 * heads; r += kPer) {
+        const unsigned char* blk = image[r >> 1];
+        uint32_t word, meta;
+        if ((r & 1) == 0) {
+            word = *reinterpret_cast<const uint32_t*>(blk + tok * L::kRow + L::k_nibble(d) / 2);
+            meta = *reinterpret_cast<const uint32_t*>(blk + L::kKMeta + tok * L::kMeta + (d / GS) * 4);
+        } else {
+            word = *reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d, tok)) |
+                   ((uint32_t)*reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, tok)) << 16);
+            meta = *reinterpret_cast<const uint32_t*>(blk + L::kVMeta + tok * L::kMeta + (d / GS) * 4);
         }
+        const float2 sl = Pair<T>::f2(meta);
+        uint32_t o[4];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int r = r0 + i * kPer;
-            if (r >= rows) continue;
-            const float2 sl = Pair<T>::f2(meta[i]);
-            uint32_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // 2^23 + code, exactly, from the bits; a single rounding to fp32, one to T
-                const float c0 = __uint_as_float(0x4B000000u | ((word[i] >> (8 * j)) & 15u)) - 8388608.f;
-                const float c1 = __uint_as_float(0x4B000000u | ((word[i] >> (8 * j + 4)) & 15u)) - 8388608.f;
-                o[j] = Pair<T>::pack(value_of<T>(c0, sl.x, sl.y), value_of<T>(c1, sl.x, sl.y));
-            }
-            T* dst = ((r & 1) ? reinterpret_cast<T*>(P.v_out) : reinterpret_cast<T*>(P.k_out)) +
-                     (token * P.c.kv_heads + h0 + (r >> 1)) * D + d;
-            *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int j = 0; j < 4; ++j) {
+            // 2^23 + code, exactly, from the bits; a single rounding to fp32, one to T
+            const float c0 = __uint_as_float(0x4B000000u | ((word >> (8 * j)) & 15u)) - 8388608.f;
+            const float c1 = __uint_as_float(0x4B000000u | ((word >> (8 * j + 4)) & 15u)) - 8388608.f;
+            o[j] = Pair<T>::pack(value_of<T>(c0, sl.x, sl.y), value_of<T>(c1, sl.x, sl.y));
         }
+        T* dst = ((r & 1) ? reinterpret_cast<T*>(P.v_out) : reinterpret_cast<T*>(P.k_out)) + out + (r >> 1) * D;
+        __stcs(reinterpret_cast<uint4*>(dst), make_uint4(o[0], o[1], o[2], o[3]));
     }
 }
 
@@ -267,13 +304,14 @@ int launch_kv4_rows(bool append, const cb_kv4_cache* c, const void* k_in, const 
     if (strides != nullptr) { P.k_tok = strides[0]; P.k_head = strides[1]; P.v_tok = strides[2]; P.v_head = strides[3]; }
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
-    // few tokens: one head to a CTA, so that a decode step spreads over the SMs; many: eight, to look pages up less often
-    const int64_t tiles = (n_tokens + kTok - 1) / kTok;
+    // few blocks: one head to a CTA, so that a decode step spreads over the SMs; many: up to eight, for fewer look-ups
+    const int64_t items = items_of(n_tokens, n_seqs, P.per_seq, cu != nullptr);
     int hp = 1;
-    while (hp < 8 && tiles * ((c->kv_heads + 2 * hp - 1) / (2 * hp)) >= 4 * sms) hp *= 2;
-    while ((c->kv_heads + hp - 1) / hp > 65535) hp *= 2;
+    while (hp < kMaxHeads && items * ((c->kv_heads + 2 * hp - 1) / (2 * hp)) >= 4 * sms) hp *= 2;
     P.heads_per_cta = hp;
-    const dim3 grid((unsigned)tiles, (unsigned)((c->kv_heads + hp - 1) / hp));
+    const int64_t head_ctas = (c->kv_heads + hp - 1) / hp;
+    if (items >= (1ll << 31) || head_ctas > 65535) { set_error("kv4: too many tokens, sequences or heads in one call"); return CB_ERR_INVALID; }
+    const dim3 grid((unsigned)items, (unsigned)head_ctas);
     const bool bf = c->dtype == CB_BF16;
 #define CB_KV4_CASE(d, g) \
     if (c->head_dim == d && c->group_size == g) \
