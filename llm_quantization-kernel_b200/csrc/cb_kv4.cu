@@ -94,6 +94,14 @@ template <> struct Pair<__half> {
         const __half2 r = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&r);
     }
+    static constexpr float kTop = 65504.f;
+    // value = code * scale + lo with one rounding, for two codes at bits 0-3 and 16-19: 1024 + code from the bits, exactly
+    __device__ static uint32_t values(uint32_t codes, uint32_t scale2, uint32_t lo2) {
+        const uint32_t u = (codes & 0x000F000Fu) | 0x64006400u, k = 0x64006400u;
+        const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&k));
+        const __half2 r = __hfma2(c, *reinterpret_cast<const __half2*>(&scale2), *reinterpret_cast<const __half2*>(&lo2));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
 };
 template <> struct Pair<__nv_bfloat16> {
     using V2 = __nv_bfloat162;
@@ -110,6 +118,14 @@ template <> struct Pair<__nv_bfloat16> {
         const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&r);
     }
+    static constexpr float kTop = 3.3895314e38f;
+    // as for fp16; 128 + code from the bits
+    __device__ static uint32_t values(uint32_t codes, uint32_t scale2, uint32_t lo2) {
+        const uint32_t u = (codes & 0x000F000Fu) | 0x43004300u, k = 0x43004300u;
+        const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&k));
+        const __nv_bfloat162 r = __hfma2(c, *reinterpret_cast<const __nv_bfloat162*>(&scale2), *reinterpret_cast<const __nv_bfloat162*>(&lo2));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
 };
 
 // The group's (scale, lo) as stored, from its exact minimum and maximum.
@@ -121,39 +137,45 @@ __device__ __forceinline__ uint32_t group_meta(float lo, float hi) {
     return Pair<T>::pack(scale, lo);
 }
 
-// round_half_even((x - lo) / scale), at most 15, for 8 values: the codes as 4-bit fields.  Adding 1.5 * 2^23 rounds and leaves
-// the code in the sum's low bits; the fields are gathered by multiply-adds of the sums' bits.  x * inv may miss a tie or fall on the wrong side of
-// one: then the remainder x - lo - code * scale, which the fused multiply-add forms without rounding, is half a step or more, and the
-// eight are done again with care.
+// Reciprocal to about 2^-22; what it gets wrong is found below.
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// round_half_even((x - lo) / scale), at most 15, for 8 values: the codes as 4-bit fields.  Adding 1.5 * 2^23 rounds; the rounded
+// quotients are gathered by multiply-adds.  The remainder x - lo - code * scale, which the fused multiply-add forms without rounding,
+// shows where the approximate quotient met a tie or fell on the wrong side of one: there it is half a step or more (`half`: half a step, or 0
+// where a code could exceed 15), and the eight are done again with care.
 template <typename T>
-__device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale, float lo) {
-    constexpr float kMagic = 12582912.f;                          // bits 0x4B400000
-    if (!(scale > 0.f)) return 0u;
-    const float inv = __frcp_rn(scale), half = 0.5f * scale;
-    uint32_t word = 0u - 0x4B400000u * 0x11111111u;
-    bool near_tie = false;
+__device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale, float lo, float inv, float half) {
+    constexpr float kMagic = 12582912.f;
+    float c[8], worst = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float2 f = Pair<T>::f2(x[j >> 1]);
         const float a = (j & 1 ? f.y : f.x) - lo;
-        const float t = fminf(fmaf(a, inv, kMagic), kMagic + 15.f);
-        const float rest = fmaf(-(t - kMagic), scale, a);
-        near_tie = near_tie || rest <= -half || (rest >= half && t < kMagic + 15.f);       // above 15 there is nothing to round up to
-        word += __float_as_uint(t) << (4 * j);
+        c[j] = fmaf(a, inv, kMagic) - kMagic;
+        worst = fmaxf(worst, fabsf(fmaf(-c[j], scale, a)));
     }
-    if (near_tie) {
-        word = 0u;
+    if (worst < half) {
+        const float p = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + kMagic;
+        const float q = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + kMagic;
+        return __byte_perm(__float_as_uint(p), __float_as_uint(q), 0x5410);
+    }
+    uint32_t word = 0u;
+    if (!(scale > 0.f)) return 0u;                                // one value, or NaN
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = Pair<T>::f2(x[j >> 1]);
-            const float a = (j & 1 ? f.y : f.x) - lo;
-            float c = rintf(a * inv);
-            const float d = fmaf(-c, scale, a);
-            const bool odd = ((int)c & 1) != 0;
-            if (d > half || (d == half && odd)) c += 1.f;
-            if (d < -half || (d == -half && odd)) c -= 1.f;
-            word |= (uint32_t)(int)fminf(c, 15.f) << (4 * j);
-        }
+    for (int j = 0; j < 8; ++j) {
+        const float2 f = Pair<T>::f2(x[j >> 1]);
+        const float a = (j & 1 ? f.y : f.x) - lo, h = 0.5f * scale;
+        float k = rintf(__fdiv_rn(a, scale));
+        const float d = fmaf(-k, scale, a);
+        const bool odd = ((int)k & 1) != 0;
+        if (d > h || (d == h && odd)) k += 1.f;
+        if (d < -h || (d == -h && odd)) k -= 1.f;
+        word |= (uint32_t)(int)fminf(k, 15.f) << (4 * j);
     }
     return word;
 }
@@ -192,22 +214,33 @@ kv4_append_kernel(const RowParams P) {
                 x[i] = __ldg(reinterpret_cast<const uint4*>(src + d));
             }
         }
+        // All lanes take part in the shuffles; what dead ones compute is dropped.  Groups' (min, -max) first, of all the rows; then each
+        // lane of a group finishes one row's, and they are passed around.
+        uint32_t both[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int r = r0 + i * kPer;
-            // all lanes take part in the shuffles; what dead ones compute is dropped
             uint32_t mn = Pair<T>::min2(Pair<T>::min2(x[i].x, x[i].y), Pair<T>::min2(x[i].z, x[i].w));
-            uint32_t mx = Pair<T>::max2(Pair<T>::max2(x[i].x, x[i].y), Pair<T>::max2(x[i].z, x[i].w));
-            mn = Pair<T>::min2(mn, __byte_perm(mn, 0u, 0x1032));
-            mx = Pair<T>::max2(mx, __byte_perm(mx, 0u, 0x1032)) ^ 0x80008000u;
-            uint32_t both = __byte_perm(mn, mx, 0x5410);                  // (min, -max)
+            uint32_t mx = Pair<T>::max2(Pair<T>::max2(x[i].x, x[i].y), Pair<T>::max2(x[i].z, x[i].w)) ^ 0x80008000u;
+            both[i] = Pair<T>::min2(__byte_perm(mn, mx, 0x5410), __byte_perm(mn, mx, 0x7632));
+        }
 #pragma unroll
-            for (int o = 1; o < GS / 8; o <<= 1) both = Pair<T>::min2(both, __shfl_xor_sync(0xffffffffu, both, o));
-            const float2 mm = Pair<T>::f2(both);
-            const uint32_t meta = group_meta<T>(mm.x, -mm.y);
+        for (int o = 1; o < GS / 8; o <<= 1)
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) both[i] = Pair<T>::min2(both[i], __shfl_xor_sync(0xffffffffu, both[i], o));
+        static_assert(kBatch == 4 && GS / 8 >= 4, "a lane for each row");
+        const float2 mm = Pair<T>::f2(tid & 2 ? (tid & 1 ? both[3] : both[2]) : (tid & 1 ? both[1] : both[0]));
+        const uint32_t my_meta = group_meta<T>(mm.x, -mm.y);
+        const float my_scale = Pair<T>::f2(my_meta).x, my_inv = rcp_approx(my_scale);
+        // the rounding of a scale of few bits can carry the largest value past 15.5 steps; NaN fails the comparison
+        const float my_half = -mm.y - mm.x < 15.4f * my_scale ? 0.5f * my_scale : 0.f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int r = r0 + i * kPer, from = (tid & 31 & ~3) | i;
+            const uint32_t meta = __shfl_sync(0xffffffffu, my_meta, from);
+            const float inv = __shfl_sync(0xffffffffu, my_inv, from), half = __shfl_sync(0xffffffffu, my_half, from);
             const float2 sl = Pair<T>::f2(meta);
             const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            const uint32_t word = codes_of<T>(xs, sl.x, sl.y);
+            const uint32_t word = codes_of<T>(xs, sl.x, sl.y, inv, half);
             if (!live || r >= rows) continue;
             unsigned char* blk = full ? image[r >> 1] : first + (r >> 1) * stride;
             if ((r & 1) == 0) {
@@ -227,14 +260,6 @@ kv4_append_kernel(const RowParams P) {
         const int h = i / kPieces, at = i % kPieces * 16;
         *reinterpret_cast<uint4*>(first + h * stride + at) = *reinterpret_cast<const uint4*>(image[h] + at);
     }
-}
-
-// code * scale + lo, at most the type's largest number in size: the rounding of scale can carry the largest value of a
-// group whose range reaches that number past it.  NaN stays.
-template <typename T>
-__device__ __forceinline__ float value_of(float code, float scale, float lo) {
-    const float v = fmaf(code, scale, lo), top = std::is_same<T, __half>::value ? 65504.f : 3.3895314e38f;
-    return v > top ? top : v < -top ? -top : v;
 }
 
 template <typename T, int D, int GS>
@@ -269,15 +294,21 @@ kv4_read_kernel(const RowParams P) {
                    ((uint32_t)*reinterpret_cast<const uint16_t*>(blk + L::kVCodes + L::v_byte(d + 4, tok)) << 16);
             meta = *reinterpret_cast<const uint32_t*>(blk + L::kVMeta + tok * L::kMeta + (d / GS) * 4);
         }
-        const float2 sl = Pair<T>::f2(meta);
-        uint32_t o[4];
+        const uint32_t scale2 = __byte_perm(meta, 0u, 0x1010), lo2 = __byte_perm(meta, 0u, 0x3232);
+        uint32_t y[4];                                            // values 0 and 4, 1 and 5, 2 and 6, 3 and 7
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // 2^23 + code, exactly, from the bits; a single rounding to fp32, one to T
-            const float c0 = __uint_as_float(0x4B000000u | ((word >> (8 * j)) & 15u)) - 8388608.f;
-            const float c1 = __uint_as_float(0x4B000000u | ((word >> (8 * j + 4)) & 15u)) - 8388608.f;
-            o[j] = Pair<T>::pack(value_of<T>(c0, sl.x, sl.y), value_of<T>(c1, sl.x, sl.y));
+        for (int j = 0; j < 4; ++j) y[j] = Pair<T>::values(word >> (4 * j), scale2, lo2);
+        const float2 sl = Pair<T>::f2(meta);
+        if (fmaf(15.f, sl.x, sl.y) > Pair<T>::kTop) {
+            // the rounding of scale can carry the largest values of such a group past the type's largest number: they are that number
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = fmaf((float)((word >> (4 * j)) & 15u), sl.x, sl.y), b = fmaf((float)((word >> (4 * j + 16)) & 15u), sl.x, sl.y);
+                y[j] = Pair<T>::pack(fminf(a, Pair<T>::kTop), fminf(b, Pair<T>::kTop));
+            }
         }
+        const uint32_t o[4] = {__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                               __byte_perm(y[2], y[3], 0x7632)};
         T* dst = ((r & 1) ? reinterpret_cast<T*>(P.v_out) : reinterpret_cast<T*>(P.k_out)) + out + (r >> 1) * D;
         __stcs(reinterpret_cast<uint4*>(dst), make_uint4(o[0], o[1], o[2], o[3]));
     }
