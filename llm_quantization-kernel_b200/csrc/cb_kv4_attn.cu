@@ -15,8 +15,8 @@
 //
 // Precision: q_r is scaled by a power of two so that its largest value lies in [2^13, 2^14) and then rounded to fp16: exact for
 // fp16 inputs down to 2^-24 of the row's largest value, and for bfloat16 inputs alike.  p * scale is scaled by a power of two so
-// that scale's part lies in [2^14, 2^15) for the largest scale met and then rounded to fp16 (relative error 2^-11; below 2^-28
-// of the largest possible weight absolute).  All sums, the softmax statistics and the lo part are fp32.
+// that scale's part lies in [2^6, 2^7) for the largest scale met and then rounded to fp16 (relative error 2^-11; below 2^-20
+// of the largest weight and scale 2^-31 of them).  p is at most 2^8, so that this fits fp16.  All sums, the softmax statistics and the lo part are fp32.
 //
 // Work: the 16-token blocks of all (sequence, row tile, key head) segments form one line that is cut into equal parts, one for each CTA (two to an
 // SM), whatever the lengths are; lengths are read on the device, so a captured launch serves any.  The 8 warps of a CTA take
@@ -48,6 +48,7 @@ struct AttnParams {
     float scale_log2;                                 // |softmax scale| * log2(e), above 0
     float q_sign;                                     // 1, or -1 where the scale is negative
     uint32_t zero;                                    // 0, unknown to the compiler
+    uint32_t bpp_mul, bpp_shift;                      // n / blocks_per_page = (n * bpp_mul) >> 32 >> bpp_shift for n < 2^31; bpp_mul 0: one block to a page
     int* counters;                                    // [B * kv_heads * row_tiles], zero between calls
     float* partial;                                   // [grid][2][rows of a tile * (D + 2)]
 };
@@ -134,6 +135,8 @@ __device__ __forceinline__ int seq_len(const AttnParams& P, int64_t b) {
     return (int)min((int64_t)max(P.lengths[b], 0), cap);
 }
 __device__ __forceinline__ int blocks_of(int len) { return (int)(((unsigned)len + kKvBlock - 1) / kKvBlock); }
+
+constexpr float kLag = 8.f;
 
 constexpr int kOpen = 12;
 __device__ __forceinline__ int units_open(int nblk) { return nblk == 0 ? 0 : nblk + kOpen; }
@@ -244,7 +247,7 @@ kv4_attention_kernel(const AttnParams P) {
         int64_t page = -1;
         int in_page = 0;
         if (lane < per && blk < blk1) {
-            const int row = blk / P.c.blocks_per_page;
+            const int row = P.bpp_mul == 0u ? blk : (int)(__umulhi((uint32_t)blk, P.bpp_mul) >> P.bpp_shift);
             in_page = blk - row * P.c.blocks_per_page;
             page = P.c.table[b * P.c.table_stride + row];
             if (page < 0 || page >= P.c.n_pages) { page = -1; atomicExch(&g_kv4_attn_status, kKv4BadPage); }
@@ -417,13 +420,11 @@ kv4_attention_kernel(const AttnParams P) {
                         }
                 }
             }
-            // ---- running maximum (of the scaled scores) and scale reference
-            float alpha[NT][2];
+            // ---- m_run follows the running maximum of the scaled scores, s_exp that of the value scales.  m_run is moved only where
+            // some score lies more than kLag above it: p stays below 2^kLag, and most stages need no exchange between lanes.
             const float smax = fmaxf(unpack2<T>(smax2).x, 0.f);
-            const int e_new = max(s_exp, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)) >> 23));
-            bool moved = e_new != s_exp;
-            const float rs = __uint_as_float((uint32_t)max(127 + s_exp - e_new, 0) << 23);
-            s_exp = e_new;
+            float mx[NT][2];
+            bool move = (int)(__float_as_uint(smax) >> 23) > s_exp;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -431,32 +432,38 @@ kv4_attention_kernel(const AttnParams P) {
                     float m = fmaxf(x[0][n][c], x[0][n][2 + c]);
 #pragma unroll
                     for (int k = 1; k < kStageBlocks; ++k) m = fmaxf(m, fmaxf(x[k][n][c], x[k][n][2 + c]));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    const float mn = fmaxf(m_run[n][c], m * qmul[n][c]);
-                    alpha[n][c] = mn == m_run[n][c] ? 1.f : ex2(m_run[n][c] - mn);
-                    moved = moved || alpha[n][c] != 1.f;
-                    m_run[n][c] = mn;
+                    mx[n][c] = m * qmul[n][c];
+                    move = move || mx[n][c] > m_run[n][c] + kLag;
                 }
-            if (__any_sync(0xffffffffu, moved)) {
+            if (__any_sync(0xffffffffu, move)) {
+                const int e_new = max(s_exp, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(smax)) >> 23));
+                const float rs = __uint_as_float((uint32_t)max(127 + s_exp - e_new, 0) << 23);
+                s_exp = e_new;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+                    float alpha[2];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        l_run[n][c] *= alpha[n][c];
+                        float m = mx[n][c];
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                        m = fmaxf(m_run[n][c], m);
+                        alpha[c] = m == m_run[n][c] ? 1.f : ex2(m_run[n][c] - m);
+                        m_run[n][c] = m;
+                        l_run[n][c] *= alpha[c];
 #pragma unroll
-                        for (int j = 0; j < NG; ++j) z[n][j][c] *= alpha[n][c];
-                        alpha[n][c] *= rs;
+                        for (int j = 0; j < NG; ++j) z[n][j][c] *= alpha[c];
+                        alpha[c] *= rs;
                     }
 #pragma unroll
                     for (int d = 0; d < D / 16; ++d) {
-                        o[n][d][0] *= alpha[n][0]; o[n][d][1] *= alpha[n][1];
-                        o[n][d][2] *= alpha[n][0]; o[n][d][3] *= alpha[n][1];
+                        o[n][d][0] *= alpha[0]; o[n][d][1] *= alpha[1];
+                        o[n][d][2] *= alpha[0]; o[n][d][3] *= alpha[1];
                     }
                 }
             }
-            const float cmul = __uint_as_float((uint32_t)(268 - s_exp) << 23);       // 2^14 / 2^(s_exp - 127)
+            const float cmul = __uint_as_float((uint32_t)(260 - s_exp) << 23);       // 2^6 / 2^(s_exp - 127)
             uint32_t words = 0u;
 #pragma unroll
             for (int k = 0; k < kStageBlocks; ++k) {
@@ -499,7 +506,6 @@ kv4_attention_kernel(const AttnParams P) {
                             pb[n][j][0] = movmatrix_t(pack_h2(h[0], h[1]));
                             pb[n][j][1] = movmatrix_t(pack_h2(h[2], h[3]));
                         }
-                        words |= pb[n][j][0] | pb[n][j][1];
                     }
                 }
                 uint32_t v0[D / 32], v1[D / 32];                                     // pairs t and t + 4
@@ -535,8 +541,8 @@ kv4_attention_kernel(const AttnParams P) {
             uint32_t seen_words;
             if (good == 3u && cnt == kStageBlocks && (first + cnt) * kKvBlock <= lim_min) seen_words = take(std::true_type{}, stage, first, good);
             else seen_words = take(std::false_type{}, stage, first, good);
-            // The slot may be overwritten once every lane has its codes in registers: the vote needs words that came last, and
-            // what was computed from the others (the bits are masked with a zero that the compiler does not know).
+            // The slot may be overwritten once every lane has its codes in registers: this vote needs the V words (masked with a zero
+            // that the compiler does not know), the vote on the maxima needed all else.
             const unsigned held = __ballot_sync(0xffffffffu, (seen_words & P.zero) != 0u);
             if (i + kSlots < mine) issue(i + kSlots, at + kSlots + held);
         }
@@ -561,7 +567,7 @@ kv4_attention_kernel(const AttnParams P) {
 
         // ---- the warps' results meet: value = o * 2^24 (2^20) / cmul + z
         {
-            const float back = __uint_as_float((uint32_t)(s_exp - 14) << 23);        // 1 / cmul
+            const float back = __uint_as_float((uint32_t)(s_exp - 6) << 23);         // 1 / cmul
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -733,6 +739,13 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     P.q_sign = scale < 0.f ? -1.f : 1.f;
     P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
     P.zero = 0u;
+    {   // with 2^s >= d > 2^(s - 1), m = ceil(2^(31 + s) / d) < 2^32 is off by less than 1, n * m / 2^(31 + s) by less than n / 2^(31 + s) < 1 / d
+        const uint32_t d = (uint32_t)P.c.blocks_per_page;
+        uint32_t s = 0;
+        while ((1u << s) < d) ++s;
+        P.bpp_mul = d == 1u ? 0u : (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+        P.bpp_shift = d == 1u ? 0u : s - 1;
+    }
     P.counters = counters; P.partial = partial;
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
