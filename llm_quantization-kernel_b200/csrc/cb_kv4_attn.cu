@@ -76,14 +76,25 @@ struct AttnCfg {
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    const long long t0 = clock64();
-    for (;;) {
-        uint32_t ok;
+    uint32_t ok;
+    long long t0 = 0;
+    for (bool again = false;; again = true) {
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n selp.u32 %0, 1, 0, p;\n}"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
-        if (clock64() - t0 > kWaitCycles) return false;
+        if (!again) t0 = clock64();
+        else if (clock64() - t0 > kWaitCycles) return false;
     }
+}
+// A word of 8 codes -> four fp16 pairs: codes 0 and 4 (times 2^-24), 1 and 5 (2^-20), 2 and 6 (2^-24), 3 and 7 (2^-20).  The last
+// pair is formed by a subtraction of the two before it, which is exact and runs beside the integer pipe, the busiest one here.
+__device__ __forceinline__ void spread(uint32_t w, uint32_t (&a)[4]) {
+    a[0] = w & 0x000F000Fu;
+    a[1] = w & 0x00F000F0u;
+    const uint32_t y = __byte_perm(w, 0u, 0x4341);                // bytes 1 and 3
+    a[2] = y & 0x000F000Fu;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&y), *reinterpret_cast<const __half2*>(&a[2]));
+    a[3] = *reinterpret_cast<const uint32_t*>(&d);
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -379,15 +390,14 @@ kv4_attention_kernel(const AttnParams P) {
 #pragma unroll
                     for (int j = 0; j < NG; ++j) {
                         const int w = j * KWG + wg;
-                        const uint32_t ya = wa[w] >> 8, yb = wb[w] >> 8;
+                        uint32_t a[4], c[4];
+                        spread(wa[w], a);
+                        spread(wb[w], c);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            if (wg == 0) mma16816_first(acc[j][n], wa[w] & 0x000F000Fu, wb[w] & 0x000F000Fu, wa[w] & 0x00F000F0u, wb[w] & 0x00F000F0u,
-                                                        qf[n][4 * w], qf[n][4 * w + 1]);
-                            else mma16816(acc[j][n], wa[w] & 0x000F000Fu, wb[w] & 0x000F000Fu, wa[w] & 0x00F000F0u, wb[w] & 0x00F000F0u,
-                                          qf[n][4 * w], qf[n][4 * w + 1]);
-                            mma16816(acc[j][n], ya & 0x000F000Fu, yb & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x00F000F0u,
-                                     qf[n][4 * w + 2], qf[n][4 * w + 3]);
+                            if (wg == 0) mma16816_first(acc[j][n], a[0], c[0], a[1], c[1], qf[n][4 * w], qf[n][4 * w + 1]);
+                            else mma16816(acc[j][n], a[0], c[0], a[1], c[1], qf[n][4 * w], qf[n][4 * w + 1]);
+                            mma16816(acc[j][n], a[2], c[2], a[3], c[3], qf[n][4 * w + 2], qf[n][4 * w + 3]);
                         }
                     }
 #pragma unroll
@@ -514,12 +524,14 @@ kv4_attention_kernel(const AttnParams P) {
 #pragma unroll
                 for (int hw = 0; hw < D / 32; ++hw) {                                // four values of this lane, two tokens each
                     const int j = hw * 4 / (GS / 8);
-                    const uint32_t x0 = v0[hw], x1 = v1[hw], y0 = x0 >> 8, y1 = x1 >> 8;
-                    words |= x0 | x1;
+                    uint32_t a[4], c[4];
+                    spread(v0[hw], a);
+                    spread(v1[hw], c);
+                    words |= v0[hw] | v1[hw];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma16816(o[n][2 * hw], x0 & 0x000F000Fu, y0 & 0x000F000Fu, x1 & 0x000F000Fu, y1 & 0x000F000Fu, pb[n][j][0], pb[n][j][1]);
-                        mma16816(o[n][2 * hw + 1], x0 & 0x00F000F0u, y0 & 0x00F000F0u, x1 & 0x00F000F0u, y1 & 0x00F000F0u, pb[n][j][0], pb[n][j][1]);
+                        mma16816(o[n][2 * hw], a[0], a[2], c[0], c[2], pb[n][j][0], pb[n][j][1]);
+                        mma16816(o[n][2 * hw + 1], a[1], a[3], c[1], c[3], pb[n][j][0], pb[n][j][1]);
                     }
                 }
             }
