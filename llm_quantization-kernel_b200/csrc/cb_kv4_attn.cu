@@ -18,8 +18,8 @@
 // that scale's part lies in [2^6, 2^7) for the largest scale met and then rounded to fp16 (relative error 2^-11; below 2^-20
 // of the largest weight and scale 2^-31 of them).  p is at most 2^8, so that this fits fp16.  All sums, the softmax statistics and the lo part are fp32.
 //
-// Work: the 16-token blocks of all (sequence, row tile, key head) segments form one line that is cut into equal parts, one for each CTA (two to an
-// SM), whatever the lengths are; lengths are read on the device, so a captured launch serves any.  The 8 warps of a CTA take
+// Work: the 16-token blocks of all (sequence, row tile, key head) segments form one line that is cut into equal parts, one for each CTA (one to an
+// SM), whatever the lengths are; lengths are read on the device, so a captured launch serves any.  The warps of a CTA take
 // pairs of blocks in turn, each with a ring of its own filled by bulk copies (one per block), and keep running maxima, sums and
 // outputs of their own; they meet in shared memory at the end of a segment.  Where a segment is cut, its parts leave
 // (max, sum, output) in scratch and the CTA that arrives last adds them in order of position: the result does not
@@ -31,7 +31,6 @@
 namespace cb {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kStageBlocks = 2;                       // blocks of a ring slot
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
 
@@ -53,15 +52,23 @@ struct AttnParams {
     float* partial;                                   // [grid][2][rows of a tile * (D + 2)]
 };
 
+// Where a CTA stands: segment `seg` of sequence b (len tokens, nb blocks, per_seg units a segment; base: the sequence's first unit, seg0: the
+// segment's), and its blocks of this CTA.
+struct Piece {
+    uint32_t u, seg0, base;
+    int per_seg, b, seg, nb, len, blk0, blk1;
+};
+struct Sched { uint32_t u0, u1, share, extra; int quota; };
+
 template <int D, int GS, int NT>
 struct AttnCfg {
     using L = KvLayout<D, GS>;
     static constexpr int kRows = 8 * NT;
+    static constexpr int kWarps = NT == 1 ? 12 : 8, kThreads = kWarps * 32;       // one CTA to an SM: 168 or 255 registers a thread
     static constexpr int kSlotBytes = kStageBlocks * L::kBytes;
-    static constexpr int kCtasPerSm = NT == 1 ? 2 : 1;
     static constexpr int kMerge = kWarps * kRows * D * 4;             // the warps' outputs; then the weights of a cut segment's parts
     // the ring fills what an SM has left; the slots of a warp are at most 8
-    static constexpr int kRingBudget = (NT == 1 ? 110 : 222) * 1024 - kMerge;
+    static constexpr int kRingBudget = 223 * 1024 - kMerge;
     static constexpr int kSlots = kRingBudget / (kWarps * kSlotBytes) > 8 ? 8 : kRingBudget / (kWarps * kSlotBytes);
     static_assert(kSlots >= 1, "a ring has a slot");
     static constexpr int kMergeOff = kWarps * kSlots * kSlotBytes;
@@ -69,8 +76,9 @@ struct AttnCfg {
     static constexpr int kBarOff = kStatsOff + 2 * kWarps * kRows * 4;
     static constexpr int kOkOff = kBarOff + kWarps * kSlots * 8;      // [kWarps][kSlots] blocks whose page is good
     static constexpr int kMiscOff = kOkOff + kWarps * kSlots * 4;
-    static constexpr int kSmem = kMiscOff + 16;
-    static_assert(kSmem <= (227 * 1024) / kCtasPerSm - 1024, "shared memory of an SM");
+    static constexpr int kPlaceOff = kMiscOff + 16, kSchedOff = kPlaceOff + kWarps * 2 * (int)sizeof(Piece);
+    static constexpr int kSmem = kSchedOff + kWarps * (int)sizeof(Sched);
+    static_assert(kSmem <= 227 * 1024, "shared memory of an SM");
     static constexpr int kPartFloats = kRows * (D + 2);
 };
 
@@ -153,11 +161,11 @@ constexpr int kOpen = 12;
 __device__ __forceinline__ int units_open(int nblk) { return nblk == 0 ? 0 : nblk + kOpen; }
 
 template <typename T, int D, int GS, int NT>
-__global__ void __launch_bounds__(kThreads, (AttnCfg<D, GS, NT>::kCtasPerSm))
+__global__ void __launch_bounds__((AttnCfg<D, GS, NT>::kThreads), 1)
 kv4_attention_kernel(const AttnParams P) {
     using C = AttnCfg<D, GS, NT>;
     using L = typename C::L;
-    constexpr int NG = L::NG, kSlots = C::kSlots, kRows = C::kRows;
+    constexpr int NG = L::NG, kSlots = C::kSlots, kRows = C::kRows, kWarps = C::kWarps, kThreads = C::kThreads;
     constexpr int KW = D / 32, KWG = GS / 32;          // code words of a lane and key row, of one group
     extern __shared__ __align__(128) unsigned char smem[];
     float* merge = reinterpret_cast<float*>(smem + C::kMergeOff);
@@ -177,90 +185,100 @@ kv4_attention_kernel(const AttnParams P) {
     }
     if (tid == 0) misc[0] = 0;
 
-    // ---- the line's length (every warp for itself), and sequences without keys: their rows are zero
-    int64_t U = 0;
-    {
-        int64_t units = 0;
-        for (int64_t b = lane; b < P.B; b += 32) units += P.aligned ? blocks_of(seq_len(P, b)) : units_open(blocks_of(seq_len(P, b)));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) units += __shfl_xor_sync(0xffffffffu, units, o);
-        U = units * segs;
-    }
-    for (int64_t b = blockIdx.x; b < P.B; b += gridDim.x)
-        if (seq_len(P, b) == 0) {
-            uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(P.out) + b * P.T * P.H * D);
-            for (int i = tid; i < P.T * P.H * D / 2; i += kThreads) o[i] = 0u;
-        }
-    if (U == 0) return;
-    __syncthreads();
+    // ---- the line's length, every warp for itself.  The caller has checked that units fit 32 bits.
+    const int B = (int)P.B, first_len = lane < B ? seq_len(P, lane) : 0;              // of sequence `lane`: all there are with up to 32
+    uint32_t U = P.aligned ? blocks_of(first_len) : units_open(blocks_of(first_len));
+    for (int s = lane + 32; s < B; s += 32) U += P.aligned ? blocks_of(seq_len(P, s)) : units_open(blocks_of(seq_len(P, s)));
+    U = __reduce_add_sync(0xffffffffu, U) * (uint32_t)segs;
     // ---- this CTA's part [u0, u1) of the line.  aligned: a segment of nb blocks is cut into ceil(nb / quota) parts, one to a CTA
-    // (quota such that there are CTAs enough), and u counts parts.  Otherwise the line is cut into equal parts, in which a segment
-    // counts kOpen units more than its blocks, ahead of them: what a CTA spends on a segment besides.
-    const int64_t nc = min((int64_t)gridDim.x, U);
-    const int quota = P.aligned ? (int)((U + gridDim.x - 1 - P.B * segs) / (gridDim.x - P.B * segs)) : 1;
+    // (quota such that there are CTAs enough), and u counts parts.  Otherwise the line is cut into equal parts (the first `extra` have a
+    // unit more), in which a segment counts kOpen units more than its blocks, ahead of them: what a CTA spends on a segment besides.
+    const uint32_t nc = min(gridDim.x, max(U, 1u)), share = U / nc, extra = U - share * nc;
+    auto unit_of_cta = [&](uint32_t c) { return share * c + min(c, extra); };
+    const uint32_t spare = gridDim.x - (uint32_t)(B * segs);                          // aligned: CTAs beyond one for each segment
+    const int quota = P.aligned ? (int)((U + spare - 1u) / spare) : 1;
     auto units_of = [&](int nblk) { return P.aligned ? (nblk + quota - 1) / quota : units_open(nblk); };     // of one segment
-    const int64_t u0 = P.aligned ? (int64_t)blockIdx.x : blockIdx.x * U / nc;
-    const int64_t u1 = P.aligned ? u0 + 1 : (blockIdx.x + 1) * U / nc;
-    if (u0 >= u1) return;
+    const uint32_t u0 = P.aligned ? blockIdx.x : unit_of_cta(blockIdx.x);
+    const uint32_t u1 = P.aligned ? u0 + 1u : unit_of_cta(blockIdx.x + 1u);
 
     // ---- the sequence that holds unit u0
-    int64_t b = -1, base = 0;
-    int len = 0, nb = 0, per_seg = 0;
-    for (int64_t b0 = 0; b0 < P.B; b0 += 32) {
-        const int my_len = b0 + lane < P.B ? seq_len(P, b0 + lane) : 0;
-        const int64_t mine = (int64_t)units_of(blocks_of(my_len)) * segs;
-        int64_t cum = mine;
+    int b = -1, len = 0, nb = 0, per_seg = 0;
+    uint32_t base = 0;
+    if (blockIdx.x < nc || P.aligned)
+        for (int b0 = 0; b0 < B; b0 += 32) {
+            const int my_len = b0 == 0 ? first_len : b0 + lane < B ? seq_len(P, b0 + lane) : 0;
+            const uint32_t units = (uint32_t)(units_of(blocks_of(my_len)) * segs);
+            uint32_t cum = units;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, cum, o);
-            if (lane >= o) cum += up;
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, cum, o);
+                if (lane >= o) cum += up;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, base + cum > u0);
+            if (past != 0u) {
+                const int l = __ffs(past) - 1;
+                b = b0 + l;
+                len = __shfl_sync(0xffffffffu, my_len, l);
+                base += __shfl_sync(0xffffffffu, cum - units, l);
+                break;
+            }
+            base += __shfl_sync(0xffffffffu, cum, 31);
         }
-        const unsigned past = __ballot_sync(0xffffffffu, base + cum > u0);
-        if (past != 0u) {
-            const int l = __ffs(past) - 1;
-            b = b0 + l;
-            len = __shfl_sync(0xffffffffu, my_len, l);
-            base += __shfl_sync(0xffffffffu, cum - mine, l);
-            break;
-        }
-        base += __shfl_sync(0xffffffffu, cum, 31);
-    }
-    if (b < 0) return;                                 // aligned: more CTAs than parts
+    // sequences without keys: their rows are zero
+    auto zero_rows = [&]() {
+        for (int s = blockIdx.x; s < B; s += gridDim.x)
+            if (seq_len(P, s) == 0) {
+                uint32_t* o = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(P.out) + (int64_t)s * P.T * P.H * D);
+                for (int i = tid; i < P.T * P.H * D / 2; i += kThreads) o[i] = 0u;
+            }
+    };
+    if (U == 0u || b < 0) { zero_rows(); return; }     // nothing to do, or (aligned) more CTAs than parts
     nb = blocks_of(len);
     per_seg = units_of(nb);
 
-    // ---- a piece: the blocks [blk0, blk1) of one segment
-    int64_t u = u0, seg0 = 0;                          // seg0: the segment's first unit
-    int seg = 0, blk0 = 0, blk1 = 0;
-    auto piece_at = [&](int64_t at) {
-        const unsigned local = (unsigned)(at - base);
-        seg = (int)(local / (unsigned)per_seg);
-        const int part = (int)(local - (unsigned)seg * (unsigned)per_seg);
-        seg0 = at - part;
+    // ---- a piece: the blocks [blk0, blk1) of one segment.  Where the CTA stands in its list is needed between pieces only: it waits in
+    // shared memory (every warp has its own), the registers are for the product.
+    Piece* place = reinterpret_cast<Piece*>(smem + C::kPlaceOff) + warp * 2;
+    Sched* sched = reinterpret_cast<Sched*>(smem + C::kSchedOff) + warp;
+    auto piece_at = [&](Piece& p, uint32_t at, uint32_t end) {
+        const uint32_t local = at - p.base;
+        p.u = at;
+        p.seg = (int)(local / (uint32_t)p.per_seg);
+        const int part = (int)(local - (uint32_t)p.seg * (uint32_t)p.per_seg);
+        p.seg0 = at - (uint32_t)part;
         if (P.aligned) {
-            blk0 = (int)((int64_t)part * nb / per_seg);
-            blk1 = (int)((int64_t)(part + 1) * nb / per_seg);
+            const int each = p.nb / p.per_seg, more = p.nb - each * p.per_seg;
+            p.blk0 = each * part + min(part, more);
+            p.blk1 = p.blk0 + each + (part < more ? 1 : 0);
         } else {
-            blk0 = max(part - kOpen, 0);
-            blk1 = (int)min((int64_t)nb, u1 - seg0 - kOpen);           // may be 0 or less: nothing but the opening
+            p.blk0 = max(part - kOpen, 0);
+            p.blk1 = min(p.nb, (int)(end - p.seg0) - kOpen);           // may be 0 or less: nothing but the opening
         }
     };
-    piece_at(u);
-    if (blk1 <= blk0) return;
+    int b_now, seg_now, len_now, blk0, blk1;
+    {
+        Piece p;
+        p.base = base; p.b = b; p.len = len; p.nb = blocks_of(len); p.per_seg = units_of(p.nb);
+        piece_at(p, u0, u1);
+        if (p.blk1 <= p.blk0) { zero_rows(); return; }
+        b_now = p.b; seg_now = p.seg; len_now = p.len; blk0 = p.blk0; blk1 = p.blk1;
+        if (lane == 0) { place[0] = p; *sched = Sched{u0, u1, share, extra, quota}; }
+    }
 
     // ---- this warp's stages of the piece: stage i holds `per` blocks from first(i) on; few blocks: one to a stage
     uint32_t it = 0;                                   // stages this warp has taken from its ring, ever
     int per = 1, mine = 0;
+    const int32_t* table_row = nullptr;
+    const unsigned char* head_pages = nullptr;
     auto first_of = [&](int i) { return blk0 + (warp + i * kWarps) * per; };
     auto issue = [&](int i, uint32_t at) {
         const uint32_t s = at % kSlots;
         const int blk = first_of(i) + lane;
-        int64_t page = -1;
-        int in_page = 0;
+        int page = -1, in_page = 0;
         if (lane < per && blk < blk1) {
             const int row = P.bpp_mul == 0u ? blk : (int)(__umulhi((uint32_t)blk, P.bpp_mul) >> P.bpp_shift);
             in_page = blk - row * P.c.blocks_per_page;
-            page = P.c.table[b * P.c.table_stride + row];
+            page = table_row[row];
             if (page < 0 || page >= P.c.n_pages) { page = -1; atomicExch(&g_kv4_attn_status, kKv4BadPage); }
         }
         const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
@@ -271,23 +289,26 @@ kv4_attention_kernel(const AttnParams P) {
         }
         __syncwarp();
         if (page >= 0) {
-            const unsigned char* src = P.c.pages + ((page * kv_heads + seg % kv_heads) * P.c.blocks_per_page + in_page) * L::kBytes;
+            const unsigned char* src = head_pages + ((int64_t)page * kv_heads * P.c.blocks_per_page + in_page) * L::kBytes;
             asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                          ::"r"(ring_u32 + s * C::kSlotBytes + lane * L::kBytes), "l"(src), "r"((uint32_t)L::kBytes), "r"(bar) : "memory");
         }
     };
-    auto begin_piece = [&]() {                         // the first stages of a piece are on their way before anything else
+    auto begin_piece = [&](int b, int seg) {           // the first stages of a piece are on their way before anything else
         const int pieces = blk1 - blk0;
-        per = pieces > kWarps ? kStageBlocks : 1;
+        per = pieces > 2 * kWarps ? kStageBlocks : 1;
         const int nstage = (pieces + per - 1) / per;
         mine = warp < nstage ? (nstage - 1 - warp) / kWarps + 1 : 0;
+        table_row = P.c.table + (int64_t)b * P.c.table_stride;
+        head_pages = P.c.pages + (int64_t)(seg % kv_heads) * P.c.blocks_per_page * L::kBytes;
         for (int i = 0; i < kSlots && i < mine; ++i) issue(i, it + i);
     };
-    begin_piece();
+    __syncthreads();                                   // barriers are there
+    begin_piece(b_now, seg_now);
+    zero_rows();
 
-    for (;;) {
-        const int kvh = seg % kv_heads, row0 = (seg / kv_heads) * kRows;
-        const bool whole = blk0 == 0 && blk1 == nb;
+    for (int bank = 0;; bank ^= 1) {
+        const int row0 = seg_now / kv_heads * kRows, len = len_now;
 
         // ---- query rows: fp16 fragments, their scales, sums and limits
         uint32_t qf[NT][KW * 4];
@@ -298,7 +319,7 @@ kv4_attention_kernel(const AttnParams P) {
             const int r = row0 + n * 8 + g;
             const bool live = r < P.R;
             const int rt = live ? r / P.G : 0, rg = live ? r % P.G : 0;
-            const T* src = reinterpret_cast<const T*>(P.q) + b * P.q_b + rt * P.q_t + (int64_t)(kvh * P.G + rg) * P.q_h;
+            const T* src = reinterpret_cast<const T*>(P.q) + (int64_t)b_now * P.q_b + rt * P.q_t + (int64_t)(seg_now % kv_heads * P.G + rg) * P.q_h;
             float x[KW][8], mx = 0.f;
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
@@ -560,21 +581,28 @@ kv4_attention_kernel(const AttnParams P) {
         }
         it += mine;
 
-        // ---- the next piece's copies start; it is finished with the values of this one kept aside
-        const int64_t this_b = b, this_u = u, this_seg0 = seg0, this_base_seg = b * segs + seg;
-        const int this_per = per_seg;
-        u = P.aligned ? u1 : seg0 + kOpen + blk1;
-        const bool more = u < u1;
+        // ---- the next piece's copies start
+        const bool whole = blk0 == 0 && blk1 == place[bank].nb;
         bool begun = false;
-        if (more && misc[0] == 0) {
-            while (u >= base + (int64_t)per_seg * segs) {
-                base += (int64_t)per_seg * segs;
-                if (++b >= P.B) break;                 // only if lengths changed while the kernel ran
-                len = seq_len(P, b);
-                nb = blocks_of(len);
-                per_seg = units_of(nb);
+        if (misc[0] == 0) {
+            Piece p = place[bank];
+            const uint32_t end = sched->u1, u = P.aligned ? end : p.seg0 + (uint32_t)(kOpen + blk1);
+            if (u < end) {
+                while (u >= p.base + (uint32_t)(p.per_seg * segs)) {
+                    p.base += (uint32_t)(p.per_seg * segs);
+                    if (++p.b >= B) break;             // only if lengths changed while the kernel ran
+                    p.len = seq_len(P, p.b);
+                    p.nb = blocks_of(p.len);
+                    p.per_seg = units_open(p.nb);
+                }
+                if (p.b < B && end - u > kOpen) {
+                    piece_at(p, u, end);
+                    b_now = p.b; seg_now = p.seg; len_now = p.len; blk0 = p.blk0; blk1 = p.blk1;
+                    if (lane == 0) place[bank ^ 1] = p;
+                    begin_piece(b_now, seg_now);
+                    begun = true;
+                }
             }
-            if (b < P.B && u1 - u > kOpen) { piece_at(u); begin_piece(); begun = true; }
         }
 
         // ---- the warps' results meet: value = o * 2^24 (2^20) / cmul + z
@@ -616,45 +644,51 @@ kv4_attention_kernel(const AttnParams P) {
                 for (int i = 0; i < kSlots && i < mine; ++i) mbar_wait(bars + 8 * ((it + i) % kSlots), ((it + i) / kSlots) & 1);
             return;
         }
-        auto store = [&](int row, int d, float4 v, float l) {           // four neighbouring values of a finished row
+        const Piece& now = place[bank];
+        auto store = [&](int row, int d, auto& v, float l) {            // neighbouring values of a finished row
+            constexpr int N = sizeof(v) / sizeof(float);
             const int r = row0 + row;
             if (r >= P.R) return;
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-            T* dst = reinterpret_cast<T*>(P.out) + ((this_b * P.T + r / P.G) * P.H + kvh * P.G + r % P.G) * D + d;
-            const T y[4] = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv), from_f32<T>(v.w * inv)};
-            *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+            T y[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = from_f32<T>(l == 0.f ? 0.f : v[i] * inv);
+            T* dst = reinterpret_cast<T*>(P.out) + (((int64_t)now.b * P.T + r / P.G) * P.H + now.seg % kv_heads * P.G + r % P.G) * D + d;
+            if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+            else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(y);
         };
-        float* my_part = P.partial + ((int64_t)blockIdx.x * 2 + (this_u == u0 ? 0 : 1)) * C::kPartFloats;
+        float* my_part = P.partial + ((int64_t)blockIdx.x * 2 + (now.u == sched->u0 ? 0 : 1)) * C::kPartFloats;
         for (int idx = tid; idx < kRows * D / 4; idx += kThreads) {
             const int row = idx / (D / 4), d = idx % (D / 4) * 4;
             float mw[kWarps], m = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) { mw[w] = st_max[w * kRows + row]; m = fmaxf(m, mw[w]); }
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
             float l = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 if (mw[w] == -INFINITY) continue;
                 const float f = ex2(mw[w] - m);
                 const float4 a = *reinterpret_cast<const float4*>(merge + ((size_t)w * kRows + row) * D + d);
-                v.x = fmaf(f, a.x, v.x); v.y = fmaf(f, a.y, v.y); v.z = fmaf(f, a.z, v.z); v.w = fmaf(f, a.w, v.w);
+                v[0] = fmaf(f, a.x, v[0]); v[1] = fmaf(f, a.y, v[1]); v[2] = fmaf(f, a.z, v[2]); v[3] = fmaf(f, a.w, v[3]);
                 l = fmaf(f, st_sum[w * kRows + row], l);
             }
             if (whole) store(row, d, v, l);
             else {
-                *reinterpret_cast<float4*>(my_part + row * D + d) = v;
+                *reinterpret_cast<float4*>(my_part + row * D + d) = make_float4(v[0], v[1], v[2], v[3]);
                 if (d == 0) { my_part[kRows * D + row] = m; my_part[kRows * D + kRows + row] = l; }
             }
         }
         if (!whole) {
-            __threadfence();
+            // CTAs that hold the segment's first and last block: c0 .. c0 + n - 1
+            const uint32_t share = sched->share, extra = sched->extra;
+            auto cta_of_unit = [&](uint32_t u) { return u < extra * (share + 1u) ? u / (share + 1u) : extra + (u - extra * (share + 1u)) / share; };
+            const uint32_t c0 = P.aligned ? now.seg0 : cta_of_unit(now.seg0 + kOpen);
+            const int n = P.aligned ? now.per_seg : (int)(cta_of_unit(now.seg0 + (uint32_t)now.per_seg - 1u) - c0) + 1;
             __syncthreads();
-            // CTAs that hold the segment's first and last unit
-            const int64_t c0 = P.aligned ? this_seg0 : ((this_seg0 + kOpen + 1) * nc - 1) / U;
-            const int n = P.aligned ? this_per : (int)(((this_seg0 + this_per) * nc - 1) / U - c0) + 1;
             if (tid == 0) {
-                int* counter = P.counters + this_base_seg;
+                int* counter = P.counters + ((int64_t)now.b * segs + now.seg);
+                __threadfence();                                        // the CTA's part, ordered before by the barrier, is visible to who sees the count
                 const bool last = atomicAdd(counter, 1) == n - 1;
                 if (last) *counter = 0;
                 __threadfence();
@@ -662,39 +696,52 @@ kv4_attention_kernel(const AttnParams P) {
             }
             __syncthreads();
             if (misc[1] != 0) {
-                // parts lie at c0 (its second one, if the segment does not begin with that CTA), c0 + 1, ...: their weights first
-                const int64_t off0 = (c0 * 2 + (P.aligned || c0 * U / nc >= this_seg0 ? 0 : 1)) * C::kPartFloats;
-                auto part = [&](int c) { return P.partial + (c == 0 ? off0 : (c0 + c) * 2 * C::kPartFloats); };
-                float* weight = merge;                                  // [kRows][n]
+                // Parts lie at c0 (its second one, if the segment does not begin with that CTA), c0 + 1, ...  A warp takes a row, a lane
+                // 4 values of it (2 at D = 64).
+                const int64_t off0 = ((int64_t)c0 * 2 + (P.aligned || share * c0 + min(c0, extra) >= now.seg0 ? 0 : 1)) * C::kPartFloats;
+                auto part = [&](int c) { return P.partial + (c == 0 ? off0 : (int64_t)(c0 + c) * 2 * C::kPartFloats); };
+                constexpr int kV = D / 32;
                 for (int row = warp; row < kRows; row += kWarps) {
+                    float* weight = merge + row * n;
                     float m = -INFINITY, l = 0.f;
-                    for (int c = lane; c < n; c += 32) {
-                        const float pm = __ldcg(part(c) + kRows * D + row);
-                        weight[row * n + c] = pm;
-                        m = fmaxf(m, pm);
-                    }
+                    for (int c = lane; c < n; c += 32) m = fmaxf(m, __ldcg(part(c) + kRows * D + row));
 #pragma unroll
                     for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
                     for (int c = lane; c < n; c += 32) {
-                        const float pm = weight[row * n + c], f = pm == -INFINITY ? 0.f : ex2(pm - m);
-                        weight[row * n + c] = f;
-                        if (f != 0.f) l = fmaf(f, __ldcg(part(c) + kRows * D + kRows + row), l);
+                        const float pm = __ldcg(part(c) + kRows * D + row), pl = __ldcg(part(c) + kRows * D + kRows + row);
+                        const float f = pm == -INFINITY ? 0.f : ex2(pm - m);
+                        weight[c] = f;
+                        if (f != 0.f) l = fmaf(f, pl, l);
                     }
 #pragma unroll
                     for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
-                    if (lane == 0) st_sum[row] = l;
-                }
-                __syncthreads();
-                for (int idx = tid; idx < kRows * D / 4; idx += kThreads) {
-                    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int c = 0; c < n; ++c) {
-                        const float f = weight[row * n + c];
-                        const float4 a = __ldcg(reinterpret_cast<const float4*>(part(c) + row * D + d));
-                        v.x = fmaf(f, a.x, v.x); v.y = fmaf(f, a.y, v.y); v.z = fmaf(f, a.z, v.z); v.w = fmaf(f, a.w, v.w);
+                    __syncwarp();
+                    float v[kV];
+#pragma unroll
+                    for (int i = 0; i < kV; ++i) v[i] = 0.f;
+                    for (int c = 0; c < n; c += 8) {
+                        float a[8][kV];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (c + k < n) {
+                                const float* src = part(c + k) + row * D + lane * kV;
+                                if constexpr (kV == 4) {
+                                    const float4 q4 = __ldcg(reinterpret_cast<const float4*>(src));
+                                    a[k][0] = q4.x; a[k][1] = q4.y; a[k][2] = q4.z; a[k][3] = q4.w;
+                                } else {
+                                    const float2 q2 = __ldcg(reinterpret_cast<const float2*>(src));
+                                    a[k][0] = q2.x; a[k][1] = q2.y;
+                                }
+                            }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (c + k < n) {
+                                const float f = weight[c + k];
+#pragma unroll
+                                for (int i = 0; i < kV; ++i) v[i] = fmaf(f, a[k][i], v[i]);
+                            }
                     }
-                    store(row, d, v, st_sum[row]);
+                    store(row, lane * kV, v, l);
                 }
             }
         }
@@ -714,8 +761,8 @@ int launch_attn_t(const AttnParams& P, int sms, cudaStream_t stream) {
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
     // a cut segment has at most one part on each CTA: their weights share the merge buffer
-    if (sms * C::kCtasPerSm > kWarps * D) { set_error("kv4_attention: more SMs than this kernel was laid out for"); return CB_ERR_UNSUPPORTED; }
-    kv4_attention_kernel<T, D, GS, NT><<<sms * C::kCtasPerSm, kThreads, C::kSmem, stream>>>(P);
+    if (sms > C::kWarps * D) { set_error("kv4_attention: more SMs than this kernel was laid out for"); return CB_ERR_UNSUPPORTED; }
+    kv4_attention_kernel<T, D, GS, NT><<<sms, C::kThreads, C::kSmem, stream>>>(P);
     CB_CUDA_TRY(cudaGetLastError());
     return CB_OK;
 }
@@ -734,7 +781,7 @@ size_t kv4_attention_partial_bytes(int64_t rows, int head_dim) {
     const int sms = sm_count_current();
     if (sms <= 0) return 0;
     const int tile = attn_tile_rows(rows);
-    return (size_t)sms * (tile == 8 ? 2 : 1) * 2 * tile * (head_dim + 2) * sizeof(float);
+    return (size_t)sms * 2 * tile * (head_dim + 2) * sizeof(float);
 }
 
 // Arguments are checked by the caller.
@@ -763,7 +810,7 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     if (sms <= 0) return CB_ERR_CUDA;
     // Few segments: parts that end with their segment, so that each CTA goes through the chain of copy, product and join once; the parts are
     // then up to a quarter longer.  Many: equal parts.
-    P.aligned = 4 * B * c->kv_heads * P.row_tiles <= (int64_t)sms * (tile == 8 ? 2 : 1);
+    P.aligned = 4 * B * c->kv_heads * P.row_tiles <= sms;
     const bool bf = c->dtype == CB_BF16;
 #define CB_KV4_NT(d, gs, nt) (bf ? launch_attn_t<__nv_bfloat16, d, gs, nt>(P, sms, stream) : launch_attn_t<__half, d, gs, nt>(P, sms, stream))
 #define CB_KV4_CASE(d, gs) \
