@@ -104,7 +104,7 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
     CB_REQUIRE(T < (1 << 24) && H < (1 << 20) && T * H * cache->head_dim < (1ll << 31), "%s: T * H out of range", who);
     const int64_t segs = cb_kv4_attention_counters(B, T, H, cache->kv_heads);
     // the kernel numbers blocks, and a few more for each segment, with 32 bits
-    CB_REQUIRE(segs < (1ll << 26) && (table_stride * (cache->page_size / kKvBlock) + 64) < (1ll << 31) / segs,
+    CB_REQUIRE(segs < (1ll << 26) && (table_stride * (cache->page_size / kKvBlock) + 256) < (1ll << 31) / segs,
                "%s: too many rows and pages", who);
     CB_REQUIRE(q && out && lengths && strides3 && (page_table || table_stride == 0), "%s: NULL pointer", who);
     CB_REQUIRE(aligned16(q) && aligned16(out), "%s: q and out must be 16-byte aligned", who);

@@ -44,6 +44,7 @@ struct AttnParams {
     int64_t B;
     int T, H, G, R, row_tiles;
     bool aligned;                                     // no CTA's part crosses a segment's end
+    int solo;                                         // segments of up to this many blocks are taken by single warps
     float scale_log2;                                 // |softmax scale| * log2(e), above 0
     float q_sign;                                     // 1, or -1 where the scale is negative
     uint32_t zero;                                    // 0, unknown to the compiler
@@ -55,10 +56,10 @@ struct AttnParams {
 // Where a CTA stands: segment `seg` of sequence b (len tokens, nb blocks, per_seg units a segment; base: the sequence's first unit, seg0: the
 // segment's), and its blocks of this CTA.
 struct Piece {
-    uint32_t u, seg0, base;
+    uint32_t u, seg0, base, next;                     // next: where the following piece is looked for
     int per_seg, b, seg, nb, len, blk0, blk1;
 };
-struct Sched { uint32_t u0, u1, share, extra; int quota; };
+struct Sched { uint32_t u0, u1, share, extra; };
 
 template <int D, int GS, int NT>
 struct AttnCfg {
@@ -157,8 +158,7 @@ __device__ __forceinline__ int blocks_of(int len) { return (int)(((unsigned)len 
 
 constexpr float kLag = 8.f;
 
-constexpr int kOpen = 12;
-__device__ __forceinline__ int units_open(int nblk) { return nblk == 0 ? 0 : nblk + kOpen; }
+constexpr int kOpen = 40;
 
 template <typename T, int D, int GS, int NT>
 __global__ void __launch_bounds__((AttnCfg<D, GS, NT>::kThreads), 1)
@@ -187,17 +187,23 @@ kv4_attention_kernel(const AttnParams P) {
 
     // ---- the line's length, every warp for itself.  The caller has checked that units fit 32 bits.
     const int B = (int)P.B, first_len = lane < B ? seq_len(P, lane) : 0;              // of sequence `lane`: all there are with up to 32
-    uint32_t U = P.aligned ? blocks_of(first_len) : units_open(blocks_of(first_len));
-    for (int s = lane + 32; s < B; s += 32) U += P.aligned ? blocks_of(seq_len(P, s)) : units_open(blocks_of(seq_len(P, s)));
-    U = __reduce_add_sync(0xffffffffu, U) * (uint32_t)segs;
-    // ---- this CTA's part [u0, u1) of the line.  aligned: a segment of nb blocks is cut into ceil(nb / quota) parts, one to a CTA
-    // (quota such that there are CTAs enough), and u counts parts.  Otherwise the line is cut into equal parts (the first `extra` have a
-    // unit more), in which a segment counts kOpen units more than its blocks, ahead of them: what a CTA spends on a segment besides.
+    // Units of a sequence's segments and how many of these there are.  aligned: a segment of nb blocks is cut into ceil(nb / quota) parts,
+    // one to a CTA (quota such that there are CTAs enough), and u counts parts (before quota is known: blocks).  Otherwise the line is cut
+    // into equal parts, in which a segment counts kOpen units more than its blocks, ahead of them: what a CTA spends on a segment besides.
+    // Short segments (solo) go to single warps, kWarps of them together as one segment that belongs to the CTA in whose part it begins.
+    const int groups = (segs + kWarps - 1) / kWarps;
+    int quota = 1;
+    auto is_solo = [&](int nblk) { return nblk <= P.solo; };
+    auto segs_of = [&](int nblk) { return is_solo(nblk) ? groups : segs; };
+    auto units_of = [&](int nblk) { return P.aligned ? (nblk + quota - 1) / quota : nblk == 0 ? 0 : is_solo(nblk) ? kOpen + nblk * kWarps : kOpen + nblk; };
+    uint32_t U = (uint32_t)(units_of(blocks_of(first_len)) * segs_of(blocks_of(first_len)));
+    for (int s = lane + 32; s < B; s += 32) { const int n = blocks_of(seq_len(P, s)); U += (uint32_t)(units_of(n) * segs_of(n)); }
+    U = __reduce_add_sync(0xffffffffu, U);
+    // ---- this CTA's part [u0, u1) of the line (the first `extra` parts have a unit more)
     const uint32_t nc = min(gridDim.x, max(U, 1u)), share = U / nc, extra = U - share * nc;
     auto unit_of_cta = [&](uint32_t c) { return share * c + min(c, extra); };
     const uint32_t spare = gridDim.x - (uint32_t)(B * segs);                          // aligned: CTAs beyond one for each segment
-    const int quota = P.aligned ? (int)((U + spare - 1u) / spare) : 1;
-    auto units_of = [&](int nblk) { return P.aligned ? (nblk + quota - 1) / quota : units_open(nblk); };     // of one segment
+    if (P.aligned) quota = (int)((U + spare - 1u) / spare);
     const uint32_t u0 = P.aligned ? blockIdx.x : unit_of_cta(blockIdx.x);
     const uint32_t u1 = P.aligned ? u0 + 1u : unit_of_cta(blockIdx.x + 1u);
 
@@ -207,7 +213,7 @@ kv4_attention_kernel(const AttnParams P) {
     if (blockIdx.x < nc || P.aligned)
         for (int b0 = 0; b0 < B; b0 += 32) {
             const int my_len = b0 == 0 ? first_len : b0 + lane < B ? seq_len(P, b0 + lane) : 0;
-            const uint32_t units = (uint32_t)(units_of(blocks_of(my_len)) * segs);
+            const uint32_t units = (uint32_t)(units_of(blocks_of(my_len)) * segs_of(blocks_of(my_len)));
             uint32_t cum = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -240,29 +246,58 @@ kv4_attention_kernel(const AttnParams P) {
     // shared memory (every warp has its own), the registers are for the product.
     Piece* place = reinterpret_cast<Piece*>(smem + C::kPlaceOff) + warp * 2;
     Sched* sched = reinterpret_cast<Sched*>(smem + C::kSchedOff) + warp;
+    // The piece that begins at unit `at` or behind it, before `end`; false where there is none.  p: a sequence, `at` not before it.
     auto piece_at = [&](Piece& p, uint32_t at, uint32_t end) {
-        const uint32_t local = at - p.base;
-        p.u = at;
-        p.seg = (int)(local / (uint32_t)p.per_seg);
-        const int part = (int)(local - (uint32_t)p.seg * (uint32_t)p.per_seg);
-        p.seg0 = at - (uint32_t)part;
-        if (P.aligned) {
-            const int each = p.nb / p.per_seg, more = p.nb - each * p.per_seg;
-            p.blk0 = each * part + min(part, more);
-            p.blk1 = p.blk0 + each + (part < more ? 1 : 0);
-        } else {
+        for (;;) {
+            while (at >= p.base + (uint32_t)(p.per_seg * segs_of(p.nb))) {
+                p.base += (uint32_t)(p.per_seg * segs_of(p.nb));
+                if (++p.b >= B) return false;
+                p.len = seq_len(P, p.b);
+                p.nb = blocks_of(p.len);
+                p.per_seg = units_of(p.nb);
+            }
+            if (at >= end) return false;
+            const uint32_t local = at - p.base;
+            p.u = at;
+            p.seg = (int)(local / (uint32_t)p.per_seg);
+            const int part = (int)(local - (uint32_t)p.seg * (uint32_t)p.per_seg);
+            p.seg0 = at - (uint32_t)part;
+            p.next = p.seg0 + (uint32_t)p.per_seg;
+            if (P.aligned) {
+                const int each = p.nb / p.per_seg, more = p.nb - each * p.per_seg;
+                p.blk0 = each * part + min(part, more);
+                p.blk1 = p.blk0 + each + (part < more ? 1 : 0);
+                p.next = end;
+                return true;
+            }
+            if (is_solo(p.nb)) {
+                p.blk0 = 0; p.blk1 = p.nb;
+                if (part == 0) return true;
+                at = p.next;                           // begun, and finished, by an earlier CTA
+                continue;
+            }
             p.blk0 = max(part - kOpen, 0);
-            p.blk1 = min(p.nb, (int)(end - p.seg0) - kOpen);           // may be 0 or less: nothing but the opening
+            p.blk1 = min(p.nb, (int)(end - p.seg0) - kOpen);
+            return p.blk1 > p.blk0;                    // else nothing but the opening
         }
     };
     int b_now, seg_now, len_now, blk0, blk1;
+    bool solo;                                         // this warp has the segment to itself
+    auto enter = [&](const Piece& p) {
+        solo = !P.aligned && is_solo(p.nb);
+        b_now = p.b; len_now = p.len; blk0 = p.blk0; blk1 = p.blk1;
+        seg_now = p.seg;
+        if (solo) {
+            seg_now = p.seg * kWarps + warp;
+            if (seg_now >= segs) { seg_now = 0; blk1 = 0; }            // nothing for this warp
+        }
+    };
     {
         Piece p;
         p.base = base; p.b = b; p.len = len; p.nb = blocks_of(len); p.per_seg = units_of(p.nb);
-        piece_at(p, u0, u1);
-        if (p.blk1 <= p.blk0) { zero_rows(); return; }
-        b_now = p.b; seg_now = p.seg; len_now = p.len; blk0 = p.blk0; blk1 = p.blk1;
-        if (lane == 0) { place[0] = p; *sched = Sched{u0, u1, share, extra, quota}; }
+        if (!piece_at(p, u0, u1)) { zero_rows(); return; }
+        enter(p);
+        if (lane == 0) { place[0] = p; *sched = Sched{u0, u1, share, extra}; }
     }
 
     // ---- this warp's stages of the piece: stage i holds `per` blocks from first(i) on; few blocks: one to a stage
@@ -270,7 +305,7 @@ kv4_attention_kernel(const AttnParams P) {
     int per = 1, mine = 0;
     const int32_t* table_row = nullptr;
     const unsigned char* head_pages = nullptr;
-    auto first_of = [&](int i) { return blk0 + (warp + i * kWarps) * per; };
+    auto first_of = [&](int i) { return blk0 + (solo ? i : warp + i * kWarps) * per; };
     auto issue = [&](int i, uint32_t at) {
         const uint32_t s = at % kSlots;
         const int blk = first_of(i) + lane;
@@ -296,9 +331,9 @@ kv4_attention_kernel(const AttnParams P) {
     };
     auto begin_piece = [&](int b, int seg) {           // the first stages of a piece are on their way before anything else
         const int pieces = blk1 - blk0;
-        per = pieces > 2 * kWarps ? kStageBlocks : 1;
+        per = solo || pieces > 2 * kWarps ? kStageBlocks : 1;
         const int nstage = (pieces + per - 1) / per;
-        mine = warp < nstage ? (nstage - 1 - warp) / kWarps + 1 : 0;
+        mine = solo ? nstage : warp < nstage ? (nstage - 1 - warp) / kWarps + 1 : 0;
         table_row = P.c.table + (int64_t)b * P.c.table_stride;
         head_pages = P.c.pages + (int64_t)(seg % kv_heads) * P.c.blocks_per_page * L::kBytes;
         for (int i = 0; i < kSlots && i < mine; ++i) issue(i, it + i);
@@ -582,26 +617,16 @@ kv4_attention_kernel(const AttnParams P) {
         it += mine;
 
         // ---- the next piece's copies start
-        const bool whole = blk0 == 0 && blk1 == place[bank].nb;
+        const bool alone = solo, idle = solo && blk1 == 0, whole = blk0 == 0 && blk1 == place[bank].nb;
+        const int64_t first_row = (int64_t)b_now * P.T * P.H + seg_now % kv_heads * P.G;      // of the output, in rows of D: row r is T's r / G, head r % G
         bool begun = false;
         if (misc[0] == 0) {
             Piece p = place[bank];
-            const uint32_t end = sched->u1, u = P.aligned ? end : p.seg0 + (uint32_t)(kOpen + blk1);
-            if (u < end) {
-                while (u >= p.base + (uint32_t)(p.per_seg * segs)) {
-                    p.base += (uint32_t)(p.per_seg * segs);
-                    if (++p.b >= B) break;             // only if lengths changed while the kernel ran
-                    p.len = seq_len(P, p.b);
-                    p.nb = blocks_of(p.len);
-                    p.per_seg = units_open(p.nb);
-                }
-                if (p.b < B && end - u > kOpen) {
-                    piece_at(p, u, end);
-                    b_now = p.b; seg_now = p.seg; len_now = p.len; blk0 = p.blk0; blk1 = p.blk1;
-                    if (lane == 0) place[bank ^ 1] = p;
-                    begin_piece(b_now, seg_now);
-                    begun = true;
-                }
+            if (piece_at(p, p.next, sched->u1)) {
+                enter(p);
+                if (lane == 0) place[bank ^ 1] = p;
+                begin_piece(b_now, seg_now);
+                begun = true;
             }
         }
 
@@ -638,7 +663,7 @@ kv4_attention_kernel(const AttnParams P) {
                 }
             }
         }
-        __syncthreads();
+        if (!alone) __syncthreads(); else __syncwarp();
         if (misc[0] != 0) {                                             // a copy was not heard of: wait (bounded) for the others in flight
             if (begun)
                 for (int i = 0; i < kSlots && i < mine; ++i) mbar_wait(bars + 8 * ((it + i) % kSlots), ((it + i) / kSlots) & 1);
@@ -653,10 +678,22 @@ kv4_attention_kernel(const AttnParams P) {
             T y[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) y[i] = from_f32<T>(l == 0.f ? 0.f : v[i] * inv);
-            T* dst = reinterpret_cast<T*>(P.out) + (((int64_t)now.b * P.T + r / P.G) * P.H + now.seg % kv_heads * P.G + r % P.G) * D + d;
+            T* dst = reinterpret_cast<T*>(P.out) + (first_row + (int64_t)(r / P.G) * P.H + r % P.G) * D + d;
             if constexpr (N == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
             else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(y);
         };
+        if (alone) {                                                    // this warp's rows are finished
+            if (!idle)
+                for (int idx = lane; idx < kRows * D / 4; idx += 32) {
+                    const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+                    const float4 a = *reinterpret_cast<const float4*>(merge + ((size_t)warp * kRows + row) * D + d);
+                    float v[4] = {a.x, a.y, a.z, a.w};
+                    store(row, d, v, st_sum[warp * kRows + row]);
+                }
+            if (!begun) return;
+            __syncwarp();
+            continue;
+        }
         float* my_part = P.partial + ((int64_t)blockIdx.x * 2 + (now.u == sched->u0 ? 0 : 1)) * C::kPartFloats;
         for (int idx = tid; idx < kRows * D / 4; idx += kThreads) {
             const int row = idx / (D / 4), d = idx % (D / 4) * 4;
@@ -811,6 +848,8 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     // Few segments: parts that end with their segment, so that each CTA goes through the chain of copy, product and join once; the parts are
     // then up to a quarter longer.  Many: equal parts.
     P.aligned = 4 * B * c->kv_heads * P.row_tiles <= sms;
+    // Segments enough to fill the SMs: the short ones (up to 128 tokens) one to a warp.
+    P.solo = !P.aligned && B * c->kv_heads * P.row_tiles >= sms ? 8 : 0;
     const bool bf = c->dtype == CB_BF16;
 #define CB_KV4_NT(d, gs, nt) (bf ? launch_attn_t<__nv_bfloat16, d, gs, nt>(P, sms, stream) : launch_attn_t<__half, d, gs, nt>(P, sms, stream))
 #define CB_KV4_CASE(d, gs) \
