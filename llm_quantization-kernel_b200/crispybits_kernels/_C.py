@@ -652,7 +652,10 @@ def kv4_block_bytes(head_dim: int, group_size: int) -> int:
 
 
 def _kv4_record(cache, who: str) -> _KV4Cache:
-    pages = cache.pages
+    """The library's record of a cache.  It is made and checked once, and kept by the cache it describes."""
+    pages, rec = cache.pages, cache.__dict__.get("_record")
+    if rec is not None and rec.pages == pages.data_ptr():
+        return rec
     if not pages.is_cuda or pages.dtype != torch.uint8 or pages.dim() != 3 or not pages.is_contiguous():
         _fail(f"{who}: the cache's pages must be a contiguous 3-D CUDA uint8 tensor")
     if cache.dtype not in (torch.float16, torch.bfloat16):
@@ -661,75 +664,90 @@ def _kv4_record(cache, who: str) -> _KV4Cache:
         _fail(f"{who}: pages do not fit the cache's head_dim, group_size and page_size")
     if pages.numel() == 0:
         _fail(f"{who}: the cache has no pages")
-    return _KV4Cache(pages.data_ptr(), pages.shape[0], pages.shape[1], cache.head_dim, cache.group_size, cache.page_size,
-                     _DTYPE[cache.dtype])
+    rec = _KV4Cache(pages.data_ptr(), pages.shape[0], pages.shape[1], cache.head_dim, cache.group_size, cache.page_size,
+                    _DTYPE[cache.dtype])
+    cache.__dict__["_record"] = rec
+    return rec
 
 
-def _check_index(t, device, shape, name: str, who: str):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device:
-        _fail(f"{who}: {name} must be an int32 tensor on the cache's device")
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        _fail(f"{who}: {name} must be contiguous of shape {list(shape)}")
+# The checks below are written for the call that is in order, which takes a few attribute reads; what is wrong with one that is not is
+# said by the function that follows.
+def _index_ok(t, device: int, n: int) -> bool:
+    return isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1)
 
 
-def _check_table(page_table, device, who: str):
-    if not isinstance(page_table, torch.Tensor) or page_table.dtype != torch.int32 or page_table.device != device:
+def _check_index(t, device: int, n: int, name: str, who: str):
+    if _index_ok(t, device, n):
+        return
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda or t.get_device() != device:
+        _fail(f"{who}: {name} must be an int32 tensor on the device of the others")
+    _fail(f"{who}: {name} must be contiguous of shape [{n}]")
+
+
+def _check_table(page_table, device: int, who: str):
+    if not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or page_table.get_device() != device:
         _fail(f"{who}: page_table must be an int32 tensor on the cache's device")
-    if page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        _fail(f"{who}: page_table must be [sequences, pages] with contiguous rows")
-    if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
-        _fail(f"{who}: page_table must be contiguous")
+    if page_table.dim() != 2 or not page_table.is_contiguous():
+        _fail(f"{who}: page_table must be contiguous [sequences, pages]")
 
 
 def _vector_rows(t: torch.Tensor) -> torch.Tensor:
     """`t` itself where every row of its last dimension is contiguous and 16-byte aligned, else a contiguous copy."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    *lead, last = t.stride()
+    for s in lead:
+        last |= (s & 7) << 1                       # 1 only if the last is 1 and the others are multiples of 8
+    if last == 1 and t.data_ptr() & 15 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def kv4_append(cache, k, v, page_table, starts, cu_seqlens):
     """k, v [tokens, kv_heads, head_dim] -> the cache's pages (struct cb_kv4_cache; cb_kv4_append)."""
-    rec, dev = _kv4_record(cache, "kv4_append"), cache.pages.device
+    rec, dev = _kv4_record(cache, "kv4_append"), cache.pages.get_device()
+    want = (rec.kv_heads, rec.head_dim)
     for t, name in ((k, "k"), (v, "v")):
-        if t.device != dev or t.dtype != cache.dtype:
+        if t.get_device() != dev or t.dtype is not cache.dtype:
             _fail(f"kv4_append: {name} must be of the cache's dtype, on its device")
-        if t.dim() != 3 or t.shape[1] != rec.kv_heads or t.shape[2] != rec.head_dim:
+        if t.dim() != 3 or t.shape[1:] != want:
             _fail(f"kv4_append: {name} must be [tokens, {rec.kv_heads}, {rec.head_dim}]")
-    if k.shape != v.shape:
+    n = k.shape[0]
+    if v.shape[0] != n:
         _fail("kv4_append: k and v must have the same shape")
     _check_table(page_table, dev, "kv4_append")
-    n, seqs = k.shape[0], page_table.shape[0]
-    _check_index(starts, dev, (seqs,), "starts", "kv4_append")
+    seqs, pages = page_table.shape
+    _check_index(starts, dev, seqs, "starts", "kv4_append")
     if cu_seqlens is not None:
-        _check_index(cu_seqlens, dev, (seqs + 1,), "cu_seqlens", "kv4_append")
+        _check_index(cu_seqlens, dev, seqs + 1, "cu_seqlens", "kv4_append")
     if n == 0:
         return
     k, v = _vector_rows(k), _vector_rows(v)
-    strides = (_i64 * 4)(k.stride(0), k.stride(1), v.stride(0), v.stride(1))
-    with _on_device(dev):
-        _rc(_lib.cb_kv4_append(ctypes.byref(rec), k.data_ptr(), v.data_ptr(), strides, n, page_table.data_ptr(),
-                               page_table.shape[1], seqs, starts.data_ptr(),
-                               0 if cu_seqlens is None else cu_seqlens.data_ptr(), _stream(k)))
+    strides = (_i64 * 4)(*k.stride()[:2], *v.stride()[:2])
+    with _on_device(k.device):
+        _rc(_lib.cb_kv4_append(rec, k.data_ptr(), v.data_ptr(), strides, n, page_table.data_ptr(), pages, seqs, starts.data_ptr(),
+                               None if cu_seqlens is None else cu_seqlens.data_ptr(), _raw_stream(dev)))
 
 
 def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
     """(k, v) [tokens, kv_heads, head_dim]: the values that the cache holds for the named tokens (cb_kv4_read)."""
-    rec, dev = _kv4_record(cache, "kv4_read"), cache.pages.device
+    rec, dev = _kv4_record(cache, "kv4_read"), cache.pages.get_device()
     _check_table(page_table, dev, "kv4_read")
-    n, seqs = int(n_tokens), page_table.shape[0]
+    seqs, pages = page_table.shape
+    n = int(n_tokens)
     if n < 0:
         _fail("kv4_read: n_tokens must not be negative")
-    _check_index(starts, dev, (seqs,), "starts", "kv4_read")
+    _check_index(starts, dev, seqs, "starts", "kv4_read")
     if cu_seqlens is not None:
-        _check_index(cu_seqlens, dev, (seqs + 1,), "cu_seqlens", "kv4_read")
-    k = torch.empty((n, rec.kv_heads, rec.head_dim), dtype=cache.dtype, device=dev)
-    v = torch.empty_like(k)
+        _check_index(cu_seqlens, dev, seqs + 1, "cu_seqlens", "kv4_read")
+    device = cache.pages.device
+    k = torch.empty((n, rec.kv_heads, rec.head_dim), dtype=cache.dtype, device=device)
+    v = torch.empty((n, rec.kv_heads, rec.head_dim), dtype=cache.dtype, device=device)
     if n:
-        with _on_device(dev):
-            _rc(_lib.cb_kv4_read(ctypes.byref(rec), k.data_ptr(), v.data_ptr(), n, page_table.data_ptr(),
-                                 page_table.shape[1], seqs, starts.data_ptr(),
-                                 0 if cu_seqlens is None else cu_seqlens.data_ptr(), _stream(k)))
+        with _on_device(device):
+            _rc(_lib.cb_kv4_read(rec, k.data_ptr(), v.data_ptr(), n, page_table.data_ptr(), pages, seqs, starts.data_ptr(),
+                                 None if cu_seqlens is None else cu_seqlens.data_ptr(), _raw_stream(dev)))
     return k, v
 
 
@@ -740,6 +758,7 @@ def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
 _kv4_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
 _kv4_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
 _KV4_SLAB = 1 << 18
+_partial_bytes: Dict[Tuple[int, bool, int], int] = {}      # (device index, more than 8 rows, head_dim) -> cb_kv4_attention_partial_bytes
 
 
 def kv4_prepare_device(device: torch.device):
@@ -752,47 +771,55 @@ def kv4_prepare_device(device: torch.device):
         _kv4_slab[index] = [slab, 0]
 
 
-def _kv4_scratch(dev, stream: int, counters: int, nbytes: int):
+def _kv4_scratch(device, dev: int, stream: int, counters: int, nbytes: int):
     if torch.cuda.is_current_stream_capturing():
-        partial = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        slab, need = _kv4_slab.get(dev.index), -(-counters // 32) * 32
+        partial = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        slab, need = _kv4_slab.get(dev), -(-counters // 32) * 32
         if slab is None or slab[1] + need > _KV4_SLAB:
-            return torch.zeros(counters, dtype=torch.int32, device=dev), partial
+            return torch.zeros(counters, dtype=torch.int32, device=device), partial
         slab[1] += need
         return slab[0][slab[1] - need:slab[1]], partial
-    have = _kv4_eager.get((dev.index, stream))
+    have = _kv4_eager.get((dev, stream))
     if have is None or have[0].numel() < counters or have[1].numel() < nbytes:
-        have = (torch.zeros(max(counters, 4096), dtype=torch.int32, device=dev),
-                torch.empty(nbytes, dtype=torch.uint8, device=dev))
-        _kv4_eager[(dev.index, stream)] = have
+        have = (torch.zeros(max(counters, 4096), dtype=torch.int32, device=device),
+                torch.empty(nbytes, dtype=torch.uint8, device=device))
+        _kv4_eager[(dev, stream)] = have
     return have
 
 
 def kv4_attention(q, cache, page_table, lengths, scale: float):
-    """q [B, T, H, head_dim] -> [B, T, H, head_dim] (cb_kv4_attention)."""
-    rec, dev = _kv4_record(cache, "kv4_attention"), cache.pages.device
-    if q.device != dev or q.dtype != cache.dtype:
+    """q [B, T, H, head_dim] or [B, H, head_dim] -> as q (cb_kv4_attention)."""
+    rec, dev = _kv4_record(cache, "kv4_attention"), cache.pages.get_device()
+    if q.get_device() != dev or q.dtype is not cache.dtype:
         _fail("kv4_attention: q must be of the cache's dtype, on its device")
-    if q.dim() != 4 or q.shape[3] != rec.head_dim:
-        _fail(f"kv4_attention: q must be [B, T, H, {rec.head_dim}]")
-    B, T, H, D = q.shape
-    if H % rec.kv_heads:
+    shape, kv, D = q.shape, rec.kv_heads, rec.head_dim
+    if len(shape) not in (3, 4) or shape[-1] != D:
+        _fail(f"kv4_attention: q must be [B, T, H, {D}] or [B, H, {D}]")
+    B, T, H = shape[0], shape[1] if len(shape) == 4 else 1, shape[-2]
+    if H % kv:
         _fail("kv4_attention: q's heads must be a multiple of the cache's")
     _check_table(page_table, dev, "kv4_attention")
     if page_table.shape[0] != B:
         _fail("kv4_attention: page_table needs one row for each sequence of q")
-    _check_index(lengths, dev, (B,), "lengths", "kv4_attention")
-    out = torch.empty((B, T, H, D), dtype=q.dtype, device=dev)
-    if out.numel() == 0:
+    _check_index(lengths, dev, B, "lengths", "kv4_attention")
+    device = q.device
+    out = torch.empty(shape, dtype=q.dtype, device=device)
+    if B == 0 or T == 0 or H == 0:
         return out
     q = _vector_rows(q)
-    with _on_device(dev):
-        st = _stream(q)
-        counters, partial = _kv4_scratch(dev, st, _lib.cb_kv4_attention_counters(B, T, H, rec.kv_heads),
-                                         _lib.cb_kv4_attention_partial_bytes(T, H, rec.kv_heads, D))
-        _rc(_lib.cb_kv4_attention(ctypes.byref(rec), q.data_ptr(), (_i64 * 3)(*q.stride()[:3]), out.data_ptr(), B, T, H,
+    st = q.stride()
+    rows = T * (H // kv)
+    counters = B * kv * (1 if rows <= 8 else -(-rows // 16))
+    with _on_device(device):
+        key = (dev, rows > 8, D)
+        nbytes = _partial_bytes.get(key)
+        if nbytes is None:
+            nbytes = _partial_bytes[key] = _lib.cb_kv4_attention_partial_bytes(T, H, kv, D)
+        stream = _raw_stream(dev)
+        counts, partial = _kv4_scratch(device, dev, stream, counters, nbytes)
+        _rc(_lib.cb_kv4_attention(rec, q.data_ptr(), (_i64 * 3)(st[0], st[1] if len(st) == 4 else 0, st[-2]), out.data_ptr(), B, T, H,
                                   page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), scale,
-                                  counters.data_ptr(), counters.numel() * 4, partial.data_ptr(), partial.numel(), st))
+                                  counts.data_ptr(), counters * 4, partial.data_ptr(), nbytes, stream))
     return out
 
 
@@ -803,7 +830,8 @@ _lib.cb_prompt_attention.restype = _int
 
 def _tma_rows(t: torch.Tensor) -> torch.Tensor:
     """As _vector_rows, and no dimension of several entries with a stride of 0 (an expanded tensor is copied)."""
-    if any(s <= 0 for s, n in zip(t.stride(), t.shape) if n > 1):
+    st = t.stride()
+    if (st[0] <= 0 and t.shape[0] > 1) or (st[1] <= 0 and t.shape[1] > 1):
         return t.clone(memory_format=torch.contiguous_format)
     return _vector_rows(t)
 
@@ -813,31 +841,37 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bo
     who = "prompt_attention"
     if not isinstance(q, torch.Tensor) or not q.is_cuda:
         _fail(f"{who}: q must be a CUDA tensor (this build has no CPU path)")
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    dtype, dev = q.dtype, q.get_device()
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         _fail(f"{who}: q must be float16 or bfloat16")
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         _fail(f"{who}: q must be [Tq, H, head_dim], k and v [Tk, Hkv, head_dim]")
-    if k.device != q.device or v.device != q.device or k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.get_device() != dev or v.get_device() != dev or k.dtype is not dtype or v.dtype is not dtype:
         _fail(f"{who}: q, k and v must be of one dtype, on one device")
-    (tq, h, d), (tk, hkv) = q.shape, k.shape[:2]
-    if k.shape != v.shape or k.shape[2] != d:
+    shape = q.shape
+    tq, h, d = shape
+    tk, hkv, dk = k.shape
+    if dk != d or v.shape != k.shape:
         _fail(f"{who}: k and v must have the same shape, with q's head_dim")
     if hkv == 0 or h % hkv:
         _fail(f"{who}: q's heads must be a multiple of k's")
-    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         _fail(f"{who}: cu_seqlens must hold the first query of each sequence and their end")
-    _check_index(cu_seqlens, q.device, tuple(cu_seqlens.shape), "cu_seqlens", who)
-    _check_index(cu_seqlens_k, q.device, tuple(cu_seqlens.shape), "cu_seqlens_k", who)
+    n = cu_seqlens.shape[0]
+    _check_index(cu_seqlens, dev, n, "cu_seqlens", who)
+    if cu_seqlens_k is not cu_seqlens:
+        _check_index(cu_seqlens_k, dev, n, "cu_seqlens_k", who)
+    device = q.device
     if out is None:
-        out = torch.empty((tq, h, d), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or out.data_ptr() % 16:
+        out = torch.empty(shape, dtype=dtype, device=device)
+    elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         _fail(f"{who}: out must be contiguous and 16-byte aligned, of q's shape, dtype and device")
-    if out.numel() == 0 or cu_seqlens.numel() == 1:
+    if tq == 0 or h == 0 or n == 1:
         return out
     q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)
     strides = (_i64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
-    with _on_device(q.device):
+    with _on_device(device):
         _rc(_lib.cb_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, out.data_ptr(), tq, tk, h, hkv, d,
-                                     _DTYPE[q.dtype], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), cu_seqlens.numel() - 1,
-                                     scale, 1 if causal else 0, _stream(q)))
+                                     _DTYPE[dtype], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), n - 1, scale,
+                                     1 if causal else 0, _raw_stream(dev)))
     return out

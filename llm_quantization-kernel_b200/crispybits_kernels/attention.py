@@ -33,7 +33,7 @@ def _C():
     return ops._C
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class KV4Cache:
     """Keys and values of one layer in 4 bits: `pages` uint8 [n_pages, kv_heads, bytes of a page and head]."""
     pages: torch.Tensor
@@ -105,10 +105,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
     among them; token j of T sees the first lengths - T + 1 + j.  A row that sees nothing (lengths 0) is 0.  scale: default head_dim ** -0.5.
     T may be any, but the cache is read once for each 16 rows (T * H / kv_heads of them) of a key head: for long pieces of
     a prompt, read the history back and use prompt attention."""
-    one = q.dim() == 3
-    out = _C().kv4_attention(q.unsqueeze(1) if one else q, cache, page_table, lengths,
-                             cache.head_dim ** -0.5 if scale is None else float(scale))
-    return out.squeeze(1) if one else out
+    return _C().kv4_attention(q, cache, page_table, lengths, cache.head_dim ** -0.5 if scale is None else float(scale))
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,

@@ -158,7 +158,7 @@ __device__ __forceinline__ int blocks_of(int len) { return (int)(((unsigned)len 
 
 constexpr float kLag = 8.f;
 
-constexpr int kOpen = 40;
+constexpr int kOpen = 64;
 
 template <typename T, int D, int GS, int NT>
 __global__ void __launch_bounds__((AttnCfg<D, GS, NT>::kThreads), 1)
