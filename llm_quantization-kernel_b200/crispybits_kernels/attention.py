@@ -30,6 +30,8 @@ from . import ops
 
 def _C():
     ops._check_ext()
+    if not hasattr(ops._C, "kv4_block_bytes"):
+        raise RuntimeError("the selected backend has no attention operators")
     return ops._C
 
 

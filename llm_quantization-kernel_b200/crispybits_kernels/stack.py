@@ -22,9 +22,12 @@ predecessor on every rank (not for a completion event on its own GPU), and a one
 publishes its completion; a block's QKV launch, which reads x and not the previous block's output, waits for one
 launch less and so overlaps the previous hand-shake.
 
-Only the linears and the gathers are in the step: attention, normalisation and residual adds of a
-real model are other kernels and are outside this path.  Each block reads the step's hidden state
-x; inside a block the data flows  x -> QKV -> (Q part) -> o_proj -> gate/up -> down.
+Only the linears and the gathers are in the plain step: normalisation and residual adds of a real model are other
+kernels and are outside this path, and so is attention unless the step is given a `StackCache`.  Each block reads the
+step's hidden state x; inside a block the data flows  x -> QKV -> (Q part) -> o_proj -> gate/up -> down, and with a cache
+    x -> QKV -> K, V into the block's 4-bit cache -> attention of Q over it -> o_proj -> gate/up -> down
+on every rank for its own heads, so that the gather after the attention is the one that Q had.  `prefill` does the same for
+whole prompts.  There is no positional rotation: the synthetic stack has no positions in its linears either.
 
 The synthetic weights are drawn on the stack's device (seeded per block and matrix, identical on every
 rank) and quantised and packed by `packer`: by default the library's GPU kernel (cb_quantize_pack, which is
@@ -39,6 +42,7 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
+from .attention import KV4Cache, kv4_append, kv4_attention, kv4_read, prompt_attention
 from .ops import PackedLinearWeight, fused_gate_up, fused_qkv, new_workspace, packed_linear
 
 LLAMA2_7B = dict(n_blocks=32, d_model=4096, d_ff=11008)
@@ -77,6 +81,24 @@ class _Block:
     gate: PackedLinearWeight
     up: PackedLinearWeight
     down: PackedLinearWeight
+
+
+class StackCache:
+    """Keys and values of `batch` sequences for every block of a DecodeStack (this rank's heads), in 4 bits: one KV4Cache for
+    each block, one page table and one vector of lengths for all.  Sequence s owns pages s * n .. s * n + n - 1."""
+
+    def __init__(self, stack: "DecodeStack", batch: int, max_tokens: int, head_dim: int = 128, page_size: int = 64,
+                 group_size: int = 64, dtype: torch.dtype = torch.float16):
+        local = stack.d_model // stack.world
+        if local % head_dim:
+            raise ValueError("a rank's rows of Q must be whole heads")
+        pages = -(-max_tokens // page_size)
+        self.batch, self.heads, self.head_dim = batch, local // head_dim, head_dim
+        self.layers = [KV4Cache.empty(batch * pages, self.heads, head_dim, page_size, group_size, dtype, stack.device)
+                       for _ in range(stack.n_blocks)]
+        self.page_table = torch.arange(batch * pages, dtype=torch.int32, device=stack.device).view(batch, pages)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=stack.device)      # cached tokens of each sequence
+        self.seen = torch.zeros_like(self.lengths)                                     # of the running step: its own tokens too
 
 
 class DecodeStack:
@@ -242,18 +264,63 @@ class DecodeStack:
             return out.view(1, self.world * nl)
         return out.view(self.world, b, nl).permute(1, 0, 2).reshape(b, self.world * nl)
 
-    def step(self, x: torch.Tensor, decode_threshold: int = 8) -> torch.Tensor:
-        """x [B, d_model] (replicated on every rank) -> the last block's down-projection output [B, d_model]."""
+    def step(self, x: torch.Tensor, decode_threshold: int = 8, cache: Optional[StackCache] = None) -> torch.Tensor:
+        """x [B, d_model] (replicated on every rank) -> the last block's down-projection output [B, d_model].  With a cache, row s is the
+        next token of sequence s: its keys and values are appended, and what o_proj reads is its attention over the cache."""
         if self.comm != "nccl":
+            if cache is not None:
+                raise ValueError("attention in the step needs comm='nccl'")
             return self._step_p2p(x)
         y = None
         kw = dict(decode_threshold=decode_threshold, workspace=self.workspace)
-        for blk in self.blocks:
-            oq, _ok, _ov = fused_qkv(x, blk.q, blk.k, blk.v, **kw)
+        if cache is not None:
+            self._check_cache(cache, x.shape[0])
+            torch.add(cache.lengths, 1, out=cache.seen)
+        for i, blk in enumerate(self.blocks):
+            oq, ok, ov = fused_qkv(x, blk.q, blk.k, blk.v, **kw)
+            if cache is not None:
+                oq, ok, ov = (t.view(-1, cache.heads, cache.head_dim) for t in (oq, ok, ov))
+                kv4_append(cache.layers[i], ok, ov, cache.page_table, cache.lengths)
+                oq = kv4_attention(oq, cache.layers[i], cache.page_table, cache.seen).flatten(1)
             a = self.gather(packed_linear(self.gather(oq), blk.o, **kw))
             m = self.gather(fused_gate_up(a, blk.gate, blk.up, **kw))
             y = self.gather(packed_linear(m, blk.down, **kw))
+        if cache is not None:
+            cache.lengths.copy_(cache.seen)
         return y                                          # the last block's output; every block ran the same launches
+
+    def _check_cache(self, cache: StackCache, batch: int):
+        if len(cache.layers) != self.n_blocks or cache.heads * cache.head_dim != self.d_model // self.world:
+            raise ValueError("the cache was made for another stack")
+        if batch != cache.batch:
+            raise ValueError("one row, or one prompt, for each sequence of the cache")
+
+    def prefill(self, x: torch.Tensor, lens: List[int], cache: StackCache, past: Optional[List[int]] = None) -> torch.Tensor:
+        """Prompts of all sequences: x [sum(lens), d_model], packed -> the last block's output [sum(lens), d_model]; their keys and
+        values enter the cache.  `past`: tokens that each sequence has cached already (default: none); the prompts then attend to
+        these too, as the cache holds them, and to themselves in the cache's 4 bits as well."""
+        if self.comm != "nccl":
+            raise ValueError("prefill needs comm='nccl'")
+        self._check_cache(cache, len(lens))
+        if sum(lens) != x.shape[0]:
+            raise ValueError("lens must add up to the rows of x")
+        bounds = lambda v: torch.tensor(np.concatenate(([0], np.cumsum(v))), dtype=torch.int32).to(self.device)
+        cu, y = bounds(lens), None
+        total = [n + p for n, p in zip(lens, past)] if past is not None else lens
+        cu_all = bounds(total) if past is not None else cu
+        nothing = torch.zeros_like(cache.lengths)
+        torch.add(cache.lengths, cu[1:] - cu[:-1], out=cache.seen)
+        for i, blk in enumerate(self.blocks):
+            q, k, v = (t.view(-1, cache.heads, cache.head_dim) for t in fused_qkv(x, blk.q, blk.k, blk.v, workspace=self.workspace))
+            kv4_append(cache.layers[i], k, v, cache.page_table, cache.lengths, cu)
+            if past is not None:
+                k, v = kv4_read(cache.layers[i], cache.page_table, nothing, cu_all, sum(total))
+            a = self.gather(prompt_attention(q, k, v, cu, cu_all).flatten(1))
+            a = self.gather(packed_linear(a, blk.o, workspace=self.workspace))
+            m = self.gather(fused_gate_up(a, blk.gate, blk.up, workspace=self.workspace))
+            y = self.gather(packed_linear(m, blk.down, workspace=self.workspace))
+        cache.lengths.copy_(cache.seen)
+        return y
 
     # -------------------------------------------------------------- check value (fp32, any device)
     @torch.no_grad()
