@@ -287,7 +287,7 @@ int cb_decode_plan(int bits, int64_t B, int64_t V, int64_t K, int64_t split_k, i
  * weights-in-TMEM kernel) = in the tensor-core GEMM role r (1 activation producer, 2 MMA issuer,
  * 3 dequantiser, 4 epilogue, 5 packed-word producer) gave up a bounded wait; 3001 = a kernel of the 4-bit cache met a position
  * outside its page table or a page number outside the cache and left it out, 3002 = a copy of the cache's attention did not
- * arrive in time and outputs were not written; 4000 + r = role r of the prompt attention (1 TMA, 2 MMA, 3 softmax, 4 epilogue) gave up a
+ * arrive in time and outputs were not written; 4000 + r = role r of the prompt attention (1 TMA, 2 MMA, 3 softmax, 4 epilogue, 5 tile ends) gave up a
  * bounded wait.  No counterpart in the reference. */
 int cb_decode_status(int* status);
 

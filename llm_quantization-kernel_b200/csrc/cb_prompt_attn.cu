@@ -12,8 +12,8 @@
 // rounding is relative.  p is rounded to the inputs' type; the sum l takes the unrounded p.
 //
 // TMEM map (512 columns): S0/P0 [0, 128), S1/P1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D).
-// Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 and 11 none (they complete the
-// warpgroup that gives registers to the softmax warps, which hold a whole row of scores).
+// Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 zeros behind the last
+// key (below), 11 nothing (it completes the warpgroup that gives registers to the softmax warps, which hold a whole row of scores).
 //
 // V rows behind the last key of a sequence belong to another sequence (or to nothing): they are zeroed in shared memory, since 0 *
 // inf is not 0.  K rows there only make scores that are masked.
@@ -31,9 +31,10 @@ namespace cb {
 namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
-constexpr int kTmaWarp = 8, kMmaWarp = 9, kThreads = 384;
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kFixWarp = 10, kThreads = 384;
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
 constexpr int kSoftRegs = 200, kOtherRegs = 104;
+constexpr int kPolyOf8 = 2;
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
 
 __device__ int g_prompt_status;
@@ -68,7 +69,7 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n selp.u32 %0, 1, 0, p;\n}"
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
@@ -93,6 +94,53 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two floats in one register pair: the packed operations of this GPU do both at once.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(uint32_t lo, uint32_t hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { return pair(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void unpair(f32x2 v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// 2^x for two x <= 2^7 without the special-function unit: x = n + f with n the nearest integer, 2^f by a polynomial of degree 4 that is within
+// 2.7e-6 of it (relative; fitted for this purpose on [-1/2, 1/2]), 2^n from n's bits.  Below 2^-126 the result is 2^-126.
+__device__ __forceinline__ f32x2 ex2_poly(f32x2 x2) {
+    float x0, x1;
+    unpair(x2, x0, x1);
+    const f32x2 x = pair(max_nan(x0, -126.f), max_nan(x1, -126.f));
+    const f32x2 t = add2(x, pair(12583039.f, 12583039.f));        // 1.5 * 2^23 + 127: the low bits hold n + 127
+    const f32x2 f = add2(x, mul2(add2(t, pair(-12583039.f, -12583039.f)), pair(-1.f, -1.f)));
+    f32x2 p = fma2(f, pair(0.00957006889f, 0.00957006889f), pair(0.0559178085f, 0.0559178085f));
+    p = fma2(p, f, pair(0.240247451f, 0.240247451f));
+    p = fma2(p, f, pair(0.693121821f, 0.693121821f));
+    p = fma2(p, f, pair(0.999999262f, 0.999999262f));
+    float t0, t1;
+    unpair(t, t0, t1);
+    return mul2(p, pair(__float_as_uint(t0) << 23, __float_as_uint(t1) << 23));
+}
 #define CB_R32(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7]), \
     "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]), "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), \
     "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]), "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), \
@@ -108,13 +156,25 @@ template <int O, int N> __device__ __forceinline__ void tmem_ld32(uint32_t addr,
                  "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                  : CB_R32(v, O) : "r"(addr));
 }
+template <int N> __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[N]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                   "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
 template <int O, int N> __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[N]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
                  "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
                  "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
                  ::"r"(addr), CB_W32(v, O) : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+#define CB_X32(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7]), \
+    "+r"(v[o + 8]), "+r"(v[o + 9]), "+r"(v[o + 10]), "+r"(v[o + 11]), "+r"(v[o + 12]), "+r"(v[o + 13]), "+r"(v[o + 14]), "+r"(v[o + 15]), \
+    "+r"(v[o + 16]), "+r"(v[o + 17]), "+r"(v[o + 18]), "+r"(v[o + 19]), "+r"(v[o + 20]), "+r"(v[o + 21]), "+r"(v[o + 22]), "+r"(v[o + 23]), \
+    "+r"(v[o + 24]), "+r"(v[o + 25]), "+r"(v[o + 26]), "+r"(v[o + 27]), "+r"(v[o + 28]), "+r"(v[o + 29]), "+r"(v[o + 30]), "+r"(v[o + 31])
+// All loads of this thread have arrived; v[O .. O + 31] are named so that nothing that uses them moves ahead of the wait.
+template <int O, int N> __device__ __forceinline__ void tmem_ld_wait32(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : CB_X32(v, O) :: "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // The work of a CTA, in order: every role walks through the same list by itself.  Tiles are ordered by their place in their
@@ -205,21 +265,22 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     auto q_full = [&](int x) { return bars + 8u * x; };
     const uint32_t q_empty = bars + 16u;
     auto s_full = [&](int x) { return bars + 24u + 8u * x; };
-    auto p_ready = [&](int x) { return bars + 40u + 8u * x; };
-    auto pv_done = [&](int x) { return bars + 56u + 8u * x; };
-    auto o_free = [&](int x) { return bars + 72u + 8u * x; };
-    auto kv_full = [&](int s) { return bars + 88u + 8u * s; };
-    auto kv_empty = [&](int s) { return bars + 88u + 8u * (kSlots + s); };
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 224);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 228);
-    static_assert(88 + 16 * kSlots <= 224, "barriers");
+    auto p_ready = [&](int x, int half) { return bars + 40u + 16u * x + 8u * half; };
+    auto pv_done = [&](int x) { return bars + 72u + 8u * x; };
+    auto o_free = [&](int x) { return bars + 88u + 8u * x; };
+    const uint32_t v_landed = bars + 104u, v_fixed = bars + 112u;
+    auto kv_full = [&](int s) { return bars + 120u + 8u * s; };
+    auto kv_empty = [&](int s) { return bars + 120u + 8u * (kSlots + s); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 248);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 252);
+    static_assert(120 + 16 * kSlots <= 248, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; ++x) {
-            mbar_init(q_full(x), 1); mbar_init(s_full(x), 1); mbar_init(p_ready(x), 4); mbar_init(pv_done(x), 1); mbar_init(o_free(x), 4);
+            mbar_init(q_full(x), 1); mbar_init(s_full(x), 1); mbar_init(p_ready(x, 0), 4); mbar_init(p_ready(x, 1), 4); mbar_init(pv_done(x), 1); mbar_init(o_free(x), 4);
         }
-        mbar_init(q_empty, 1);
+        mbar_init(q_empty, 1); mbar_init(v_landed, 1); mbar_init(v_fixed, 1);
         for (int s = 0; s < kSlots; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -272,88 +333,102 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 while (!mbar_try_wait(q_full(x), (tiles - 1) & 1) && clock64() - t0 < kWaitCycles) {}
         }
     } else if (warp == kMmaWarp) {
-        // ================= MMA issuer =================
+        // ================= MMA issuer: one thread =================
         constexpr uint32_t fmt = BF ? ((1u << 7) | (1u << 10)) : 0u;
         const uint32_t idesc_s = (1u << 4) | fmt | ((uint32_t)P.negate << 13) | ((uint32_t)(kTileK >> 3) << 17) | ((uint32_t)(kSub >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kSub >> 4) << 24);
         const uint64_t dk = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);                            // K-major, 128-byte swizzle, 8-row atoms 1024 bytes apart
         const uint64_t dv = ((uint64_t)(C::kBox >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);        // N-major: 64-value boxes kBox apart, 8-key groups 1024 bytes apart
-        uint32_t it = 0, tiles = 0, pcount[2] = {0, 0}, ocount[2] = {0, 0};
+        uint32_t it = 0, tiles = 0, fixes = 0, pcount[2] = {0, 0}, ocount[2] = {0, 0};
         // the ring place of K tile j of the present query tile is it + 2 j, of V tile j it + 2 j + 1
-        auto wait_kv = [&](uint32_t place) { return __all_sync(0xffffffffu, mbar_wait(kv_full(place % kSlots), (place / kSlots) & 1, abort_flag)); };
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+            if (!mbar_wait(bar, parity, abort_flag)) gave_up = 2;
+            return gave_up == 0;
+        };
         auto scores = [&](int x, int j, bool release) {
             const uint32_t place = it + 2 * j;
-            if (!wait_kv(place)) { gave_up = 2; return; }
-            fence_after();
-            if (lane == 0) {
-                const uint32_t qa = base + C::kQOff + x * C::kTileBytes, ka = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+            const uint32_t qa = base + C::kQOff + x * C::kTileBytes, ka = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k / 4) * C::kBox + (k % 4) * 32;
-                    const uint64_t ad = dk | (uint64_t)(((qa + off) >> 4) & 0x3FFF), bd = dk | (uint64_t)(((ka + off) >> 4) & 0x3FFF);
-                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
-                                 ::"r"(tmem + x * 128), "l"(ad), "l"(bd), "r"(idesc_s), "r"(k > 0 ? 1u : 0u), "r"(0u) : "memory");
-                }
-                commit(s_full(x));
-                if (release) commit(kv_empty(place % kSlots));
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (k / 4) * C::kBox + (k % 4) * 32;
+                const uint64_t ad = dk | (uint64_t)(((qa + off) >> 4) & 0x3FFF), bd = dk | (uint64_t)(((ka + off) >> 4) & 0x3FFF);
+                asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                             " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
+                             ::"r"(tmem + x * 128), "l"(ad), "l"(bd), "r"(idesc_s), "r"(k > 0 ? 1u : 0u), "r"(0u) : "memory");
             }
-            __syncwarp();
+            commit(s_full(x));
+            if (release) commit(kv_empty(place % kSlots));
         };
         auto values = [&](int x, int j, bool release) {
             const uint32_t place = it + 2 * j + 1;
-            if (!wait_kv(place)) { gave_up = 2; return; }
-            if (!__all_sync(0xffffffffu, mbar_wait(p_ready(x), pcount[x] & 1, abort_flag))) { gave_up = 2; return; }
-            ++pcount[x];
-            fence_after();
-            if (lane == 0) {
-                const uint32_t va = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+            const uint32_t va = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+            for (int half = 0; half < 2; ++half) {                // the first 64 keys' product while the others' weights are made
+                if (!wait(p_ready(x, half), pcount[x] & 1)) return;
+                fence_after();
 #pragma unroll
-                for (int k = 0; k < kTileK / 16; ++k) {
+                for (int k4 = 0; k4 < kTileK / 32; ++k4) {
+                    const int k = half * (kTileK / 32) + k4;
                     const uint64_t bd = dv | (uint64_t)(((va + k * 2048) >> 4) & 0x3FFF);
                     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                                  " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
                                  ::"r"(tmem + 256 + x * 128), "r"(tmem + x * 128 + k * 8), "l"(bd), "r"(idesc_o), "r"(j > 0 || k > 0 ? 1u : 0u), "r"(0u) : "memory");
                 }
-                commit(pv_done(x));
-                if (release) commit(kv_empty(place % kSlots));
             }
-            __syncwarp();
+            commit(pv_done(x));
+            if (release) commit(kv_empty(place % kSlots));
+            ++pcount[x];
         };
         while (!gave_up && walk.next(w)) {
             const int n = max(w.n[0], w.n[1]);
             if (n == 0) continue;
-            for (int x = 0; x < 2; ++x)                           // both halves of Q are always loaded
-                if (!__all_sync(0xffffffffu, mbar_wait(q_full(x), tiles & 1, abort_flag))) gave_up = 2;
-            ++tiles;
-            for (int x = 0; x < 2 && !gave_up; ++x)
-                if (w.n[x] > 0) scores(x, 0, x == 1 || w.n[1] == 0);
-            for (int j = 0; j < n && !gave_up; ++j) {
-                const int valid = w.lk - j * kTileK;
-                if (valid < kTileK) {
-                    // rows behind the sequence's last key: zeros, before any product reads them
-                    const uint32_t place = it + 2 * j + 1;
-                    if (!wait_kv(place)) { gave_up = 2; break; }
-                    unsigned char* v = smem + C::kRingOff + (place % kSlots) * C::kTileBytes;
-                    for (int i = lane; i < (kTileK - valid) * 8; i += 32)
-                        for (int h = 0; h < D / 64; ++h) *reinterpret_cast<uint4*>(v + h * C::kBox + valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
+            if (lane == 0) {
+                // both halves of Q are always loaded
+                if (wait(q_full(0), tiles & 1) && wait(q_full(1), tiles & 1) && wait(kv_full(it % kSlots), (it / kSlots) & 1)) {
+                    fence_after();
+                    for (int x = 0; x < 2; ++x)
+                        if (w.n[x] > 0) scores(x, 0, x == 1 || w.n[1] == 0);
                 }
-                for (int x = 0; x < 2 && !gave_up; ++x) {
-                    if (j < w.n[x]) {
-                        if (j == 0) {                             // the previous tile's O must have been read
-                            if (ocount[x] > 0 && !__all_sync(0xffffffffu, mbar_wait(o_free(x), (ocount[x] - 1) & 1, abort_flag))) { gave_up = 2; break; }
-                            ++ocount[x];
-                        }
-                        values(x, j, x == 1 || j >= w.n[1]);
+                for (int j = 0; j < n && !gave_up; ++j) {
+                    const uint32_t v = it + 2 * j + 1, k = v + 1;
+                    if (!wait(kv_full(v % kSlots), (v / kSlots) & 1)) break;
+                    if (w.lk - j * kTileK < kTileK) {
+                        mbar_arrive(v_landed);                    // only now: the fixing warp does not follow the ring itself
+                        if (!wait(v_fixed, fixes++ & 1)) break;
                     }
-                    if (!gave_up && j + 1 < w.n[x]) scores(x, j + 1, x == 1 || j + 1 >= w.n[1]);
+                    if (j + 1 < n && !wait(kv_full(k % kSlots), (k / kSlots) & 1)) break;
+                    for (int x = 0; x < 2 && !gave_up; ++x) {
+                        if (j < w.n[x]) {
+                            if (j == 0) {                         // the previous tile's O must have been read
+                                if (ocount[x] > 0 && !wait(o_free(x), (ocount[x] - 1) & 1)) break;
+                                ++ocount[x];
+                            }
+                            values(x, j, x == 1 || j >= w.n[1]);
+                        }
+                        if (!gave_up && j + 1 < w.n[x]) scores(x, j + 1, x == 1 || j + 1 >= w.n[1]);
+                    }
                 }
+                if (!gave_up) commit(q_empty);
             }
+            ++tiles;
             it += 2 * n;
-            if (lane == 0 && !gave_up) commit(q_empty);
+            gave_up = __shfl_sync(0xffffffffu, gave_up, 0);
+        }
+    } else if (warp == kFixWarp) {
+        // ================= the last V tile of a sequence: zeros behind its last key, before any product reads it =================
+        uint32_t it = 0, fixes = 0;
+        while (!gave_up && walk.next(w)) {
+            const int n = max(w.n[0], w.n[1]), valid = w.lk - (n - 1) * kTileK;
+            if (n == 0) continue;
+            it += 2 * n;
+            if (valid >= kTileK) continue;
+            const uint32_t place = it - 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(v_landed, fixes++ & 1, abort_flag))) { gave_up = 5; break; }
+            unsigned char* v = smem + C::kRingOff + (place % kSlots) * C::kTileBytes;
+            for (int i = lane; i < (kTileK - valid) * 8; i += 32)
+                for (int h = 0; h < D / 64; ++h) *reinterpret_cast<uint4*>(v + h * C::kBox + valid * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
+            if (lane == 0) mbar_arrive(v_fixed);
         }
     }
     } else {
@@ -378,17 +453,27 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 if (!__all_sync(0xffffffffu, mbar_wait(s_full(x), count & 1, abort_flag))) { gave_up = 3; break; }
                 fence_after();
                 uint32_t s[128];
-                tmem_ld32<0>(s_addr, s); tmem_ld32<32>(s_addr + 32, s); tmem_ld32<64>(s_addr + 64, s); tmem_ld32<96>(s_addr + 96, s);
-                tmem_ld_wait();
+                tmem_ld32<0>(s_addr, s); tmem_ld32<32>(s_addr + 32, s);
+                tmem_ld_wait32<0>(s); tmem_ld_wait32<32>(s);
+                tmem_ld32<64>(s_addr + 64, s); tmem_ld32<96>(s_addr + 96, s);
                 const int seen = limit - j * kTileK;
-                if (__any_sync(0xffffffffu, seen < kTileK)) {
-#pragma unroll
-                    for (int i = 0; i < 128; ++i)
-                        if (i >= seen) s[i] = 0xff800000u;
-                }
+                const bool masked = __any_sync(0xffffffffu, seen < kTileK);
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (masked)
 #pragma unroll
-                for (int i = 0; i < 128; i += 8)
+                    for (int i = 0; i < 64; ++i)
+                        if (i >= seen) s[i] = 0xff800000u;
+#pragma unroll
+                for (int i = 0; i < 64; i += 8)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], fmaxf(__uint_as_float(s[i + c]), __uint_as_float(s[i + 4 + c])));
+                tmem_ld_wait32<64>(s); tmem_ld_wait32<96>(s);
+                if (masked)
+#pragma unroll
+                    for (int i = 64; i < 128; ++i)
+                        if (i >= seen) s[i] = 0xff800000u;
+#pragma unroll
+                for (int i = 64; i < 128; i += 8)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], fmaxf(__uint_as_float(s[i + c]), __uint_as_float(s[i + 4 + c])));
                 const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * P.scale_log2;
@@ -404,7 +489,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                         for (int c = 0; c < D; c += 32) {
                             uint32_t v[32];
                             tmem_ld32<0>(o_addr + c, v);
-                            tmem_ld_wait();
+                            tmem_ld_wait32<0>(v);
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
                             tmem_st32<0>(o_addr + c, v);
@@ -412,22 +497,44 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                         tmem_st_wait();
                     }
                 }
+                // ---- weights: 32 keys at a time.  Of unmasked tiles kPolyOf8 of 8 pairs go to the polynomial: the special-function units are as
+                // busy as the tensor cores otherwise.
                 const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-                float l4[4] = {0.f, 0.f, 0.f, 0.f};
+                const f32x2 neg2 = pair(neg, neg), mul = pair(P.scale_log2, P.scale_log2);
+                f32x2 sum[2] = {0ull, 0ull};
+                auto weights = [&](auto plain) {
 #pragma unroll
-                for (int i = 0; i < 128; i += 4) {
-                    float p[4];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t out[16];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) { p[c] = ex2(fmaf(__uint_as_float(s[i + c]), P.scale_log2, neg)); l4[c] += p[c]; }
-                    s[i / 2] = pack2<T>(p[0], p[1]);
-                    s[i / 2 + 1] = pack2<T>(p[2], p[3]);
-                }
-                l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
-                tmem_st32<0>(s_addr, s); tmem_st32<32>(s_addr + 32, s);
-                tmem_st_wait();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_ready(x));
+                        for (int i = 0; i < 16; ++i) {
+                            const f32x2 e = fma2(pair(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), mul, neg2);
+                            f32x2 p2;
+                            float p0, p1;
+                            if (decltype(plain)::value && i % 8 < kPolyOf8) {
+                                p2 = ex2_poly(e);
+                                unpair(p2, p0, p1);
+                            } else {
+                                unpair(e, p0, p1);
+                                p0 = ex2(p0); p1 = ex2(p1);
+                                p2 = pair(p0, p1);
+                            }
+                            sum[i & 1] = add2(sum[i & 1], p2);
+                            out[i] = pack2<T>(p0, p1);
+                        }
+                        tmem_st16(s_addr + 16 * c, out);
+                        if (c & 1) {
+                            tmem_st_wait();
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(p_ready(x, c >> 1));
+                        }
+                    }
+                };
+                if (masked) weights(std::false_type{}); else weights(std::true_type{});
+                float l0, l1;
+                unpair(add2(sum[0], sum[1]), l0, l1);
+                l += l0 + l1;
             }
             if (gave_up) break;
             if (!__all_sync(0xffffffffu, mbar_wait(pv_done(x), (count - 1) & 1, abort_flag))) { gave_up = 4; break; }
@@ -437,7 +544,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             for (int c = 0; c < D; c += 32) {
                 uint32_t v[32];
                 tmem_ld32<0>(o_addr + c, v);
-                tmem_ld_wait();
+                tmem_ld_wait32<0>(v);
                 if (c + 32 == D) {
                     fence_before();
                     __syncwarp();
