@@ -87,6 +87,22 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// The same value from every lane, known to the compiler as such: it then lives in a uniform register, which is where
+// tcgen05.mma takes its operands from (moving them there one by one was measured to cost twice the products' own time).
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -333,85 +349,90 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 while (!mbar_try_wait(q_full(x), (tiles - 1) & 1) && clock64() - t0 < kWaitCycles) {}
         }
     } else if (warp == kMmaWarp) {
-        // ================= MMA issuer: one thread =================
+        // ================= MMA issuer: the warp goes through the list together, one elected thread issues =================
         constexpr uint32_t fmt = BF ? ((1u << 7) | (1u << 10)) : 0u;
         const uint32_t idesc_s = (1u << 4) | fmt | ((uint32_t)P.negate << 13) | ((uint32_t)(kTileK >> 3) << 17) | ((uint32_t)(kSub >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | fmt | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(kSub >> 4) << 24);
-        const uint64_t dk = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);                            // K-major, 128-byte swizzle, 8-row atoms 1024 bytes apart
-        const uint64_t dv = ((uint64_t)(C::kBox >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);        // N-major: 64-value boxes kBox apart, 8-key groups 1024 bytes apart
+        constexpr uint64_t dk = (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);                        // K-major, 128-byte swizzle, 8-row atoms 1024 bytes apart
+        constexpr uint64_t dv = ((uint64_t)(C::kBox >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);    // N-major: 64-value boxes kBox apart, 8-key groups 1024 bytes apart
+        const uint32_t tm = uniform(tmem), ring = uniform((base + C::kRingOff) >> 4), q_at = uniform((base + C::kQOff) >> 4);
         uint32_t it = 0, tiles = 0, fixes = 0, pcount[2] = {0, 0}, ocount[2] = {0, 0};
         // the ring place of K tile j of the present query tile is it + 2 j, of V tile j it + 2 j + 1
         auto wait = [&](uint32_t bar, uint32_t parity) {
-            if (!mbar_wait(bar, parity, abort_flag)) gave_up = 2;
+            if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))) gave_up = 2;
             return gave_up == 0;
         };
-        auto scores = [&](int x, int j, bool release) {
-            const uint32_t place = it + 2 * j;
-            const uint32_t qa = base + C::kQOff + x * C::kTileBytes, ka = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+        auto scores = [&](int x, uint32_t place, bool release) {
+            const uint32_t slot = place % kSlots;
+            const uint64_t ad = dk | (uint64_t)(q_at + x * (C::kTileBytes >> 4)), bd = dk | (uint64_t)(ring + slot * (C::kTileBytes >> 4));
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (k / 4) * C::kBox + (k % 4) * 32;
-                const uint64_t ad = dk | (uint64_t)(((qa + off) >> 4) & 0x3FFF), bd = dk | (uint64_t)(((ka + off) >> 4) & 0x3FFF);
-                asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                             " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
-                             ::"r"(tmem + x * 128), "l"(ad), "l"(bd), "r"(idesc_s), "r"(k > 0 ? 1u : 0u), "r"(0u) : "memory");
+                for (int k = 0; k < D / 16; ++k) {
+                    constexpr uint32_t kBox16 = C::kBox >> 4;
+                    const uint32_t off = (k / 4) * kBox16 + (k % 4) * 2;
+                    mma_ss(tm + x * 128, ad + off, bd + off, idesc_s, k > 0 ? 1u : 0u);
+                }
+                commit(s_full(x));
+                if (release) commit(kv_empty(slot));
             }
-            commit(s_full(x));
-            if (release) commit(kv_empty(place % kSlots));
+            __syncwarp();
         };
-        auto values = [&](int x, int j, bool release) {
-            const uint32_t place = it + 2 * j + 1;
-            const uint32_t va = base + C::kRingOff + (place % kSlots) * C::kTileBytes;
+        auto values = [&](int x, uint32_t place, bool first, bool release) {
+            const uint32_t slot = place % kSlots;
+            const uint64_t bd = dv | (uint64_t)(ring + slot * (C::kTileBytes >> 4));
+#pragma unroll
             for (int half = 0; half < 2; ++half) {                // the first 64 keys' product while the others' weights are made
                 if (!wait(p_ready(x, half), pcount[x] & 1)) return;
                 fence_after();
+                if (elect_one()) {
 #pragma unroll
-                for (int k4 = 0; k4 < kTileK / 32; ++k4) {
-                    const int k = half * (kTileK / 32) + k4;
-                    const uint64_t bd = dv | (uint64_t)(((va + k * 2048) >> 4) & 0x3FFF);
-                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
-                                 ::"r"(tmem + 256 + x * 128), "r"(tmem + x * 128 + k * 8), "l"(bd), "r"(idesc_o), "r"(j > 0 || k > 0 ? 1u : 0u), "r"(0u) : "memory");
+                    for (int k4 = 0; k4 < kTileK / 32; ++k4) {
+                        const int k = half * (kTileK / 32) + k4;
+                        mma_ts(tm + 256 + x * 128, tm + x * 128 + k * 8, bd + k * 128, idesc_o, first && k == 0 ? 0u : 1u);
+                    }
+                    if (half == 1) {
+                        commit(pv_done(x));
+                        if (release) commit(kv_empty(slot));
+                    }
                 }
+                __syncwarp();
             }
-            commit(pv_done(x));
-            if (release) commit(kv_empty(place % kSlots));
             ++pcount[x];
         };
         while (!gave_up && walk.next(w)) {
-            const int n = max(w.n[0], w.n[1]);
+            const int n0 = (int)uniform(w.n[0]), n1 = (int)uniform(w.n[1]), lk = (int)uniform(w.lk), n = max(n0, n1);
             if (n == 0) continue;
-            if (lane == 0) {
-                // both halves of Q are always loaded
-                if (wait(q_full(0), tiles & 1) && wait(q_full(1), tiles & 1) && wait(kv_full(it % kSlots), (it / kSlots) & 1)) {
-                    fence_after();
-                    for (int x = 0; x < 2; ++x)
-                        if (w.n[x] > 0) scores(x, 0, x == 1 || w.n[1] == 0);
-                }
-                for (int j = 0; j < n && !gave_up; ++j) {
-                    const uint32_t v = it + 2 * j + 1, k = v + 1;
-                    if (!wait(kv_full(v % kSlots), (v / kSlots) & 1)) break;
-                    if (w.lk - j * kTileK < kTileK) {
-                        mbar_arrive(v_landed);                    // only now: the fixing warp does not follow the ring itself
-                        if (!wait(v_fixed, fixes++ & 1)) break;
-                    }
-                    if (j + 1 < n && !wait(kv_full(k % kSlots), (k / kSlots) & 1)) break;
-                    for (int x = 0; x < 2 && !gave_up; ++x) {
-                        if (j < w.n[x]) {
-                            if (j == 0) {                         // the previous tile's O must have been read
-                                if (ocount[x] > 0 && !wait(o_free(x), (ocount[x] - 1) & 1)) break;
-                                ++ocount[x];
-                            }
-                            values(x, j, x == 1 || j >= w.n[1]);
-                        }
-                        if (!gave_up && j + 1 < w.n[x]) scores(x, j + 1, x == 1 || j + 1 >= w.n[1]);
-                    }
-                }
-                if (!gave_up) commit(q_empty);
-            }
+            // both halves of Q are always loaded
+            if (!wait(q_full(0), tiles & 1) || !wait(q_full(1), tiles & 1) || !wait(kv_full(it % kSlots), (it / kSlots) & 1)) break;
             ++tiles;
+            fence_after();
+            if (n0 > 0) scores(0, it, n1 == 0);
+            if (n1 > 0) scores(1, it, true);
+            for (int j = 0; j < n && !gave_up; ++j) {
+                const uint32_t v = it + 2 * j + 1, k = v + 1;
+                if (!wait(kv_full(v % kSlots), (v / kSlots) & 1)) break;
+                if (lk - j * kTileK < kTileK) {
+                    if (lane == 0) mbar_arrive(v_landed);         // only now: the fixing warp does not follow the ring itself
+                    if (!wait(v_fixed, fixes++ & 1)) break;
+                }
+                if (j + 1 < n && !wait(kv_full(k % kSlots), (k / kSlots) & 1)) break;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int nx = x == 0 ? n0 : n1;
+                    if (j < nx) {
+                        if (j == 0) {                             // the previous tile's O must have been read
+                            if (ocount[x] > 0 && !wait(o_free(x), (ocount[x] - 1) & 1)) break;
+                            ++ocount[x];
+                        }
+                        values(x, v, j == 0, x == 1 || j >= n1);
+                    }
+                    if (gave_up) break;
+                    if (j + 1 < nx) scores(x, k, x == 1 || j + 1 >= n1);
+                }
+            }
             it += 2 * n;
-            gave_up = __shfl_sync(0xffffffffu, gave_up, 0);
+            if (!gave_up && elect_one()) commit(q_empty);
+            __syncwarp();
         }
     } else if (warp == kFixWarp) {
         // ================= the last V tile of a sequence: zeros behind its last key, before any product reads it =================
