@@ -34,7 +34,6 @@ constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kFixWarp = 10, kThreads = 384;
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
 constexpr int kSoftRegs = 200, kOtherRegs = 104;
-constexpr int kPolyOf8 = 2;
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
 
 __device__ int g_prompt_status;
@@ -52,6 +51,8 @@ template <int D>
 struct PromptCfg {
     static constexpr uint32_t kBox = 64 * 2 * kTileK;                       // 64 values x 128 rows
     static constexpr uint32_t kTileBytes = kBox * (D / 64);
+    // D = 64: the products are half as long, and the special-function units would be the slowest part
+    static constexpr int kPolyOf8 = D == 64 ? 2 : 0;
     static constexpr int kSlots = D == 128 ? 4 : 8;                         // ring of K and V tiles
     static constexpr uint32_t kQOff = 0, kRingOff = 2 * kTileBytes, kBarOff = kRingOff + kSlots * kTileBytes;
     static constexpr uint32_t kSmem = kBarOff + 256 + 1024;
@@ -95,13 +96,13 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
     return p != 0;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(hi) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(hi) : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -364,13 +365,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         };
         auto scores = [&](int x, uint32_t place, bool release) {
             const uint32_t slot = place % kSlots;
-            const uint64_t ad = dk | (uint64_t)(q_at + x * (C::kTileBytes >> 4)), bd = dk | (uint64_t)(ring + slot * (C::kTileBytes >> 4));
+            const uint32_t ad = (uint32_t)dk | (q_at + x * (C::kTileBytes >> 4)), bd = (uint32_t)dk | (ring + slot * (C::kTileBytes >> 4));
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     constexpr uint32_t kBox16 = C::kBox >> 4;
                     const uint32_t off = (k / 4) * kBox16 + (k % 4) * 2;
-                    mma_ss(tm + x * 128, ad + off, bd + off, idesc_s, k > 0 ? 1u : 0u);
+                    mma_ss(tm + x * 128, ad + off, bd + off, (uint32_t)(dk >> 32), idesc_s, k > 0 ? 1u : 0u);
                 }
                 commit(s_full(x));
                 if (release) commit(kv_empty(slot));
@@ -379,7 +380,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         };
         auto values = [&](int x, uint32_t place, bool first, bool release) {
             const uint32_t slot = place % kSlots;
-            const uint64_t bd = dv | (uint64_t)(ring + slot * (C::kTileBytes >> 4));
+            const uint32_t bd = (uint32_t)dv | (ring + slot * (C::kTileBytes >> 4));
 #pragma unroll
             for (int half = 0; half < 2; ++half) {                // the first 64 keys' product while the others' weights are made
                 if (!wait(p_ready(x, half), pcount[x] & 1)) return;
@@ -388,7 +389,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
 #pragma unroll
                     for (int k4 = 0; k4 < kTileK / 32; ++k4) {
                         const int k = half * (kTileK / 32) + k4;
-                        mma_ts(tm + 256 + x * 128, tm + x * 128 + k * 8, bd + k * 128, idesc_o, first && k == 0 ? 0u : 1u);
+                        mma_ts(tm + 256 + x * 128, tm + x * 128 + k * 8, bd + k * 128, (uint32_t)(dv >> 32), idesc_o, first && k == 0 ? 0u : 1u);
                     }
                     if (half == 1) {
                         commit(pv_done(x));
@@ -518,8 +519,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                         tmem_st_wait();
                     }
                 }
-                // ---- weights: 32 keys at a time.  Of unmasked tiles kPolyOf8 of 8 pairs go to the polynomial: the special-function units are as
-                // busy as the tensor cores otherwise.
+                // ---- weights: 32 keys at a time.  Of unmasked tiles kPolyOf8 of 8 pairs go to the polynomial.
                 const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
                 const f32x2 neg2 = pair(neg, neg), mul = pair(P.scale_log2, P.scale_log2);
                 f32x2 sum[2] = {0ull, 0ull};
@@ -532,7 +532,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                             const f32x2 e = fma2(pair(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), mul, neg2);
                             f32x2 p2;
                             float p0, p1;
-                            if (decltype(plain)::value && i % 8 < kPolyOf8) {
+                            if (decltype(plain)::value && i % 8 < C::kPolyOf8) {
                                 p2 = ex2_poly(e);
                                 unpair(p2, p0, p1);
                             } else {
