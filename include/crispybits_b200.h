@@ -355,10 +355,16 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * cu_k[s + 1] - 1 (device memory; bounds outside the tensors are cut to them).  Head h reads key head h / (H / Hkv).  head_dim 64 or 128,
  * dtype CB_F16 or CB_BF16.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
  * behind a query's last one are not used, except that an infinity or a NaN in v makes NaN of that value for
- * queries up to 127 positions before it. */
+ * queries up to 127 positions before it.
+ * Scratch lets few prompts use all SMs: the keys of their tiles are cut into parts and joined in order, so that the result stays the same
+ * from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, any content) and, in *counter_bytes, of
+ * `counters` (zeroed ONCE, left zero by every call); 0: nothing would be cut.  Both may be NULL: then nothing is.  Calls that may overlap
+ * on the GPU need their own. */
 int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
                         int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
-                        float scale, int causal, void* stream);
+                        float scale, int causal, void* counters, size_t counter_bytes, void* partial, size_t partial_bytes,
+                        void* stream);
+size_t cb_prompt_attention_scratch(int64_t Tq, int64_t Tk, int64_t H, int64_t B, int head_dim, size_t* counter_bytes);
 
 #ifdef __cplusplus
 }

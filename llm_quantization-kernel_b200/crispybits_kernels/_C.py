@@ -751,39 +751,40 @@ def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
     return k, v
 
 
-# Scratch of the cache's attention.  Eager calls: counters (zeroed when made; every call leaves them zero) and partial
+# Scratch of the attention operators.  Eager calls: counters (zeroed when made; every call leaves them zero) and partial
 # sums of one (device, stream), where calls run one after another.  Captured calls: partial sums from the graph's own
 # pool, and counters that no other call ever gets, cut from a slab zeroed beforehand -- two graphs may then run at the
 # same time.  A capture that finds no slab, or an empty one, zeroes its counters inside the graph.
-_kv4_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
-_kv4_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
-_KV4_SLAB = 1 << 18
+_attention_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
+_attention_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
+_ATTENTION_SLAB = 1 << 18
 _partial_bytes: Dict[Tuple[int, bool, int], int] = {}      # (device index, more than 8 rows, head_dim) -> cb_kv4_attention_partial_bytes
 
 
-def kv4_prepare_device(device: torch.device):
+def prepare_attention(device: torch.device):
     """Make the slab of zeroed counters that captured calls on this device draw from (not inside a capture)."""
     index = device.index if device.index is not None else torch.cuda.current_device()
-    if index not in _kv4_slab and not torch.cuda.is_current_stream_capturing():
+    if index not in _attention_slab and not torch.cuda.is_current_stream_capturing():
         with _on_device(torch.device("cuda", index)):
-            slab = torch.zeros(_KV4_SLAB, dtype=torch.int32, device=torch.device("cuda", index))
+            slab = torch.zeros(_ATTENTION_SLAB, dtype=torch.int32, device=torch.device("cuda", index))
             torch.cuda.current_stream(index).synchronize()       # visible to whatever stream a graph will run on
-        _kv4_slab[index] = [slab, 0]
+        _attention_slab[index] = [slab, 0]
 
 
-def _kv4_scratch(device, dev: int, stream: int, counters: int, nbytes: int):
+def _attention_scratch(device, dev: int, stream: int, counters: int, nbytes: int):
     if torch.cuda.is_current_stream_capturing():
         partial = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        slab, need = _kv4_slab.get(dev), -(-counters // 32) * 32
-        if slab is None or slab[1] + need > _KV4_SLAB:
+        slab, need = _attention_slab.get(dev), -(-counters // 32) * 32
+        if slab is None or slab[1] + need > _ATTENTION_SLAB:
             return torch.zeros(counters, dtype=torch.int32, device=device), partial
         slab[1] += need
         return slab[0][slab[1] - need:slab[1]], partial
-    have = _kv4_eager.get((dev, stream))
+    have = _attention_eager.get((dev, stream))
     if have is None or have[0].numel() < counters or have[1].numel() < nbytes:
-        have = (torch.zeros(max(counters, 4096), dtype=torch.int32, device=device),
+        prepare_attention(device)
+        have = (torch.zeros(max(counters, 8192), dtype=torch.int32, device=device),
                 torch.empty(nbytes, dtype=torch.uint8, device=device))
-        _kv4_eager[(dev, stream)] = have
+        _attention_eager[(dev, stream)] = have
     return have
 
 
@@ -816,7 +817,7 @@ def kv4_attention(q, cache, page_table, lengths, scale: float):
         if nbytes is None:
             nbytes = _partial_bytes[key] = _lib.cb_kv4_attention_partial_bytes(T, H, kv, D)
         stream = _raw_stream(dev)
-        counts, partial = _kv4_scratch(device, dev, stream, counters, nbytes)
+        counts, partial = _attention_scratch(device, dev, stream, counters, nbytes)
         _rc(_lib.cb_kv4_attention(rec, q.data_ptr(), (_i64 * 3)(st[0], st[1] if len(st) == 4 else 0, st[-2]), out.data_ptr(), B, T, H,
                                   page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), scale,
                                   counts.data_ptr(), counters * 4, partial.data_ptr(), nbytes, stream))
@@ -824,8 +825,10 @@ def kv4_attention(q, cache, page_table, lengths, scale: float):
 
 
 _lib.cb_prompt_attention.argtypes = [_vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _i64,
-                                     ctypes.c_float, _int, _vp]
+                                     ctypes.c_float, _int, _vp, _sz, _vp, _sz, _vp]
 _lib.cb_prompt_attention.restype = _int
+_lib.cb_prompt_attention_scratch.argtypes = [_i64, _i64, _i64, _i64, _int, ctypes.POINTER(_sz)]
+_lib.cb_prompt_attention_scratch.restype = _sz
 
 
 def _tma_rows(t: torch.Tensor) -> torch.Tensor:
@@ -871,7 +874,11 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bo
     q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)
     strides = (_i64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
     with _on_device(device):
+        stream, cbytes = _raw_stream(dev), _sz(0)
+        nbytes = _lib.cb_prompt_attention_scratch(tq, tk, h, n - 1, d, cbytes)
+        counts, partial = _attention_scratch(device, dev, stream, cbytes.value // 4, nbytes) if nbytes else (None, None)
         _rc(_lib.cb_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, out.data_ptr(), tq, tk, h, hkv, d,
                                      _DTYPE[dtype], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), n - 1, scale,
-                                     1 if causal else 0, _raw_stream(dev)))
+                                     1 if causal else 0, None if counts is None else counts.data_ptr(), cbytes.value,
+                                     None if partial is None else partial.data_ptr(), nbytes, stream))
     return out

@@ -61,7 +61,7 @@ class KV4Cache:
             raise ValueError("KV4Cache: dtype must be float16 or bfloat16")
         pages = torch.empty(n_pages, kv_heads, page_size // 16 * block, dtype=torch.uint8, device=device)
         if pages.is_cuda:
-            c.kv4_prepare_device(pages.device)
+            c.prepare_attention(pages.device)
         return KV4Cache(pages, int(head_dim), int(page_size), int(group_size), dtype)
 
     @property

@@ -31,9 +31,10 @@ namespace cb {
 namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
+constexpr int kMinPart = 6, kPartsOfGrid = 2;         // a part has that many key tiles or more, and there are about that many to a CTA
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kFixWarp = 10, kThreads = 384;
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
-constexpr int kSoftRegs = 200, kOtherRegs = 104;
+constexpr int kSoftRegs = 216, kOtherRegs = 72;
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
 
 __device__ int g_prompt_status;
@@ -45,6 +46,11 @@ struct PromptParams {
     float scale_log2;                                 // |scale| * log2(e), above 0
     int negate;                                       // the scale is negative: the products with q are negated
     int causal;
+    // Few tiles: their keys are cut into parts, which leave (O, m, l) in `partial`, one slot for an item of the list; the last of a
+    // tile's parts to finish joins them.  counters: 8 for an item (of a tile's first part: one for each softmax warp), zero between calls.
+    float* partial;                                   // nullptr: tiles are not cut
+    int* counters;
+    int64_t items;                                    // that there is room for
 };
 
 template <int D>
@@ -195,18 +201,25 @@ template <int O, int N> __device__ __forceinline__ void tmem_ld_wait32(uint32_t 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // The work of a CTA, in order: every role walks through the same list by itself.  Tiles are ordered by their place in their
-// sequence, the last ones (with the causal bound: the longest) first, heads innermost; CTA i takes item i of the first
+// sequence, the last ones (with the causal bound: the longest) first, then parts of their keys, heads innermost; CTA i takes item i of the first
 // gridDim.x, then in turn the mirrored and the same place of the following ones.
 struct Work {
-    int head, row0, lq, lk, q_first, k_first;         // row0: the tile's first query row in its sequence
-    int n[2];                                         // key tiles of the sub-tiles
+    int head, row0, lq, lk, q_first, k_first;         // row0: the tile's first query row in its sequence; k_first, lk: from the part's first key on
+    int n[2];                                         // key tiles of the sub-tiles, in this part
+    int parts, part, slot0;                           // slot0: item of the tile's and head's first part; part i's is slot0 + i * H
 };
 struct Walk {
     const PromptParams& P;
-    int lane, level, round = 0, my_tiles = 0;
+    int lane, level, round = 0, my_tiles = 0, cut = 0x7fffffff;       // cut: key tiles of a part, at most
     int64_t above = 0;                                // tiles of higher levels
+    int64_t rank_now = 0, items_before = 0;           // of cut lists: the tile last looked at, and the items before it
     __device__ __forceinline__ int lens(int b, int& first) const {
         const int s = min(max(P.cu_q[b], 0), P.Tq), e = min(max(P.cu_q[b + 1], s), P.Tq);
+        first = s;
+        return e - s;
+    }
+    __device__ __forceinline__ int keys(int b, int& first) const {
+        const int s = min(max(P.cu_k[b], 0), P.Tk), e = min(max(P.cu_k[b + 1], s), P.Tk);
         first = s;
         return e - s;
     }
@@ -214,18 +227,29 @@ struct Walk {
         int first;
         return b < P.B ? (int)(((int64_t)lens(b, first) + kTileQ - 1) / kTileQ) : 0;
     }
+    // key tiles that the `rows` query rows from r0 on see together
+    __device__ __forceinline__ int key_tiles(int r0, int rows, int lq, int lk) const {
+        int64_t n = lk;
+        if (P.causal) n = min(n, (int64_t)r0 + rows + (lk - lq));
+        return rows <= 0 || n <= 0 ? 0 : (int)((n + kTileK - 1) / kTileK);
+    }
     __device__ Walk(const PromptParams& p, int l) : P(p), lane(l) {
         int top = 0;
         my_tiles = tiles_of(lane);                    // of sequence `lane`: all there are with up to 32 sequences
         for (int b0 = 0; b0 < P.B; b0 += 32) top = max(top, tiles_of(b0 + lane));
         level = __reduce_max_sync(0xffffffffu, top) - 1;
+        if (P.partial == nullptr) return;
+        int all = 0;                                  // key tiles of a head (there are few: the list is cut only where tiles are)
+        for (int b = lane; b < P.B; b += 32) {
+            int first;
+            const int lq = lens(b, first), lk = keys(b, first);
+            for (int r0 = 0; r0 < lq; r0 += kTileQ) all += key_tiles(r0, min(lq - r0, kTileQ), lq, lk);
+        }
+        all = __reduce_add_sync(0xffffffffu, all);
+        cut = max(kMinPart, (int)(((int64_t)all * P.H + kPartsOfGrid * gridDim.x - 1) / (kPartsOfGrid * gridDim.x)));
     }
-    __device__ bool next(Work& w) {
-        const int64_t place = (round & 1) ? (int64_t)(gridDim.x - 1 - blockIdx.x) : (int64_t)blockIdx.x;
-        const int64_t item = (int64_t)round * gridDim.x + place;
-        ++round;
-        const int64_t rank = item / P.H;
-        w.head = (int)(item - rank * P.H);
+    // The rank-th tile of a head, ranks rising from call to call.
+    __device__ bool tile_at(int64_t rank, Work& w) {
         for (; level >= 0; --level) {
             int64_t seen = above;
             for (int b0 = 0; b0 < P.B; b0 += 32) {
@@ -237,17 +261,10 @@ struct Walk {
                     const bool me = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == want;
                     const int b = b0 + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
                     w.lq = lens(b, w.q_first);
-                    const int s = min(max(P.cu_k[b], 0), P.Tk), e = min(max(P.cu_k[b + 1], s), P.Tk);
-                    w.k_first = s;
-                    w.lk = e - s;
+                    w.lk = keys(b, w.k_first);
                     w.row0 = level * kTileQ;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int r0 = w.row0 + x * kSub, rows = min(w.lq - r0, kSub);
-                        int64_t keys = w.lk;
-                        if (P.causal) keys = min(keys, (int64_t)r0 + rows + (w.lk - w.lq));
-                        w.n[x] = rows <= 0 || keys <= 0 ? 0 : (int)((keys + kTileK - 1) / kTileK);
-                    }
+                    for (int x = 0; x < 2; ++x) w.n[x] = key_tiles(w.row0 + x * kSub, min(w.lq - w.row0 - x * kSub, kSub), w.lq, w.lk);
                     return true;
                 }
                 seen += cnt;
@@ -255,6 +272,36 @@ struct Walk {
             above = seen;
         }
         return false;
+    }
+    __device__ bool next(Work& w) {
+        const int64_t place = (round & 1) ? (int64_t)(gridDim.x - 1 - blockIdx.x) : (int64_t)blockIdx.x;
+        const int64_t item = (int64_t)round * gridDim.x + place;
+        ++round;
+        if (P.partial == nullptr) {
+            const int64_t rank = item / P.H;
+            w.head = (int)(item - rank * P.H);
+            w.parts = 1; w.part = 0;
+            return tile_at(rank, w);
+        }
+        for (;; ++rank_now) {
+            if (!tile_at(rank_now, w)) return false;
+            const int n = max(w.n[0], w.n[1]);
+            w.parts = n <= cut ? 1 : (n + cut - 1) / cut;
+            if (items_before + (int64_t)w.parts * P.H > P.items) w.parts = 1;       // only if sequences overlap
+            const int64_t count = (int64_t)w.parts * P.H;
+            if (item < items_before + count) break;
+            items_before += count;
+        }
+        const int local = (int)(item - items_before), n = max(w.n[0], w.n[1]);
+        w.part = local / P.H;
+        w.head = local - w.part * P.H;
+        w.slot0 = (int)items_before + w.head;
+        const int each = n / w.parts, more = n - each * w.parts, j0 = each * w.part + min(w.part, more), cnt = each + (w.part < more ? 1 : 0);
+        w.k_first += j0 * kTileK;
+        w.lk -= j0 * kTileK;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) w.n[x] = min(max(w.n[x] - j0, 0), cnt);
+        return true;
     }
 };
 
@@ -464,7 +511,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             const int n = w.n[x], r = w.row0 + x * kSub + row;    // query row in its sequence
             const bool live = r < w.lq;
             T* dst = reinterpret_cast<T*>(P.out) + ((int64_t)(w.q_first + r) * P.H + w.head) * D;
-            if (n == 0) {                                         // rows that see no key
+            if (n == 0 && w.parts == 1) {                         // rows that see no key
                 if (live)
                     for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4*>(dst + d) = make_uint4(0u, 0u, 0u, 0u);
                 continue;
@@ -558,29 +605,85 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 l += l0 + l1;
             }
             if (gave_up) break;
-            if (!__all_sync(0xffffffffu, mbar_wait(pv_done(x), (count - 1) & 1, abort_flag))) { gave_up = 4; break; }
-            fence_after();
+            if (n > 0) {
+                if (!__all_sync(0xffffffffu, mbar_wait(pv_done(x), (count - 1) & 1, abort_flag))) { gave_up = 4; break; }
+                fence_after();
+            }
+            // a cut tile: O[d][row], m[row], l[row] of this part and sub-tile
+            constexpr int kPart = kSub * (D + 2);
+            auto part_at = [&](int part) { return P.partial + ((int64_t)(w.slot0 + part * P.H) * 2 + x) * kPart + row; };
             const float inv = l == 0.f ? 0.f : 1.f / l;
+            auto store32 = [&](int c, const uint32_t (&v)[32]) {  // 32 finished values
+                if (!live) return;
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-                uint32_t v[32];
-                tmem_ld32<0>(o_addr + c, v);
-                tmem_ld_wait32<0>(v);
-                if (c + 32 == D) {
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(o_free(x));
+                for (int i = 0; i < 32; i += 8) {
+                    uint32_t y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        y[k] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[i + 2 * k]) * inv, __uint_as_float(v[i + 2 * k + 1]) * inv);
+                    *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
-                if (live) {
+            };
+            if (n > 0) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint32_t y[4];
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld32<0>(o_addr + c, v);
+                    tmem_ld_wait32<0>(v);
+                    if (c + 32 == D) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(o_free(x));
+                    }
+                    if (w.parts == 1) store32(c, v);
+                    else {
+                        float* at = part_at(w.part) + c * kSub;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            y[k] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[i + 2 * k]) * inv, __uint_as_float(v[i + 2 * k + 1]) * inv);
-                        *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        for (int i = 0; i < 32; ++i) __stcg(at + i * kSub, __uint_as_float(v[i]));
                     }
                 }
+            }
+            if (w.parts == 1) continue;
+            __stcg(part_at(w.part) + D * kSub, m_ref);
+            __stcg(part_at(w.part) + (D + 1) * kSub, l);
+            __syncwarp();
+            int last = 0;
+            if (lane == 0) {
+                int* counter = P.counters + ((int64_t)w.slot0 * 2 + x) * 4 + quad;
+                __threadfence();
+                last = atomicAdd(counter, 1) == w.parts - 1;
+                if (last) *counter = 0;
+                __threadfence();
+            }
+            if (__shfl_sync(0xffffffffu, last, 0) == 0) continue;
+            // this warp's rows are complete in all parts: joined in their order
+            float top = -INFINITY, sum = 0.f;
+            for (int i = 0; i < w.parts; ++i) top = fmaxf(top, __ldcg(part_at(i) + D * kSub));
+            for (int i = 0; i < w.parts; ++i) {
+                const float m = __ldcg(part_at(i) + D * kSub);
+                if (m != -INFINITY) sum = fmaf(ex2(m - top), __ldcg(part_at(i) + (D + 1) * kSub), sum);
+            }
+            const float rsum = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 64) {                     // 64 loads on their way at a time
+                float v[64];
+#pragma unroll
+                for (int k = 0; k < 64; ++k) v[k] = 0.f;
+#pragma unroll 1
+                for (int i = 0; i < w.parts; ++i) {
+                    const float* at = part_at(i);
+                    const float m = __ldcg(at + D * kSub);
+                    float o[64];
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) o[k] = __ldcg(at + (c + k) * kSub);
+                    const float f = m == -INFINITY ? 0.f : ex2(m - top) * rsum;
+#pragma unroll
+                    for (int k = 0; k < 64; ++k) v[k] = m == -INFINITY ? v[k] : fmaf(f, o[k], v[k]);
+                }
+                if (live)
+#pragma unroll
+                    for (int k = 0; k < 64; k += 8)
+                        *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(pack2<T>(v[k], v[k + 1]), pack2<T>(v[k + 2], v[k + 3]), pack2<T>(v[k + 4], v[k + 5]), pack2<T>(v[k + 6], v[k + 7]));
             }
         }
     }
@@ -627,10 +730,19 @@ int launch_prompt_t(const CUtensorMap (&maps)[3], const PromptParams& P, int gri
 
 }  // namespace
 
+// How many items a list of these sizes can have when its tiles may be cut (0: they are not).  Cut where there are fewer tiles than two for each SM and a
+// sequence has 1024 keys or more on average: below that a tile's keys are few, above it the tiles alone keep the SMs busy.
+int64_t prompt_attention_items(int64_t Tq, int64_t Tk, int64_t H, int64_t B) {
+    const int sms = sm_count_current();
+    const int64_t tiles = (Tq / kTileQ + B) * H;
+    return sms <= 0 || tiles >= 2 * (int64_t)sms || Tk < 1024 * B ? 0 : tiles + kPartsOfGrid * sms;
+}
+size_t prompt_attention_partial_bytes(int64_t items, int head_dim) { return (size_t)items * kTileQ * (head_dim + 2) * sizeof(float); }
+
 // Arguments are checked by the caller.  strides: {q token, q head, k token, k head, v token, v head} in elements.
 int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
                             int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
-                            float scale, int causal, cudaStream_t stream) {
+                            float scale, int causal, int* counters, float* partial, cudaStream_t stream) {
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
     EncodeTiledFn enc = encode_fn();
@@ -656,8 +768,9 @@ int launch_prompt_attention(const void* q, const void* k, const void* v, const i
     P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
     P.negate = scale < 0.f ? 1 : 0;
     P.causal = causal ? 1 : 0;
+    P.counters = counters; P.partial = partial; P.items = partial != nullptr ? prompt_attention_items(Tq, Tk, H, B) : 0;
     const int64_t most = (Tq / kTileQ + B) * H;                   // tiles there can be
-    const int grid = (int)std::min<int64_t>(sms, most);
+    const int grid = partial != nullptr ? sms : (int)std::min<int64_t>(sms, most);
     const bool bf = dtype == CB_BF16;
     if (head_dim == 128) return bf ? launch_prompt_t<__nv_bfloat16, 128>(maps, P, grid, stream) : launch_prompt_t<__half, 128>(maps, P, grid, stream);
     return bf ? launch_prompt_t<__nv_bfloat16, 64>(maps, P, grid, stream) : launch_prompt_t<__half, 64>(maps, P, grid, stream);

@@ -14,7 +14,7 @@ def test_c_entry_point_refuses_bad_arguments():
     lib, s6 = _C._lib, (ctypes.c_int64 * 6)(*[128] * 6)
 
     def call(q=256, k=256, v=256, st=s6, out=256, tq=4, tk=4, h=2, hkv=2, d=64, dt=1, cq=256, ck=256, b=1):
-        return lib.cb_prompt_attention(q, k, v, st, out, tq, tk, h, hkv, d, dt, cq, ck, b, 1.0, 1, 0)
+        return lib.cb_prompt_attention(q, k, v, st, out, tq, tk, h, hkv, d, dt, cq, ck, b, 1.0, 1, 0, 0, 0, 0, 0)
 
     for bad in (dict(dt=0), dict(dt=3), dict(d=96), dict(d=256), dict(tq=-1), dict(tk=-1), dict(tq=1 << 30), dict(h=3), dict(hkv=0), dict(b=-1),
                 dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(cq=0), dict(ck=0), dict(st=None), dict(q=8), dict(k=8), dict(v=8),
@@ -132,6 +132,53 @@ def test_a_long_prompt_and_rising_scores():
         check(ck.prompt_attention(q, k, v, i32([0, n])), reference(q, k, v, [0, n], [0, n]))
         k = k.flip(0).contiguous()
         check(ck.prompt_attention(q, k, v, i32([0, n])), reference(q, k, v, [0, n], [0, n]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d,causal", [(torch.float16, 64, True), (torch.bfloat16, 128, True), (torch.float16, 128, False)])
+@pytest.mark.parametrize("lens,past", [([300], [9000]), ([1], [4096]), ([130, 0, 257, 5], [5000, 700, 0, 6001]), ([3000], [0]), ([64, 64], [3968, 0])])
+def test_keys_cut_into_parts(dtype, d, causal, lens, past):
+    """Few tiles over many keys: their keys are shared out among the SMs."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    cq, ckv = offsets(lens), offsets([n + p for n, p in zip(lens, past)])
+    assert _C._lib.cb_prompt_attention_scratch(cq[-1], ckv[-1], 4, len(lens), d, None) > 0
+    q, k, v = rand(cq[-1], 4, d, dtype, 1), rand(ckv[-1], 2, d, dtype, 2), rand(ckv[-1], 2, d, dtype, 3)
+    k = (k.float() * torch.linspace(0.1, 2.0, ckv[-1], device=DEV)[:, None, None]).to(dtype)
+    want = reference(q, k, v, cq, ckv, causal=causal)
+    first = ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal)
+    check(first, want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for s in streams * 3:
+        with torch.cuda.stream(s):
+            outs.append(ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal))
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        a, b = i32(cq), i32(ckv)
+        with torch.cuda.graph(g):
+            outs.append(ck.prompt_attention(q, k, v, a, b, causal=causal))
+        graphs.append((g, a, b))
+    for _ in range(3):
+        for (g, *_), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(first, o) for o in outs)
+
+
+@pytest.mark.gpu
+def test_bounds_that_overlap_stay_inside_the_scratch():
+    """Sequences that name the same rows again and again: more tiles than the list has room for in parts."""
+    import crispybits_kernels as ck
+    n = 3000
+    q, k, v = rand(n, 1, 64, torch.float16, 1), rand(4 * n, 1, 64, torch.float16, 2), rand(4 * n, 1, 64, torch.float16, 3)
+    B = 11
+    cu, cu_k = i32([0, n] * (B // 2) + [0, n]), i32([0, 4 * n] * (B // 2) + [0, 4 * n])
+    got = ck.prompt_attention(q, k, v, cu, cu_k, causal=False)
+    check(got, reference(q, k, v, [0, n], [0, 4 * n], causal=False))
 
 
 @pytest.mark.gpu
