@@ -287,7 +287,7 @@ int cb_decode_plan(int bits, int64_t B, int64_t V, int64_t K, int64_t split_k, i
  * weights-in-TMEM kernel) = in the tensor-core GEMM role r (1 activation producer, 2 MMA issuer,
  * 3 dequantiser, 4 epilogue, 5 packed-word producer) gave up a bounded wait; 3001 = a kernel of the 4-bit cache met a position
  * outside its page table or a page number outside the cache and left it out, 3002 = a copy of the cache's attention did not
- * arrive in time and outputs were not written; 4000 + r = role r of the prompt attention (1 TMA, 2 MMA, 3 softmax, 4 epilogue, 5 tile ends) gave up a
+ * arrive in time and outputs were not written; 4000 + r = role r of the prompt attention (1 TMA, 2 MMA, 3 softmax, 4 epilogue, 5 tile ends, 6 the walk) gave up a
  * bounded wait.  No counterpart in the reference. */
 int cb_decode_status(int* status);
 
@@ -356,15 +356,14 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * dtype CB_F16 or CB_BF16.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
  * behind a query's last one are not used, except that an infinity or a NaN in v makes NaN of that value for
  * queries up to 127 positions before it.
- * Scratch lets few prompts use all SMs: the keys of their tiles are cut into parts and joined in order, so that the result stays the same
- * from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, any content) and, in *counter_bytes, of
- * `counters` (zeroed ONCE, left zero by every call); 0: nothing would be cut.  Both may be NULL: then nothing is.  Calls that may overlap
- * on the GPU need their own. */
+ * The work is cut into equal parts for the SMs, whatever the lengths are; where a cut falls inside a tile, its parts meet in scratch and are joined in
+ * order, so that the result is the same from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, of any
+ * content) and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call).  Calls that may overlap on the GPU need their own. */
 int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
                         int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
                         float scale, int causal, void* counters, size_t counter_bytes, void* partial, size_t partial_bytes,
                         void* stream);
-size_t cb_prompt_attention_scratch(int64_t Tq, int64_t Tk, int64_t H, int64_t B, int head_dim, size_t* counter_bytes);
+size_t cb_prompt_attention_scratch(int head_dim, size_t* counter_bytes);
 
 #ifdef __cplusplus
 }

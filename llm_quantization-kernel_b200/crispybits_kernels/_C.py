@@ -758,6 +758,7 @@ def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
 _attention_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
 _attention_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
 _ATTENTION_SLAB = 1 << 18
+_prompt_bytes: Dict[Tuple[int, int], Tuple[int, int]] = {}   # (device index, head_dim) -> bytes of counters and partial, cb_prompt_attention_scratch
 _partial_bytes: Dict[Tuple[int, bool, int], int] = {}      # (device index, more than 8 rows, head_dim) -> cb_kv4_attention_partial_bytes
 
 
@@ -827,7 +828,7 @@ def kv4_attention(q, cache, page_table, lengths, scale: float):
 _lib.cb_prompt_attention.argtypes = [_vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _i64,
                                      ctypes.c_float, _int, _vp, _sz, _vp, _sz, _vp]
 _lib.cb_prompt_attention.restype = _int
-_lib.cb_prompt_attention_scratch.argtypes = [_i64, _i64, _i64, _i64, _int, ctypes.POINTER(_sz)]
+_lib.cb_prompt_attention_scratch.argtypes = [_int, ctypes.POINTER(_sz)]
 _lib.cb_prompt_attention_scratch.restype = _sz
 
 
@@ -874,11 +875,13 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bo
     q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)
     strides = (_i64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
     with _on_device(device):
-        stream, cbytes = _raw_stream(dev), _sz(0)
-        nbytes = _lib.cb_prompt_attention_scratch(tq, tk, h, n - 1, d, cbytes)
-        counts, partial = _attention_scratch(device, dev, stream, cbytes.value // 4, nbytes) if nbytes else (None, None)
+        stream, sizes = _raw_stream(dev), _prompt_bytes.get((dev, d))
+        if sizes is None:
+            cbytes = _sz(0)
+            nbytes = _lib.cb_prompt_attention_scratch(d, cbytes)
+            sizes = _prompt_bytes[(dev, d)] = (cbytes.value, nbytes)
+        counts, partial = _attention_scratch(device, dev, stream, sizes[0] // 4, sizes[1])
         _rc(_lib.cb_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, out.data_ptr(), tq, tk, h, hkv, d,
                                      _DTYPE[dtype], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), n - 1, scale,
-                                     1 if causal else 0, None if counts is None else counts.data_ptr(), cbytes.value,
-                                     None if partial is None else partial.data_ptr(), nbytes, stream))
+                                     1 if causal else 0, counts.data_ptr(), sizes[0], partial.data_ptr(), sizes[1], stream))
     return out

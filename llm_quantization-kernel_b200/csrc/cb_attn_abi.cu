@@ -16,8 +16,8 @@ size_t kv4_attention_partial_bytes(int64_t rows, int head_dim);
 int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
                             int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
                             float scale, int causal, int* counters, float* partial, cudaStream_t stream);
-int64_t prompt_attention_items(int64_t Tq, int64_t Tk, int64_t H, int64_t B);
-size_t prompt_attention_partial_bytes(int64_t items, int head_dim);
+size_t prompt_attention_partial_bytes(int head_dim);
+size_t prompt_attention_counter_bytes();
 
 namespace {
 
@@ -119,10 +119,9 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
                                 reinterpret_cast<cudaStream_t>(stream));
 }
 
-size_t cb_prompt_attention_scratch(int64_t Tq, int64_t Tk, int64_t H, int64_t B, int head_dim, size_t* counter_bytes) {
-    const int64_t items = Tq > 0 && Tk > 0 && H > 0 && B > 0 ? prompt_attention_items(Tq, Tk, H, B) : 0;
-    if (counter_bytes != nullptr) *counter_bytes = (size_t)items * 8 * sizeof(int);
-    return prompt_attention_partial_bytes(items, head_dim);
+size_t cb_prompt_attention_scratch(int head_dim, size_t* counter_bytes) {
+    if (counter_bytes != nullptr) *counter_bytes = prompt_attention_counter_bytes();
+    return prompt_attention_partial_bytes(head_dim);
 }
 
 int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
@@ -143,13 +142,11 @@ int cb_prompt_attention(const void* q, const void* k, const void* v, const int64
         CB_REQUIRE(used <= 1 || (strides6[i] > 0 && strides6[i] % 8 == 0 && strides6[i] < (1ll << 38)),
                    "%s: strides must be positive multiples of 8 elements", who);
     }
-    const int64_t items = counters != nullptr && partial != nullptr ? prompt_attention_items(Tq, Tk, H, B) : 0;
-    if (items > 0)
-        CB_REQUIRE(counter_bytes >= (size_t)items * 8 * sizeof(int) && partial_bytes >= prompt_attention_partial_bytes(items, head_dim) && aligned16(partial),
-                   "%s: scratch is too small (cb_prompt_attention_scratch)", who);
+    CB_REQUIRE(counters != nullptr && counter_bytes >= prompt_attention_counter_bytes() && partial != nullptr && aligned16(partial) &&
+                   partial_bytes >= prompt_attention_partial_bytes(head_dim),
+               "%s: scratch is missing or too small (cb_prompt_attention_scratch)", who);
     return launch_prompt_attention(q, k, v, strides6, out, Tq, Tk, H, Hkv, head_dim, dtype, cu_q, cu_k, B, scale, causal,
-                                   items > 0 ? reinterpret_cast<int*>(counters) : nullptr, items > 0 ? reinterpret_cast<float*>(partial) : nullptr,
-                                   reinterpret_cast<cudaStream_t>(stream));
+                                   reinterpret_cast<int*>(counters), reinterpret_cast<float*>(partial), reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

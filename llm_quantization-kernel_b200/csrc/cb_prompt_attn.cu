@@ -12,8 +12,8 @@
 // rounding is relative.  p is rounded to the inputs' type; the sum l takes the unrounded p.
 //
 // TMEM map (512 columns): S0/P0 [0, 128), S1/P1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D).
-// Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 zeros behind the last
-// key (below), 11 nothing (it completes the warpgroup that gives registers to the softmax warps, which hold a whole row of scores).
+// Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 the walk through
+// the work, 11 zeros behind the last key (below).  Warps 8-11 give registers to the softmax warps, which hold a whole row of scores.
 //
 // V rows behind the last key of a sequence belong to another sequence (or to nothing): they are zeroed in shared memory, since 0 *
 // inf is not 0.  K rows there only make scores that are masked.
@@ -31,8 +31,9 @@ namespace cb {
 namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
-constexpr int kMinPart = 6, kPartsOfGrid = 2;         // a part has that many key tiles or more, and there are about that many to a CTA
-constexpr int kTmaWarp = 8, kMmaWarp = 9, kFixWarp = 10, kThreads = 384;
+constexpr int kOpen = 4;                              // what a CTA spends on a (tile, head) besides its products, in key tiles
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kWalkWarp = 10, kFixWarp = 11, kThreads = 384;
+constexpr int kQueue = 4, kReaders = 11;              // steps of work handed on at a time, to 8 softmax warps, TMA, MMA and the fixing warp
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
 constexpr int kSoftRegs = 216, kOtherRegs = 72;
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
@@ -46,11 +47,10 @@ struct PromptParams {
     float scale_log2;                                 // |scale| * log2(e), above 0
     int negate;                                       // the scale is negative: the products with q are negated
     int causal;
-    // Few tiles: their keys are cut into parts, which leave (O, m, l) in `partial`, one slot for an item of the list; the last of a
-    // tile's parts to finish joins them.  counters: 8 for an item (of a tile's first part: one for each softmax warp), zero between calls.
-    float* partial;                                   // nullptr: tiles are not cut
+    // Where the line of work is cut inside a (tile, head), the parts leave (O, m, l) in `partial`, two slots for a CTA, and the last to finish joins
+    // them.  counters: 8 for a CTA (of a cut tile's first part: one for each softmax warp), zero between calls.
+    float* partial;
     int* counters;
-    int64_t items;                                    // that there is room for
 };
 
 template <int D>
@@ -61,7 +61,8 @@ struct PromptCfg {
     static constexpr int kPolyOf8 = D == 64 ? 2 : 0;
     static constexpr int kSlots = D == 128 ? 4 : 8;                         // ring of K and V tiles
     static constexpr uint32_t kQOff = 0, kRingOff = 2 * kTileBytes, kBarOff = kRingOff + kSlots * kTileBytes;
-    static constexpr uint32_t kSmem = kBarOff + 256 + 1024;
+    static constexpr uint32_t kQueueOff = kBarOff + 384;                    // kQueue steps of work
+    static constexpr uint32_t kSmem = kQueueOff + kQueue * 64 + 1024;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -200,110 +201,132 @@ template <int O, int N> __device__ __forceinline__ void tmem_ld_wait32(uint32_t 
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The work of a CTA, in order: every role walks through the same list by itself.  Tiles are ordered by their place in their
-// sequence, the last ones (with the causal bound: the longest) first, then parts of their keys, heads innermost; CTA i takes item i of the first
-// gridDim.x, then in turn the mirrored and the same place of the following ones.
-struct Work {
-    int head, row0, lq, lk, q_first, k_first;         // row0: the tile's first query row in its sequence; k_first, lk: from the part's first key on
+// The work: all (tile of 256 query rows, head) pairs, sequence after sequence, heads innermost, form one line of key tiles (and kOpen more ahead of each
+// pair's) that is cut into equal parts, one for each CTA.  One warp walks through the CTA's part, a few steps ahead, and hands the steps to the others
+// through a queue in shared memory.
+struct Work {                                         // head < 0: the end
+    int head, row0, lq, lk, q_first, k_first;         // row0: the tile's first query row in its sequence; k_first, lk: from this part's first key on
     int n[2];                                         // key tiles of the sub-tiles, in this part
-    int parts, part, slot0;                           // slot0: item of the tile's and head's first part; part i's is slot0 + i * H
+    int parts, slot, cta0, odd0;                      // parts of this tile and head; this one's slot of scratch; part i's is (cta0 + i) * 2 (+ odd0 for i = 0)
 };
 struct Walk {
-    const PromptParams& P;
-    int lane, level, round = 0, my_tiles = 0, cut = 0x7fffffff;       // cut: key tiles of a part, at most
-    int64_t above = 0;                                // tiles of higher levels
-    int64_t rank_now = 0, items_before = 0;           // of cut lists: the tile last looked at, and the items before it
-    __device__ __forceinline__ int lens(int b, int& first) const {
-        const int s = min(max(P.cu_q[b], 0), P.Tq), e = min(max(P.cu_q[b + 1], s), P.Tq);
-        first = s;
-        return e - s;
+    int64_t u, u0, u1, base, share, extra;            // base: the present sequence's first unit
+    int b, lq, lk, q_first, k_first;
+};
+__device__ __forceinline__ int row_range(const int32_t* cu, int b, int rows, int& first) {
+    const int s = min(max(cu[b], 0), rows), e = min(max(cu[b + 1], s), rows);
+    first = s;
+    return e - s;
+}
+// Key tiles that the `rows` query rows from r0 on see together.
+__device__ __forceinline__ int key_tiles(const PromptParams& P, int r0, int rows, int lq, int lk) {
+    int64_t n = lk;
+    if (P.causal) n = min(n, (int64_t)r0 + rows + (lk - lq));
+    return rows <= 0 || n <= 0 ? 0 : (int)((n + kTileK - 1) / kTileK);
+}
+// Units of the first t tiles of a sequence.  Under the causal bound tile i (of 256 rows) sees 2 (i + 1) + o key tiles, o = ceil((lk - lq) / 128),
+// or none; only the last tile may have fewer rows.
+__device__ __forceinline__ int64_t units_before(const PromptParams& P, int t, int lq, int lk) {
+    const int tiles = (int)(((int64_t)lq + kTileQ - 1) / kTileQ), full = min(t, tiles - 1);
+    int64_t n = 0;
+    if (!P.causal) n = (int64_t)full * key_tiles(P, 0, 1, lq, lk);
+    else {
+        const int64_t off = (int64_t)lk - lq, o = off >= 0 ? (off + kTileK - 1) / kTileK : -(-off / kTileK);
+        const int64_t from = o < 0 ? min(-o / 2, (int64_t)full) : 0;      // tiles before it see nothing
+        n = ((int64_t)full * (full + 1) - from * (from + 1)) + (full - from) * o;
     }
-    __device__ __forceinline__ int keys(int b, int& first) const {
-        const int s = min(max(P.cu_k[b], 0), P.Tk), e = min(max(P.cu_k[b + 1], s), P.Tk);
-        first = s;
-        return e - s;
-    }
-    __device__ __forceinline__ int tiles_of(int b) const {
+    if (t >= tiles && tiles > 0) n += key_tiles(P, (tiles - 1) * kTileQ, lq - (tiles - 1) * kTileQ, lq, lk);
+    return (n + (int64_t)kOpen * max(t, 0)) * P.H;
+}
+__device__ __forceinline__ int64_t units_of(const PromptParams& P, int lq, int lk) {
+    return lq <= 0 ? 0 : units_before(P, (int)(((int64_t)lq + kTileQ - 1) / kTileQ), lq, lk);
+}
+
+// All lanes of a warp call these two together.  false: this CTA has nothing (more) to do.
+__device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk& walk) {
+    int64_t U = 0;
+    for (int b = lane; b < P.B; b += 32) {
         int first;
-        return b < P.B ? (int)(((int64_t)lens(b, first) + kTileQ - 1) / kTileQ) : 0;
+        U += units_of(P, row_range(P.cu_q, b, P.Tq, first), row_range(P.cu_k, b, P.Tk, first));
     }
-    // key tiles that the `rows` query rows from r0 on see together
-    __device__ __forceinline__ int key_tiles(int r0, int rows, int lq, int lk) const {
-        int64_t n = lk;
-        if (P.causal) n = min(n, (int64_t)r0 + rows + (lk - lq));
-        return rows <= 0 || n <= 0 ? 0 : (int)((n + kTileK - 1) / kTileK);
-    }
-    __device__ Walk(const PromptParams& p, int l) : P(p), lane(l) {
-        int top = 0;
-        my_tiles = tiles_of(lane);                    // of sequence `lane`: all there are with up to 32 sequences
-        for (int b0 = 0; b0 < P.B; b0 += 32) top = max(top, tiles_of(b0 + lane));
-        level = __reduce_max_sync(0xffffffffu, top) - 1;
-        if (P.partial == nullptr) return;
-        int all = 0;                                  // key tiles of a head (there are few: the list is cut only where tiles are)
-        for (int b = lane; b < P.B; b += 32) {
-            int first;
-            const int lq = lens(b, first), lk = keys(b, first);
-            for (int r0 = 0; r0 < lq; r0 += kTileQ) all += key_tiles(r0, min(lq - r0, kTileQ), lq, lk);
-        }
-        all = __reduce_add_sync(0xffffffffu, all);
-        cut = max(kMinPart, (int)(((int64_t)all * P.H + kPartsOfGrid * gridDim.x - 1) / (kPartsOfGrid * gridDim.x)));
-    }
-    // The rank-th tile of a head, ranks rising from call to call.
-    __device__ bool tile_at(int64_t rank, Work& w) {
-        for (; level >= 0; --level) {
-            int64_t seen = above;
-            for (int b0 = 0; b0 < P.B; b0 += 32) {
-                const int nt = P.B <= 32 ? my_tiles : tiles_of(b0 + lane);
-                const unsigned has = __ballot_sync(0xffffffffu, nt > level);
-                const int cnt = __popc(has);
-                if (rank < seen + cnt) {
-                    const int want = (int)(rank - seen);
-                    const bool me = ((has >> lane) & 1u) && __popc(has & ((1u << lane) - 1u)) == want;
-                    const int b = b0 + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
-                    w.lq = lens(b, w.q_first);
-                    w.lk = keys(b, w.k_first);
-                    w.row0 = level * kTileQ;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) w.n[x] = key_tiles(w.row0 + x * kSub, min(w.lq - w.row0 - x * kSub, kSub), w.lq, w.lk);
-                    return true;
-                }
-                seen += cnt;
-            }
-            above = seen;
-        }
-        return false;
-    }
-    __device__ bool next(Work& w) {
-        const int64_t place = (round & 1) ? (int64_t)(gridDim.x - 1 - blockIdx.x) : (int64_t)blockIdx.x;
-        const int64_t item = (int64_t)round * gridDim.x + place;
-        ++round;
-        if (P.partial == nullptr) {
-            const int64_t rank = item / P.H;
-            w.head = (int)(item - rank * P.H);
-            w.parts = 1; w.part = 0;
-            return tile_at(rank, w);
-        }
-        for (;; ++rank_now) {
-            if (!tile_at(rank_now, w)) return false;
-            const int n = max(w.n[0], w.n[1]);
-            w.parts = n <= cut ? 1 : (n + cut - 1) / cut;
-            if (items_before + (int64_t)w.parts * P.H > P.items) w.parts = 1;       // only if sequences overlap
-            const int64_t count = (int64_t)w.parts * P.H;
-            if (item < items_before + count) break;
-            items_before += count;
-        }
-        const int local = (int)(item - items_before), n = max(w.n[0], w.n[1]);
-        w.part = local / P.H;
-        w.head = local - w.part * P.H;
-        w.slot0 = (int)items_before + w.head;
-        const int each = n / w.parts, more = n - each * w.parts, j0 = each * w.part + min(w.part, more), cnt = each + (w.part < more ? 1 : 0);
-        w.k_first += j0 * kTileK;
-        w.lk -= j0 * kTileK;
+    for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
+    const int64_t nc = min((int64_t)gridDim.x, U);
+    if ((int64_t)blockIdx.x >= nc) return false;
+    const int64_t share = U / nc, extra = U - share * nc, c = blockIdx.x;
+    const int64_t u0 = share * c + min(c, extra), u1 = share * (c + 1) + min(c + 1, extra);
+    int64_t base = 0;
+    for (int b0 = 0; b0 < P.B; b0 += 32) {
+        int first_q = 0, first_k = 0;
+        const int b = b0 + lane;
+        const int lq = b < P.B ? row_range(P.cu_q, b, P.Tq, first_q) : 0, lk = b < P.B ? row_range(P.cu_k, b, P.Tk, first_k) : 0;
+        const int64_t mine = units_of(P, lq, lk);
+        int64_t cum = mine;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) w.n[x] = min(max(w.n[x] - j0, 0), cnt);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, cum, o);
+            if (lane >= o) cum += up;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, base + cum > u0);
+        if (past != 0u) {
+            const int l = __ffs(past) - 1;
+            walk.u = walk.u0 = u0; walk.u1 = u1; walk.share = share; walk.extra = extra;
+            walk.base = base + __shfl_sync(0xffffffffu, cum - mine, l);
+            walk.b = b0 + l;
+            walk.lq = __shfl_sync(0xffffffffu, lq, l); walk.lk = __shfl_sync(0xffffffffu, lk, l);
+            walk.q_first = __shfl_sync(0xffffffffu, first_q, l); walk.k_first = __shfl_sync(0xffffffffu, first_k, l);
+            return true;
+        }
+        base += __shfl_sync(0xffffffffu, cum, 31);
+    }
+    return false;
+}
+__device__ __forceinline__ bool walk_next(const PromptParams& P, Walk& walk, Work& w) {
+    int64_t& u = walk.u;
+    int64_t& base = walk.base;
+    const int64_t u0 = walk.u0, u1 = walk.u1, share = walk.share, extra = walk.extra;
+    int &lq = walk.lq, &lk = walk.lk, &q_first = walk.q_first, &k_first = walk.k_first;
+    while (u < u1) {
+        for (int64_t n = units_of(P, lq, lk); u >= base + n; n = units_of(P, lq, lk)) {
+            base += n;
+            if (++walk.b >= P.B) return false;        // only if the bounds changed while the kernel ran
+            lq = row_range(P.cu_q, walk.b, P.Tq, q_first);
+            lk = row_range(P.cu_k, walk.b, P.Tk, k_first);
+        }
+        int lo = 0, hi = (int)(((int64_t)lq + kTileQ - 1) / kTileQ);      // the tile: units_before(lo) <= u - base < units_before(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (units_before(P, mid, lq, lk) <= u - base) lo = mid; else hi = mid;
+        }
+        w.row0 = lo * kTileQ;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) w.n[x] = key_tiles(P, w.row0 + x * kSub, min(lq - w.row0 - x * kSub, kSub), lq, lk);
+        const int n = max(w.n[0], w.n[1]), per = n + kOpen;
+        const int64_t in_tile = u - base - units_before(P, lo, lq, lk);
+        w.head = (int)(in_tile / per);
+        const int part = (int)(in_tile - (int64_t)w.head * per), j0 = max(part - kOpen, 0);
+        const int64_t seg0 = u - part;
+        const int j1 = (int)min((int64_t)n, u1 - seg0 - kOpen);
+        const bool first = u == u0;
+        u = seg0 + per;
+        if (n == 0 ? part > 0 : j1 <= j0) continue;   // rows without keys belong to the CTA of the first unit; of others this is the opening only
+        w.lq = lq; w.q_first = q_first;
+        w.lk = lk - j0 * kTileK; w.k_first = k_first + j0 * kTileK;
+        w.parts = 1; w.slot = w.cta0 = w.odd0 = 0;
+        if (n > 0 && (j0 > 0 || j1 < n)) {
+            auto cta_of = [&](int64_t unit) { return unit < extra * (share + 1) ? unit / (share + 1) : extra + (unit - extra * (share + 1)) / share; };
+            const int64_t c0 = cta_of(seg0 + kOpen);
+            w.cta0 = (int)c0;
+            w.parts = (int)(cta_of(seg0 + per - 1) - c0) + 1;
+            w.slot = (int)blockIdx.x * 2 + (first ? 0 : 1);
+            w.odd0 = share * c0 + min(c0, extra) < seg0 ? 1 : 0;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) w.n[x] = min(max(w.n[x] - j0, 0), j1 - j0);
+        }
         return true;
     }
-};
+    return false;
+}
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
@@ -335,15 +358,20 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     const uint32_t v_landed = bars + 104u, v_fixed = bars + 112u;
     auto kv_full = [&](int s) { return bars + 120u + 8u * s; };
     auto kv_empty = [&](int s) { return bars + 120u + 8u * (kSlots + s); };
-    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 248);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 252);
-    static_assert(120 + 16 * kSlots <= 248, "barriers");
+    auto w_full = [&](uint32_t i) { return bars + 256u + 8u * (i % kQueue); };
+    auto w_empty = [&](uint32_t i) { return bars + 256u + 8u * (kQueue + i % kQueue); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 352);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 356);
+    static_assert(120 + 16 * kSlots <= 256 && 256 + 16 * kQueue <= 352, "barriers");
+    Work* queue = reinterpret_cast<Work*>(smem + C::kQueueOff);
+    static_assert(sizeof(Work) <= 64, "a step of work");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int x = 0; x < 2; ++x) {
             mbar_init(q_full(x), 1); mbar_init(s_full(x), 1); mbar_init(p_ready(x, 0), 4); mbar_init(p_ready(x, 1), 4); mbar_init(pv_done(x), 1); mbar_init(o_free(x), 4);
         }
+        for (int i = 0; i < kQueue; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), kReaders); }
         mbar_init(q_empty, 1); mbar_init(v_landed, 1); mbar_init(v_fixed, 1);
         for (int s = 0; s < kSlots; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
         *abort_flag = 0;
@@ -359,14 +387,43 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     const uint32_t tmem = *tmem_slot;
     int gave_up = 0;
 
-    Work w;
+    // The steps of work, as a reader sees them: next() waits for one, done() hands it back.
+    uint32_t step = 0;
+    const Work* wp = queue;
+    auto next = [&]() {
+        if (gave_up) return false;
+        if (!__all_sync(0xffffffffu, mbar_wait(w_full(step), (step / kQueue) & 1, abort_flag))) { gave_up = 6; return false; }
+        wp = queue + step % kQueue;
+        return wp->head >= 0;
+    };
+    auto done = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(w_empty(step));
+        ++step;
+    };
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-    Walk walk(P, lane);
-    if (warp == kTmaWarp) {
+    if (warp == kWalkWarp) {
+        // ================= the walk =================
+        Walk walk;
+        Work w;
+        bool more = walk_begin(P, lane, walk);
+        for (; !gave_up; ++step) {
+            more = more && walk_next(P, walk, w);
+            if (!more) w.head = -1;
+            if (step >= kQueue && !__all_sync(0xffffffffu, mbar_wait(w_empty(step), (step / kQueue - 1) & 1, abort_flag))) { gave_up = 6; break; }
+            if (lane == 0) {
+                queue[step % kQueue] = w;
+                mbar_arrive(w_full(step));
+            }
+            __syncwarp();
+            if (!more) break;
+        }
+    } else if (warp == kTmaWarp) {
         // ================= TMA: Q once a tile, K and V tiles through the ring =================
         uint32_t it = 0, tiles = 0;
-        while (!gave_up && walk.next(w)) {
+        for (; next(); done()) {
+            const Work w = *wp;
             const int n = max(w.n[0], w.n[1]);
             if (n == 0) continue;
             if (tiles > 0 && !__all_sync(0xffffffffu, mbar_wait(q_empty, (tiles - 1) & 1, abort_flag))) { gave_up = 1; break; }
@@ -447,7 +504,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             }
             ++pcount[x];
         };
-        while (!gave_up && walk.next(w)) {
+        for (; next(); done()) {
+            const Work& w = *wp;
             const int n0 = (int)uniform(w.n[0]), n1 = (int)uniform(w.n[1]), lk = (int)uniform(w.lk), n = max(n0, n1);
             if (n == 0) continue;
             // both halves of Q are always loaded
@@ -485,7 +543,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     } else if (warp == kFixWarp) {
         // ================= the last V tile of a sequence: zeros behind its last key, before any product reads it =================
         uint32_t it = 0, fixes = 0;
-        while (!gave_up && walk.next(w)) {
+        for (; next(); done()) {
+            const Work& w = *wp;
             const int n = max(w.n[0], w.n[1]), valid = w.lk - (n - 1) * kTileK;
             if (n == 0) continue;
             it += 2 * n;
@@ -503,11 +562,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     } else {
         // ================= softmax and epilogue: a thread owns a row =================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-        Walk walk(P, lane);
         const int x = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
         const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), s_addr = lane_base + x * 128, o_addr = lane_base + 256 + x * 128;
         uint32_t count = 0;                                       // score tiles of this sub-tile so far
-        while (!gave_up && walk.next(w)) {
+        for (; next(); done()) {
+            const Work& w = *wp;
             const int n = w.n[x], r = w.row0 + x * kSub + row;    // query row in its sequence
             const bool live = r < w.lq;
             T* dst = reinterpret_cast<T*>(P.out) + ((int64_t)(w.q_first + r) * P.H + w.head) * D;
@@ -611,7 +670,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             }
             // a cut tile: O[d][row], m[row], l[row] of this part and sub-tile
             constexpr int kPart = kSub * (D + 2);
-            auto part_at = [&](int part) { return P.partial + ((int64_t)(w.slot0 + part * P.H) * 2 + x) * kPart + row; };
+            auto slot_at = [&](int slot) { return P.partial + ((int64_t)slot * 2 + x) * kPart + row; };
+            auto part_at = [&](int i) { return slot_at((w.cta0 + i) * 2 + (i == 0 ? w.odd0 : 0)); };
             const float inv = l == 0.f ? 0.f : 1.f / l;
             auto store32 = [&](int c, const uint32_t (&v)[32]) {  // 32 finished values
                 if (!live) return;
@@ -637,19 +697,19 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                     }
                     if (w.parts == 1) store32(c, v);
                     else {
-                        float* at = part_at(w.part) + c * kSub;
+                        float* at = slot_at(w.slot) + c * kSub;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) __stcg(at + i * kSub, __uint_as_float(v[i]));
                     }
                 }
             }
             if (w.parts == 1) continue;
-            __stcg(part_at(w.part) + D * kSub, m_ref);
-            __stcg(part_at(w.part) + (D + 1) * kSub, l);
+            __stcg(slot_at(w.slot) + D * kSub, m_ref);
+            __stcg(slot_at(w.slot) + (D + 1) * kSub, l);
             __syncwarp();
             int last = 0;
             if (lane == 0) {
-                int* counter = P.counters + ((int64_t)w.slot0 * 2 + x) * 4 + quad;
+                int* counter = P.counters + (w.cta0 * 2 + x) * 4 + quad;
                 __threadfence();
                 last = atomicAdd(counter, 1) == w.parts - 1;
                 if (last) *counter = 0;
@@ -730,14 +790,14 @@ int launch_prompt_t(const CUtensorMap (&maps)[3], const PromptParams& P, int gri
 
 }  // namespace
 
-// How many items a list of these sizes can have when its tiles may be cut (0: they are not).  Cut where there are fewer tiles than two for each SM and a
-// sequence has 1024 keys or more on average: below that a tile's keys are few, above it the tiles alone keep the SMs busy.
-int64_t prompt_attention_items(int64_t Tq, int64_t Tk, int64_t H, int64_t B) {
+size_t prompt_attention_partial_bytes(int head_dim) {
     const int sms = sm_count_current();
-    const int64_t tiles = (Tq / kTileQ + B) * H;
-    return sms <= 0 || tiles >= 2 * (int64_t)sms || Tk < 1024 * B ? 0 : tiles + kPartsOfGrid * sms;
+    return sms <= 0 ? 0 : (size_t)sms * 2 * kTileQ * (head_dim + 2) * sizeof(float);
 }
-size_t prompt_attention_partial_bytes(int64_t items, int head_dim) { return (size_t)items * kTileQ * (head_dim + 2) * sizeof(float); }
+size_t prompt_attention_counter_bytes() {
+    const int sms = sm_count_current();
+    return sms <= 0 ? 0 : (size_t)sms * 8 * sizeof(int);
+}
 
 // Arguments are checked by the caller.  strides: {q token, q head, k token, k head, v token, v head} in elements.
 int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
@@ -768,9 +828,8 @@ int launch_prompt_attention(const void* q, const void* k, const void* v, const i
     P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
     P.negate = scale < 0.f ? 1 : 0;
     P.causal = causal ? 1 : 0;
-    P.counters = counters; P.partial = partial; P.items = partial != nullptr ? prompt_attention_items(Tq, Tk, H, B) : 0;
-    const int64_t most = (Tq / kTileQ + B) * H;                   // tiles there can be
-    const int grid = partial != nullptr ? sms : (int)std::min<int64_t>(sms, most);
+    P.counters = counters; P.partial = partial;
+    const int grid = sms;
     const bool bf = dtype == CB_BF16;
     if (head_dim == 128) return bf ? launch_prompt_t<__nv_bfloat16, 128>(maps, P, grid, stream) : launch_prompt_t<__half, 128>(maps, P, grid, stream);
     return bf ? launch_prompt_t<__nv_bfloat16, 64>(maps, P, grid, stream) : launch_prompt_t<__half, 64>(maps, P, grid, stream);

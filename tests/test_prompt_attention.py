@@ -13,12 +13,12 @@ def test_c_entry_point_refuses_bad_arguments():
     from crispybits_kernels import _C
     lib, s6 = _C._lib, (ctypes.c_int64 * 6)(*[128] * 6)
 
-    def call(q=256, k=256, v=256, st=s6, out=256, tq=4, tk=4, h=2, hkv=2, d=64, dt=1, cq=256, ck=256, b=1):
-        return lib.cb_prompt_attention(q, k, v, st, out, tq, tk, h, hkv, d, dt, cq, ck, b, 1.0, 1, 0, 0, 0, 0, 0)
+    def call(q=256, k=256, v=256, st=s6, out=256, tq=4, tk=4, h=2, hkv=2, d=64, dt=1, cq=256, ck=256, b=1, cnt=256, part=256):
+        return lib.cb_prompt_attention(q, k, v, st, out, tq, tk, h, hkv, d, dt, cq, ck, b, 1.0, 1, cnt, 1 << 20, part, 1 << 40, 0)
 
     for bad in (dict(dt=0), dict(dt=3), dict(d=96), dict(d=256), dict(tq=-1), dict(tk=-1), dict(tq=1 << 30), dict(h=3), dict(hkv=0), dict(b=-1),
                 dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(cq=0), dict(ck=0), dict(st=None), dict(q=8), dict(k=8), dict(v=8),
-                dict(out=8), dict(st=(ctypes.c_int64 * 6)(128, 128, 128, 4, 128, 128)), dict(st=(ctypes.c_int64 * 6)(0, *[128] * 5)),
+                dict(out=8), dict(cnt=0), dict(part=0), dict(part=8), dict(st=(ctypes.c_int64 * 6)(128, 128, 128, 4, 128, 128)), dict(st=(ctypes.c_int64 * 6)(0, *[128] * 5)),
                 dict(st=(ctypes.c_int64 * 6)(128, 128, -128, 128, 128, 128))):
         assert call(**bad) == 1 and lib.cb_last_error(), bad
     assert call(tq=0) == 0 and call(b=0) == 0 and call(h=0) == 0
@@ -140,9 +140,7 @@ def test_a_long_prompt_and_rising_scores():
 def test_keys_cut_into_parts(dtype, d, causal, lens, past):
     """Few tiles over many keys: their keys are shared out among the SMs."""
     import crispybits_kernels as ck
-    from crispybits_kernels import _C
     cq, ckv = offsets(lens), offsets([n + p for n, p in zip(lens, past)])
-    assert _C._lib.cb_prompt_attention_scratch(cq[-1], ckv[-1], 4, len(lens), d, None) > 0
     q, k, v = rand(cq[-1], 4, d, dtype, 1), rand(ckv[-1], 2, d, dtype, 2), rand(ckv[-1], 2, d, dtype, 3)
     k = (k.float() * torch.linspace(0.1, 2.0, ckv[-1], device=DEV)[:, None, None]).to(dtype)
     want = reference(q, k, v, cq, ckv, causal=causal)
@@ -170,8 +168,8 @@ def test_keys_cut_into_parts(dtype, d, causal, lens, past):
 
 
 @pytest.mark.gpu
-def test_bounds_that_overlap_stay_inside_the_scratch():
-    """Sequences that name the same rows again and again: more tiles than the list has room for in parts."""
+def test_bounds_that_overlap():
+    """Sequences that name the same rows again and again: more tiles than the rows make."""
     import crispybits_kernels as ck
     n = 3000
     q, k, v = rand(n, 1, 64, torch.float16, 1), rand(4 * n, 1, 64, torch.float16, 2), rand(4 * n, 1, 64, torch.float16, 3)
