@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
 constexpr int kOpen = 4;                              // what a CTA spends on a (tile, head) besides its products, in key tiles
+constexpr int kRoundUnits = 100, kMaxRounds = 4;      // a round is that many units for a CTA, or more
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kWalkWarp = 10, kFixWarp = 11, kThreads = 384;
 constexpr int kQueue = 4, kReaders = 11;              // steps of work handed on at a time, to 8 softmax warps, TMA, MMA and the fixing warp
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
@@ -47,8 +48,8 @@ struct PromptParams {
     float scale_log2;                                 // |scale| * log2(e), above 0
     int negate;                                       // the scale is negative: the products with q are negated
     int causal;
-    // Where the line of work is cut inside a (tile, head), the parts leave (O, m, l) in `partial`, two slots for a CTA, and the last to finish joins
-    // them.  counters: 8 for a CTA (of a cut tile's first part: one for each softmax warp), zero between calls.
+    // Where the line of work is cut inside a (head, tile), the pieces leave (O, m, l) in `partial`, two slots for a part of the line, and the last to
+    // finish joins them.  counters: 8 for a part (that of the first piece; one for each softmax warp), zero between calls.
     float* partial;
     int* counters;
 };
@@ -201,17 +202,18 @@ template <int O, int N> __device__ __forceinline__ void tmem_ld_wait32(uint32_t 
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// The work: all (tile of 256 query rows, head) pairs, sequence after sequence, heads innermost, form one line of key tiles (and kOpen more ahead of each
-// pair's) that is cut into equal parts, one for each CTA.  One warp walks through the CTA's part, a few steps ahead, and hands the steps to the others
-// through a queue in shared memory.
+// The work: all (head, tile of 256 query rows) pairs, sequence after sequence, tiles innermost, form one line of key tiles (and kOpen more ahead of each
+// pair's) that is cut into equal parts: `rounds` for each CTA, CTA i taking parts i, i + CTAs, ...  In a round all CTAs are in one stretch of the
+// line, a few heads wide, whose keys and values the L2 holds.  One warp walks through the CTA's parts, a few steps ahead, and hands the steps to the
+// others through a queue in shared memory.
 struct Work {                                         // head < 0: the end
     int head, row0, lq, lk, q_first, k_first;         // row0: the tile's first query row in its sequence; k_first, lk: from this part's first key on
     int n[2];                                         // key tiles of the sub-tiles, in this part
-    int parts, slot, cta0, odd0;                      // parts of this tile and head; this one's slot of scratch; part i's is (cta0 + i) * 2 (+ odd0 for i = 0)
+    int parts, slot, first, odd0;                     // pieces of this tile and head; this one's slot of scratch; piece i's is (first + i) * 2 (+ odd0 for i = 0)
 };
 struct Walk {
-    int64_t u, u0, u1, base, share, extra;            // base: the present sequence's first unit
-    int b, lq, lk, q_first, k_first;
+    int64_t u, u0, u1, base, share, extra;            // the present part [u0, u1) of the line; base: the present sequence's first unit
+    int part, rounds, b, lq, lk, q_first, k_first;
 };
 __device__ __forceinline__ int row_range(const int32_t* cu, int b, int rows, int& first) {
     const int s = min(max(cu[b], 0), rows), e = min(max(cu[b + 1], s), rows);
@@ -224,7 +226,7 @@ __device__ __forceinline__ int key_tiles(const PromptParams& P, int r0, int rows
     if (P.causal) n = min(n, (int64_t)r0 + rows + (lk - lq));
     return rows <= 0 || n <= 0 ? 0 : (int)((n + kTileK - 1) / kTileK);
 }
-// Units of the first t tiles of a sequence.  Under the causal bound tile i (of 256 rows) sees 2 (i + 1) + o key tiles, o = ceil((lk - lq) / 128),
+// Units of the first t tiles of a head of a sequence.  Under the causal bound tile i (of 256 rows) sees 2 (i + 1) + o key tiles, o = ceil((lk - lq) / 128),
 // or none; only the last tile may have fewer rows.
 __device__ __forceinline__ int64_t units_before(const PromptParams& P, int t, int lq, int lk) {
     const int tiles = (int)(((int64_t)lq + kTileQ - 1) / kTileQ), full = min(t, tiles - 1);
@@ -236,25 +238,16 @@ __device__ __forceinline__ int64_t units_before(const PromptParams& P, int t, in
         n = ((int64_t)full * (full + 1) - from * (from + 1)) + (full - from) * o;
     }
     if (t >= tiles && tiles > 0) n += key_tiles(P, (tiles - 1) * kTileQ, lq - (tiles - 1) * kTileQ, lq, lk);
-    return (n + (int64_t)kOpen * max(t, 0)) * P.H;
+    return n + (int64_t)kOpen * max(t, 0);
 }
 __device__ __forceinline__ int64_t units_of(const PromptParams& P, int lq, int lk) {
-    return lq <= 0 ? 0 : units_before(P, (int)(((int64_t)lq + kTileQ - 1) / kTileQ), lq, lk);
+    return lq <= 0 ? 0 : units_before(P, (int)(((int64_t)lq + kTileQ - 1) / kTileQ), lq, lk) * P.H;
 }
 
-// All lanes of a warp call these two together.  false: this CTA has nothing (more) to do.
-__device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk& walk) {
-    int64_t U = 0;
-    for (int b = lane; b < P.B; b += 32) {
-        int first;
-        U += units_of(P, row_range(P.cu_q, b, P.Tq, first), row_range(P.cu_k, b, P.Tk, first));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
-    const int64_t nc = min((int64_t)gridDim.x, U);
-    if ((int64_t)blockIdx.x >= nc) return false;
-    const int64_t share = U / nc, extra = U - share * nc, c = blockIdx.x;
-    const int64_t u0 = share * c + min(c, extra), u1 = share * (c + 1) + min(c + 1, extra);
+// All lanes of a warp call these together.  false: there is nothing (more) to do.
+__device__ __forceinline__ bool walk_part(const PromptParams& P, int lane, Walk& walk, int part) {
+    const int64_t c = part, u0 = walk.share * c + min(c, walk.extra), u1 = walk.share * (c + 1) + min(c + 1, walk.extra);
+    walk.part = part;
     int64_t base = 0;
     for (int b0 = 0; b0 < P.B; b0 += 32) {
         int first_q = 0, first_k = 0;
@@ -270,7 +263,7 @@ __device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk
         const unsigned past = __ballot_sync(0xffffffffu, base + cum > u0);
         if (past != 0u) {
             const int l = __ffs(past) - 1;
-            walk.u = walk.u0 = u0; walk.u1 = u1; walk.share = share; walk.extra = extra;
+            walk.u = walk.u0 = u0; walk.u1 = u1;
             walk.base = base + __shfl_sync(0xffffffffu, cum - mine, l);
             walk.b = b0 + l;
             walk.lq = __shfl_sync(0xffffffffu, lq, l); walk.lk = __shfl_sync(0xffffffffu, lk, l);
@@ -281,51 +274,68 @@ __device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk
     }
     return false;
 }
-__device__ __forceinline__ bool walk_next(const PromptParams& P, Walk& walk, Work& w) {
-    int64_t& u = walk.u;
-    int64_t& base = walk.base;
-    const int64_t u0 = walk.u0, u1 = walk.u1, share = walk.share, extra = walk.extra;
-    int &lq = walk.lq, &lk = walk.lk, &q_first = walk.q_first, &k_first = walk.k_first;
-    while (u < u1) {
-        for (int64_t n = units_of(P, lq, lk); u >= base + n; n = units_of(P, lq, lk)) {
-            base += n;
-            if (++walk.b >= P.B) return false;        // only if the bounds changed while the kernel ran
-            lq = row_range(P.cu_q, walk.b, P.Tq, q_first);
-            lk = row_range(P.cu_k, walk.b, P.Tk, k_first);
+__device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk& walk) {
+    int64_t U = 0;
+    for (int b = lane; b < P.B; b += 32) {
+        int first;
+        U += units_of(P, row_range(P.cu_q, b, P.Tq, first), row_range(P.cu_k, b, P.Tk, first));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
+    const int rounds = (int)min(max(U / ((int64_t)gridDim.x * kRoundUnits), (int64_t)1), (int64_t)kMaxRounds);
+    const int64_t nc = min((int64_t)gridDim.x * rounds, U);
+    if ((int64_t)blockIdx.x >= nc) return false;
+    const int64_t share = U / nc, extra = U - share * nc;
+    walk.share = share; walk.extra = extra; walk.rounds = rounds;
+    return walk_part(P, lane, walk, blockIdx.x);
+}
+__device__ __forceinline__ bool walk_next(const PromptParams& P, int lane, Walk& walk, Work& w) {
+    for (;;) {
+        if (walk.u >= walk.u1) {                      // the next round's part
+            const int64_t part = (int64_t)walk.part + gridDim.x;
+            if (part >= (int64_t)gridDim.x * walk.rounds || !walk_part(P, lane, walk, (int)part)) return false;
         }
-        int lo = 0, hi = (int)(((int64_t)lq + kTileQ - 1) / kTileQ);      // the tile: units_before(lo) <= u - base < units_before(hi)
-        while (hi - lo > 1) {
+        const int64_t u = walk.u;
+        for (int64_t n = units_of(P, walk.lq, walk.lk); u >= walk.base + n; n = units_of(P, walk.lq, walk.lk)) {
+            walk.base += n;
+            if (++walk.b >= P.B) return false;        // only if the bounds changed while the kernel ran
+            walk.lq = row_range(P.cu_q, walk.b, P.Tq, walk.q_first);
+            walk.lk = row_range(P.cu_k, walk.b, P.Tk, walk.k_first);
+        }
+        const int lq = walk.lq, lk = walk.lk;
+        int lo = 0, hi = (int)(((int64_t)lq + kTileQ - 1) / kTileQ);
+        const int64_t each = units_before(P, hi, lq, lk);                 // of a head
+        w.head = (int)((u - walk.base) / each);
+        const int64_t local = u - walk.base - w.head * each;
+        while (hi - lo > 1) {                         // the tile: units_before(lo) <= local < units_before(hi)
             const int mid = (lo + hi) >> 1;
-            if (units_before(P, mid, lq, lk) <= u - base) lo = mid; else hi = mid;
+            if (units_before(P, mid, lq, lk) <= local) lo = mid; else hi = mid;
         }
         w.row0 = lo * kTileQ;
 #pragma unroll
         for (int x = 0; x < 2; ++x) w.n[x] = key_tiles(P, w.row0 + x * kSub, min(lq - w.row0 - x * kSub, kSub), lq, lk);
         const int n = max(w.n[0], w.n[1]), per = n + kOpen;
-        const int64_t in_tile = u - base - units_before(P, lo, lq, lk);
-        w.head = (int)(in_tile / per);
-        const int part = (int)(in_tile - (int64_t)w.head * per), j0 = max(part - kOpen, 0);
-        const int64_t seg0 = u - part;
-        const int j1 = (int)min((int64_t)n, u1 - seg0 - kOpen);
-        const bool first = u == u0;
-        u = seg0 + per;
-        if (n == 0 ? part > 0 : j1 <= j0) continue;   // rows without keys belong to the CTA of the first unit; of others this is the opening only
-        w.lq = lq; w.q_first = q_first;
-        w.lk = lk - j0 * kTileK; w.k_first = k_first + j0 * kTileK;
-        w.parts = 1; w.slot = w.cta0 = w.odd0 = 0;
+        const int at = (int)(local - units_before(P, lo, lq, lk)), j0 = max(at - kOpen, 0);
+        const int64_t seg0 = u - at;
+        const int j1 = (int)min((int64_t)n, walk.u1 - seg0 - kOpen);
+        walk.u = seg0 + per;
+        if (n == 0 ? at > 0 : j1 <= j0) continue;     // rows without keys belong to the part with their first unit; of others this is the opening only
+        w.lq = lq; w.q_first = walk.q_first;
+        w.lk = lk - j0 * kTileK; w.k_first = walk.k_first + j0 * kTileK;
+        w.parts = 1; w.slot = w.first = w.odd0 = 0;
         if (n > 0 && (j0 > 0 || j1 < n)) {
-            auto cta_of = [&](int64_t unit) { return unit < extra * (share + 1) ? unit / (share + 1) : extra + (unit - extra * (share + 1)) / share; };
-            const int64_t c0 = cta_of(seg0 + kOpen);
-            w.cta0 = (int)c0;
-            w.parts = (int)(cta_of(seg0 + per - 1) - c0) + 1;
-            w.slot = (int)blockIdx.x * 2 + (first ? 0 : 1);
-            w.odd0 = share * c0 + min(c0, extra) < seg0 ? 1 : 0;
+            const int64_t share = walk.share, extra = walk.extra;
+            auto part_of = [&](int64_t unit) { return unit < extra * (share + 1) ? unit / (share + 1) : extra + (unit - extra * (share + 1)) / share; };
+            const int64_t p0 = part_of(seg0 + kOpen);
+            w.first = (int)p0;
+            w.parts = (int)(part_of(seg0 + per - 1) - p0) + 1;
+            w.slot = walk.part * 2 + (u == walk.u0 ? 0 : 1);
+            w.odd0 = share * p0 + min(p0, extra) < seg0 ? 1 : 0;
 #pragma unroll
             for (int x = 0; x < 2; ++x) w.n[x] = min(max(w.n[x] - j0, 0), j1 - j0);
         }
         return true;
     }
-    return false;
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -409,7 +419,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         Work w;
         bool more = walk_begin(P, lane, walk);
         for (; !gave_up; ++step) {
-            more = more && walk_next(P, walk, w);
+            more = more && walk_next(P, lane, walk, w);
             if (!more) w.head = -1;
             if (step >= kQueue && !__all_sync(0xffffffffu, mbar_wait(w_empty(step), (step / kQueue - 1) & 1, abort_flag))) { gave_up = 6; break; }
             if (lane == 0) {
@@ -671,7 +681,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             // a cut tile: O[d][row], m[row], l[row] of this part and sub-tile
             constexpr int kPart = kSub * (D + 2);
             auto slot_at = [&](int slot) { return P.partial + ((int64_t)slot * 2 + x) * kPart + row; };
-            auto part_at = [&](int i) { return slot_at((w.cta0 + i) * 2 + (i == 0 ? w.odd0 : 0)); };
+            auto part_at = [&](int i) { return slot_at((w.first + i) * 2 + (i == 0 ? w.odd0 : 0)); };
             const float inv = l == 0.f ? 0.f : 1.f / l;
             auto store32 = [&](int c, const uint32_t (&v)[32]) {  // 32 finished values
                 if (!live) return;
@@ -709,7 +719,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             __syncwarp();
             int last = 0;
             if (lane == 0) {
-                int* counter = P.counters + (w.cta0 * 2 + x) * 4 + quad;
+                int* counter = P.counters + (w.first * 2 + x) * 4 + quad;
                 __threadfence();
                 last = atomicAdd(counter, 1) == w.parts - 1;
                 if (last) *counter = 0;
@@ -792,11 +802,11 @@ int launch_prompt_t(const CUtensorMap (&maps)[3], const PromptParams& P, int gri
 
 size_t prompt_attention_partial_bytes(int head_dim) {
     const int sms = sm_count_current();
-    return sms <= 0 ? 0 : (size_t)sms * 2 * kTileQ * (head_dim + 2) * sizeof(float);
+    return sms <= 0 ? 0 : (size_t)sms * kMaxRounds * 2 * kTileQ * (head_dim + 2) * sizeof(float);
 }
 size_t prompt_attention_counter_bytes() {
     const int sms = sm_count_current();
-    return sms <= 0 ? 0 : (size_t)sms * 8 * sizeof(int);
+    return sms <= 0 ? 0 : (size_t)sms * kMaxRounds * 8 * sizeof(int);
 }
 
 // Arguments are checked by the caller.  strides: {q token, q head, k token, k head, v token, v head} in elements.
