@@ -31,7 +31,7 @@ namespace cb {
 namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
-constexpr int kOpen = 4;                              // what a CTA spends on a (tile, head) besides its products, in key tiles
+constexpr int kOpen = 3;                              // what a CTA spends on a (tile, head) besides its products, in key tiles
 constexpr int kRoundUnits = 100, kMaxRounds = 4;      // a round is that many units for a CTA, or more
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kWalkWarp = 10, kFixWarp = 11, kThreads = 384;
 constexpr int kQueue = 4, kReaders = 11;              // steps of work handed on at a time, to 8 softmax warps, TMA, MMA and the fixing warp
@@ -226,6 +226,11 @@ __device__ __forceinline__ int key_tiles(const PromptParams& P, int r0, int rows
     if (P.causal) n = min(n, (int64_t)r0 + rows + (lk - lq));
     return rows <= 0 || n <= 0 ? 0 : (int)((n + kTileK - 1) / kTileK);
 }
+// a / b, both not negative, mostly by the much shorter 32-bit division.
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+    return a / b;
+}
 // Units of the first t tiles of a head of a sequence.  Under the causal bound tile i (of 256 rows) sees 2 (i + 1) + o key tiles, o = ceil((lk - lq) / 128),
 // or none; only the last tile may have fewer rows.
 __device__ __forceinline__ int64_t units_before(const PromptParams& P, int t, int lq, int lk) {
@@ -282,10 +287,10 @@ __device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
-    const int rounds = (int)min(max(U / ((int64_t)gridDim.x * kRoundUnits), (int64_t)1), (int64_t)kMaxRounds);
+    const int rounds = (int)min(max(div64(U, (int64_t)gridDim.x * kRoundUnits), (int64_t)1), (int64_t)kMaxRounds);
     const int64_t nc = min((int64_t)gridDim.x * rounds, U);
     if ((int64_t)blockIdx.x >= nc) return false;
-    const int64_t share = U / nc, extra = U - share * nc;
+    const int64_t share = nc == 0 ? 0 : div64(U, nc), extra = U - share * nc;
     walk.share = share; walk.extra = extra; walk.rounds = rounds;
     return walk_part(P, lane, walk, blockIdx.x);
 }
@@ -305,7 +310,7 @@ __device__ __forceinline__ bool walk_next(const PromptParams& P, int lane, Walk&
         const int lq = walk.lq, lk = walk.lk;
         int lo = 0, hi = (int)(((int64_t)lq + kTileQ - 1) / kTileQ);
         const int64_t each = units_before(P, hi, lq, lk);                 // of a head
-        w.head = (int)((u - walk.base) / each);
+        w.head = (int)div64(u - walk.base, each);
         const int64_t local = u - walk.base - w.head * each;
         while (hi - lo > 1) {                         // the tile: units_before(lo) <= local < units_before(hi)
             const int mid = (lo + hi) >> 1;
@@ -325,7 +330,7 @@ __device__ __forceinline__ bool walk_next(const PromptParams& P, int lane, Walk&
         w.parts = 1; w.slot = w.first = w.odd0 = 0;
         if (n > 0 && (j0 > 0 || j1 < n)) {
             const int64_t share = walk.share, extra = walk.extra;
-            auto part_of = [&](int64_t unit) { return unit < extra * (share + 1) ? unit / (share + 1) : extra + (unit - extra * (share + 1)) / share; };
+            auto part_of = [&](int64_t unit) { return unit < extra * (share + 1) ? div64(unit, share + 1) : extra + div64(unit - extra * (share + 1), share); };
             const int64_t p0 = part_of(seg0 + kOpen);
             w.first = (int)p0;
             w.parts = (int)(part_of(seg0 + per - 1) - p0) + 1;
@@ -524,6 +529,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             fence_after();
             if (n0 > 0) scores(0, it, n1 == 0);
             if (n1 > 0) scores(1, it, true);
+            if (n == 1 && elect_one()) commit(q_empty);           // the last scores: the next tile's Q may come
             for (int j = 0; j < n && !gave_up; ++j) {
                 const uint32_t v = it + 2 * j + 1, k = v + 1;
                 if (!wait(kv_full(v % kSlots), (v / kSlots) & 1)) break;
@@ -545,10 +551,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                     if (gave_up) break;
                     if (j + 1 < nx) scores(x, k, x == 1 || j + 1 >= n1);
                 }
+                if (j + 2 == n && !gave_up && elect_one()) commit(q_empty);
+                __syncwarp();
             }
             it += 2 * n;
-            if (!gave_up && elect_one()) commit(q_empty);
-            __syncwarp();
         }
     } else if (warp == kFixWarp) {
         // ================= the last V tile of a sequence: zeros behind its last key, before any product reads it =================
