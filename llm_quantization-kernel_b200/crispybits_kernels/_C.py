@@ -672,12 +672,8 @@ def _kv4_record(cache, who: str) -> _KV4Cache:
 
 # The checks below are written for the call that is in order, which takes a few attribute reads; what is wrong with one that is not is
 # said by the function that follows.
-def _index_ok(t, device: int, n: int) -> bool:
-    return isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == device and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1)
-
-
 def _check_index(t, device: int, n: int, name: str, who: str):
-    if _index_ok(t, device, n):
+    if getattr(t, "dtype", None) is torch.int32 and t.get_device() == device and t.shape == (n,) and t.is_contiguous():
         return
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda or t.get_device() != device:
         _fail(f"{who}: {name} must be an int32 tensor on the device of the others")
@@ -685,20 +681,29 @@ def _check_index(t, device: int, n: int, name: str, who: str):
 
 
 def _check_table(page_table, device: int, who: str):
-    if not isinstance(page_table, torch.Tensor) or page_table.dtype is not torch.int32 or page_table.get_device() != device:
+    if getattr(page_table, "dtype", None) is not torch.int32 or page_table.get_device() != device:
         _fail(f"{who}: page_table must be an int32 tensor on the cache's device")
     if page_table.dim() != 2 or not page_table.is_contiguous():
         _fail(f"{who}: page_table must be contiguous [sequences, pages]")
 
 
-def _vector_rows(t: torch.Tensor) -> torch.Tensor:
-    """`t` itself where every row of its last dimension is contiguous and 16-byte aligned, else a contiguous copy."""
-    *lead, last = t.stride()
-    for s in lead:
-        last |= (s & 7) << 1                       # 1 only if the last is 1 and the others are multiples of 8
-    if last == 1 and t.data_ptr() & 15 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _vector_rows(t: torch.Tensor, positive: bool = False):
+    """(t, its strides) where every row of the last dimension is contiguous and 16-byte aligned (`positive`: and no
+    other stride is 0, as in an expanded tensor), else of a contiguous copy."""
+    st = t.stride()
+    if st[-1] == 1 and not (t.data_ptr() & 15):
+        bits = 0
+        for s in st[:-1]:
+            bits |= s
+        if not bits & 7 and not (positive and 0 in st):
+            return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
+
+
+def _empty(like: torch.Tensor) -> torch.Tensor:
+    """Contiguous, uninitialised, of the shape, dtype and device of `like` (by the shorter way where there is one)."""
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype, device=like.device)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -723,8 +728,8 @@ def kv4_append(cache, k, v, page_table, starts, cu_seqlens):
         _check_index(cu_seqlens, dev, seqs + 1, "cu_seqlens", "kv4_append")
     if n == 0:
         return
-    k, v = _vector_rows(k), _vector_rows(v)
-    strides = (_i64 * 4)(*k.stride()[:2], *v.stride()[:2])
+    (k, sk), (v, sv) = _vector_rows(k), _vector_rows(v)
+    strides = (_i64 * 4)(sk[0], sk[1], sv[0], sv[1])
     with _on_device(k.device):
         _rc(_lib.cb_kv4_append(rec, k.data_ptr(), v.data_ptr(), strides, n, page_table.data_ptr(), pages, seqs, starts.data_ptr(),
                                None if cu_seqlens is None else cu_seqlens.data_ptr(), _raw_stream(dev)))
@@ -743,7 +748,7 @@ def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
         _check_index(cu_seqlens, dev, seqs + 1, "cu_seqlens", "kv4_read")
     device = cache.pages.device
     k = torch.empty((n, rec.kv_heads, rec.head_dim), dtype=cache.dtype, device=device)
-    v = torch.empty((n, rec.kv_heads, rec.head_dim), dtype=cache.dtype, device=device)
+    v = torch.empty_like(k)
     if n:
         with _on_device(device):
             _rc(_lib.cb_kv4_read(rec, k.data_ptr(), v.data_ptr(), n, page_table.data_ptr(), pages, seqs, starts.data_ptr(),
@@ -805,11 +810,10 @@ def kv4_attention(q, cache, page_table, lengths, scale: float):
         _fail("kv4_attention: page_table needs one row for each sequence of q")
     _check_index(lengths, dev, B, "lengths", "kv4_attention")
     device = q.device
-    out = torch.empty(shape, dtype=q.dtype, device=device)
+    out = _empty(q)
     if B == 0 or T == 0 or H == 0:
         return out
-    q = _vector_rows(q)
-    st = q.stride()
+    q, st = _vector_rows(q)
     rows = T * (H // kv)
     counters = B * kv * (1 if rows <= 8 else -(-rows // 16))
     with _on_device(device):
@@ -832,14 +836,6 @@ _lib.cb_prompt_attention_scratch.argtypes = [_int, ctypes.POINTER(_sz)]
 _lib.cb_prompt_attention_scratch.restype = _sz
 
 
-def _tma_rows(t: torch.Tensor) -> torch.Tensor:
-    """As _vector_rows, and no dimension of several entries with a stride of 0 (an expanded tensor is copied)."""
-    st = t.stride()
-    if (st[0] <= 0 and t.shape[0] > 1) or (st[1] <= 0 and t.shape[1] > 1):
-        return t.clone(memory_format=torch.contiguous_format)
-    return _vector_rows(t)
-
-
 def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bool, out=None):
     """q [Tq, H, D], k and v [Tk, Hkv, D] -> [Tq, H, D] (cb_prompt_attention)."""
     who = "prompt_attention"
@@ -859,7 +855,7 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bo
         _fail(f"{who}: k and v must have the same shape, with q's head_dim")
     if hkv == 0 or h % hkv:
         _fail(f"{who}: q's heads must be a multiple of k's")
-    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
+    if not isinstance(cu_seqlens, torch.Tensor) or cu_seqlens.dim() != 1 or len(cu_seqlens) < 1:
         _fail(f"{who}: cu_seqlens must hold the first query of each sequence and their end")
     n = cu_seqlens.shape[0]
     _check_index(cu_seqlens, dev, n, "cu_seqlens", who)
@@ -867,13 +863,13 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bo
         _check_index(cu_seqlens_k, dev, n, "cu_seqlens_k", who)
     device = q.device
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = _empty(q)
     elif out.shape != shape or out.dtype != dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         _fail(f"{who}: out must be contiguous and 16-byte aligned, of q's shape, dtype and device")
     if tq == 0 or h == 0 or n == 1:
         return out
-    q, k, v = _tma_rows(q), _tma_rows(k), _tma_rows(v)
-    strides = (_i64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    (q, sq), (k, sk), (v, sv) = _vector_rows(q, True), _vector_rows(k, True), _vector_rows(v, True)
+    strides = (_i64 * 6)(sq[0], sq[1], sk[0], sk[1], sv[0], sv[1])
     with _on_device(device):
         stream, sizes = _raw_stream(dev), _prompt_bytes.get((dev, d))
         if sizes is None:
