@@ -354,8 +354,8 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * out [Tq, H, head_dim] contiguous, 16-byte aligned.  Sequence s has queries cu_q[s] .. cu_q[s + 1] - 1 and keys cu_k[s] ..
  * cu_k[s + 1] - 1 (device memory; bounds outside the tensors are cut to them).  Head h reads key head h / (H / Hkv).  head_dim 64 or 128,
  * dtype CB_F16 or CB_BF16.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
- * behind a query's last one are not used, except that an infinity or a NaN in v makes NaN of that value for
- * queries up to 127 positions before it.
+ * behind a query's last one do not touch it, infinities and NaN among them; a value of v that is not finite makes the
+ * same value of the queries that see it inf or NaN.
  * The work is cut into equal parts for the SMs, whatever the lengths are; where a cut falls inside a tile, its parts meet in scratch and are joined in
  * order, so that the result is the same from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, of any
  * content) and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call).  Calls that may overlap on the GPU need their own. */

@@ -15,8 +15,10 @@
 // Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 the walk through
 // the work, 11 zeros behind the last key (below).  Warps 8-11 give registers to the softmax warps, which hold a whole row of scores.
 //
-// V rows behind the last key of a sequence belong to another sequence (or to nothing): they are zeroed in shared memory, since 0 *
-// inf is not 0.  K rows there only make scores that are masked.
+// What a row does not see gets weight 0, but 0 * inf is not 0.  V rows behind the last key of a sequence belong to another sequence (or to
+// nothing) and are zeroed in shared memory.  Inside a sequence, where a value that is not finite follows a row within its last key tiles, the row's
+// sum comes out as NaN; the epilogue looks for that (it adds the row up) and forms such a sum again, from memory and without the tensor cores.
+// K needs nothing: scores are masked by selection.
 //
 // What bounds it at D = 128: 4 * 128 * 128 * D operations of a sub-tile and key tile are 1024 clocks of the tensor cores, and
 // its 128 * 128 exponentials are 1024 clocks of the special-function units.
@@ -43,6 +45,8 @@ __device__ int g_prompt_status;
 
 struct PromptParams {
     void* out;                                        // [Tq, H, D]
+    const void* q; const void* k; const void* v;      // only for what mend() does; the products read them through tensor maps
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;      // strides in elements
     const int32_t* cu_q; const int32_t* cu_k;
     int Tq, Tk, H, group, B;                          // group: query heads of a key head
     float scale_log2;                                 // |scale| * log2(e), above 0
@@ -351,6 +355,39 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) 
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// One row's 32 columns from d0 on of O, some of them NaN.  If a key of this row's key tiles that the row does not see holds a value that is not finite in
+// such a column, the column's sum over the keys that the row does see is formed again: keys [0, limit) of the step.
+template <typename T, int D>
+__device__ void mend(const PromptParams& P, const Work& w, int row, int limit, int tiles, int d0, float m_ref, uint32_t (&v)[32]) {
+    const int64_t kv_head = w.head / P.group;
+    const T* q = reinterpret_cast<const T*>(P.q) + (int64_t)(w.q_first + row) * P.q_tok + w.head * P.q_head;
+    const T* k = reinterpret_cast<const T*>(P.k) + (int64_t)w.k_first * P.k_tok + kv_head * P.k_head;
+    const T* val = reinterpret_cast<const T*>(P.v) + (int64_t)w.k_first * P.v_tok + kv_head * P.v_head + d0;
+    uint32_t spoilt = 0u;
+    for (int key = limit; key < min(tiles * kTileK, w.lk); ++key)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (!(fabsf(to_f32(val[key * P.v_tok + i])) < INFINITY)) spoilt |= 1u << i;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        if (__uint_as_float(v[i]) == __uint_as_float(v[i])) spoilt &= ~(1u << i);
+        if ((spoilt >> i) & 1u) v[i] = 0u;
+    }
+    if (spoilt == 0u) return;
+    const float neg = m_ref == -INFINITY ? 0.f : -m_ref, mul = P.negate ? -P.scale_log2 : P.scale_log2;
+    for (int key = 0; key < limit; ++key) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (int d = 0; d < D; d += 4)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[c] = fmaf(to_f32(q[d + c]), to_f32(k[key * P.k_tok + d + c]), s[c]);
+        const float p = ex2(fmaf((s[0] + s[1]) + (s[2] + s[3]), mul, neg));
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if ((spoilt >> i) & 1u) v[i] = __float_as_uint(fmaf(p, to_f32(val[key * P.v_tok + i]), __uint_as_float(v[i])));
+    }
 }
 
 template <typename T, int D>
@@ -700,24 +737,44 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                     *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             };
+            auto put32 = [&](int c, const uint32_t (&v)[32]) {
+                if (w.parts == 1) store32(c, v);
+                else {
+                    float* at = slot_at(w.slot) + c * kSub;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) __stcg(at + i * kSub, __uint_as_float(v[i]));
+                }
+            };
             if (n > 0) {
+                f32x2 sums[2] = {0ull, 0ull};                     // not finite if a value is not
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
                     uint32_t v[32];
                     tmem_ld32<0>(o_addr + c, v);
                     tmem_ld_wait32<0>(v);
-                    if (c + 32 == D) {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(o_free(x));
-                    }
-                    if (w.parts == 1) store32(c, v);
-                    else {
-                        float* at = slot_at(w.slot) + c * kSub;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) __stcg(at + i * kSub, __uint_as_float(v[i]));
+                    for (int i = 0; i < 16; ++i) sums[i & 1] = add2(sums[i & 1], pair(v[2 * i], v[2 * i + 1]));
+                    put32(c, v);
+                }
+                float s0, s1;
+                unpair(add2(sums[0], sums[1]), s0, s1);
+                const bool mine = !(fabsf(s0 + s1) < INFINITY) && live && l == l;
+                if (__any_sync(0xffffffffu, mine)) {
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t v[32];
+                        tmem_ld32<0>(o_addr + c, v);
+                        tmem_ld_wait32<0>(v);
+                        if (mine) {
+                            mend<T, D>(P, w, r, limit, n, c, m_ref, v);
+                            put32(c, v);
+                        }
+                        __syncwarp();
                     }
                 }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(o_free(x));
             }
             if (w.parts == 1) continue;
             __stcg(slot_at(w.slot) + D * kSub, m_ref);
@@ -840,6 +897,8 @@ int launch_prompt_attention(const void* q, const void* k, const void* v, const i
     }
     PromptParams P{};
     P.out = out; P.cu_q = cu_q; P.cu_k = cu_k;
+    P.q = q; P.k = k; P.v = v;
+    P.q_tok = strides[0]; P.q_head = strides[1]; P.k_tok = strides[2]; P.k_head = strides[3]; P.v_tok = strides[4]; P.v_head = strides[5];
     P.Tq = (int)Tq; P.Tk = (int)Tk; P.H = (int)H; P.group = (int)(H / Hkv); P.B = (int)B;
     P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
     P.negate = scale < 0.f ? 1 : 0;

@@ -243,6 +243,31 @@ def test_nan_in_a_sequence_reaches_only_that_sequence():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,past", [(300, 0), (200, 65), (130, 3000), (700, -40)])
+def test_values_that_are_not_finite_reach_the_queries_that_see_them(dtype, d, n, past):
+    """An infinity or a NaN in v, anywhere: queries before it are what they are without it, later ones are not finite in that value only."""
+    import crispybits_kernels as ck
+    cq, ckv = [0, n, n + 50], [0, n + past, n + past + 50]
+    q, k, v = rand(cq[-1], 2, d, dtype, 1), rand(ckv[-1], 1, d, dtype, 2), rand(ckv[-1], 1, d, dtype, 3)
+    gen = torch.Generator().manual_seed(n)
+    spots = [(int(torch.randint(0, n + past, (1,), generator=gen)), int(torch.randint(0, d, (1,), generator=gen))) for _ in range(5)]
+    spots += [(n + past - 1, 0), (max(0, n + past - 129), d - 1)]
+    bad = v.clone()
+    for i, (key, col) in enumerate(spots):
+        v[key, 0, col] = 0
+        bad[key, 0, col] = (math.nan, math.inf, -math.inf)[i % 3]
+    want, tol = reference(q, k, v, cq, ckv)
+    got = ck.prompt_attention(q, k, bad, i32(cq), i32(ckv))
+    hit = torch.zeros(cq[-1], 2, d, dtype=torch.bool, device=DEV)
+    for key, col in spots:
+        hit[max(0, key - past):n, :, col] = True
+    assert torch.equal(~torch.isfinite(got), hit)
+    assert ((got.double() - want).abs() <= tol)[~hit].all()      # a sum formed again has fewer roundings, not more
+
+
+@pytest.mark.gpu
 def test_the_same_every_time_on_any_stream_and_captured():
     import crispybits_kernels as ck
     from crispybits_kernels import _C
