@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 import weakref
 from typing import Dict, List, Tuple
 
@@ -763,6 +764,7 @@ def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
 _attention_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
 _attention_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
 _ATTENTION_SLAB = 1 << 18
+_attention_lock = threading.Lock()
 _prompt_bytes: Dict[Tuple[int, int], Tuple[int, int]] = {}   # (device index, head_dim) -> bytes of counters and partial, cb_prompt_attention_scratch
 _partial_bytes: Dict[Tuple[int, bool, int], int] = {}      # (device index, more than 8 rows, head_dim) -> cb_kv4_attention_partial_bytes
 
@@ -771,20 +773,24 @@ def prepare_attention(device: torch.device):
     """Make the slab of zeroed counters that captured calls on this device draw from (not inside a capture)."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     if index not in _attention_slab and not torch.cuda.is_current_stream_capturing():
-        with _on_device(torch.device("cuda", index)):
+        with _attention_lock, _on_device(torch.device("cuda", index)):
             slab = torch.zeros(_ATTENTION_SLAB, dtype=torch.int32, device=torch.device("cuda", index))
             torch.cuda.current_stream(index).synchronize()       # visible to whatever stream a graph will run on
-        _attention_slab[index] = [slab, 0]
+            _attention_slab.setdefault(index, [slab, 0])
 
 
 def _attention_scratch(device, dev: int, stream: int, counters: int, nbytes: int):
     if torch.cuda.is_current_stream_capturing():
         partial = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        slab, need = _attention_slab.get(dev), -(-counters // 32) * 32
-        if slab is None or slab[1] + need > _ATTENTION_SLAB:
+        need = -(-counters // 32) * 32
+        with _attention_lock:
+            slab = _attention_slab.get(dev)
+            at = _ATTENTION_SLAB if slab is None else slab[1]
+            if at + need <= _ATTENTION_SLAB:
+                slab[1] = at + need
+        if at + need > _ATTENTION_SLAB:
             return torch.zeros(counters, dtype=torch.int32, device=device), partial
-        slab[1] += need
-        return slab[0][slab[1] - need:slab[1]], partial
+        return slab[0][at:at + need], partial
     have = _attention_eager.get((dev, stream))
     if have is None or have[0].numel() < counters or have[1].numel() < nbytes:
         prepare_attention(device)

@@ -64,6 +64,9 @@ class KV4Cache:
             c.prepare_attention(pages.device)
         return KV4Cache(pages, int(head_dim), int(page_size), int(group_size), dtype)
 
+    def __getstate__(self):
+        return {f: v for f, v in self.__dict__.items() if f != "_record"}      # the library's record names addresses of this process
+
     @property
     def n_pages(self) -> int:
         return self.pages.shape[0]

@@ -357,10 +357,11 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One row's 32 columns from d0 on of O, some of them NaN.  If a key of this row's key tiles that the row does not see holds a value that is not finite in
-// such a column, the column's sum over the keys that the row does see is formed again: keys [0, limit) of the step.
+// One row's 32 columns from d0 on, as this thread has just stored them: at `out`, finished (O times inv), or without it at `part`, O itself.  If a key of
+// the row's key tiles that the row does not see holds a value that is not finite in a column that came out as NaN, the column's sum over the keys
+// that the row does see is formed again: keys [0, limit) of the step.
 template <typename T, int D>
-__device__ void mend(const PromptParams& P, const Work& w, int row, int limit, int tiles, int d0, float m_ref, uint32_t (&v)[32]) {
+__device__ void mend(const PromptParams& P, const Work& w, int row, int limit, int tiles, int d0, float m_ref, float inv, T* out, float* part) {
     const int64_t kv_head = w.head / P.group;
     const T* q = reinterpret_cast<const T*>(P.q) + (int64_t)(w.q_first + row) * P.q_tok + w.head * P.q_head;
     const T* k = reinterpret_cast<const T*>(P.k) + (int64_t)w.k_first * P.k_tok + kv_head * P.k_head;
@@ -370,10 +371,12 @@ __device__ void mend(const PromptParams& P, const Work& w, int row, int limit, i
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             if (!(fabsf(to_f32(val[key * P.v_tok + i])) < INFINITY)) spoilt |= 1u << i;
+    float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-        if (__uint_as_float(v[i]) == __uint_as_float(v[i])) spoilt &= ~(1u << i);
-        if ((spoilt >> i) & 1u) v[i] = 0u;
+        v[i] = out != nullptr ? to_f32(out[i]) : part[i * kSub];
+        if (v[i] == v[i]) spoilt &= ~(1u << i);
+        v[i] = 0.f;
     }
     if (spoilt == 0u) return;
     const float neg = m_ref == -INFINITY ? 0.f : -m_ref, mul = P.negate ? -P.scale_log2 : P.scale_log2;
@@ -386,8 +389,14 @@ __device__ void mend(const PromptParams& P, const Work& w, int row, int limit, i
         const float p = ex2(fmaf((s[0] + s[1]) + (s[2] + s[3]), mul, neg));
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-            if ((spoilt >> i) & 1u) v[i] = __float_as_uint(fmaf(p, to_f32(val[key * P.v_tok + i]), __uint_as_float(v[i])));
+            if ((spoilt >> i) & 1u) v[i] = fmaf(p, to_f32(val[key * P.v_tok + i]), v[i]);
     }
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if ((spoilt >> i) & 1u) {
+            if (out != nullptr) out[i] = from_f32<T>(v[i] * inv);
+            else __stcg(part + i * kSub, v[i]);
+        }
 }
 
 template <typename T, int D>
@@ -752,29 +761,21 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                     uint32_t v[32];
                     tmem_ld32<0>(o_addr + c, v);
                     tmem_ld_wait32<0>(v);
+                    if (c + 32 == D) {
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(o_free(x));
+                    }
+                    put32(c, v);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) sums[i & 1] = add2(sums[i & 1], pair(v[2 * i], v[2 * i + 1]));
-                    put32(c, v);
                 }
                 float s0, s1;
                 unpair(add2(sums[0], sums[1]), s0, s1);
-                const bool mine = !(fabsf(s0 + s1) < INFINITY) && live && l == l;
-                if (__any_sync(0xffffffffu, mine)) {
+                if (!(fabsf(s0 + s1) < INFINITY) && live && l == l) {
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t v[32];
-                        tmem_ld32<0>(o_addr + c, v);
-                        tmem_ld_wait32<0>(v);
-                        if (mine) {
-                            mend<T, D>(P, w, r, limit, n, c, m_ref, v);
-                            put32(c, v);
-                        }
-                        __syncwarp();
-                    }
+                    for (int c = 0; c < D; c += 32) mend<T, D>(P, w, r, limit, n, c, m_ref, inv, w.parts == 1 ? dst + c : nullptr, slot_at(w.slot) + c * kSub);
                 }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(o_free(x));
             }
             if (w.parts == 1) continue;
             __stcg(slot_at(w.slot) + D * kSub, m_ref);

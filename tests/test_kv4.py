@@ -570,6 +570,50 @@ def test_pages_beyond_32_bit_offsets():
 
 
 @pytest.mark.gpu
+def test_a_cache_can_be_copied_and_pickled():
+    import copy
+    import dataclasses
+    import io
+
+    import crispybits_kernels as ck
+    f = Filled([40], 1, 64, 32, 16, torch.float16)
+    q = rand_q(1, 1, 2, 64, torch.float16)
+    want = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    buf = io.BytesIO()
+    torch.save(f.cache, buf)
+    buf.seek(0)
+    moved = dataclasses.replace(f.cache, pages=f.cache.pages.clone())
+    for other in (copy.deepcopy(f.cache), torch.load(buf, weights_only=False), moved):
+        assert other.pages.data_ptr() != f.cache.pages.data_ptr()
+        assert torch.equal(want, ck.kv4_attention(q, other, f.table, f.lengths))
+        other.pages.zero_()
+        assert torch.equal(want, ck.kv4_attention(q, f.cache, f.table, f.lengths))
+
+
+@pytest.mark.gpu
+def test_captures_beyond_the_prepared_counters():
+    """Counters cut from the slab are never given out twice; when it is used up, a graph zeroes its own."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    f = Filled([2000, 30], 2, 64, 64, 64, torch.float16)
+    q = rand_q(2, 1, 4, 64, torch.float16)
+    want = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    slab = _C._attention_slab[torch.cuda.current_device()]
+    before = slab[1]
+    slab[1] = slab[0].numel() - 40                                 # room for one call more
+    try:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = [ck.kv4_attention(q, f.cache, f.table, f.lengths) for _ in range(3)]
+        for _ in range(3):
+            g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(want, o) for o in outs) and slab[1] == slab[0].numel() - 8
+    finally:
+        slab[1] = before
+
+
+@pytest.mark.gpu
 def test_shapes_and_devices_that_do_not_fit_are_refused():
     import crispybits_kernels as ck
     f = Filled([20], 2, 64, 32, 16, torch.float16)
