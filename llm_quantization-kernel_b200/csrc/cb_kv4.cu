@@ -12,6 +12,7 @@
 // owns 8 consecutive values of a row (token, head, K or V).
 #include <algorithm>
 
+#include "cb_f32x2.cuh"
 #include "cb_kv4.cuh"
 
 namespace cb {
@@ -147,37 +148,35 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // round_half_even((x - lo) / scale), at most 15, for 8 values: the codes as 4-bit fields.  Adding 1.5 * 2^23 rounds; the rounded
 // quotients are gathered by multiply-adds.  The remainder x - lo - code * scale, which the fused multiply-add forms without rounding,
 // shows where the approximate quotient met a tie or fell on the wrong side of one: there it is half a step or more (`half`: half a step, or 0
-// where a code could exceed 15), and the eight are done again with care.
+// where a code could exceed 15), and the eight are put right one by one.  (A tie in 8 values is met by 7 % of the warps for normal fp16
+// values, by 38 % for bfloat16.)
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale, float lo, float inv, float half) {
     constexpr float kMagic = 12582912.f;
-    float c[8], worst = 0.f;
+    const f32x2 minus_lo = pair(-lo, -lo), inv2 = pair(inv, inv), minus_scale = pair(-scale, -scale), magic = pair(kMagic, kMagic), back = pair(-kMagic, -kMagic);
+    float c[8], rest[8], worst = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 f = Pair<T>::f2(x[j >> 1]);
-        const float a = (j & 1 ? f.y : f.x) - lo;
-        c[j] = fmaf(a, inv, kMagic) - kMagic;
-        worst = fmaxf(worst, fabsf(fmaf(-c[j], scale, a)));
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = Pair<T>::f2(x[j]);
+        const f32x2 a = add2(pair(f.x, f.y), minus_lo), q = add2(fma2(a, inv2, magic), back);
+        unpair(q, c[2 * j], c[2 * j + 1]);
+        unpair(fma2(q, minus_scale, a), rest[2 * j], rest[2 * j + 1]);
+        worst = fmaxf(worst, fmaxf(fabsf(rest[2 * j]), fabsf(rest[2 * j + 1])));
     }
-    if (worst < half) {
-        const float p = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + kMagic;
-        const float q = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + kMagic;
-        return __byte_perm(__float_as_uint(p), __float_as_uint(q), 0x5410);
-    }
-    uint32_t word = 0u;
-    if (!(scale > 0.f)) return 0u;                                // one value, or NaN
+    if (!(worst < half)) {
+        if (!(scale > 0.f)) return 0u;                            // one value, or NaN
+        const float h = 0.5f * scale;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 f = Pair<T>::f2(x[j >> 1]);
-        const float a = (j & 1 ? f.y : f.x) - lo, h = 0.5f * scale;
-        float k = rintf(__fdiv_rn(a, scale));
-        const float d = fmaf(-k, scale, a);
-        const bool odd = ((int)k & 1) != 0;
-        if (d > h || (d == h && odd)) k += 1.f;
-        if (d < -h || (d == -h && odd)) k -= 1.f;
-        word |= (uint32_t)(int)fminf(k, 15.f) << (4 * j);
+        for (int j = 0; j < 8; ++j) {
+            const bool odd = ((int)c[j] & 1) != 0;
+            if (rest[j] > h || (rest[j] == h && odd)) c[j] += 1.f;
+            if (rest[j] < -h || (rest[j] == -h && odd)) c[j] -= 1.f;
+            c[j] = fminf(c[j], 15.f);
+        }
     }
-    return word;
+    const float p = fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + kMagic;
+    const float q = fmaf(fmaf(fmaf(c[7], 16.f, c[6]), 16.f, c[5]), 16.f, c[4]) + kMagic;
+    return __byte_perm(__float_as_uint(p), __float_as_uint(q), 0x5410);
 }
 
 // Where thread `tid` stands: 8 values from `d` on, of block position `tok`, in every kPer-th row from `sub` on.
