@@ -68,7 +68,8 @@ struct PromptCfg {
     static constexpr int kSlots = D == 128 ? 4 : 8;                         // ring of K and V tiles
     static constexpr uint32_t kQOff = 0, kRingOff = 2 * kTileBytes, kBarOff = kRingOff + kSlots * kTileBytes;
     static constexpr uint32_t kQueueOff = kBarOff + 384;                    // kQueue steps of work
-    static constexpr uint32_t kSmem = kQueueOff + kQueue * 64 + 1024;
+    static constexpr uint32_t kStageOff = kQueueOff + kQueue * 64;          // 32 rows x 32 finished values for each softmax warp
+    static constexpr uint32_t kSmem = kStageOff + 8 * 2048 + 1024;
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -332,7 +333,7 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One row's 32 columns from d0 on, as this thread has just stored them: at `out`, finished (O times inv), or without it at `part`, O itself.  If a key of
+// One row's 32 columns from d0 on, as this warp has just stored them: at `out`, finished (O times inv), or without it at `part`, O itself.  If a key of
 // the row's key tiles that the row does not see holds a value that is not finite in a column that came out as NaN, the column's sum over the keys
 // that the row does see is formed again: keys [0, limit) of the step.
 template <typename T, int D>
@@ -349,7 +350,7 @@ __device__ void mend(const PromptParams& P, const Work& w, int row, int limit, i
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-        v[i] = out != nullptr ? to_f32(out[i]) : part[i * kSub];
+        v[i] = out != nullptr ? to_f32(*reinterpret_cast<const volatile T*>(out + i)) : __ldcg(part + i * kSub);
         if (v[i] == v[i]) spoilt &= ~(1u << i);
         v[i] = 0.f;
     }
@@ -695,7 +696,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                         }
                     }
                 };
-                if (masked) weights(std::false_type{}); else weights(std::true_type{});
+                if (C::kPolyOf8 == 0 || masked) weights(std::false_type{}); else weights(std::true_type{});
                 float l0, l1;
                 unpair(add2(sum[0], sum[1]), l0, l1);
                 l += l0 + l1;
@@ -710,15 +711,27 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             auto slot_at = [&](int slot) { return P.partial + ((int64_t)slot * 2 + x) * kPart + row; };
             auto part_at = [&](int i) { return slot_at((w.first + i) * 2 + (i == 0 ? w.odd0 : 0)); };
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            auto store32 = [&](int c, const uint32_t (&v)[32]) {  // 32 finished values
-                if (!live) return;
+            // 32 finished values of every row of the warp: turned over in shared memory, so that a store covers 64 contiguous bytes of each of 8 rows (a
+            // lane's own row, 16 bytes at a time, takes a line for each lane: the stores of a tile were then 2 us).  Pieces of 16 bytes stand
+            // where eight lanes that write or read together meet different banks.
+            auto store32 = [&](int c, const uint32_t (&v)[32]) {
+                unsigned char* stage = smem + C::kStageOff + warp * 2048;
+                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
+                for (int i = 0; i < 4; ++i) {
                     uint32_t y[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        y[k] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[i + 2 * k]) * inv, __uint_as_float(v[i + 2 * k + 1]) * inv);
-                    *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(y[0], y[1], y[2], y[3]);
+                        y[k] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[8 * i + 2 * k]) * inv, __uint_as_float(v[8 * i + 2 * k + 1]) * inv);
+                    *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int of = i * 8 + (lane >> 2), piece = lane & 3, at = w.row0 + x * kSub + quad * 32 + of;      // another lane's row
+                    const uint4 y = *reinterpret_cast<const uint4*>(stage + of * 64 + ((piece ^ ((of >> 1) & 3)) * 16));
+                    if (at < w.lq)
+                        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(P.out) + ((int64_t)(w.q_first + at) * P.H + w.head) * D + c + piece * 8) = y;
                 }
             };
             auto put32 = [&](int c, const uint32_t (&v)[32]) {
@@ -731,7 +744,8 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             };
             if (n > 0) {
                 f32x2 sums[2] = {0ull, 0ull};                     // not finite if a value is not
-#pragma unroll
+                // not unrolled, as little here is: code that runs once a tile comes from afar each time, and was measured to cost more than its work
+#pragma unroll 1
                 for (int c = 0; c < D; c += 32) {
                     uint32_t v[32];
                     tmem_ld32<0>(o_addr + c, v);
@@ -747,6 +761,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 }
                 float s0, s1;
                 unpair(add2(sums[0], sums[1]), s0, s1);
+                __syncwarp();                                     // other lanes have stored this row
                 if (!(fabsf(s0 + s1) < INFINITY) && live && l == l) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) mend<T, D>(P, w, r, limit, n, c, m_ref, inv, w.parts == 1 ? dst + c : nullptr, slot_at(w.slot) + c * kSub);
