@@ -337,7 +337,7 @@ int cb_kv4_read(const cb_kv4_cache* cache, void* k, void* v, int64_t n_tokens, c
 /* Attention of the newest T tokens of each of B sequences over the cache: out[b, j] = softmax(scale * q[b, j] K^T) V over the first
  * lengths[b] - T + 1 + j cached tokens of sequence b; head h reads key head h / (H / kv_heads).  A row that sees
  * nothing is 0.  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
- * strides3 = {b, t, h} in elements, multiples of 8; out [B, T, H, head_dim] contiguous.  Tokens on a page whose number
+ * strides3 = {b, t, h} in elements, multiples of 8; out [B, T, H, head_dim] contiguous, sharing no memory with q.  Tokens on a page whose number
  * lies outside the cache are left out and set the status word (3001).  counters: cb_kv4_attention_counters() int32, zeroed ONCE,
  * left zero by every call; partial: cb_kv4_attention_partial_bytes() bytes, 16-byte aligned, of any content.  Calls that may overlap on
  * the GPU need their own counters and partial. */
@@ -351,7 +351,7 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * the first Lk - Lq + r + 1 of them for the sequence's query r of Lq (a prompt's keys, or a longer past and then its own).
  * q [Tq, H, head_dim], k and v [Tk, Hkv, head_dim]: rows of contiguous values, 16-byte aligned; strides6 = {q token, q head,
  * k token, k head, v token, v head} in elements, multiples of 8 and positive (that of a dimension of one entry is not used);
- * out [Tq, H, head_dim] contiguous, 16-byte aligned.  Sequence s has queries cu_q[s] .. cu_q[s + 1] - 1 and keys cu_k[s] ..
+ * out [Tq, H, head_dim] contiguous, 16-byte aligned, outside the memory from the first to the last value of q, k and v.  Sequence s has queries cu_q[s] .. cu_q[s + 1] - 1 and keys cu_k[s] ..
  * cu_k[s + 1] - 1 (device memory; bounds outside the tensors are cut to them).  Head h reads key head h / (H / Hkv).  head_dim 64 or 128,
  * dtype CB_F16 or CB_BF16.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
  * behind a query's last one do not touch it, infinities and NaN among them; a value of v that is not finite makes the

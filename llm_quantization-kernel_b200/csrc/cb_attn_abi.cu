@@ -23,6 +23,17 @@ namespace {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// Does `out` (bytes) meet the stretch from the first to the last byte of the 16-bit values at p[i0 * s0 + i1 * s1 + i2 * s2 + d]?  A CTA writes rows of the
+// output while others still read the queries, keys and values of theirs.
+bool meets(const void* out, int64_t bytes, const void* p, int head_dim, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2 = 1, int64_t s2 = 0) {
+    if (p == nullptr || n0 <= 0 || n1 <= 0 || n2 <= 0) return false;
+    const int64_t ends[3] = {(n0 - 1) * s0, (n1 - 1) * s1, (n2 - 1) * s2};
+    intptr_t lo = reinterpret_cast<intptr_t>(p), hi = lo + 2ll * head_dim;
+    for (int64_t e : ends) (e < 0 ? lo : hi) += 2 * e;
+    const intptr_t o = reinterpret_cast<intptr_t>(out);
+    return o < hi && lo < o + bytes;
+}
+
 int64_t block_bytes(int head_dim, int group_size) {
     if ((head_dim != 64 && head_dim != 128) || (group_size != 32 && group_size != 64 && group_size != 128) || group_size > head_dim) return 0;
     return 2 * kKvBlock * (head_dim / 2 + 4 * (head_dim / group_size));
@@ -114,6 +125,8 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
     CB_REQUIRE(counters != nullptr && counter_bytes >= (size_t)segs * sizeof(int), "%s: needs %lld zeroed counters", who, (long long)segs);
     const size_t need = cb_kv4_attention_partial_bytes(T, H, cache->kv_heads, cache->head_dim);
     CB_REQUIRE(partial != nullptr && partial_bytes >= need && aligned16(partial), "%s: needs %zu bytes of 16-byte aligned scratch", who, need);
+    CB_REQUIRE(!meets(out, 2 * B * T * H * cache->head_dim, q, cache->head_dim, B, strides3[0], T, strides3[1], H, strides3[2]),
+               "%s: out and q share memory", who);
     return launch_kv4_attention(cache, q, strides3, out, B, T, H, page_table, table_stride, lengths, scale,
                                 reinterpret_cast<int*>(counters), reinterpret_cast<float*>(partial),
                                 reinterpret_cast<cudaStream_t>(stream));
@@ -145,6 +158,9 @@ int cb_prompt_attention(const void* q, const void* k, const void* v, const int64
     CB_REQUIRE(counters != nullptr && counter_bytes >= prompt_attention_counter_bytes() && partial != nullptr && aligned16(partial) &&
                    partial_bytes >= prompt_attention_partial_bytes(head_dim),
                "%s: scratch is missing or too small (cb_prompt_attention_scratch)", who);
+    const int64_t out_bytes = 2 * Tq * H * head_dim;
+    CB_REQUIRE(!meets(out, out_bytes, q, head_dim, Tq, strides6[0], H, strides6[1]) && !meets(out, out_bytes, k, head_dim, Tk, strides6[2], Hkv, strides6[3]) &&
+                   !meets(out, out_bytes, v, head_dim, Tk, strides6[4], Hkv, strides6[5]), "%s: out shares memory with q, k or v", who);
     return launch_prompt_attention(q, k, v, strides6, out, Tq, Tk, H, Hkv, head_dim, dtype, cu_q, cu_k, B, scale, causal,
                                    reinterpret_cast<int*>(counters), reinterpret_cast<float*>(partial), reinterpret_cast<cudaStream_t>(stream));
 }

@@ -24,6 +24,24 @@ def test_c_entry_point_refuses_bad_arguments():
     assert call(tq=0) == 0 and call(b=0) == 0 and call(h=0) == 0
 
 
+def test_c_entry_point_refuses_an_output_on_its_inputs():
+    """Other rows may still be read while one is written."""
+    from crispybits_kernels import _C
+    lib, s6 = _C._lib, (ctypes.c_int64 * 6)(256, 64, 128, 64, 128, 64)
+    size = 4 * 256 * 2                                          # 4 queries of 4 heads (k and v: 4 keys of 2 heads), 64 values
+    q, k, v, out, far = 1 << 20, 2 << 20, 3 << 20, 4 << 20, 1 << 30
+
+    def message(out):
+        assert lib.cb_prompt_attention(q, k, v, s6, out, 4, 4, 4, 2, 64, 1, far, far, 1, 1.0, 1, far, 1 << 30, far, 1 << 40, 0) != 0
+        return lib.cb_last_error().decode()
+
+    for near in (q, q + size - 16, q - size + 16, k, k + 1024 - 16, v - size + 16):
+        assert "shares memory" in message(near), near
+    if not torch.cuda.is_available():                           # (nothing is launched without a device)
+        for apart in (out, q + size, q - size, k + 1024, v - size):
+            assert "shares memory" not in message(apart), apart
+
+
 def test_python_entry_point_refuses_cpu_tensors():
     import crispybits_kernels as ck
     x = torch.zeros(2, 2, 64).half()
@@ -306,6 +324,11 @@ def test_refusals_on_the_device():
     for out in (torch.empty(10, 4, 64, device=DEV), torch.empty(10, 4, 128, device=DEV, dtype=q.dtype)[..., :64], torch.empty(9, 4, 64, device=DEV, dtype=q.dtype)):
         with pytest.raises(RuntimeError):
             ck.prompt_attention(q, k, k, cu, out=out)
+    both = torch.zeros(2, 10, 4, 64, device=DEV, dtype=q.dtype)
+    for out in (q, both.view(20, 4, 64)[5:15]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            ck.prompt_attention(q if out is q else both[0], k, k, cu, out=out)
+    assert (ck.prompt_attention(both[0], k, k, cu, out=both[1]) == ck.prompt_attention(both[0], k, k, cu)).all()
     assert ck.prompt_attention(q[:0], k, k, i32([0, 0])).shape == (0, 4, 64)
     none = ck.prompt_attention(q, k[:0], k[:0], cu, i32([0, 0]))
     assert (none == 0).all()
