@@ -63,8 +63,6 @@ template <int D>
 struct PromptCfg {
     static constexpr uint32_t kBox = 64 * 2 * kTileK;                       // 64 values x 128 rows
     static constexpr uint32_t kTileBytes = kBox * (D / 64);
-    // D = 64: the products are half as long, and the special-function units would be the slowest part
-    static constexpr int kPolyOf8 = D == 64 ? 2 : 0;
     static constexpr int kSlots = D == 128 ? 4 : 8;                         // ring of K and V tiles
     static constexpr uint32_t kQOff = 0, kRingOff = 2 * kTileBytes, kBarOff = kRingOff + kSlots * kTileBytes;
     static constexpr uint32_t kQueueOff = kBarOff + 384;                    // kQueue steps of work
@@ -124,27 +122,6 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-// 2^x for two x <= 2^7 without the special-function unit: x = n + f with n the nearest integer, 2^f by a polynomial of degree 4 that is within
-// 2.7e-6 of it (relative; fitted for this purpose on [-1/2, 1/2]), 2^n from n's bits.  Below 2^-126 the result is 2^-126.
-__device__ __forceinline__ f32x2 ex2_poly(f32x2 x2) {
-    float x0, x1;
-    unpair(x2, x0, x1);
-    const f32x2 x = pair(max_nan(x0, -126.f), max_nan(x1, -126.f));
-    const f32x2 t = add2(x, pair(12583039.f, 12583039.f));        // 1.5 * 2^23 + 127: the low bits hold n + 127
-    const f32x2 f = add2(x, mul2(add2(t, pair(-12583039.f, -12583039.f)), pair(-1.f, -1.f)));
-    f32x2 p = fma2(f, pair(0.00957006889f, 0.00957006889f), pair(0.0559178085f, 0.0559178085f));
-    p = fma2(p, f, pair(0.240247451f, 0.240247451f));
-    p = fma2(p, f, pair(0.693121821f, 0.693121821f));
-    p = fma2(p, f, pair(0.999999262f, 0.999999262f));
-    float t0, t1;
-    unpair(t, t0, t1);
-    return mul2(p, pair(__float_as_uint(t0) << 23, __float_as_uint(t1) << 23));
 }
 #define CB_R32(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7]), \
     "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]), "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), \
@@ -663,40 +640,29 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                         tmem_st_wait();
                     }
                 }
-                // ---- weights: 32 keys at a time.  Of unmasked tiles kPolyOf8 of 8 pairs go to the polynomial.
+                // ---- weights, 32 keys at a time
                 const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
                 const f32x2 neg2 = pair(neg, neg), mul = pair(P.scale_log2, P.scale_log2);
                 f32x2 sum[2] = {0ull, 0ull};
-                auto weights = [&](auto plain) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t out[16];
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t out[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const f32x2 e = fma2(pair(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), mul, neg2);
-                            f32x2 p2;
-                            float p0, p1;
-                            if (decltype(plain)::value && i % 8 < C::kPolyOf8) {
-                                p2 = ex2_poly(e);
-                                unpair(p2, p0, p1);
-                            } else {
-                                unpair(e, p0, p1);
-                                p0 = ex2(p0); p1 = ex2(p1);
-                                p2 = pair(p0, p1);
-                            }
-                            sum[i & 1] = add2(sum[i & 1], p2);
-                            out[i] = pack2<T>(p0, p1);
-                        }
-                        tmem_st16(s_addr + 16 * c, out);
-                        if (c & 1) {
-                            tmem_st_wait();
-                            fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(p_ready(x, c >> 1));
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        float p0, p1;
+                        unpair(fma2(pair(s[32 * c + 2 * i], s[32 * c + 2 * i + 1]), mul, neg2), p0, p1);
+                        p0 = ex2(p0); p1 = ex2(p1);
+                        sum[i & 1] = add2(sum[i & 1], pair(p0, p1));
+                        out[i] = pack2<T>(p0, p1);
                     }
-                };
-                if (C::kPolyOf8 == 0 || masked) weights(std::false_type{}); else weights(std::true_type{});
+                    tmem_st16(s_addr + 16 * c, out);
+                    if (c & 1) {
+                        tmem_st_wait();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_ready(x, c >> 1));
+                    }
+                }
                 float l0, l1;
                 unpair(add2(sum[0], sum[1]), l0, l1);
                 l += l0 + l1;
