@@ -21,7 +21,13 @@
 // K needs nothing: scores are masked by selection.
 //
 // What bounds it at D = 128: 4 * 128 * 128 * D operations of a sub-tile and key tile are 1024 clocks of the tensor cores, and
-// its 128 * 128 exponentials are 1024 clocks of the special-function units.
+// its 128 * 128 exponentials are 1024 clocks of the special-function units; at D = 64 these are twice the products' time.  So the softmax warps may not
+// lose issue slots: packed fp32 arithmetic, a row to a thread, nothing unrolled that runs once a tile.
+//   16384 tokens, 32 heads, D = 128, causal, bf16:            1.69 to 1.73 ms, 1270 to 1300 TFLOP/s (the GPU at its power limit)
+//   12 prompts of 1 to 4096 tokens, 32 heads over 8, D = 128: 258 us, 930 TFLOP/s of what the pairs need; tiles on the diagonal and at prompts'
+//                                                              ends, and a tile's opening and epilogue (kOpen), are the rest
+//   16384 tokens, 16 heads, D = 64, causal, fp16:             768 us, 720 TFLOP/s
+//   one prompt of 37 tokens, 32 heads:                        10 us: launch, tensor maps, TMEM, one pass through the roles
 //
 // Every wait is bounded; a wait that runs out raises a flag in shared memory and the status word, every role leaves its
 // loops, TMEM is released, and the kernel returns.
@@ -34,8 +40,10 @@ namespace cb {
 namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
-constexpr int kOpen = 3;                              // what a CTA spends on a (tile, head) besides its products, in key tiles
-constexpr int kRoundUnits = 100, kMaxRounds = 4;      // a round is that many units for a CTA, or more
+constexpr int kOpen = 3;                              // what a CTA spends on a (tile, head) besides its products, in key tiles (the 12 prompts with 1: 272 us)
+// A round is kRoundUnits units for a CTA, or more: 16384 tokens, 32 heads take 1.69 to 1.73 ms in four rounds, 1.81 in one, whose keys do not stay in the L2.
+// Work of less than two such rounds is one round: each cut tile costs a join.
+constexpr int kRoundUnits = 100, kMaxRounds = 4;
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kWalkWarp = 10, kFixWarp = 11, kThreads = 384;
 constexpr int kQueue = 4, kReaders = 11;              // steps of work handed on at a time, to 8 softmax warps, TMA, MMA and the fixing warp
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
