@@ -155,6 +155,11 @@ template <int N> __device__ __forceinline__ void lds_words(const unsigned char* 
     else w[0] = *reinterpret_cast<const uint32_t*>(p);
 }
 
+__device__ __forceinline__ int arrive(int* counter) {
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
+}
 // Cached tokens and blocks of a sequence.  The caller has checked that the table's capacity in blocks, times the segments
 // of a sequence, fits 31 bits.
 __device__ __forceinline__ int seq_len(const AttnParams& P, int64_t b) {
@@ -743,10 +748,9 @@ kv4_attention_kernel(const AttnParams P) {
             __syncthreads();
             if (tid == 0) {
                 int* counter = P.counters + ((int64_t)now.b * segs + now.seg);
-                __threadfence();                                        // the CTA's part, ordered before by the barrier, is visible to who sees the count
-                const bool last = atomicAdd(counter, 1) == n - 1;
+                // the CTA's part, ordered before by the barrier, is visible to who sees the count, and the others' to this CTA if it is the last
+                const bool last = arrive(counter) == n - 1;
                 if (last) *counter = 0;
-                __threadfence();
                 misc[1] = last;
             }
             __syncthreads();

@@ -308,6 +308,11 @@ __device__ __forceinline__ bool walk_next(const PromptParams& P, int lane, Walk&
     }
 }
 
+__device__ __forceinline__ int arrive(int* counter) {
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+    return before;
+}
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -748,12 +753,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             int last = 0;
             if (lane == 0) {
                 int* counter = P.counters + (w.first * 2 + x) * 4 + quad;
-                __threadfence();
-                last = atomicAdd(counter, 1) == w.parts - 1;
+                // this warp's rows, ordered before by its barrier, are visible to who sees the count, and the others' to this warp if it is the last
+                last = arrive(counter) == w.parts - 1;
                 if (last) *counter = 0;
-                __threadfence();
             }
-            if (__shfl_sync(0xffffffffu, last, 0) == 0) continue;
+            last = __shfl_sync(0xffffffffu, last, 0);
+            __syncwarp();
+            if (last == 0) continue;
             // this warp's rows are complete in all parts: joined in their order
             float top = -INFINITY, sum = 0.f;
             for (int i = 0; i < w.parts; ++i) top = fmaxf(top, __ldcg(part_at(i) + D * kSub));
