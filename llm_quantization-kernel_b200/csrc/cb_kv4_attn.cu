@@ -50,7 +50,7 @@ struct AttnParams {
     const int32_t* lengths;
     int64_t B;
     int T, H, G, R, row_tiles;
-    bool aligned;                                     // no CTA's part crosses a segment's end
+    bool aligned;                                     // no CTA's part crosses a segment's end, unless there is too much work for that
     int solo;                                         // segments of up to this many blocks are taken by single warps
     float scale_log2;                                 // |softmax scale| * log2(e), above 0
     float q_sign;                                     // 1, or -1 where the scale is negative
@@ -175,6 +175,9 @@ constexpr float kLag = 8.f;
 // heads take 28.4 us with it and 39 with 8; 12 short ones with 12 heads 17.3 and 29; one long sequence is indifferent.
 constexpr int kOpen = 64;
 
+// Blocks of a CTA up to which parts end with their segment although a tenth of the CTAs or more may then be idle.
+constexpr uint32_t kAlignedBlocks = 16;
+
 template <typename T, int D, int GS, int NT>
 __global__ void __launch_bounds__((AttnCfg<D, GS, NT>::kThreads), 1)
 kv4_attention_kernel(const AttnParams P) {
@@ -210,22 +213,32 @@ kv4_attention_kernel(const AttnParams P) {
     int quota = 1;
     auto is_solo = [&](int nblk) { return nblk <= P.solo; };
     auto segs_of = [&](int nblk) { return is_solo(nblk) ? groups : segs; };
-    auto units_of = [&](int nblk) { return P.aligned ? (nblk + quota - 1) / quota : nblk == 0 ? 0 : is_solo(nblk) ? kOpen + nblk * kWarps : kOpen + nblk; };
-    uint32_t U = (uint32_t)(units_of(blocks_of(first_len)) * segs_of(blocks_of(first_len)));
-    for (int s = lane + 32; s < B; s += 32) { const int n = blocks_of(seq_len(P, s)); U += (uint32_t)(units_of(n) * segs_of(n)); }
-    U = __reduce_add_sync(0xffffffffu, U);
+    bool aligned = P.aligned;
+    auto units_of = [&](int nblk) { return aligned ? (nblk + quota - 1) / quota : nblk == 0 ? 0 : is_solo(nblk) ? kOpen + nblk * kWarps : kOpen + nblk; };
+    auto all_units = [&]() {
+        uint32_t n = (uint32_t)(units_of(blocks_of(first_len)) * segs_of(blocks_of(first_len)));
+        for (int s = lane + 32; s < B; s += 32) { const int m = blocks_of(seq_len(P, s)); n += (uint32_t)(units_of(m) * segs_of(m)); }
+        return __reduce_add_sync(0xffffffffu, n);
+    };
+    uint32_t U = all_units();
+    // With few CTAs to a segment those that are left over stay idle: only where that costs little beside the rest (32 segments of 131071 tokens on 148
+    // SMs: 4 CTAs each, 144 us, cut into equal parts 130; 32 segments of 777 tokens: 10.2 and 10.5).
+    if (aligned && 16 * B * segs > (int)gridDim.x && U > kAlignedBlocks * gridDim.x) {
+        aligned = false;
+        U = all_units();
+    }
     // ---- this CTA's part [u0, u1) of the line (the first `extra` parts have a unit more)
     const uint32_t nc = min(gridDim.x, max(U, 1u)), share = U / nc, extra = U - share * nc;
     auto unit_of_cta = [&](uint32_t c) { return share * c + min(c, extra); };
     const uint32_t spare = gridDim.x - (uint32_t)(B * segs);                          // aligned: CTAs beyond one for each segment
-    if (P.aligned) quota = (int)((U + spare - 1u) / spare);
-    const uint32_t u0 = P.aligned ? blockIdx.x : unit_of_cta(blockIdx.x);
-    const uint32_t u1 = P.aligned ? u0 + 1u : unit_of_cta(blockIdx.x + 1u);
+    if (aligned) quota = (int)((U + spare - 1u) / spare);
+    const uint32_t u0 = aligned ? blockIdx.x : unit_of_cta(blockIdx.x);
+    const uint32_t u1 = aligned ? u0 + 1u : unit_of_cta(blockIdx.x + 1u);
 
     // ---- the sequence that holds unit u0
     int b = -1, len = 0, nb = 0, per_seg = 0;
     uint32_t base = 0;
-    if (blockIdx.x < nc || P.aligned)
+    if (blockIdx.x < nc || aligned)
         for (int b0 = 0; b0 < B; b0 += 32) {
             const int my_len = b0 == 0 ? first_len : b0 + lane < B ? seq_len(P, b0 + lane) : 0;
             const uint32_t units = (uint32_t)(units_of(blocks_of(my_len)) * segs_of(blocks_of(my_len)));
@@ -278,7 +291,7 @@ kv4_attention_kernel(const AttnParams P) {
             const int part = (int)(local - (uint32_t)p.seg * (uint32_t)p.per_seg);
             p.seg0 = at - (uint32_t)part;
             p.next = p.seg0 + (uint32_t)p.per_seg;
-            if (P.aligned) {
+            if (aligned) {
                 const int each = p.nb / p.per_seg, more = p.nb - each * p.per_seg;
                 p.blk0 = each * part + min(part, more);
                 p.blk1 = p.blk0 + each + (part < more ? 1 : 0);
@@ -299,7 +312,7 @@ kv4_attention_kernel(const AttnParams P) {
     int b_now, seg_now, len_now, blk0, blk1;
     bool solo;                                         // this warp has the segment to itself
     auto enter = [&](const Piece& p) {
-        solo = !P.aligned && is_solo(p.nb);
+        solo = !aligned && is_solo(p.nb);
         b_now = p.b; len_now = p.len; blk0 = p.blk0; blk1 = p.blk1;
         seg_now = p.seg;
         if (solo) {
@@ -743,8 +756,8 @@ kv4_attention_kernel(const AttnParams P) {
             // CTAs that hold the segment's first and last block: c0 .. c0 + n - 1
             const uint32_t share = sched->share, extra = sched->extra;
             auto cta_of_unit = [&](uint32_t u) { return u < extra * (share + 1u) ? u / (share + 1u) : extra + (u - extra * (share + 1u)) / share; };
-            const uint32_t c0 = P.aligned ? now.seg0 : cta_of_unit(now.seg0 + kOpen);
-            const int n = P.aligned ? now.per_seg : (int)(cta_of_unit(now.seg0 + (uint32_t)now.per_seg - 1u) - c0) + 1;
+            const uint32_t c0 = aligned ? now.seg0 : cta_of_unit(now.seg0 + kOpen);
+            const int n = aligned ? now.per_seg : (int)(cta_of_unit(now.seg0 + (uint32_t)now.per_seg - 1u) - c0) + 1;
             __syncthreads();
             if (tid == 0) {
                 int* counter = P.counters + ((int64_t)now.b * segs + now.seg);
@@ -757,7 +770,7 @@ kv4_attention_kernel(const AttnParams P) {
             if (misc[1] != 0) {
                 // Parts lie at c0 (its second one, if the segment does not begin with that CTA), c0 + 1, ...  A warp takes a row, a lane
                 // 4 values of it (2 at D = 64).
-                const int64_t off0 = ((int64_t)c0 * 2 + (P.aligned || share * c0 + min(c0, extra) >= now.seg0 ? 0 : 1)) * C::kPartFloats;
+                const int64_t off0 = ((int64_t)c0 * 2 + (aligned || share * c0 + min(c0, extra) >= now.seg0 ? 0 : 1)) * C::kPartFloats;
                 auto part = [&](int c) { return P.partial + (c == 0 ? off0 : (int64_t)(c0 + c) * 2 * C::kPartFloats); };
                 constexpr int kV = D / 32;
                 for (int row = warp; row < kRows; row += kWarps) {
