@@ -334,28 +334,45 @@ kv4_attention_kernel(const AttnParams P) {
     const int32_t* table_row = nullptr;
     const unsigned char* head_pages = nullptr;
     auto first_of = [&](int i) { return blk0 + (solo ? i : warp + i * kWarps) * per; };
+    auto page_of = [&](int blk, int& in_page) {        // of a block of this piece, or -1
+        const int row = P.bpp_mul == 0u ? blk : (int)(__umulhi((uint32_t)blk, P.bpp_mul) >> P.bpp_shift);
+        in_page = blk - row * P.c.blocks_per_page;
+        const int page = table_row[row];
+        if (page >= 0 && page < P.c.n_pages) return page;
+        atomicExch(&g_kv4_attn_status, kKv4BadPage);
+        return -1;
+    };
+    auto expect = [&](uint32_t s, unsigned good) {     // one lane
+        slot_ok[s] = good;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bars + 8 * s), "r"((uint32_t)(__popc(good) * L::kBytes)) : "memory");
+    };
+    auto copy = [&](uint32_t s, int c, int page, int in_page) {
+        const unsigned char* src = head_pages + ((int64_t)page * kv_heads * P.c.blocks_per_page + in_page) * L::kBytes;
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(ring_u32 + s * C::kSlotBytes + c * L::kBytes), "l"(src), "r"((uint32_t)L::kBytes), "r"(bars + 8 * s) : "memory");
+    };
     auto issue = [&](int i, uint32_t at) {
         const uint32_t s = at % kSlots;
         const int blk = first_of(i) + lane;
         int page = -1, in_page = 0;
-        if (lane < per && blk < blk1) {
-            const int row = P.bpp_mul == 0u ? blk : (int)(__umulhi((uint32_t)blk, P.bpp_mul) >> P.bpp_shift);
-            in_page = blk - row * P.c.blocks_per_page;
-            page = table_row[row];
-            if (page < 0 || page >= P.c.n_pages) { page = -1; atomicExch(&g_kv4_attn_status, kKv4BadPage); }
-        }
+        if (lane < per && blk < blk1) page = page_of(blk, in_page);
         const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
-        const uint32_t bar = bars + 8 * s;
-        if (lane == 0) {
-            slot_ok[s] = good;
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((uint32_t)(__popc(good) * L::kBytes)) : "memory");
-        }
+        if (lane == 0) expect(s, good);
         __syncwarp();
-        if (page >= 0) {
-            const unsigned char* src = head_pages + ((int64_t)page * kv_heads * P.c.blocks_per_page + in_page) * L::kBytes;
-            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                         ::"r"(ring_u32 + s * C::kSlotBytes + lane * L::kBytes), "l"(src), "r"((uint32_t)L::kBytes), "r"(bar) : "memory");
-        }
+        if (page >= 0) copy(s, lane, page, in_page);
+    };
+    // The first stages of a piece: lane 2 i + c brings block c of stage i, so that all look-ups wait for memory together (one after another they took 3 us).
+    static_assert(kSlots * kStageBlocks <= 32, "a lane for each block of the ring");
+    auto issue_first = [&]() {
+        const int i = lane / kStageBlocks, c = lane % kStageBlocks, blk = first_of(i) + c;
+        const uint32_t s = (it + i) % kSlots;
+        const bool some = i < kSlots && i < mine;
+        int page = -1, in_page = 0;
+        if (some && c < per && blk < blk1) page = page_of(blk, in_page);
+        const unsigned good = __ballot_sync(0xffffffffu, page >= 0);
+        if (some && c == 0) expect(s, (good >> lane) & ((1u << kStageBlocks) - 1u));
+        __syncwarp();
+        if (page >= 0) copy(s, c, page, in_page);
     };
     auto begin_piece = [&](int b, int seg) {           // the first stages of a piece are on their way before anything else
         const int pieces = blk1 - blk0;
@@ -364,7 +381,7 @@ kv4_attention_kernel(const AttnParams P) {
         mine = solo ? nstage : warp < nstage ? (nstage - 1 - warp) / kWarps + 1 : 0;
         table_row = P.c.table + (int64_t)b * P.c.table_stride;
         head_pages = P.c.pages + (int64_t)(seg % kv_heads) * P.c.blocks_per_page * L::kBytes;
-        for (int i = 0; i < kSlots && i < mine; ++i) issue(i, it + i);
+        issue_first();
     };
     __syncthreads();                                   // barriers are there
     begin_piece(b_now, seg_now);
@@ -775,26 +792,13 @@ kv4_attention_kernel(const AttnParams P) {
                 constexpr int kV = D / 32;
                 for (int row = warp; row < kRows; row += kWarps) {
                     float* weight = merge + row * n;
-                    float m = -INFINITY, l = 0.f;
-                    for (int c = lane; c < n; c += 32) m = fmaxf(m, __ldcg(part(c) + kRows * D + row));
+                    // a part's maximum and sum for each lane (further ones where there are more than 32), and the first outputs, on their way together
+                    constexpr int kAhead = 8;
+                    float pm = lane < n ? __ldcg(part(lane) + kRows * D + row) : -INFINITY, pl = lane < n ? __ldcg(part(lane) + kRows * D + kRows + row) : 0.f;
+                    float a[kAhead][kV];
+                    auto fetch = [&](int c) {
 #pragma unroll
-                    for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
-                    for (int c = lane; c < n; c += 32) {
-                        const float pm = __ldcg(part(c) + kRows * D + row), pl = __ldcg(part(c) + kRows * D + kRows + row);
-                        const float f = pm == -INFINITY ? 0.f : ex2(pm - m);
-                        weight[c] = f;
-                        if (f != 0.f) l = fmaf(f, pl, l);
-                    }
-#pragma unroll
-                    for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
-                    __syncwarp();
-                    float v[kV];
-#pragma unroll
-                    for (int i = 0; i < kV; ++i) v[i] = 0.f;
-                    for (int c = 0; c < n; c += 8) {
-                        float a[8][kV];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k)
+                        for (int k = 0; k < kAhead; ++k)
                             if (c + k < n) {
                                 const float* src = part(c + k) + row * D + lane * kV;
                                 if constexpr (kV == 4) {
@@ -805,13 +809,34 @@ kv4_attention_kernel(const AttnParams P) {
                                     a[k][0] = q2.x; a[k][1] = q2.y;
                                 }
                             }
+                    };
+                    fetch(0);
+                    float m = pm, l = 0.f;
+                    for (int c = lane + 32; c < n; c += 32) m = fmaxf(m, __ldcg(part(c) + kRows * D + row));
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
+                    for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
+                    for (int c = lane; c < n; c += 32) {
+                        if (c >= 32) { pm = __ldcg(part(c) + kRows * D + row); pl = __ldcg(part(c) + kRows * D + kRows + row); }
+                        const float f = pm == -INFINITY ? 0.f : ex2(pm - m);
+                        weight[c] = f;
+                        if (f != 0.f) l = fmaf(f, pl, l);
+                    }
+#pragma unroll
+                    for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
+                    __syncwarp();
+                    float v[kV];
+#pragma unroll
+                    for (int i = 0; i < kV; ++i) v[i] = 0.f;
+                    for (int c = 0;;) {
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k)
                             if (c + k < n) {
                                 const float f = weight[c + k];
 #pragma unroll
                                 for (int i = 0; i < kV; ++i) v[i] = fmaf(f, a[k][i], v[i]);
                             }
+                        if ((c += kAhead) >= n) break;
+                        fetch(c);
                     }
                     store(row, lane * kV, v, l);
                 }
