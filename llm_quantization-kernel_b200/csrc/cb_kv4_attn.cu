@@ -28,9 +28,10 @@
 // (max, sum, output) in scratch and the CTA that arrives last adds them in order of position: the result does not
 // depend on timing.
 //
-// Measured (D = 128, groups of 64): one sequence of 131071 tokens, 64 heads over 8, in 42.8 us, 3.5 TB/s or 0.54 of a copy's rate: the stages of
-// a pair of blocks (16 x 128 codes twice, unpacked and multiplied, and their softmax) fill the issue slots of the SM.  24 sequences of 0 to 8192
-// tokens, 32 heads over 8: 28.4 us (2.0 TB/s); one of 777, 32 heads: 11 us.  There the chain of a launch counts: schedule, first copies, join.
+// Measured (D = 128, groups of 64): one sequence of 131071 tokens, 64 heads over 8, in 42.2 us, 3.6 TB/s or 0.55 of a copy's rate; sixteen of them
+// in 483, 0.77.  The steady state runs at about 0.83 of that rate (the stages of unpacking, products and softmax share the issue slots of three warps on
+// each scheduler); the rest is the chain of a launch, 12 us long: lengths, schedule, look-ups, first copies, the warps' meeting, the join.  24 sequences of
+// 0 to 8192 tokens, 32 heads over 8: 27.1 us (2.1 TB/s), one of 777, 32 heads: 9.8 us, of which that chain is most.
 #include <algorithm>
 
 #include "cb_kv4.cuh"
@@ -172,7 +173,8 @@ __device__ __forceinline__ int blocks_of(int len) { return (int)(((unsigned)len 
 constexpr float kLag = 8.f;
 
 // What a segment costs besides its blocks (query rows, the warps' meeting, the join), in blocks.  24 sequences of up to 8192 tokens with 8 key
-// heads take 28.4 us with it and 39 with 8; 12 short ones with 12 heads 17.3 and 29; one long sequence is indifferent.
+// heads take 27.1 us with it, 27.3 with 48, 32.3 with 96 and 37.7 with 8; 12 short ones with 12 heads 15.8, 15.9, 16.0 and 28.7; one long
+// sequence is indifferent.
 constexpr int kOpen = 64;
 
 // Blocks of a CTA up to which parts end with their segment although a tenth of the CTAs or more may then be idle.
@@ -222,7 +224,7 @@ kv4_attention_kernel(const AttnParams P) {
     };
     uint32_t U = all_units();
     // With few CTAs to a segment those that are left over stay idle: only where that costs little beside the rest (32 segments of 131071 tokens on 148
-    // SMs: 4 CTAs each, 144 us, cut into equal parts 130; 32 segments of 777 tokens: 10.2 and 10.5).
+    // SMs: 4 CTAs each, 144 us, cut into equal parts 130; 32 segments of 777 tokens: 9.8 and 10.3).
     if (aligned && 16 * B * segs > (int)gridDim.x && U > kAlignedBlocks * gridDim.x) {
         aligned = false;
         U = all_units();
@@ -866,7 +868,7 @@ int launch_attn_t(const AttnParams& P, int sms, cudaStream_t stream) {
 
 }  // namespace
 
-// Query rows of a tile: 8, or 16 where a key head has more than 8.  (4 to 8 rows in tiles of 16: 39 us for 28, 73 for 42.)
+// Query rows of a tile: 8, or 16 where a key head has more than 8.  (4 to 8 rows in tiles of 16: 38.7 us for 27.1, 73.1 for 42.2.)
 static int attn_tile_rows(int64_t rows) { return rows > 8 ? 16 : 8; }
 
 int64_t kv4_attention_segments(int64_t B, int64_t rows, int64_t kv_heads) {
@@ -906,10 +908,10 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
     // Few segments: parts that end with their segment, so that each CTA goes through the chain of copy, product and join once (8 segments of
-    // 131071 tokens: 42.2 us, cut into equal parts 43.7); the parts are then up to a quarter longer.  Many: equal parts.
+    // 131071 tokens: 42.2 us, cut into equal parts 43.6); the parts are then up to a quarter longer.  Many: equal parts.
     P.aligned = 4 * B * c->kv_heads * P.row_tiles <= sms;
-    // Segments enough to fill the SMs: the short ones (up to 128 tokens) one to a warp (512 segments of 100 tokens: 13.5 us, by whole CTAs
-    // 24.2; where few are that short: 28.4 and 29.5).
+    // Segments enough to fill the SMs: the short ones (up to 128 tokens) one to a warp (512 segments of 100 tokens: 13.2 us, by whole CTAs
+    // 23.9; where few are that short: 27.1 and 28.6).
     P.solo = !P.aligned && B * c->kv_heads * P.row_tiles >= sms ? 8 : 0;
     const bool bf = c->dtype == CB_BF16;
 #define CB_KV4_NT(d, gs, nt) (bf ? launch_attn_t<__nv_bfloat16, d, gs, nt>(P, sms, stream) : launch_attn_t<__half, d, gs, nt>(P, sms, stream))
