@@ -336,9 +336,12 @@ class Filled:
     def reference(self, q, scale=None, drop=None):
         """(out, tolerance) for q [B, T, H, D]; drop[b]: positions left out.
 
-        Tolerance, for each output: the final rounding; the weights' rounding to fp16, 2^-11 of the code part (v - lo)
-        that they multiply; the scores' error -- fp32 sums of 2 D products, and of D code products each cut to the
-        accumulator's width, 2^-20 of their absolute sum is ample -- which moves every weight and their sum by exp of it."""
+        Tolerance, for each output: the final rounding; the weights' rounding to fp16; the scores' error -- fp32 sums of 2 D products, and
+        of D code products each cut to the accumulator's width, 2^-20 of their absolute sum is ample -- which moves every weight
+        and their sum by exp of it.
+        The weights' rounding: with x = p s (s the group's scale) and w = fp16(x), |w - x| <= 2^-11 x, the kernel forms
+        sum w code + sum (p (lo + 7.5 s) - 7.5 w) = sum p (code s + lo) + sum (w - x) (code - 7.5), so 2^-11 sum p s |code - 7.5|; its fp32 sums of
+        terms as large as 7.5 p s, which cancel, are off by 2^-20 of those at most."""
         B, T, H, D = q.shape
         scale = D ** -0.5 if scale is None else scale
         heads = self.cache.kv_heads
@@ -349,6 +352,7 @@ class Filled:
             (kc, ks, kl), (vc, vs, vl) = ([t[at[b]:at[b + 1]] for t in part] for part in parts)
             kv, vv = values64(kc, ks, kl), values64(vc, vs, vl)
             vcode = values64(vc, vs, torch.zeros_like(vl))
+            vhalf = 7.5 * values64(torch.ones_like(vc), vs, torch.zeros_like(vl))
             kabs = values64(kc, ks, kl.abs())
             pos = torch.arange(n, device=DEV)
             for j in range(T):
@@ -364,7 +368,8 @@ class Filled:
                     w = torch.softmax((kv[seen, g] @ qq) * scale, 0)
                     err = 2.0 ** -20 * ((kabs[seen, g] @ qq.abs()) * abs(scale)).max()
                     out[b, j, h] = w @ vv[seen, g]
-                    tol[b, j, h] = (torch.finfo(q.dtype).eps / 2 * out[b, j, h].abs() * 1.01 + 2.0 ** -11 * 1.01 * (w @ vcode[seen, g])
+                    tol[b, j, h] = (torch.finfo(q.dtype).eps / 2 * out[b, j, h].abs() * 1.01 + 2.0 ** -11 * 1.01 * (w @ (vcode - vhalf)[seen, g].abs())
+                                    + 2.0 ** -20 * (w @ vhalf[seen, g])
                                     + 2 * (err + 2.0 ** -21) * (w @ (vcode[seen, g] + vl.abs().repeat_interleave(self.gs, -1)[seen, g])) + 1e-7)
         return out, tol
 
@@ -434,6 +439,20 @@ def test_attention_value_scales_of_very_different_size():
     f.v[5] *= 64.0
     ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0]), i32([0, 600]))
     q = rand_q(1, 2, 4, 64, torch.float16)
+    check(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n", [2, 33, 700])
+def test_attention_groups_with_one_large_value(dtype, n):
+    """Most codes of a group are then at one end."""
+    import crispybits_kernels as ck
+    f = Filled([n], 2, 128, 64, 64, dtype)
+    f.v[..., 7::64] = f.v[..., 7::64].abs() * 100
+    f.v[..., 64:] *= -1
+    ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0]), i32([0, n]))
+    q = rand_q(1, 2, 8, 128, dtype)
     check(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
 
 
