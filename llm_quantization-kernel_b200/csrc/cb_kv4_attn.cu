@@ -418,7 +418,9 @@ kv4_attention_kernel(const AttnParams P) {
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const int e = min(max((int)(__float_as_uint(mx) >> 23), 14), 254);
-            const float f = P.q_sign * __uint_as_float((uint32_t)(267 - e) << 23);   // 2^(140 - e)
+            // 2^(140 - e).  With an infinity among a row's values each score is an infinity or NaN, and none above -inf if they are infinities of one
+            // sign: no softmax survives that, so the row's values become NaN at once, and its sum with them.
+            const float f = mx < INFINITY ? P.q_sign * __uint_as_float((uint32_t)(267 - e) << 23) : __int_as_float(0x7fffffff);
             float sum[NG];
 #pragma unroll
             for (int w = 0; w < KW; ++w) {
@@ -759,11 +761,12 @@ kv4_attention_kernel(const AttnParams P) {
             float l = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                if (mw[w] == -INFINITY) continue;
+                const float sw = st_sum[w * kRows + row];
+                if (mw[w] == -INFINITY && sw == 0.f) continue;          // saw nothing; where all scores are NaN the sum is NaN, and stays
                 const float f = ex2(mw[w] - m);
                 const float4 a = *reinterpret_cast<const float4*>(merge + ((size_t)w * kRows + row) * D + d);
                 v[0] = fmaf(f, a.x, v[0]); v[1] = fmaf(f, a.y, v[1]); v[2] = fmaf(f, a.z, v[2]); v[3] = fmaf(f, a.w, v[3]);
-                l = fmaf(f, st_sum[w * kRows + row], l);
+                l = fmaf(f, sw, l);
             }
             if (whole) store(row, d, v, l);
             else {
@@ -819,9 +822,9 @@ kv4_attention_kernel(const AttnParams P) {
                     for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
                     for (int c = lane; c < n; c += 32) {
                         if (c >= 32) { pm = __ldcg(part(c) + kRows * D + row); pl = __ldcg(part(c) + kRows * D + kRows + row); }
-                        const float f = pm == -INFINITY ? 0.f : ex2(pm - m);
+                        const float f = pm == -INFINITY && pl == 0.f ? 0.f : ex2(pm - m);     // nothing seen: 0; NaN stays
                         weight[c] = f;
-                        if (f != 0.f) l = fmaf(f, pl, l);
+                        l = fmaf(f, pl, l);
                     }
 #pragma unroll
                     for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);

@@ -658,3 +658,52 @@ def test_shapes_and_devices_that_do_not_fit_are_refused():
         ck.kv4_attention(rand_q(1, 1, 4, 128, torch.float16), wrong, *ok)
     assert ck.kv4_attention(q[:, :0], f.cache, *ok).shape == (1, 0, 4, 64)
     ck.kv4_append(f.cache, k[:0], k[:0], *ok, i32([0, 0]))
+
+
+# ------------------------------------------------------------------------------------------------ GPU: values that are not finite
+def check_with_nan(got, want):
+    """NaN exactly where the definition has NaN, everything else within its tolerance."""
+    out, tol = want
+    assert torch.equal(got.isnan(), out.isnan()), f"{int((got.isnan() != out.isnan()).sum())} of {got.numel()} values"
+    there = ~out.isnan()
+    assert ((got.double() - out).abs() <= tol)[there].all() and torch.isfinite(got[there]).all()
+
+
+# One path through the work each: parts of long sequences, whole segments and parts of several CTAs, segments of single warps, the last two mixed.
+NON_FINITE_SHAPES = [([2500, 1, 700, 16], 2), ([900, 333, 1, 64, 5, 700] * 3, 4), ([20, 1, 128, 50] * 19, 2), ([100, 1, 129, 600] * 10, 4)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,heads", NON_FINITE_SHAPES)
+@pytest.mark.parametrize("T,group", [(1, 1), (2, 8)])
+def test_queries_that_are_not_finite_give_nan_on_every_path(dtype, lens, heads, T, group):
+    """A NaN or an infinity among a query's values makes each of its scores NaN or infinite, none of which a softmax survives: its row is NaN,
+    unless it sees nothing, and the rows beside it are untouched."""
+    import crispybits_kernels as ck
+    f = Filled(lens, heads, 64, 32, 32, dtype)
+    q = rand_q(len(lens), T, heads * group, 64, dtype)
+    want = f.reference(q)
+    rows = torch.zeros(q.shape[:3], dtype=torch.bool, device=DEV)
+    for i, (b, h) in enumerate((b, h) for b in range(len(lens)) for h in (0, heads * group - 1)):
+        q[b, T - 1, h, (7 * i) % 64] = (math.nan, math.inf, -math.inf)[i % 3]
+        rows[b, T - 1, h] = True
+    out = torch.where(rows[..., None] & (f.lengths > 0)[:, None, None, None], math.nan, want[0])
+    check_with_nan(ck.kv4_attention(q, f.cache, f.table, f.lengths), (out, want[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,heads", NON_FINITE_SHAPES)
+def test_keys_that_are_not_finite_give_nan_on_every_path(lens, heads):
+    """One token, a block, hundreds of tokens or a whole sequence of keys with a NaN or an infinity: every row that sees one is NaN."""
+    import crispybits_kernels as ck
+    d, gs, T = 64, 64, 2
+    f = Filled(lens, heads, d, gs, 32, torch.float16)
+    at = offsets(lens)
+    stretches = [(0, 1), (16, 32), (0, 1), (128, 700), (48, 64), (0, 1 << 30)]
+    for b, n in enumerate(lens):
+        a, e = (min(n, x) for x in stretches[b % len(stretches)])
+        f.k[at[b] + a:at[b] + e, b % heads, 3] = (math.nan, math.inf, -math.inf)[b % 3]
+    ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0] * len(lens)), i32(at))
+    q = rand_q(len(lens), T, 2 * heads, d, torch.float16)
+    check_with_nan(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
