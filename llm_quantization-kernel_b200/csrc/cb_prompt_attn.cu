@@ -685,11 +685,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 if (!__all_sync(0xffffffffu, mbar_wait(pv_done(x), (count - 1) & 1, abort_flag))) { gave_up = 4; break; }
                 fence_after();
             }
-            // a cut tile: O[d][row], m[row], l[row] of this part and sub-tile
+            // Of this part's keys this row sees none: its O is 0, whatever the values that met its weights of 0 are.  A row that sees keys has l = 0
+            // only if all their scores are -inf, and l NaN if one is NaN or +inf: O / l is NaN then, as the definition has it.
+            const bool blind = limit <= 0;
+            // a cut tile: O[d][row], m[row], l[row] of this part and sub-tile; l is -1, and O anything, where the row is blind
             constexpr int kPart = kSub * (D + 2);
             auto slot_at = [&](int slot) { return P.partial + ((int64_t)slot * 2 + x) * kPart + row; };
             auto part_at = [&](int i) { return slot_at((w.first + i) * 2 + (i == 0 ? w.odd0 : 0)); };
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = 1.f / l;
             // 32 finished values of every row of the warp: turned over in shared memory, so that a store covers 64 contiguous bytes of each of 8 rows (a
             // lane's own row, 16 bytes at a time, takes a line for each lane: the stores of a tile were then 2 us).  Pieces of 16 bytes stand
             // where eight lanes that write or read together meet different banks.
@@ -701,7 +704,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                     uint32_t y[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        y[k] = l == 0.f ? 0u : pack2<T>(__uint_as_float(v[8 * i + 2 * k]) * inv, __uint_as_float(v[8 * i + 2 * k + 1]) * inv);
+                        y[k] = blind ? 0u : pack2<T>(__uint_as_float(v[8 * i + 2 * k]) * inv, __uint_as_float(v[8 * i + 2 * k + 1]) * inv);
                     *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
                 __syncwarp();
@@ -741,14 +744,14 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 float s0, s1;
                 unpair(add2(sums[0], sums[1]), s0, s1);
                 __syncwarp();                                     // other lanes have stored this row
-                if (!(fabsf(s0 + s1) < INFINITY) && live && l == l) {
+                if (!(fabsf(s0 + s1) < INFINITY) && live && !blind && l == l) {
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) mend<T, D>(P, w, r, limit, n, c, m_ref, inv, w.parts == 1 ? dst + c : nullptr, slot_at(w.slot) + c * kSub);
                 }
             }
             if (w.parts == 1) continue;
             __stcg(slot_at(w.slot) + D * kSub, m_ref);
-            __stcg(slot_at(w.slot) + (D + 1) * kSub, l);
+            __stcg(slot_at(w.slot) + (D + 1) * kSub, blind ? -1.f : l);
             __syncwarp();
             int last = 0;
             if (lane == 0) {
@@ -760,14 +763,15 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             last = __shfl_sync(0xffffffffu, last, 0);
             __syncwarp();
             if (last == 0) continue;
-            // this warp's rows are complete in all parts: joined in their order
+            // this warp's rows are complete in all parts: joined in their order.  Parts that are blind count for nothing; one with a sum of NaN makes the
+            // row NaN, as do scores of -inf in all that are not (top - top is NaN).
             float top = -INFINITY, sum = 0.f;
             for (int i = 0; i < w.parts; ++i) top = fmaxf(top, __ldcg(part_at(i) + D * kSub));
             for (int i = 0; i < w.parts; ++i) {
-                const float m = __ldcg(part_at(i) + D * kSub);
-                if (m != -INFINITY) sum = fmaf(ex2(m - top), __ldcg(part_at(i) + (D + 1) * kSub), sum);
+                const float m = __ldcg(part_at(i) + D * kSub), s = __ldcg(part_at(i) + (D + 1) * kSub);
+                if (!(s < 0.f)) sum = fmaf(ex2(m - top), s, sum);
             }
-            const float rsum = sum == 0.f ? 0.f : 1.f / sum;
+            const float rsum = 1.f / sum;
 #pragma unroll 1
             for (int c = 0; c < D; c += 64) {                     // 64 loads on their way at a time
                 float v[64];
@@ -776,13 +780,13 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
 #pragma unroll 1
                 for (int i = 0; i < w.parts; ++i) {
                     const float* at = part_at(i);
-                    const float m = __ldcg(at + D * kSub);
+                    const float m = __ldcg(at + D * kSub), s = __ldcg(at + (D + 1) * kSub);
                     float o[64];
 #pragma unroll
                     for (int k = 0; k < 64; ++k) o[k] = __ldcg(at + (c + k) * kSub);
-                    const float f = m == -INFINITY ? 0.f : ex2(m - top) * rsum;
+                    const float f = ex2(m - top) * rsum;
 #pragma unroll
-                    for (int k = 0; k < 64; ++k) v[k] = m == -INFINITY ? v[k] : fmaf(f, o[k], v[k]);
+                    for (int k = 0; k < 64; ++k) v[k] = s < 0.f ? v[k] : fmaf(f, o[k], v[k]);
                 }
                 if (live)
 #pragma unroll

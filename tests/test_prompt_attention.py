@@ -332,3 +332,76 @@ def test_refusals_on_the_device():
     assert ck.prompt_attention(q[:0], k, k, i32([0, 0])).shape == (0, 4, 64)
     none = ck.prompt_attention(q, k[:0], k[:0], cu, i32([0, 0]))
     assert (none == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ GPU: queries and keys that are not finite
+def check_with_nan(got, want):
+    """NaN exactly where the definition has NaN, everything else within its tolerance."""
+    out, tol = want
+    assert torch.equal(got.isnan(), out.isnan()), f"{int((got.isnan() != out.isnan()).sum())} of {got.numel()} values"
+    there = ~out.isnan()
+    assert ((got.double() - out).abs() <= tol)[there].all() and torch.isfinite(got[there]).all()
+
+
+def reference_with_nan(q, k, v, cu_q, cu_k, causal=True):
+    """`reference`, with NaN where a row that sees a key has a score that is NaN, two that are +inf, or none above -inf.  Its tolerance is formed of the
+    weights w that these scores give: sum w |v| is another where a key of score -inf has none.  The scores' error is that of the finite keys."""
+    def finite(x):
+        return torch.where(torch.isfinite(x), x, 0).double()
+    share, half = q.shape[1] // k.shape[1], torch.finfo(q.dtype).eps / 2
+    out, tol = torch.zeros(q.shape, dtype=torch.double, device=DEV), torch.zeros(q.shape, dtype=torch.double, device=DEV)
+    for b in range(len(cu_q) - 1):
+        (q0, q1), (k0, k1) = cu_q[b:b + 2], cu_k[b:b + 2]
+        if q1 <= q0 or k1 <= k0:
+            continue
+        qq = q[q0:q1].transpose(0, 1)
+        kk, vv = (x[k0:k1].transpose(0, 1).repeat_interleave(share, 0) for x in (k, v))
+        s = qq.double() @ kk.double().transpose(1, 2) * q.shape[2] ** -0.5
+        err = 2.0 ** -20 * (finite(qq).abs() @ finite(kk).abs().transpose(1, 2)) * q.shape[2] ** -0.5
+        hidden = torch.zeros(s.shape[1:], dtype=torch.bool, device=DEV)
+        if causal:
+            hidden = torch.arange(k1 - k0, device=DEV)[None] > torch.arange(q1 - q0, device=DEV)[:, None] + (k1 - k0) - (q1 - q0)
+        w = torch.softmax(s.masked_fill(hidden, -math.inf), -1)
+        w = torch.where(hidden.all(-1)[None, :, None], 0.0, w)
+        o, e = w @ vv.double(), err.masked_fill(hidden, 0).amax(-1, keepdim=True) + 2.0 ** -21
+        out[q0:q1] = o.transpose(0, 1)
+        tol[q0:q1] = (half * o.abs() * 1.01 + (half * 1.01 + 2 * e) * (w @ vv.double().abs()) + 1e-7).transpose(0, 1)
+    return out, tol
+
+
+# whole tiles, tiles cut into parts, and both; keys fewer than queries among them
+NON_FINITE_SHAPES = [([300], [0]), ([130, 5], [6000, 700]), ([513, 70, 40, 1], [0, 3000, -10, 9000]), ([1], [0])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("lens,past", NON_FINITE_SHAPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_queries_that_are_not_finite_give_nan_wherever_the_work_is_cut(dtype, d, lens, past, causal):
+    import crispybits_kernels as ck
+    cq, ckv = offsets(lens), offsets([n + p for n, p in zip(lens, past)])
+    q, k, v = rand(cq[-1], 4, d, dtype, 1), rand(ckv[-1], 2, d, dtype, 2), rand(ckv[-1], 2, d, dtype, 3)
+    k[:, :, 9] = k[:, :, 9].abs() + 0.125                            # an infinity in q's value 9 makes all scores one infinity
+    for i, r in enumerate(sorted({0, cq[-1] - 1, *cq[1:-1], *(c - 1 for c in cq[1:])} - {cq[-1]})):
+        q[r, i % 4, 9] = (math.nan, math.inf, -math.inf)[i % 3]
+        q[r, (i + 1) % 4, 20] = (-math.inf, math.nan, math.inf)[i % 3]
+    want = reference_with_nan(q, k, v, cq, ckv, causal)
+    assert want[0].isnan().any()
+    check_with_nan(ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,d", [(torch.float16, 128), (torch.bfloat16, 64)])
+@pytest.mark.parametrize("lens,past", NON_FINITE_SHAPES)
+@pytest.mark.parametrize("first,last", [(0, 1), (0, 128), (2, 1 << 30), (100, 1400), (0, 1 << 30)])
+def test_keys_that_are_not_finite_wherever_the_work_is_cut(dtype, d, lens, past, first, last):
+    """NaN keys make the rows that see them NaN; scores of -inf have no weight, and a row that has no others is NaN."""
+    import crispybits_kernels as ck
+    cq, ckv = offsets(lens), offsets([n + p for n, p in zip(lens, past)])
+    q, k, v = rand(cq[-1], 2, d, dtype, 1), rand(ckv[-1], 2, d, dtype, 2), rand(ckv[-1], 2, d, dtype, 3)
+    q[:, :, 5] = q[:, :, 5].abs() + 0.125
+    for b, (a, e) in enumerate(zip(ckv, ckv[1:])):
+        k[min(a + first, e):min(a + last, e), 0, 5] = math.nan
+        k[min(a + first, e):min(a + last, e), 1, 5] = -math.inf      # scores of -inf for every query
+    want = reference_with_nan(q, k, v, cq, ckv)
+    check_with_nan(ck.prompt_attention(q, k, v, i32(cq), i32(ckv)), want)
