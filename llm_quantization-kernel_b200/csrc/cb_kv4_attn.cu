@@ -616,12 +616,12 @@ kv4_attention_kernel(const AttnParams P) {
                             pb[n][j][0] = movmatrix_t(wa);
                             pb[n][j][1] = movmatrix_t(wb);
                         } else {
-                            // what a row does not see adds nothing, whatever is stored there
+                            // what a row does not see adds nothing, whatever is stored there; what it sees with a weight too small for a float does
                             float h[4] = {p[n][0] * fa, p[n][1] * fa, p[n][2] * fb, p[n][3] * fb};
                             float y[4] = {p[n][0] * mid_a, p[n][1] * mid_a, p[n][2] * mid_b, p[n][3] * mid_b};
 #pragma unroll
                             for (int c = 0; c < 4; ++c)
-                                if (p[n][c] == 0.f) h[c] = y[c] = 0.f;
+                                if (x[k][n][c] == -INFINITY) h[c] = y[c] = 0.f;
                             const uint32_t wa = pack_h2(h[0], h[1]), wb = pack_h2(h[2], h[3]);
                             const float2 ga = unpack2<__half>(wa), gb = unpack2<__half>(wb);
                             z[n][j][0] += fmaf(ga.x, centre, y[0]) + fmaf(gb.x, centre, y[2]);

@@ -707,3 +707,20 @@ def test_keys_that_are_not_finite_give_nan_on_every_path(lens, heads):
     ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0] * len(lens)), i32(at))
     q = rand_q(len(lens), T, 2 * heads, d, torch.float16)
     check_with_nan(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [32, 33, 47, 700])
+@pytest.mark.parametrize("T,group", [(1, 8), (1, 4), (2, 8)])
+def test_nan_values_with_a_vanishing_weight_are_nan(n, T, group):
+    """A weight below the smallest float is not 0 in the definition: NaN times it is NaN, in whole blocks and in those that need masks."""
+    import crispybits_kernels as ck
+    f = Filled([n, n], 1, 64, 32, 32, torch.float16)
+    q = rand_q(2, T, group, 64, torch.float16).abs() + 0.5
+    for b, t in ((0, 3), (1, n - 1 - T)):
+        f.k[b * n + t] = -500.0                                    # scores some 3000 below the others
+        f.v[b * n + t, 0, 40] = math.nan
+    ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0, 0]), i32([0, n, 2 * n]))
+    got, (out, tol) = ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q)
+    out[..., 32:] = math.nan
+    check_with_nan(got, (out, tol))
