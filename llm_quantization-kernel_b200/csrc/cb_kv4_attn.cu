@@ -172,6 +172,12 @@ __device__ __forceinline__ int blocks_of(int len) { return (int)(((unsigned)len 
 // How far a score may lie above the reference (in powers of two) before that is moved: p stays below 2^8.
 constexpr float kLag = 8.f;
 
+// A weight is 2^(x qmul - m) by one fused operation, and the rounding of the reference m is a factor that all weights of a row share.  It is at most
+// 2^0.5 up to m = 2^24; beyond, it would carry p out of fp16's range and then out of a float's.  A warp that has met such an m goes through its blocks
+// again, from the references that it has found, halved with their qmul until they are no larger: scores are then held to a step of 1 where they have a
+// step of 1 or more in fp32 anyway.
+constexpr float kLargeScore = 16777216.f;
+
 // What a segment costs besides its blocks (query rows, the warps' meeting, the join), in blocks.  24 sequences of up to 8192 tokens with 8 key
 // heads take 27.1 us with it, 27.3 with 48, 32.3 with 96 and 37.7 with 8; 12 short ones with 12 heads 15.8, 15.9, 16.0 and 28.7; one long
 // sequence is indifferent.
@@ -389,6 +395,7 @@ kv4_attention_kernel(const AttnParams P) {
     begin_piece(b_now, seg_now);
     zero_rows();
 
+    bool again = false;                                // this warp's second time through the piece
     for (int bank = 0;; bank ^= 1) {
         const int row0 = seg_now / kv_heads * kRows, len = len_now;
 
@@ -462,6 +469,8 @@ kv4_attention_kernel(const AttnParams P) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 m_run[n][c] = -INFINITY; l_run[n][c] = 0.f;
+                if (again)
+                    for (m_run[n][c] = st_max[warp * kRows + n * 8 + 2 * t + c]; fabsf(m_run[n][c]) > kLargeScore && fabsf(m_run[n][c]) < INFINITY; m_run[n][c] *= 0.5f) qmul[n][c] *= 0.5f;
 #pragma unroll
                 for (int j = 0; j < NG; ++j) z[n][j][c] = 0.f;
             }
@@ -672,19 +681,37 @@ kv4_attention_kernel(const AttnParams P) {
             if (i + kSlots < mine) issue(i + kSlots, at + kSlots + held);
         }
         it += mine;
+        bool large = false;                            // a reference is, or was, beyond kLargeScore
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                large = large || (fabsf(m_run[n][c]) > kLargeScore && fabsf(m_run[n][c]) < INFINITY) || !(fabsf(l_run[n][c] + z[n][0][c]) < INFINITY);
+        const bool redo = __any_sync(0xffffffffu, large) && !again;
 
-        // ---- the next piece's copies start
+        // ---- the next piece's copies start, or this one's again
         const bool alone = solo, idle = solo && blk1 == 0, whole = blk0 == 0 && blk1 == place[bank].nb;
         const int64_t first_row = (int64_t)b_now * P.T * P.H + seg_now % kv_heads * P.G;      // of the output, in rows of D: row r is T's r / G, head r % G
         bool begun = false;
         if (misc[0] == 0) {
             Piece p = place[bank];
-            if (piece_at(p, p.next, sched->u1)) {
-                enter(p);
-                if (lane == 0) place[bank ^ 1] = p;
+            if (redo || piece_at(p, p.next, sched->u1)) {
+                if (!redo) {
+                    enter(p);
+                    if (lane == 0) place[bank ^ 1] = p;
+                }
                 begin_piece(b_now, seg_now);
                 begun = true;
             }
+        }
+        if (redo && begun) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) st_max[warp * kRows + n * 8 + 2 * t + c] = m_run[n][c];      // the same from every g
+            again = true;
+            bank ^= 1;
+            continue;
         }
 
         // ---- the warps' results meet: value = o * 2^24 (2^20) / cmul + z
@@ -704,7 +731,10 @@ kv4_attention_kernel(const AttnParams P) {
                         for (int d = 4; d < 32; d <<= 1) zz[j] += __shfl_xor_sync(0xffffffffu, zz[j], d);
                     }
                     const int row = n * 8 + 2 * t + c;
-                    if (g == 0) { st_max[warp * kRows + row] = m_run[n][c]; st_sum[warp * kRows + row] = l; }
+                    if (g == 0) {
+                        if (!again) st_max[warp * kRows + row] = m_run[n][c];           // the second time it stands there, before any halving
+                        st_sum[warp * kRows + row] = l;
+                    }
                     float* dst = merge + ((size_t)warp * kRows + row) * D;
 #pragma unroll
                     for (int hw = 0; hw < D / 32; ++hw) {
@@ -720,6 +750,7 @@ kv4_attention_kernel(const AttnParams P) {
                 }
             }
         }
+        again = false;
         if (!alone) __syncthreads(); else __syncwarp();
         if (misc[0] != 0) {                                             // a copy was not heard of: wait (bounded) for the others in flight
             if (begun)

@@ -48,6 +48,11 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9, kWalkWarp = 10, kFixWarp = 11, kThread
 constexpr int kQueue = 4, kReaders = 11;              // steps of work handed on at a time, to 8 softmax warps, TMA, MMA and the fixing warp
 // registers a thread: 384 x 168 at launch = 128 x kOtherRegs + 256 x kSoftRegs
 constexpr int kSoftRegs = 216, kOtherRegs = 72;
+// A weight is 2^(c s - m) by one fused operation, and the rounding of the reference m is a factor that all weights of a row share.  It is at most 2^0.5
+// up to m = 2^24; beyond, it would carry p out of fp16's range and then out of a float's.  So m is kept to that by halving the row's c, as often as the
+// maximum itself asks for: scores are then held to a step of 1 where they have a step of 1 or more in fp32 anyway.  (The reference is then moved without
+// a lag, which would be one of halved units: parts compare their references in whole ones.)
+constexpr float kLargeScore = 16777216.f;
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
 
 __device__ int g_prompt_status;
@@ -327,7 +332,7 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
 // the row's key tiles that the row does not see holds a value that is not finite in a column that came out as NaN, the column's sum over the keys
 // that the row does see is formed again: keys [0, limit) of the step.
 template <typename T, int D>
-__device__ void mend(const PromptParams& P, const Work& w, int row, int limit, int tiles, int d0, float m_ref, float inv, T* out, float* part) {
+__device__ void mend(const PromptParams& P, const Work& w, int row, int limit, int tiles, int d0, float factor, float m_ref, float inv, T* out, float* part) {
     const int64_t kv_head = w.head / P.group;
     const T* q = reinterpret_cast<const T*>(P.q) + (int64_t)(w.q_first + row) * P.q_tok + w.head * P.q_head;
     const T* k = reinterpret_cast<const T*>(P.k) + (int64_t)w.k_first * P.k_tok + kv_head * P.k_head;
@@ -345,7 +350,7 @@ __device__ void mend(const PromptParams& P, const Work& w, int row, int limit, i
         v[i] = 0.f;
     }
     if (spoilt == 0u) return;
-    const float neg = m_ref == -INFINITY ? 0.f : -m_ref, mul = P.negate ? -P.scale_log2 : P.scale_log2;
+    const float neg = m_ref == -INFINITY ? 0.f : -m_ref, mul = P.negate ? -factor : factor;
     for (int key = 0; key < limit; ++key) {
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
@@ -604,7 +609,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 continue;
             }
             const int limit = P.causal ? (int)min((int64_t)w.lk, max((int64_t)0, (int64_t)r + 1 + w.lk - w.lq)) : w.lk;      // keys this row sees
-            float m_ref = -INFINITY, l = 0.f;
+            float m_ref = -INFINITY, l = 0.f, factor = P.scale_log2, lag = 8.f;
             for (int j = 0; j < n; ++j, ++count) {
                 if (!__all_sync(0xffffffffu, mbar_wait(s_full(x), count & 1, abort_flag))) { gave_up = 3; break; }
                 fence_after();
@@ -632,9 +637,16 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 for (int i = 64; i < 128; i += 8)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], fmaxf(__uint_as_float(s[i + c]), __uint_as_float(s[i + 4 + c])));
-                const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * P.scale_log2;
-                const bool move = m > m_ref + 8.f;
+                const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                float m = top * factor;
+                const bool move = m > m_ref + lag;
                 if (__any_sync(0xffffffffu, move)) {
+                    if (move && (lag == 0.f || fabsf(m) > kLargeScore) && fabsf(top) < INFINITY) {
+                        float mul = P.scale_log2;
+                        for (m = top * mul; fabsf(m) > kLargeScore; m = top * mul) { mul *= 0.5f; lag = 0.f; }
+                        m_ref *= mul / factor;
+                        factor = mul;
+                    }
                     const float a = move ? ex2(m_ref - m) : 1.f;
                     if (move) m_ref = m;
                     l *= a;
@@ -655,7 +667,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 }
                 // ---- weights, 32 keys at a time
                 const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
-                const f32x2 neg2 = pair(neg, neg), mul = pair(P.scale_log2, P.scale_log2);
+                const f32x2 neg2 = pair(neg, neg), mul = pair(factor, factor);
                 f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -746,11 +758,11 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 __syncwarp();                                     // other lanes have stored this row
                 if (!(fabsf(s0 + s1) < INFINITY) && live && !blind && l == l) {
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) mend<T, D>(P, w, r, limit, n, c, m_ref, inv, w.parts == 1 ? dst + c : nullptr, slot_at(w.slot) + c * kSub);
+                    for (int c = 0; c < D; c += 32) mend<T, D>(P, w, r, limit, n, c, factor, m_ref, inv, w.parts == 1 ? dst + c : nullptr, slot_at(w.slot) + c * kSub);
                 }
             }
             if (w.parts == 1) continue;
-            __stcg(slot_at(w.slot) + D * kSub, m_ref);
+            __stcg(slot_at(w.slot) + D * kSub, lag == 0.f ? m_ref * (P.scale_log2 / factor) : m_ref);
             __stcg(slot_at(w.slot) + (D + 1) * kSub, blind ? -1.f : l);
             __syncwarp();
             int last = 0;

@@ -724,3 +724,32 @@ def test_nan_values_with_a_vanishing_weight_are_nan(n, T, group):
     got, (out, tol) = ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q)
     out[..., 32:] = math.nan
     check_with_nan(got, (out, tol))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gain", [(torch.float16, 300.0), (torch.float16, 10000.0), (torch.bfloat16, 1e6), (torch.bfloat16, 1e12)])
+@pytest.mark.parametrize("lens,heads", [([700, 33, 2500], 2), ([600, 5, 129] * 14, 4), ([100, 16, 33] * 50, 1)])
+def test_scores_of_any_size(dtype, gain, lens, heads):
+    """Queries and keys up to fp16's largest values and beyond: a row is the value of its best key, or the mean of those that share the best score.
+    Scores are made of few bits, so that their fp32 sums are exact and neighbours 2^-6 of the largest apart, or equal."""
+    import crispybits_kernels as ck
+    d, n = 64, sum(lens)
+    f = Filled(lens, heads, d, 64, 32, dtype)
+    gen = torch.Generator().manual_seed(5)
+    f.k.zero_()
+    f.k[:, :, 0] = (torch.randint(1, 5, (n, heads), generator=gen) * 15 * 2.0 ** int(math.log2(gain) - 4)).to(dtype).to(DEV)   # code 15, a scale of few bits
+    ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0] * len(lens)), i32(offsets(lens)))
+    q = torch.zeros(len(lens), 1, 2 * heads, d, dtype=dtype, device=DEV)
+    q[..., 0] = 2.0 ** int(math.log2(gain))
+    q[:, :, 1::2] *= -1
+    got = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    at, (vc, vs, vl) = offsets(lens), quantise64(f.v, 64)
+    for b in range(len(lens)):
+        for h in range(2 * heads):
+            s = f.k[at[b]:at[b + 1], h // 2, 0].double() * q[b, 0, h, 0].double()
+            best = (s == s.max()).nonzero()[:, 0] + at[b]
+            val, step = values64(vc[best], vs[best], vl[best])[:, h // 2], vs[best][:, h // 2].repeat_interleave(64, -1)
+            want = val.mean(0)
+            # weights alike: 2^-11 of |code - 7.5| steps each for their rounding, 2^-20 of all magnitudes for the fp32 sums
+            tol = torch.finfo(dtype).eps / 2 * 1.01 * want.abs() + (2.0 ** -11 * 1.01 + 2.0 ** -18) * 7.5 * step.mean(0) + 2.0 ** -18 * val.abs().mean(0) + 1e-7
+            assert ((got[b, 0, h].double() - want).abs() <= tol).all()

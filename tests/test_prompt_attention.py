@@ -405,3 +405,26 @@ def test_keys_that_are_not_finite_wherever_the_work_is_cut(dtype, d, lens, past,
         k[min(a + first, e):min(a + last, e), 1, 5] = -math.inf      # scores of -inf for every query
     want = reference_with_nan(q, k, v, cq, ckv)
     check_with_nan(ck.prompt_attention(q, k, v, i32(cq), i32(ckv)), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gain", [(torch.float16, 300.0), (torch.float16, 10000.0), (torch.bfloat16, 1e6), (torch.bfloat16, 1e12)])
+@pytest.mark.parametrize("n,past", [(300, 0), (130, 6000)])
+@pytest.mark.parametrize("scale", [None, -0.125])
+def test_scores_of_any_size(dtype, gain, n, past, scale):
+    """Queries and keys up to fp16's largest values and beyond: a row is the value of its best key, or the mean of those that share the best score.
+    Scores are made of few bits, so that they are exact, and neighbours are 1/4 of the largest apart, or equal."""
+    import crispybits_kernels as ck
+    gen = torch.Generator().manual_seed(5)
+    q, k, v = torch.zeros(n, 2, 64, dtype=dtype, device=DEV), torch.zeros(n + past, 1, 64, dtype=dtype, device=DEV), rand(n + past, 1, 64, dtype, 3)
+    power = 2.0 ** int(math.log2(gain))
+    k[:, 0, 0] = (torch.randint(1, 5, (n + past,), generator=gen) * power).to(dtype).to(DEV)
+    q[:, 0, 0], q[:, 1, 0] = power, -power
+    got = ck.prompt_attention(q, k, v, i32([0, n]), i32([0, n + past]), scale=scale)
+    s = torch.einsum("qh,k->hqk", q[:, :, 0].double(), k[:, 0, 0].double()) * (0.125 if scale is None else scale)
+    s = s.masked_fill(torch.arange(n + past, device=DEV)[None] > torch.arange(n, device=DEV)[:, None] + past, -math.inf)
+    w = (s == s.amax(-1, keepdim=True)).double()
+    w /= w.sum(-1, keepdim=True)
+    want, size = (torch.einsum("hqk,kd->qhd", w, x) for x in (v[:, 0].double(), v[:, 0].double().abs()))
+    half = torch.finfo(dtype).eps / 2
+    assert ((got.double() - want).abs() <= half * 1.01 * want.abs() + (half * 1.01 + 2.0 ** -18) * size + 1e-7).all()
