@@ -33,6 +33,7 @@
 // each scheduler); the rest is the chain of a launch, 12 us long: lengths, schedule, look-ups, first copies, the warps' meeting, the join.  24 sequences of
 // 0 to 8192 tokens, 32 heads over 8: 27.1 us (2.1 TB/s), one of 777, 32 heads: 9.8 us, of which that chain is most.
 #include <algorithm>
+#include <cfloat>
 
 #include "cb_kv4.cuh"
 
@@ -54,7 +55,7 @@ struct AttnParams {
     bool aligned;                                     // no CTA's part crosses a segment's end, unless there is too much work for that
     int solo;                                         // segments of up to this many blocks are taken by single warps
     float scale_log2;                                 // |softmax scale| * log2(e), above 0
-    float q_sign;                                     // 1, or -1 where the scale is negative
+    float q_sign;                                     // 1, or -1 where the scale is negative, 0 where it is 0
     uint32_t zero;                                    // 0, unknown to the compiler
     uint32_t bpp_mul, bpp_shift;                      // n / blocks_per_page = (n * bpp_mul) >> 32 >> bpp_shift for n < 2^31; bpp_mul 0: one block to a page
     int* counters;                                    // [B * kv_heads * row_tiles], zero between calls
@@ -441,7 +442,9 @@ kv4_attention_kernel(const AttnParams P) {
                 const float part = ((h[0] + h[1]) + (h[2] + h[3])) + ((h[4] + h[5]) + (h[6] + h[7]));
                 if (w % KWG == 0) sum[w / KWG] = part; else sum[w / KWG] += part;
             }
-            const float mul = P.scale_log2 * __uint_as_float((uint32_t)(e - 13) << 23) * 16777216.f;
+            // Kept among the normal floats: 0 times the -inf of an unseen token, or an infinity times a score, would be NaN.  Where that changes it, the row's
+            // values are all below 2^-112 (the scores are then 0 in effect) or above 2^119 (one key has all the weight).
+            const float mul = fminf(fmaxf(P.scale_log2 * 16777216.f * __uint_as_float((uint32_t)(e - 13) << 23), FLT_MIN), FLT_MAX);
             const int limit = live ? len - P.T + 1 + rt : 0;
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
@@ -928,8 +931,8 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     P.R = P.T * P.G;
     const int tile = attn_tile_rows(P.R);
     P.row_tiles = (P.R + tile - 1) / tile;
-    P.q_sign = scale < 0.f ? -1.f : 1.f;
-    P.scale_log2 = scale == 0.f ? 1e-30f : fabsf(scale) * 1.4426950408889634f;      // a scale of 0 weighs all keys alike
+    P.q_sign = scale < 0.f ? -1.f : scale > 0.f ? 1.f : 0.f;
+    P.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;         // a scale of 0 weighs all keys alike: queries of 0 do
     P.zero = 0u;
     {   // with 2^s >= d > 2^(s - 1), m = ceil(2^(31 + s) / d) < 2^32 is off by less than 1, n * m / 2^(31 + s) by less than n / 2^(31 + s) < 1 / d
         const uint32_t d = (uint32_t)P.c.blocks_per_page;

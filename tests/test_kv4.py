@@ -753,3 +753,37 @@ def test_scores_of_any_size(dtype, gain, lens, heads):
             # weights alike: 2^-11 of |code - 7.5| steps each for their rounding, 2^-20 of all magnitudes for the fp32 sums
             tol = torch.finfo(dtype).eps / 2 * 1.01 * want.abs() + (2.0 ** -11 * 1.01 + 2.0 ** -18) * 7.5 * step.mean(0) + 2.0 ** -18 * val.abs().mean(0) + 1e-7
             assert ((got[b, 0, h].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, 1e-9, None])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_queries_of_zeros_and_a_scale_of_zero_weigh_all_keys_alike(scale, dtype):
+    import crispybits_kernels as ck
+    lens = [20, 333, 1, 64]
+    f = Filled(lens, 2, 64, 32, 32, dtype)
+    q = rand_q(4, 3, 8, 64, dtype)
+    q[:, :, ::2] = 0.0
+    q[:, 1] *= 2.0 ** -20
+    check(ck.kv4_attention(q, f.cache, f.table, f.lengths, scale=scale), f.reference(q, scale))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [110, 119, 120, 121, 127])
+def test_the_largest_bfloat16_queries(power):
+    """One value of q and k alone, so that scores are 2^(power - 63 - t) / 8 for token t: the first has all the weight, exactly."""
+    import crispybits_kernels as ck
+    n = 20
+    f = Filled([n], 1, 64, 32, 32, torch.bfloat16)
+    f.k.zero_()
+    f.k[:, 0, 0] = 2.0 ** (-60 - torch.arange(n, device=DEV))
+    ck.kv4_append(f.cache, f.k, f.v, f.table, i32([0]), i32([0, n]))
+    q = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 2.0 ** power
+    q[:, :, 1] *= -1                                               # the last token's is the largest score, and 2^(power - 83) / 8 above the next
+    got = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    codes, scale, lo = quantise64(f.v, 32)
+    for h, t in ((0, 0), (1, n - 1)):
+        want = values64(codes, scale, lo)[t, 0]
+        tol = torch.finfo(torch.bfloat16).eps / 2 * 1.01 * want.abs() + 2.0 ** -20 * (15 * scale + lo.abs())[t, 0].repeat_interleave(32)
+        assert ((got[0, 0, h].double() - want).abs() <= tol).all()

@@ -428,3 +428,14 @@ def test_scores_of_any_size(dtype, gain, n, past, scale):
     want, size = (torch.einsum("hqk,kd->qhd", w, x) for x in (v[:, 0].double(), v[:, 0].double().abs()))
     half = torch.finfo(dtype).eps / 2
     assert ((got.double() - want).abs() <= half * 1.01 * want.abs() + (half * 1.01 + 2.0 ** -18) * size + 1e-7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,past", [(200, 0), (100, 5000)])
+def test_a_scale_of_zero_weighs_large_keys_alike_too(n, past):
+    """Scores of up to 2^120, times a scale of 0: each row is the mean of the values that it sees."""
+    import crispybits_kernels as ck
+    cq, ckv = [0, n], [0, n + past]
+    q, k, v = rand(n, 2, 64, torch.bfloat16, 1, 2.0 ** 56), rand(n + past, 1, 64, torch.bfloat16, 2, 2.0 ** 56), rand(n + past, 1, 64, torch.bfloat16, 3)
+    got = ck.prompt_attention(q, k, v, i32(cq), i32(ckv), scale=0.0)
+    check(got, reference(torch.zeros_like(q), k, v, cq, ckv, 0.0))
