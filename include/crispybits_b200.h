@@ -336,7 +336,7 @@ int cb_kv4_read(const cb_kv4_cache* cache, void* k, void* v, int64_t n_tokens, c
 
 /* Attention of the newest T tokens of each of B sequences over the cache: out[b, j] = softmax(scale * q[b, j] K^T) V over the first
  * lengths[b] - T + 1 + j cached tokens of sequence b; head h reads key head h / (H / kv_heads).  A row that sees
- * nothing is 0.  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
+ * nothing is 0.  scale is finite (this and prompt attention).  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
  * strides3 = {b, t, h} in elements, multiples of 8; out [B, T, H, head_dim] contiguous, sharing no memory with q.  Tokens on a page whose number
  * lies outside the cache are left out and set the status word (3001).  counters: cb_kv4_attention_counters() int32, zeroed ONCE,
  * left zero by every call; partial: cb_kv4_attention_partial_bytes() bytes, 16-byte aligned, of any content.  Calls that may overlap on

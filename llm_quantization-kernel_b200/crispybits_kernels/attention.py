@@ -107,7 +107,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
 
     q: [B, H, head_dim], one token of each sequence, or [B, T, H, head_dim], the T newest; any strides.  H is a multiple of the
     cache's heads, and query head h reads key head h // (H // kv_heads).  `lengths` [B]: cached tokens of each sequence, q's own
-    among them; token j of T sees the first lengths - T + 1 + j.  A row that sees nothing (lengths 0) is 0.  scale: default head_dim ** -0.5.
+    among them; token j of T sees the first lengths - T + 1 + j.  A row that sees nothing (lengths 0) is 0.  scale: finite, default head_dim ** -0.5.
     T may be any, but the cache is read once for each 16 rows (T * H / kv_heads of them) of a key head: for long pieces of
     a prompt, read the history back and use prompt attention."""
     return _C().kv4_attention(q, cache, page_table, lengths, cache.head_dim ** -0.5 if scale is None else float(scale))
@@ -123,7 +123,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     `cu_seqlens` int32 [B + 1]: the first query of each sequence and the end of the last; `cu_seqlens_k` the same for the keys where
     they differ: a piece of a prompt attends to what came before it and to itself.  causal: query r of Lq sees the first
     Lk - Lq + r + 1 keys.  A query that sees none gives 0.  Rows of no sequence are left as they are in `out` (and are
-    undefined without it; it shares no memory with q, k and v).  scale: default head_dim ** -0.5.  Keys and values that a query does not see do not
+    undefined without it; it shares no memory with q, k and v).  scale: finite, default head_dim ** -0.5.  Keys and values that a query does not see do not
     touch it, infinities and NaN among them.  Scratch for tiles that are cut between SMs (158 MB at head_dim 128 on 148 SMs) is kept for each
     stream that calls this eagerly, and comes from the graph's pool in a capture."""
     return _C().prompt_attention(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k,

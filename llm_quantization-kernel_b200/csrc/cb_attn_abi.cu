@@ -1,4 +1,6 @@
 // extern "C" entry points of the attention operators: argument checks and kernel choice.
+#include <cmath>
+
 #include "cb_common.cuh"
 #include "cb_kv4.cuh"
 
@@ -112,6 +114,7 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
     if (rc != CB_OK) return rc;
     CB_REQUIRE(B >= 0 && B < (1ll << 31) && T >= 0 && H >= 0, "%s: negative or too large batch, T or H", who);
     CB_REQUIRE(table_stride >= 0 && table_stride < (1ll << 31), "%s: page table out of range", who);
+    CB_REQUIRE(std::isfinite(scale), "%s: scale must be finite", who);
     if (B == 0 || T == 0 || H == 0) return CB_OK;
     CB_REQUIRE(H % cache->kv_heads == 0, "%s: H must be a multiple of kv_heads", who);
     CB_REQUIRE(T < (1 << 24) && H < (1 << 20) && T * H * cache->head_dim < (1ll << 31), "%s: T * H out of range", who);
@@ -146,6 +149,7 @@ int cb_prompt_attention(const void* q, const void* k, const void* v, const int64
     CB_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128 (got %d)", who, head_dim);
     CB_REQUIRE(Tq >= 0 && Tk >= 0 && Tq < (1ll << 30) && Tk < (1ll << 30), "%s: too many tokens", who);
     CB_REQUIRE(H >= 0 && Hkv >= 0 && H < (1 << 20) && Hkv < (1 << 20) && B >= 0 && B < (1ll << 30), "%s: heads or sequences out of range", who);
+    CB_REQUIRE(std::isfinite(scale), "%s: scale must be finite", who);
     if (Tq == 0 || H == 0 || B == 0) return CB_OK;
     CB_REQUIRE(Hkv > 0 && H % Hkv == 0, "%s: H must be a multiple of Hkv", who);
     CB_REQUIRE(q && out && cu_q && cu_k && strides6 && (Tk == 0 || (k && v)), "%s: NULL pointer", who);

@@ -787,3 +787,26 @@ def test_the_largest_bfloat16_queries(power):
         want = values64(codes, scale, lo)[t, 0]
         tol = torch.finfo(torch.bfloat16).eps / 2 * 1.01 * want.abs() + 2.0 ** -20 * (15 * scale + lo.abs())[t, 0].repeat_interleave(32)
         assert ((got[0, 0, h].double() - want).abs() <= tol).all()
+
+
+def test_a_scale_that_is_not_finite_is_refused():
+    from crispybits_kernels import _C
+    lib, c = _C._lib, _C._KV4Cache(256, 4, 2, 128, 64, 64, 1)
+    s3, s6 = (ctypes.c_int64 * 3)(8, 8, 8), (ctypes.c_int64 * 6)(*[128] * 6)
+    for scale in (math.nan, math.inf, -math.inf, 1e39):
+        assert lib.cb_kv4_attention(ctypes.byref(c), 256, s3, 256, 2, 1, 4, 256, 2, 256, scale, 256, 1 << 20, 256, 1 << 30, 0) == 1
+        assert b"scale" in lib.cb_last_error()
+        assert lib.cb_prompt_attention(256, 256, 256, s6, 256, 4, 4, 2, 2, 64, 1, 256, 256, 1, scale, 1, 256, 1 << 20, 256, 1 << 40, 0) == 1
+        assert b"scale" in lib.cb_last_error()
+
+
+@pytest.mark.gpu
+def test_a_scale_that_is_not_finite_is_refused_in_python():
+    import crispybits_kernels as ck
+    f = Filled([20], 2, 64, 32, 16, torch.float16)
+    q = rand_q(1, 1, 4, 64, torch.float16)
+    for scale in (math.nan, math.inf, 1e39):
+        with pytest.raises(RuntimeError, match="scale"):
+            ck.kv4_attention(q, f.cache, f.table, f.lengths, scale=scale)
+        with pytest.raises(RuntimeError, match="scale"):
+            ck.prompt_attention(q[0], q[0], q[0], i32([0, 1]), scale=scale)
