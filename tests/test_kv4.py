@@ -810,3 +810,15 @@ def test_a_scale_that_is_not_finite_is_refused_in_python():
             ck.kv4_attention(q, f.cache, f.table, f.lengths, scale=scale)
         with pytest.raises(RuntimeError, match="scale"):
             ck.prompt_attention(q[0], q[0], q[0], i32([0, 1]), scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 7, 8, 9, 13, 17])
+@pytest.mark.parametrize("T", [1, 2, 3])
+def test_tiles_with_rows_to_spare(group, T):
+    """Fewer rows than a tile has, in whole blocks, blocks that the newest tokens see in part, and blocks that end inside."""
+    import crispybits_kernels as ck
+    lens = [2, 31, 32, 33, 800, 1311]
+    f = Filled(lens, 2, 64, 32, 32, torch.float16, seed=group)
+    q = rand_q(len(lens), T, 2 * group, 64, torch.float16)
+    check(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
