@@ -81,14 +81,19 @@ def kv4_append(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, page_table: to
     """Quantise the keys and values of new tokens into the cache.
 
     k, v: packed [tokens, kv_heads, head_dim] with `cu_seqlens` [B + 1], the first token of each sequence; or, without it,
-    [B, kv_heads, head_dim] (a decode step) or [B, T, kv_heads, head_dim].  Any strides; rows that are not contiguous or not
+    [B, T, kv_heads, head_dim], or packed with as many tokens of each sequence (a decode step: one).  Any strides; rows that are not contiguous or not
     16-byte aligned are copied first.  `starts` [B]: the position of each sequence's first new token.  No position
     may be written twice in one call.  A token whose position has no page (beyond the table, or a page number outside the cache) is left out,
     and `_C.decode_status()` then reports 3001."""
-    if cu_seqlens is None and k.dim() == 4:
-        k, v = (t.flatten(0, 1) if t.dim() == 4 else t for t in (k, v))
-    if cu_seqlens is None and page_table.dim() == 2 and page_table.shape[0] and k.shape[0] % page_table.shape[0]:
-        raise ValueError("kv4_append: without cu_seqlens every sequence brings as many tokens")
+    if cu_seqlens is None:
+        if k.dim() == 4 or v.dim() == 4:
+            if k.shape != v.shape:
+                raise ValueError("kv4_append: k and v must have the same shape")
+            if page_table.dim() == 2 and k.shape[0] != page_table.shape[0]:
+                raise ValueError("kv4_append: page_table needs one row for each sequence of k and v")
+            k, v = k.flatten(0, 1), v.flatten(0, 1)
+        if page_table.dim() == 2 and page_table.shape[0] and k.shape[0] % page_table.shape[0]:
+            raise ValueError("kv4_append: without cu_seqlens every sequence brings as many tokens")
     _C().kv4_append(cache, k, v, page_table, starts, cu_seqlens)
 
 

@@ -169,3 +169,19 @@ def test_stack_with_attention_on_gpu(head_dim):
     assert cache.lengths.tolist() == [86, 49, 27]
     from crispybits_kernels import _C
     assert _C.decode_status() == 0
+
+
+def test_append_refuses_batches_that_do_not_fit_the_page_table(stand_in):
+    """A batch of another number of sequences, or k and v of different [B, T], would put tokens into sequences that are not theirs."""
+    from crispybits_kernels import KV4Cache, kv4_append, kv4_read
+    cache = KV4Cache.empty(4, 2, 64, 16, device="cpu")
+    table, starts = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    x = torch.randn(8, 2, 64).half()
+    for k, v in ((x.view(4, 2, 2, 64), x.view(4, 2, 2, 64)), (x.view(1, 8, 2, 64), x.view(1, 8, 2, 64)), (x.view(2, 4, 2, 64), x.view(4, 2, 2, 64)),
+                 (x.view(2, 4, 2, 64), x), (x, x.view(2, 4, 2, 64)), (x[:7], x[:7])):
+        with pytest.raises(ValueError):
+            kv4_append(cache, k, v, table, starts)
+    kv4_append(cache, x.view(2, 4, 2, 64), x.view(2, 4, 2, 64), table, starts)
+    a = kv4_read(cache, table, starts, None, 8)
+    kv4_append(cache, x, x, table, starts)                         # packed, as many tokens of each
+    assert torch.equal(a[0], kv4_read(cache, table, starts, None, 8)[0])
