@@ -85,7 +85,8 @@ class _Block:
 
 class StackCache:
     """Keys and values of `batch` sequences for every block of a DecodeStack (this rank's heads), in 4 bits: one KV4Cache for
-    each block, one page table and one vector of lengths for all.  Sequence s owns pages s * n .. s * n + n - 1."""
+    each block, one page table and one vector of lengths for all.  Sequence s owns pages s * n .. s * n + n - 1, with room for
+    `capacity` tokens: max_tokens, rounded up to whole pages."""
 
     def __init__(self, stack: "DecodeStack", batch: int, max_tokens: int, head_dim: int = 128, page_size: int = 64,
                  group_size: int = 64, dtype: torch.dtype = torch.float16):
@@ -93,12 +94,29 @@ class StackCache:
         if local % head_dim:
             raise ValueError("a rank's rows of Q must be whole heads")
         pages = -(-max_tokens // page_size)
-        self.batch, self.heads, self.head_dim = batch, local // head_dim, head_dim
+        self.batch, self.heads, self.head_dim, self.capacity = batch, local // head_dim, head_dim, pages * page_size
         self.layers = [KV4Cache.empty(batch * pages, self.heads, head_dim, page_size, group_size, dtype, stack.device)
                        for _ in range(stack.n_blocks)]
         self.page_table = torch.arange(batch * pages, dtype=torch.int32, device=stack.device).view(batch, pages)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=stack.device)      # cached tokens of each sequence
         self.seen = torch.zeros_like(self.lengths)                                     # of the running step: its own tokens too
+        self._longest, self._at, self._replayed = 0, None, False      # the largest of `lengths`, and the version of them that it was read from
+
+    def longest(self) -> int:
+        """Tokens of the longest sequence.  The lengths are read from the device only where they may have changed behind the eager calls that
+        advance them: by hand, or by replays of a captured step."""
+        version = None if self.lengths.is_inference() else self.lengths._version
+        if version is None or version != self._at or self._replayed:
+            self._longest, self._at = max(self.lengths.tolist(), default=0), version
+        return self._longest
+
+    def advance(self, longest: int):
+        """`seen` becomes `lengths`; `longest` of them, from an eager call."""
+        self.lengths.copy_(self.seen)
+        if self.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
+            self._replayed = True
+        elif not self.lengths.is_inference():
+            self._longest, self._at = longest, self.lengths._version
 
 
 class DecodeStack:
@@ -266,7 +284,9 @@ class DecodeStack:
 
     def step(self, x: torch.Tensor, decode_threshold: int = 8, cache: Optional[StackCache] = None) -> torch.Tensor:
         """x [B, d_model] (replicated on every rank) -> the last block's down-projection output [B, d_model].  With a cache, row s is the
-        next token of sequence s: its keys and values are appended, and what o_proj reads is its attention over the cache."""
+        next token of sequence s: its keys and values are appended, and what o_proj reads is its attention over the cache.  A cache with no
+        room for it is refused; replays of a captured step have to stay within `capacity` by themselves (a token beyond it is left out, and
+        the library's status is then 3001)."""
         if self.comm != "nccl":
             if cache is not None:
                 raise ValueError("attention in the step needs comm='nccl'")
@@ -275,6 +295,11 @@ class DecodeStack:
         kw = dict(decode_threshold=decode_threshold, workspace=self.workspace)
         if cache is not None:
             self._check_cache(cache, x.shape[0])
+            longest = 0
+            if not (cache.lengths.is_cuda and torch.cuda.is_current_stream_capturing()):
+                longest = cache.longest() + 1
+                if longest > cache.capacity:
+                    raise ValueError(f"the cache is full: {cache.capacity} tokens of a sequence")
             torch.add(cache.lengths, 1, out=cache.seen)
         for i, blk in enumerate(self.blocks):
             oq, ok, ov = fused_qkv(x, blk.q, blk.k, blk.v, **kw)
@@ -286,7 +311,7 @@ class DecodeStack:
             m = self.gather(fused_gate_up(a, blk.gate, blk.up, **kw))
             y = self.gather(packed_linear(m, blk.down, **kw))
         if cache is not None:
-            cache.lengths.copy_(cache.seen)
+            cache.advance(longest)
         return y                                          # the last block's output; every block ran the same launches
 
     def _check_cache(self, cache: StackCache, batch: int):
@@ -298,12 +323,18 @@ class DecodeStack:
     def prefill(self, x: torch.Tensor, lens: List[int], cache: StackCache, past: Optional[List[int]] = None) -> torch.Tensor:
         """Prompts of all sequences: x [sum(lens), d_model], packed -> the last block's output [sum(lens), d_model]; their keys and
         values enter the cache.  `past`: tokens that each sequence has cached already (default: none); the prompts then attend to
-        these too, as the cache holds them, and to themselves in the cache's 4 bits as well."""
+        these too, as the cache holds them, and to themselves in the cache's 4 bits as well.  It has to be what the cache's lengths
+        say (which are read, so the call waits for the device), and the cache has to have room for the prompts."""
         if self.comm != "nccl":
             raise ValueError("prefill needs comm='nccl'")
         self._check_cache(cache, len(lens))
         if sum(lens) != x.shape[0]:
             raise ValueError("lens must add up to the rows of x")
+        held = cache.lengths.tolist()
+        if held != (list(past) if past is not None else [0] * cache.batch):
+            raise ValueError(f"past must be what the sequences have cached: {held}")
+        if min(lens, default=0) < 0 or max((n + p for n, p in zip(lens, held)), default=0) > cache.capacity:
+            raise ValueError(f"the cache has room for {cache.capacity} tokens of a sequence")
         bounds = lambda v: torch.tensor(np.concatenate(([0], np.cumsum(v))), dtype=torch.int32).to(self.device)
         cu, y = bounds(lens), None
         total = [n + p for n, p in zip(lens, past)] if past is not None else lens
@@ -319,7 +350,7 @@ class DecodeStack:
             a = self.gather(packed_linear(a, blk.o, workspace=self.workspace))
             m = self.gather(fused_gate_up(a, blk.gate, blk.up, workspace=self.workspace))
             y = self.gather(packed_linear(m, blk.down, workspace=self.workspace))
-        cache.lengths.copy_(cache.seen)
+        cache.advance(max(total))
         return y
 
     # -------------------------------------------------------------- check value (fp32, any device)

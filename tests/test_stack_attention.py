@@ -185,3 +185,65 @@ def test_append_refuses_batches_that_do_not_fit_the_page_table(stand_in):
     a = kv4_read(cache, table, starts, None, 8)
     kv4_append(cache, x, x, table, starts)                         # packed, as many tokens of each
     assert torch.equal(a[0], kv4_read(cache, table, starts, None, 8)[0])
+
+
+def test_a_past_that_is_not_the_caches_and_tokens_without_room_are_refused(stand_in):
+    """Nothing is appended by a call that is refused."""
+    st, cache = make()
+    assert cache.capacity == 48                                    # 40 tokens in pages of 16
+    x = lambda n: torch.randn(n, 256, generator=torch.Generator().manual_seed(n)).half()
+    st.prefill(x(8), [5, 1, 2], cache)
+    for lens, past in (([5, 1, 2], None), ([5, 1, 2], [5, 1, 3]), ([5, 1, 2], [5, 1]), ([5, 1, 2], [0, 0, 0]), ([44, 0, 0], [5, 1, 2]), ([-1, 1, 1], [5, 1, 2])):
+        with pytest.raises(ValueError):
+            st.prefill(x(sum(lens)), lens, cache, past=past)
+        assert cache.lengths.tolist() == [5, 1, 2]
+    st.prefill(x(41), [41, 0, 0], cache, past=[5, 1, 2])
+    for n in (47, 48):
+        st.step(x(3), cache=cache)
+        assert cache.lengths.tolist()[0] == n
+    with pytest.raises(ValueError):
+        st.step(x(3), cache=cache)
+    assert cache.lengths.tolist() == [48, 3, 4]
+    cache.lengths.copy_(torch.tensor([47, 0, 1]))                  # sequences start again: the lengths are theirs who own the cache
+    st.step(x(3), cache=cache)
+    with pytest.raises(ValueError):
+        st.step(x(3), cache=cache)
+    cache.lengths.zero_()
+    st.prefill(x(8), [5, 1, 2], cache)
+    assert cache.lengths.tolist() == [5, 1, 2]
+
+
+def test_a_cache_made_in_inference_mode(stand_in):
+    with torch.inference_mode():
+        from crispybits_kernels.stack import StackCache
+        st = make()[0]
+        cache = StackCache(st, 3, 16, head_dim=64, page_size=16)
+        x = torch.randn(3, 256, generator=torch.Generator().manual_seed(1)).half()
+        st.prefill(x.repeat(16, 1), [16, 16, 16], cache)
+        cache.lengths.fill_(15)
+        st.step(x, cache=cache)
+        with pytest.raises(ValueError):
+            st.step(x, cache=cache)
+
+
+@pytest.mark.gpu
+def test_replays_of_a_captured_step_count_for_the_eager_ones():
+    import crispybits_kernels as ck
+    from crispybits_kernels import ops
+    from crispybits_kernels.stack import DecodeStack, StackCache
+    ops.set_backend("cuda")
+    st = DecodeStack(1, 256, 512, bitmap=[4], device="cuda", std=0.05)
+    cache = StackCache(st, 2, 16, head_dim=64, page_size=16)
+    x, graph = torch.randn(2, 256, device="cuda").half(), torch.cuda.CUDAGraph()
+    st.step(x, cache=cache)
+    with torch.cuda.graph(graph):
+        st.step(x, cache=cache)
+    for _ in range(14):
+        graph.replay()
+    st.step(x, cache=cache)
+    assert cache.lengths.tolist() == [16, 16]
+    with pytest.raises(ValueError):
+        st.step(x, cache=cache)
+    graph.replay()                                                 # left out, and said so
+    from crispybits_kernels import _C
+    assert _C.decode_status() == 3001 and ck.kv4_read(cache.layers[0], cache.page_table, torch.zeros_like(cache.lengths), None, 32)[0].shape[0] == 32
