@@ -100,6 +100,7 @@ template <> struct Pair<__half> {
         return *reinterpret_cast<const uint32_t*>(&r);
     }
     static constexpr float kTop = 65504.f;
+    static constexpr uint32_t kTie = 0x1000u;                     // the bits of a float that a normal fp16 has not, half way between two
     // value = code * scale + lo with one rounding, for two codes at bits 0-3 and 16-19: 1024 + code from the bits, exactly
     __device__ static uint32_t values(uint32_t codes, uint32_t scale2, uint32_t lo2) {
         const uint32_t u = (codes & 0x000F000Fu) | 0x64006400u, k = 0x64006400u;
@@ -124,6 +125,7 @@ template <> struct Pair<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t*>(&r);
     }
     static constexpr float kTop = 3.3895314e38f;
+    static constexpr uint32_t kTie = 0x8000u;
     // as for fp16; 128 + code from the bits
     __device__ static uint32_t values(uint32_t codes, uint32_t scale2, uint32_t lo2) {
         const uint32_t u = (codes & 0x000F000Fu) | 0x43004300u, k = 0x43004300u;
@@ -133,10 +135,24 @@ template <> struct Pair<__nv_bfloat16> {
     }
 };
 
-// The group's (scale, lo) as stored, from its exact minimum and maximum.
+// What rounding took from d = a - b, exactly.
+__device__ __forceinline__ float lost(float a, float b, float d) {
+    const float bb = d - a;
+    return (a - (d - bb)) - (b + bb);
+}
+
+// The group's (scale, lo) as stored, from its exact minimum and maximum.  The range hi - lo may need more bits than a float has; what it loses
+// matters only where the quotient lies half way between two values of T.  (It lies there exactly if it looks so: 15 times such a value is a float, and
+// other floats are at least a 2^-24th of it away, a quotient's rounding half as much at most.)
 template <typename T>
 __device__ __forceinline__ uint32_t group_meta(float lo, float hi) {
-    float scale = to_f32(from_f32<T>(__fdiv_rn(hi - lo, 15.0f)));
+    const float range = hi - lo;
+    float q = __fdiv_rn(range, 15.0f);
+    if ((__float_as_uint(q) & (2 * Pair<T>::kTie - 1)) == Pair<T>::kTie) {
+        const float e = lost(hi, lo, range);
+        if (e != 0.f) q = __uint_as_float(__float_as_uint(q) + (e > 0.f ? 1 : -1));
+    }
+    float scale = to_f32(from_f32<T>(q));
     if (scale < 1.17549435e-38f) scale = 0.f;
     if (!(scale < INFINITY) || !(fabsf(lo) < INFINITY)) scale = lo = __int_as_float(0x7fffffff);
     return Pair<T>::pack(scale, lo);
@@ -150,10 +166,11 @@ __device__ __forceinline__ float rcp_approx(float x) {
 }
 
 // round_half_even((x - lo) / scale), at most 15, for 8 values: the codes as 4-bit fields.  Adding 1.5 * 2^23 rounds; the rounded
-// quotients are gathered by multiply-adds.  The remainder x - lo - code * scale, which the fused multiply-add forms without rounding,
+// quotients are gathered by multiply-adds.  The remainder a - code * scale of a = x - lo, which the fused multiply-add forms without rounding,
 // shows where the approximate quotient met a tie or fell on the wrong side of one: there it is half a step or more (`half`: half a step, or 0
 // where a code could exceed 15), and the eight are put right one by one.  (A tie in 8 values is met by 7 % of the warps for normal fp16
-// values, by 38 % for bfloat16.)
+// values, by 38 % for bfloat16.)  a itself is rounded where x and lo are of very different size; that is less than the step in which remainders and half
+// steps lie, so that it decides where the remainder is half a step and nowhere else.
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale, float lo, float inv, float half) {
     constexpr float kMagic = 12582912.f;
@@ -172,9 +189,14 @@ __device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale
         const float h = 0.5f * scale;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const bool odd = ((int)c[j] & 1) != 0;
-            if (rest[j] > h || (rest[j] == h && odd)) c[j] += 1.f;
-            if (rest[j] < -h || (rest[j] == -h && odd)) c[j] -= 1.f;
+            float past = fabsf(rest[j]) - h;                      // beyond half a step, in the remainder's direction
+            if (past == 0.f) {
+                const float2 f = Pair<T>::f2(x[j / 2]);
+                const float v = j & 1 ? f.y : f.x;
+                past = copysignf(1.f, rest[j]) * lost(v, lo, v - lo);
+                if (past == 0.f) past = (float)((int)c[j] & 1);   // a tie: to even
+            }
+            if (past > 0.f) c[j] += copysignf(1.f, rest[j]);
             c[j] = fminf(c[j], 15.f);
         }
     }
@@ -190,7 +212,7 @@ template <int D> struct Place {
 };
 
 template <typename T, int D, int GS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)              // 64 registers; with three CTAs to an SM the prompts above take 136 us for 125
 kv4_append_kernel(const RowParams P) {
     using L = KvLayout<D, GS>;
     constexpr int kTpr = Place<D>::kTpr, kPer = Place<D>::kPer, kBatch = 4;       // kBatch: loads in flight

@@ -822,3 +822,56 @@ def test_tiles_with_rows_to_spare(group, T):
     f = Filled(lens, 2, 64, 32, 32, torch.float16, seed=group)
     q = rand_q(len(lens), T, 2 * group, 64, torch.float16)
     check(ck.kv4_attention(q, f.cache, f.table, f.lengths), f.reference(q))
+
+
+def exact_codes(row, gs, dtype):
+    """Codes, scale and lo of one row, in rational arithmetic."""
+    from fractions import Fraction as Fr
+    codes, scales, los = [], [], []
+    for g in range(0, len(row), gs):
+        x = [Fr(v) for v in row[g:g + gs]]
+        lo, want = min(x), (max(x) - min(x)) / 15
+        near = torch.tensor(float(want), dtype=torch.double).to(dtype)
+        around = torch.stack((near, torch.nextafter(near, torch.tensor(0.0).to(dtype)), torch.nextafter(near, torch.tensor(math.inf).to(dtype)))).double().tolist()
+        even = lambda v: torch.tensor(v, dtype=torch.double).to(dtype).view(torch.int16).item() & 1
+        scale = min((Fr(v) for v in around if math.isfinite(v)), key=lambda v: (abs(v - want), even(float(v))))
+        codes += [0 if scale == 0 else min(15, round((v - lo) / scale)) for v in x]                     # Fraction rounds half to even
+        scales.append(float(scale)); los.append(float(lo))
+    return codes, scales, los
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_codes_at_half_steps_beside_a_tiny_minimum(dtype):
+    """A minimum some 2^-30 of the other values: what a float loses of x - lo, and of the range, decides the ties.  Every byte as defined."""
+    import crispybits_kernels as ck
+    d, gs = 64, 32
+    tiny = (2.0 ** -24, 2.0 ** -22) if dtype == torch.float16 else (2.0 ** -30, 2.0 ** -100)
+    ends = [(lo, top) for top in (15.0, 15.0 * 2 ** -6) for lo in (*tiny, *(-t for t in tiny))]
+    if dtype == torch.float16:
+        # ranges hi - lo beside 15 t, t half way between two scales: hi = 15 t - r, lo = -r (1 +- 2^-10) with r of one bit, 2^-15 or 2^-14 of hi
+        # (bfloat16 has none that a float does not hold: 15 t has 13 bits, hi 8, so that r is 2^-12 of it or more and lo a multiple of 2^-19)
+        fits = lambda v: torch.tensor(v, dtype=torch.double).to(dtype).double().item() == v
+        found = [(-r * e, 15 * t - r) for k in range(1 << 10, 1 << 11) for t in [(2 * k + 1) * 2.0 ** -11] for r in (2.0 ** -12, 2.0 ** -11, 2.0 ** -10)
+                 if fits(15 * t - r) for e in (1 + 2.0 ** -10, 1 - 2.0 ** -11, 1.0)]
+        assert len(found) >= 30
+        ends += found[:12] + found[-12:]
+    rows = []
+    for lo, top in ends:
+        step = torch.tensor((top - lo) / 15, dtype=torch.double).to(dtype).double().item()
+        x = [lo, top, *((i + 0.5) * step for i in range(15))]
+        rows.append((x + [1.0 * step] * (gs - len(x))) * 2)
+    x = torch.tensor(rows, dtype=torch.double).to(dtype)
+    x[:, gs:] *= -1
+    n = x.shape[0]
+    c = ck.KV4Cache.empty(1, 1, d, 64, gs, dtype)
+    c.pages.zero_()
+    xs = x[:, None].to(DEV)
+    ck.kv4_append(c, xs, xs, i32([[0]]), i32([0]), i32([0, n]))
+    page, lay = torch.zeros(c.pages.shape[2], dtype=torch.uint8), Layout(d, gs)
+    for i in range(n):
+        codes, scale, lo = exact_codes(x[i].double().tolist(), gs, dtype)
+        for which in "kv":
+            lay.put(page, which, i, codes, torch.tensor(scale), torch.tensor(lo), dtype)
+    got = c.pages[0, 0].cpu()
+    assert torch.equal(got, page), f"{int((got != page).sum())} bytes differ"
