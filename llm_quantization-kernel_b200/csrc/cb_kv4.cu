@@ -143,19 +143,25 @@ __device__ __forceinline__ float lost(float a, float b, float d) {
 
 // The group's (scale, lo) as stored, from its exact minimum and maximum.  The range hi - lo may need more bits than a float has; what it loses
 // matters only where the quotient lies half way between two values of T.  (It lies there exactly if it looks so: 15 times such a value is a float, and
-// other floats are at least a 2^-24th of it away, a quotient's rounding half as much at most.)
+// other floats are at least a 2^-24th of it away, a quotient's rounding half as much at most.)  A range beyond the largest float is formed of halves,
+// which are exact: a float holds half of any value of T.
+constexpr float kWide = 2.2e37f;                                  // scales above it may have such a range: 15 of them are 3.3e38
 template <typename T>
-__device__ __forceinline__ uint32_t group_meta(float lo, float hi) {
+__device__ __forceinline__ uint32_t group_meta(float low, float hi) {
+    const bool wide = Pair<T>::kTop > 15.f * kWide && hi - low == INFINITY && hi < INFINITY && low > -INFINITY;
+    const float part = wide ? 0.5f : 1.f, lo = part * low;
+    hi *= part;
     const float range = hi - lo;
     float q = __fdiv_rn(range, 15.0f);
     if ((__float_as_uint(q) & (2 * Pair<T>::kTie - 1)) == Pair<T>::kTie) {
         const float e = lost(hi, lo, range);
         if (e != 0.f) q = __uint_as_float(__float_as_uint(q) + (e > 0.f ? 1 : -1));
     }
-    float scale = to_f32(from_f32<T>(q));
+    float scale = to_f32(from_f32<T>(q)), stored = low;
+    if (wide) scale += scale;
     if (scale < 1.17549435e-38f) scale = 0.f;
-    if (!(scale < INFINITY) || !(fabsf(lo) < INFINITY)) scale = lo = __int_as_float(0x7fffffff);
-    return Pair<T>::pack(scale, lo);
+    if (!(scale < INFINITY) || !(fabsf(low) < INFINITY)) scale = stored = __int_as_float(0x7fffffff);
+    return Pair<T>::pack(scale, stored);
 }
 
 // Reciprocal to about 2^-22; what it gets wrong is found below.
@@ -163,6 +169,26 @@ __device__ __forceinline__ float rcp_approx(float x) {
     float y;
     asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// round_half_even((x - lo) / scale), at most 15, for 8 bfloat16 values of a group whose range may be beyond the largest float: from halves.  Not inlined, since
+// hardly ever called.
+__device__ __noinline__ uint32_t wide_codes(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, float scale, float lo) {
+    uint32_t word = 0u;
+    const float step = 0.5f * scale, low = 0.5f * lo, h = 0.5f * step;
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t two = j < 2 ? x0 : j < 4 ? x1 : j < 6 ? x2 : x3;
+        const float v = 0.5f * __uint_as_float(j & 1 ? two & 0xFFFF0000u : two << 16), a = v - low;
+        float c = floorf(__fdiv_rn(a, step));                     // the quotient's rounding up to a whole number: the remainder is then below 0
+        float rest = fmaf(-c, step, a);
+        if (rest < 0.f) { c -= 1.f; rest += step; }
+        float past = rest - h;                                    // beyond half a step
+        if (past == 0.f) past = lost(v, low, a);
+        if (past == 0.f) past = (float)((int)c & 1);
+        if (past > 0.f) c += 1.f;
+        word |= (uint32_t)fminf(c, 15.f) << (4 * j);
+    }
+    return word;
 }
 
 // round_half_even((x - lo) / scale), at most 15, for 8 values: the codes as 4-bit fields.  Adding 1.5 * 2^23 rounds; the rounded
@@ -186,6 +212,7 @@ __device__ __forceinline__ uint32_t codes_of(const uint32_t (&x)[4], float scale
     }
     if (!(worst < half)) {
         if (!(scale > 0.f)) return 0u;                            // one value, or NaN
+        if (Pair<T>::kTop > 15.f * kWide && scale > kWide) return wide_codes(x[0], x[1], x[2], x[3], scale, lo);
         const float h = 0.5f * scale;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {

@@ -875,3 +875,36 @@ def test_codes_at_half_steps_beside_a_tiny_minimum(dtype):
             lay.put(page, which, i, codes, torch.tensor(scale), torch.tensor(lo), dtype)
     got = c.pages[0, 0].cpu()
     assert torch.equal(got, page), f"{int((got != page).sum())} bytes differ"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gs", [32, 64])
+def test_groups_whose_range_is_no_float(gs):
+    """Finite bfloat16 values more than the largest float apart: bytes as defined, and values read back (those beyond the largest are the largest)."""
+    import crispybits_kernels as ck
+    d, top = 64, torch.finfo(torch.bfloat16).max
+    gen = torch.Generator().manual_seed(1)
+    rows = [torch.linspace(-1, 1, d, dtype=torch.double) * top, torch.where(torch.rand(d, generator=gen) < 0.5, -top, top).double(),
+            torch.cat((torch.full((63,), -top), torch.tensor([2.0 ** -133]))).double(), (torch.rand(d, generator=gen).double() * 2 - 1) * top,
+            (torch.rand(d, generator=gen).double() * 1.1 - 0.1) * top, torch.tensor([-top, top, *(-top + (i % 15 + 0.5) * (top / 7.5) for i in range(62))]),
+            torch.tensor([-top * 0.51, top * 0.51, *([1.0, -2.0 ** -133] * 31)])]
+    x = torch.stack([r.double() for r in rows]).to(torch.bfloat16)
+    x = torch.where(torch.isfinite(x), x, torch.tensor(top).to(x.dtype))
+    x = torch.cat((x, -x))
+    n = x.shape[0]
+    c = ck.KV4Cache.empty(1, 1, d, 64, gs, torch.bfloat16)
+    c.pages.zero_()
+    xs = x[:, None].to(DEV)
+    ck.kv4_append(c, xs, xs, i32([[0]]), i32([0]), i32([0, n]))
+    page, lay, want = torch.zeros(c.pages.shape[2], dtype=torch.uint8), Layout(d, gs), []
+    for i in range(n):
+        codes, scale, lo = exact_codes(x[i].double().tolist(), gs, torch.bfloat16)
+        want.append([k * scale[j // gs] + lo[j // gs] for j, k in enumerate(codes)])
+        for which in "kv":
+            lay.put(page, which, i, codes, torch.tensor(scale, dtype=torch.double), torch.tensor(lo, dtype=torch.double), torch.bfloat16)
+    got = c.pages[0, 0].cpu()
+    assert torch.equal(got, page), f"{int((got != page).sum())} bytes differ"
+    want = torch.tensor(want, dtype=torch.double).clamp(-top, top)
+    for y in ck.kv4_read(c, i32([[0]]), i32([0]), i32([0, n]), n):
+        # one rounding of the type, of a sum of two that fp32 may have rounded first
+        assert ((y[:, 0].cpu().double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20) + 2.0 ** -24 * 2 * top + 2.0 ** -133).all()
