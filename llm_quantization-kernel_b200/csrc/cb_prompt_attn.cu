@@ -54,6 +54,7 @@ constexpr int kSoftRegs = 216, kOtherRegs = 72;
 // a lag, which would be one of halved units: parts compare their references in whole ones.)
 constexpr float kLargeScore = 16777216.f;
 constexpr long long kWaitCycles = 2000000000ll;       // about a second
+constexpr long long kBeatCycles = 1 << 24;            // and as much for each stretch of 4096 keys that mend() has gone through: several times what it takes
 
 __device__ int g_prompt_status;
 
@@ -103,7 +104,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
     while (!mbar_try_wait(bar, parity))
-        if (*abort_flag != 0 || clock64() - t0 > kWaitCycles) return false;
+        if (abort_flag[0] != 0 || clock64() - t0 > kWaitCycles + abort_flag[1] * kBeatCycles) return false;
     return true;
 }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
@@ -318,6 +319,11 @@ __device__ __forceinline__ int arrive(int* counter) {
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
     return before;
 }
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -328,52 +334,91 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One row's 32 columns from d0 on, as this warp has just stored them: at `out`, finished (O times inv), or without it at `part`, O itself.  If a key of
-// the row's key tiles that the row does not see holds a value that is not finite in a column that came out as NaN, the column's sum over the keys
-// that the row does see is formed again: keys [0, limit) of the step.
+// 16-bit values d .. d + 7 of a row times those of another, added up in four sums.
+template <typename T> __device__ __forceinline__ void dot8(const uint4& a, const uint4& b, float (&s)[4]) {
+    const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 u = unpack2<T>(x[i]), v = unpack2<T>(y[i]);
+        s[i] = fmaf(u.x, v.x, fmaf(u.y, v.y, s[i]));
+    }
+}
+
+// One row, as this warp has just stored it: finished at `out` (O times inv), or O itself at `part` (column c at part[c * kSub]).  If a key of the row's key
+// tiles that the row does not see holds a value that is not finite in a column that came out as NaN, the column's sum over the keys that the row
+// does see is formed again: keys [0, limit) of the step.  The warp does this together, a key to a lane for the weights, D / 32 columns to a lane for the
+// sums; about 100 ns a key.  `beat` counts its stretches, for those who wait for this warp.  (As a call it is 0.2 us slower where it is not called.)
 template <typename T, int D>
-__device__ void mend(const PromptParams& P, const Work& w, int row, int limit, int tiles, int d0, float factor, float m_ref, float inv, T* out, float* part) {
-    const int64_t kv_head = w.head / P.group;
-    const T* q = reinterpret_cast<const T*>(P.q) + (int64_t)(w.q_first + row) * P.q_tok + w.head * P.q_head;
-    const T* k = reinterpret_cast<const T*>(P.k) + (int64_t)w.k_first * P.k_tok + kv_head * P.k_head;
-    const T* val = reinterpret_cast<const T*>(P.v) + (int64_t)w.k_first * P.v_tok + kv_head * P.v_head + d0;
+__device__ __forceinline__ void mend(const PromptParams& P, int lane, int head, int64_t q_row, int64_t k_first, int limit, int end, float factor, float m_ref,
+                                  float inv, T* out, float* part, int* beat) {
+    constexpr int kV = D / 32;
+    const int64_t kv_head = head / P.group;
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(P.q) + q_row * P.q_tok + head * P.q_head);
+    const T* k = reinterpret_cast<const T*>(P.k) + k_first * P.k_tok + kv_head * P.k_head;
+    const T* val = reinterpret_cast<const T*>(P.v) + k_first * P.v_tok + kv_head * P.v_head + lane * kV;
+    auto values = [&](int key, float (&x)[kV]) {                  // this lane's columns of a key's values
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(val + key * P.v_tok);
+#pragma unroll
+        for (int i = 0; i < kV / 2; ++i) { const float2 f = unpack2<T>(at[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+    };
     uint32_t spoilt = 0u;
-    for (int key = limit; key < min(tiles * kTileK, w.lk); ++key)
+#pragma unroll 4
+    for (int key = limit; key < end; ++key) {
+        float x[kV];
+        values(key, x);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (!(fabsf(to_f32(val[key * P.v_tok + i])) < INFINITY)) spoilt |= 1u << i;
-    float v[32];
+        for (int i = 0; i < kV; ++i)
+            if (!(fabsf(x[i]) < INFINITY)) spoilt |= 1u << i;
+    }
+    float v[kV];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        v[i] = out != nullptr ? to_f32(*reinterpret_cast<const volatile T*>(out + i)) : __ldcg(part + i * kSub);
+    for (int i = 0; i < kV; ++i) {
+        v[i] = out != nullptr ? to_f32(*reinterpret_cast<const volatile T*>(out + lane * kV + i)) : __ldcg(part + (lane * kV + i) * kSub);
         if (v[i] == v[i]) spoilt &= ~(1u << i);
         v[i] = 0.f;
     }
-    if (spoilt == 0u) return;
+    if (!__any_sync(0xffffffffu, spoilt != 0u)) return;
     const float neg = m_ref == -INFINITY ? 0.f : -m_ref, mul = P.negate ? -factor : factor;
-    for (int key = 0; key < limit; ++key) {
+    for (int key0 = 0; key0 < limit; key0 += 32) {
         float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int d = 0; d < D; d += 4)
+        if (key0 + lane < limit) {
+            const uint4* row = reinterpret_cast<const uint4*>(k + (key0 + lane) * P.k_tok);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) s[c] = fmaf(to_f32(q[d + c]), to_f32(k[key * P.k_tok + d + c]), s[c]);
+            for (int d = 0; d < D / 8; ++d) dot8<T>(q[d], row[d], s);
+        }
         const float p = ex2(fmaf((s[0] + s[1]) + (s[2] + s[3]), mul, neg));
+        const int n = min(limit - key0, 32);
+        if (n == 32) {
+#pragma unroll 16
+            for (int i = 0; i < 32; ++i) {
+                float x[kV];
+                values(key0 + i, x);
+                const float pi = __shfl_sync(0xffffffffu, p, i);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if ((spoilt >> i) & 1u) v[i] = fmaf(p, to_f32(val[key * P.v_tok + i]), v[i]);
+                for (int c = 0; c < kV; ++c) v[c] = fmaf(pi, x[c], v[c]);
+            }
+        } else
+            for (int i = 0; i < n; ++i) {
+                float x[kV];
+                values(key0 + i, x);
+                const float pi = __shfl_sync(0xffffffffu, p, i);
+#pragma unroll
+                for (int c = 0; c < kV; ++c) v[c] = fmaf(pi, x[c], v[c]);
+            }
+        if ((key0 & 4095) == 0 && lane == 0) atomicAdd(beat, 1);
     }
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < kV; ++i)
         if ((spoilt >> i) & 1u) {
-            if (out != nullptr) out[i] = from_f32<T>(v[i] * inv);
-            else __stcg(part + i * kSub, v[i]);
+            if (out != nullptr) out[lane * kV + i] = from_f32<T>(v[i] * inv);
+            else __stcg(part + (lane * kV + i) * kSub, v[i]);
         }
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                        const __grid_constant__ CUtensorMap vmap, const PromptParams P) {
+                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptParams P) {
     using C = PromptCfg<D>;
     constexpr int kSlots = C::kSlots;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
@@ -393,7 +438,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     auto w_full = [&](uint32_t i) { return bars + 256u + 8u * (i % kQueue); };
     auto w_empty = [&](uint32_t i) { return bars + 256u + 8u * (kQueue + i % kQueue); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 352);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 356);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 356);        // [1]: stretches of mend()
     static_assert(120 + 16 * kSlots <= 256 && 256 + 16 * kQueue <= 352, "barriers");
     Work* queue = reinterpret_cast<Work*>(smem + C::kQueueOff);
     static_assert(sizeof(Work) <= 64, "a step of work");
@@ -406,7 +451,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
         for (int i = 0; i < kQueue; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), kReaders); }
         mbar_init(q_empty, 1); mbar_init(v_landed, 1); mbar_init(v_fixed, 1);
         for (int s = 0; s < kSlots; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
-        *abort_flag = 0;
+        abort_flag[0] = abort_flag[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kMmaWarp) {
@@ -756,9 +801,12 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 float s0, s1;
                 unpair(add2(sums[0], sums[1]), s0, s1);
                 __syncwarp();                                     // other lanes have stored this row
-                if (!(fabsf(s0 + s1) < INFINITY) && live && !blind && l == l) {
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 32) mend<T, D>(P, w, r, limit, n, c, factor, m_ref, inv, w.parts == 1 ? dst + c : nullptr, slot_at(w.slot) + c * kSub);
+                for (unsigned left = __ballot_sync(0xffffffffu, !(fabsf(s0 + s1) < INFINITY) && live && !blind && l == l); left != 0u; left &= left - 1u) {
+                    const int of = __ffs(left) - 1, at = w.row0 + x * kSub + quad * 32 + of;      // the row of another lane
+                    const float f = __shfl_sync(0xffffffffu, factor, of), m = __shfl_sync(0xffffffffu, m_ref, of), i = __shfl_sync(0xffffffffu, inv, of);
+                    const int see = __shfl_sync(0xffffffffu, limit, of);
+                    mend<T, D>(P, lane, w.head, w.q_first + at, w.k_first, see, min(n * kTileK, w.lk), f, m, i,
+                               w.parts == 1 ? reinterpret_cast<T*>(P.out) + ((int64_t)(w.q_first + at) * P.H + w.head) * D : nullptr, slot_at(w.slot) - lane + of, const_cast<int*>(abort_flag) + 1);
                 }
             }
             if (w.parts == 1) continue;

@@ -439,3 +439,28 @@ def test_a_scale_of_zero_weighs_large_keys_alike_too(n, past):
     q, k, v = rand(n, 2, 64, torch.bfloat16, 1, 2.0 ** 56), rand(n + past, 1, 64, torch.bfloat16, 2, 2.0 ** 56), rand(n + past, 1, 64, torch.bfloat16, 3)
     got = ck.prompt_attention(q, k, v, i32(cq), i32(ckv), scale=0.0)
     check(got, reference(torch.zeros_like(q), k, v, cq, ckv, 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_a_value_that_is_not_finite_behind_very_many_keys(d, dtype):
+    """The rows before it form their sums again over tens of thousands of keys each; who waits for them meanwhile does not give up."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    n = 131072
+    q, k, v = rand(n, 1, d, dtype, 1), rand(n, 1, d, dtype, 2), rand(n, 1, d, dtype, 3)
+    spots = [(n - 70, 3, math.nan), (n - 60, d - 1, math.inf), (60000, 17, -math.inf)]
+    clean = v.clone()
+    for key, col, x in spots:
+        clean[key, 0, col], v[key, 0, col] = 0.0, x
+    _C.decode_status()
+    got = ck.prompt_attention(q, k, v, i32([0, n]))
+    assert _C.decode_status() == 0
+    hit = torch.zeros(n, 1, d, dtype=torch.bool, device=DEV)
+    for key, col, _ in spots:
+        hit[key:, :, col] = True
+    assert torch.equal(~torch.isfinite(got), hit)
+    for a in (n - 256, n - 128, 59904):                              # sequences that end with the rows of a tile: the same rows, from their definition
+        want, tol = reference(q[a:a + 128], k[:a + 128], clean[:a + 128], [0, 128], [0, a + 128])
+        seen = ~hit[a:a + 128]
+        assert ((got[a:a + 128].double() - want).abs() <= tol)[seen].all()
