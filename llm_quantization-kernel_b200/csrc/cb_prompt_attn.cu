@@ -439,7 +439,9 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     auto w_empty = [&](uint32_t i) { return bars + 256u + 8u * (kQueue + i % kQueue); };
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 352);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kBarOff + 356);        // [1]: stretches of mend()
-    static_assert(120 + 16 * kSlots <= 256 && 256 + 16 * kQueue <= 352, "barriers");
+    volatile uint32_t* copied = reinterpret_cast<volatile uint32_t*>(smem + C::kBarOff + 364);       // K and V tiles, and tiles of Q, that copies were issued for
+    const uint32_t drained = bars + 376u;
+    static_assert(120 + 16 * kSlots <= 256 && 256 + 16 * kQueue <= 352 && C::kQueueOff >= C::kBarOff + 384, "barriers");
     Work* queue = reinterpret_cast<Work*>(smem + C::kQueueOff);
     static_assert(sizeof(Work) <= 64, "a step of work");
 
@@ -449,7 +451,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
             mbar_init(q_full(x), 1); mbar_init(s_full(x), 1); mbar_init(p_ready(x, 0), 4); mbar_init(p_ready(x, 1), 4); mbar_init(pv_done(x), 1); mbar_init(o_free(x), 4);
         }
         for (int i = 0; i < kQueue; ++i) { mbar_init(w_full(i), 1); mbar_init(w_empty(i), kReaders); }
-        mbar_init(q_empty, 1); mbar_init(v_landed, 1); mbar_init(v_fixed, 1);
+        mbar_init(q_empty, 1); mbar_init(drained, 1); mbar_init(v_landed, 1); mbar_init(v_fixed, 1);
         for (int s = 0; s < kSlots; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
         abort_flag[0] = abort_flag[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -523,13 +525,7 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 }
             }
         }
-        if (gave_up) {                                            // own copies in flight, again with a limit
-            const long long t0 = clock64();
-            for (uint32_t i = it > kSlots ? it - kSlots : 0; i < it; ++i)
-                while (!mbar_try_wait(kv_full(i % kSlots), (i / kSlots) & 1) && clock64() - t0 < kWaitCycles) {}
-            for (int x = 0; x < 2 && tiles > 0; ++x)
-                while (!mbar_try_wait(q_full(x), (tiles - 1) & 1) && clock64() - t0 < kWaitCycles) {}
-        }
+        if (lane == 0) { copied[0] = it; copied[1] = tiles; }
     } else if (warp == kMmaWarp) {
         // ================= MMA issuer: the warp goes through the list together, one elected thread issues =================
         constexpr uint32_t fmt = BF ? ((1u << 7) | (1u << 10)) : 0u;
@@ -861,6 +857,24 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
     }
     fence_before();
     __syncthreads();
+    if (*abort_flag != 0) {
+        // Some role gave up, and others may have ended in good order before: copies and products that nobody waited for are still on their way into this
+        // CTA's memory.  They are waited for, again with a limit, before it is given back.
+        const long long t0 = clock64();
+        auto drain = [&](uint32_t bar, uint32_t parity) { while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {} };
+        if (warp == kTmaWarp) {
+            const uint32_t it = copied[0], tiles = copied[1];
+            for (uint32_t i = it > kSlots ? it - kSlots : 0; i < it; ++i) drain(kv_full(i % kSlots), (i / kSlots) & 1);
+            for (int x = 0; x < 2 && tiles > 0; ++x) drain(q_full(x), (tiles - 1) & 1);
+        }
+        if (warp == kMmaWarp) {
+            if (elect_one()) commit(drained);                     // by the thread that issued the products
+            __syncwarp();
+            drain(drained, 0);
+            fence_before();
+        }
+        __syncthreads();
+    }
     if (warp == kMmaWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
