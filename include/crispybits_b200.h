@@ -288,7 +288,8 @@ int cb_decode_plan(int bits, int64_t B, int64_t V, int64_t K, int64_t split_k, i
  * 3 dequantiser, 4 epilogue, 5 packed-word producer) gave up a bounded wait; 3001 = a kernel of the 4-bit cache met a position
  * outside its page table or a page number outside the cache and left it out, 3002 = a copy of the cache's attention did not
  * arrive in time and outputs were not written; 4000 + r = role r of the prompt attention (1 TMA, 2 MMA, 3 softmax, 4 epilogue, 5 tile ends, 6 the walk) gave up a
- * bounded wait.  No counterpart in the reference. */
+ * bounded wait.  After 3002 and 4000 + r the counters that attention calls were given may not be zero: zero them before they are used again.
+ * No counterpart in the reference. */
 int cb_decode_status(int* status);
 
 /* Introspection used by the Split-K policy (packed_gemv.cu:339-347; bindings.cpp:37-39). */
@@ -339,7 +340,7 @@ int cb_kv4_read(const cb_kv4_cache* cache, void* k, void* v, int64_t n_tokens, c
  * nothing is 0.  scale is finite (this and prompt attention).  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
  * strides3 = {b, t, h} in elements, multiples of 8; out [B, T, H, head_dim] contiguous, sharing no memory with q.  Tokens on a page whose number
  * lies outside the cache are left out and set the status word (3001).  counters: cb_kv4_attention_counters() int32, zeroed ONCE,
- * left zero by every call; partial: cb_kv4_attention_partial_bytes() bytes, 16-byte aligned, of any content.  Calls that may overlap on
+ * left zero by every call that ends well (cb_decode_status); partial: cb_kv4_attention_partial_bytes() bytes, 16-byte aligned, of any content.  Calls that may overlap on
  * the GPU need their own counters and partial. */
 int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* strides3, void* out, int64_t B, int64_t T,
                      int64_t H, const int32_t* page_table, int64_t table_stride, const int32_t* lengths, float scale,
@@ -358,7 +359,7 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * same value of the queries that see it inf or NaN.
  * The work is cut into equal parts for the SMs, whatever the lengths are; where a cut falls inside a tile, its parts meet in scratch and are joined in
  * order, so that the result is the same from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, of any
- * content) and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call).  Calls that may overlap on the GPU need their own. */
+ * content) and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call that ends well).  Calls that may overlap on the GPU need their own. */
 int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
                         int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
                         float scale, int causal, void* counters, size_t counter_bytes, void* partial, size_t partial_bytes,

@@ -618,6 +618,8 @@ def decode_status() -> int:
     """Synchronise, then read and clear the decode kernels' error word (0 = fine)."""
     out = _int(0)
     _rc(_lib.cb_decode_status(ctypes.byref(out)))
+    if out.value:
+        _zero_attention_counters(torch.cuda.current_device())
     return int(out.value)
 
 
@@ -777,6 +779,17 @@ def prepare_attention(device: torch.device):
             slab = torch.zeros(_ATTENTION_SLAB, dtype=torch.int32, device=torch.device("cuda", index))
             torch.cuda.current_stream(index).synchronize()       # visible to whatever stream a graph will run on
             _attention_slab.setdefault(index, [slab, 0])
+
+
+def _zero_attention_counters(index: int):
+    """A launch that gave up a wait leaves counters that are not zero, and later launches would join parts that are not there.  Any status is taken
+    for one: it may hide another."""
+    torch.cuda.synchronize(index)
+    with _attention_lock, _on_device(torch.device("cuda", index)):
+        kept = [have[0] for (dev, _), have in _attention_eager.items() if dev == index]
+        for counters in kept + [slab[0] for dev, slab in _attention_slab.items() if dev == index]:
+            counters.zero_()
+    torch.cuda.synchronize(index)
 
 
 def _attention_scratch(device, dev: int, stream: int, counters: int, nbytes: int):

@@ -908,3 +908,39 @@ def test_groups_whose_range_is_no_float(gs):
     for y in ck.kv4_read(c, i32([[0]]), i32([0]), i32([0, n]), n):
         # one rounding of the type, of a sum of two that fp32 may have rounded first
         assert ((y[:, 0].cpu().double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20) + 2.0 ** -24 * 2 * top + 2.0 ** -133).all()
+
+
+@pytest.mark.gpu
+def test_counters_left_by_a_launch_that_gave_up_are_zeroed_with_its_status(monkeypatch):
+    """A launch that gives up leaves counts behind.  They are planted here, with the status that such a launch sets: once the status is read, eager and
+    captured calls are right again."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    f = Filled([3000, 40, 900], 2, 64, 64, 64, torch.float16)
+    q, cu = rand_q(3, 1, 4, 64, torch.float16), i32([0, 300])
+    pq, pk, cu_k = rand_kv(300, 4, 64, torch.float16, 1), rand_kv(9300, 2, 64, torch.float16, 2), i32([0, 9300])
+
+    def both():
+        return ck.kv4_attention(q, f.cache, f.table, f.lengths), ck.prompt_attention(pq, pk, pk, cu, cu_k)
+
+    want = both()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = both()
+    torch.cuda.synchronize()
+    dev = torch.cuda.current_device()
+    for (d, _), have in _C._attention_eager.items():
+        if d == dev:
+            have[0].fill_(1)
+    _C._attention_slab[dev][0].fill_(1)
+    with monkeypatch.context() as m:
+        def status(out):
+            out._obj.value = 3002
+            return 0
+        m.setattr(_C._lib, "cb_decode_status", status)
+        assert _C.decode_status() == 3002
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(both(), want))
+        g.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert _C.decode_status() == 0
