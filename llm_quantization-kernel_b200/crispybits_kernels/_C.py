@@ -807,9 +807,12 @@ def _attention_scratch(device, dev: int, stream: int, counters: int, nbytes: int
     have = _attention_eager.get((dev, stream))
     if have is None or have[0].numel() < counters or have[1].numel() < nbytes:
         prepare_attention(device)
-        have = (torch.zeros(max(counters, 8192), dtype=torch.int32, device=device),
-                torch.empty(nbytes, dtype=torch.uint8, device=device))
-        _attention_eager[(dev, stream)] = have
+        counts, partial = have or (None, None)                   # what is large enough stays: other calls may need it as it is
+        if counts is None or counts.numel() < counters:
+            counts = torch.zeros(max(counters, 8192), dtype=torch.int32, device=device)
+        if partial is None or partial.numel() < nbytes:
+            partial = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        have = _attention_eager[(dev, stream)] = (counts, partial)
     return have
 
 

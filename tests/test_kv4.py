@@ -944,3 +944,24 @@ def test_counters_left_by_a_launch_that_gave_up_are_zeroed_with_its_status(monke
         g.replay()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
     assert _C.decode_status() == 0
+
+
+@pytest.mark.gpu
+def test_calls_of_different_needs_share_scratch_without_making_it_anew():
+    """Many counters and little scratch, then the other way round: after one round of both nothing is allocated any more."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    B, heads = 260, 40                                             # 10400 counters
+    f = Filled([1] * B, heads, 64, 64, 16, torch.float16)
+    q, x, cu = rand_q(B, 1, heads, 64, torch.float16), rand_kv(2000, 2, 128, torch.float16, 1), i32([0, 2000])
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        kept = []
+        for _ in range(3):
+            ck.kv4_attention(q, f.cache, f.table, f.lengths)
+            ck.prompt_attention(x, x, x, cu)
+            have = _C._attention_eager[(torch.cuda.current_device(), s.cuda_stream)]
+            kept.append([t.data_ptr() for t in have])
+            assert have[0].numel() >= B * heads
+    torch.cuda.synchronize()
+    assert kept[0] == kept[1] == kept[2]
