@@ -359,12 +359,14 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * same value of the queries that see it inf or NaN.
  * The work is cut into equal parts for the SMs, whatever the lengths are; where a cut falls inside a tile, its parts meet in scratch and are joined in
  * order, so that the result is the same from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, of any
- * content) and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call that ends well).  Calls that may overlap on the GPU need their own. */
+ * content) that suffice for every call and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call that ends well).  Calls that may overlap on the GPU need their own. */
 int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
                         int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
                         float scale, int causal, void* counters, size_t counter_bytes, void* partial, size_t partial_bytes,
                         void* stream);
 size_t cb_prompt_attention_scratch(int head_dim, size_t* counter_bytes);
+/* The same for calls of these sizes alone: between none, where no tile has more than 128 keys, and the above. */
+size_t cb_prompt_attention_scratch_for(int64_t Tq, int64_t Tk, int64_t H, int64_t B, int head_dim, size_t* counter_bytes);
 
 #ifdef __cplusplus
 }

@@ -762,12 +762,14 @@ def kv4_read(cache, page_table, starts, cu_seqlens, n_tokens: int):
 # Scratch of the attention operators.  Eager calls: counters (zeroed when made; every call leaves them zero) and partial
 # sums of one (device, stream), where calls run one after another.  Captured calls: partial sums from the graph's own
 # pool, and counters that no other call ever gets, cut from a slab zeroed beforehand -- two graphs may then run at the
-# same time.  A capture that finds no slab, or an empty one, zeroes its counters inside the graph.
+# same time.  A capture that finds no slab, or an empty one, zeroes its counters inside the graph; eager calls see to it that the next finds one at
+# least half full.
 _attention_eager: Dict[Tuple[int, int], Tuple[torch.Tensor, torch.Tensor]] = {}
 _attention_slab: Dict[int, List] = {}          # device index -> [tensor, next free element]
+_attention_spent: List[torch.Tensor] = []      # slabs that graphs count in and nothing more is cut from
 _ATTENTION_SLAB = 1 << 18
 _attention_lock = threading.Lock()
-_prompt_bytes: Dict[Tuple[int, int], Tuple[int, int]] = {}   # (device index, head_dim) -> bytes of counters and partial, cb_prompt_attention_scratch
+_prompt_bytes: Dict[Tuple[int, ...], Tuple[int, int]] = {}   # (device index, head_dim, sizes) -> bytes of counters and partial, cb_prompt_attention_scratch_for
 _partial_bytes: Dict[Tuple[int, bool, int], int] = {}      # (device index, more than 8 rows, head_dim) -> cb_kv4_attention_partial_bytes
 
 
@@ -781,13 +783,24 @@ def prepare_attention(device: torch.device):
             _attention_slab.setdefault(index, [slab, 0])
 
 
+def _renew_attention_slab(device, slab: List):
+    """Half of the counters for captures are given out: the next captures draw from another slab.  The old one stays, graphs count in it."""
+    fresh = torch.zeros(_ATTENTION_SLAB, dtype=torch.int32, device=device)
+    torch.cuda.current_stream(device).synchronize()
+    with _attention_lock:
+        if slab[1] > _ATTENTION_SLAB // 2:
+            _attention_spent.append(slab[0])
+            slab[0], slab[1] = fresh, 0
+
+
 def _zero_attention_counters(index: int):
     """A launch that gave up a wait leaves counters that are not zero, and later launches would join parts that are not there.  Any status is taken
     for one: it may hide another."""
     torch.cuda.synchronize(index)
     with _attention_lock, _on_device(torch.device("cuda", index)):
         kept = [have[0] for (dev, _), have in _attention_eager.items() if dev == index]
-        for counters in kept + [slab[0] for dev, slab in _attention_slab.items() if dev == index]:
+        slabs = [slab[0] for slab in _attention_slab.values()] + _attention_spent
+        for counters in kept + [slab for slab in slabs if slab.get_device() == index]:
             counters.zero_()
     torch.cuda.synchronize(index)
 
@@ -804,6 +817,9 @@ def _attention_scratch(device, dev: int, stream: int, counters: int, nbytes: int
         if at + need > _ATTENTION_SLAB:
             return torch.zeros(counters, dtype=torch.int32, device=device), partial
         return slab[0][at:at + need], partial
+    slab = _attention_slab.get(dev)
+    if slab is not None and slab[1] > _ATTENTION_SLAB // 2:
+        _renew_attention_slab(device, slab)
     have = _attention_eager.get((dev, stream))
     if have is None or have[0].numel() < counters or have[1].numel() < nbytes:
         prepare_attention(device)
@@ -854,8 +870,8 @@ def kv4_attention(q, cache, page_table, lengths, scale: float):
 _lib.cb_prompt_attention.argtypes = [_vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _i64, _i64, _i64, _i64, _int, _int, _vp, _vp, _i64,
                                      ctypes.c_float, _int, _vp, _sz, _vp, _sz, _vp]
 _lib.cb_prompt_attention.restype = _int
-_lib.cb_prompt_attention_scratch.argtypes = [_int, ctypes.POINTER(_sz)]
-_lib.cb_prompt_attention_scratch.restype = _sz
+_lib.cb_prompt_attention_scratch_for.argtypes = [_i64, _i64, _i64, _i64, _int, ctypes.POINTER(_sz)]
+_lib.cb_prompt_attention_scratch_for.restype = _sz
 
 
 def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bool, out=None):
@@ -893,11 +909,14 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, scale: float, causal: bo
     (q, sq), (k, sk), (v, sv) = _vector_rows(q, True), _vector_rows(k, True), _vector_rows(v, True)
     strides = (_i64 * 6)(sq[0], sq[1], sk[0], sk[1], sv[0], sv[1])
     with _on_device(device):
-        stream, sizes = _raw_stream(dev), _prompt_bytes.get((dev, d))
+        key = (dev, d, tq, tk, h, n)
+        stream, sizes = _raw_stream(dev), _prompt_bytes.get(key)
         if sizes is None:
+            if len(_prompt_bytes) > 4096:
+                _prompt_bytes.clear()
             cbytes = _sz(0)
-            nbytes = _lib.cb_prompt_attention_scratch(d, cbytes)
-            sizes = _prompt_bytes[(dev, d)] = (cbytes.value, nbytes)
+            nbytes = _lib.cb_prompt_attention_scratch_for(tq, tk, h, n - 1, d, cbytes)
+            sizes = _prompt_bytes[key] = (max(cbytes.value, 4), max(nbytes, 16))
         counts, partial = _attention_scratch(device, dev, stream, sizes[0] // 4, sizes[1])
         _rc(_lib.cb_prompt_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, out.data_ptr(), tq, tk, h, hkv, d,
                                      _DTYPE[dtype], cu_seqlens.data_ptr(), cu_seqlens_k.data_ptr(), n - 1, scale,

@@ -129,7 +129,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     they differ: a piece of a prompt attends to what came before it and to itself.  causal: query r of Lq sees the first
     Lk - Lq + r + 1 keys.  A query that sees none gives 0.  Rows of no sequence are left as they are in `out` (and are
     undefined without it; it shares no memory with q, k and v).  scale: finite, default head_dim ** -0.5.  Keys and values that a query does not see do not
-    touch it, infinities and NaN among them.  Scratch for tiles that are cut between SMs (158 MB at head_dim 128 on 148 SMs) is kept for each
-    stream that calls this eagerly, and comes from the graph's pool in a capture."""
+    touch it, infinities and NaN among them.  Scratch for tiles that are cut between SMs (on 148 SMs at head_dim 128 158 MB for long prompts, 39 MB for
+    a few thousand tokens, none for up to 128) is kept for each stream that calls this eagerly, and comes from the graph's pool in a capture."""
     return _C().prompt_attention(q, k, v, cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k,
                                  q.shape[-1] ** -0.5 if scale is None else float(scale), causal, out)

@@ -18,8 +18,10 @@ size_t kv4_attention_partial_bytes(int64_t rows, int head_dim);
 int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
                             int64_t H, int64_t Hkv, int head_dim, int dtype, const int32_t* cu_q, const int32_t* cu_k, int64_t B,
                             float scale, int causal, int* counters, float* partial, cudaStream_t stream);
-size_t prompt_attention_partial_bytes(int head_dim);
-size_t prompt_attention_counter_bytes();
+int64_t prompt_attention_parts(int64_t Tq, int64_t Tk, int64_t H, int64_t B);
+int64_t prompt_attention_most_parts();
+size_t prompt_attention_partial_bytes(int64_t parts, int head_dim);
+size_t prompt_attention_counter_bytes(int64_t parts);
 
 namespace {
 
@@ -136,8 +138,15 @@ int cb_kv4_attention(const cb_kv4_cache* cache, const void* q, const int64_t* st
 }
 
 size_t cb_prompt_attention_scratch(int head_dim, size_t* counter_bytes) {
-    if (counter_bytes != nullptr) *counter_bytes = prompt_attention_counter_bytes();
-    return prompt_attention_partial_bytes(head_dim);
+    const int64_t parts = prompt_attention_most_parts();
+    if (counter_bytes != nullptr) *counter_bytes = prompt_attention_counter_bytes(parts);
+    return prompt_attention_partial_bytes(parts, head_dim);
+}
+
+size_t cb_prompt_attention_scratch_for(int64_t Tq, int64_t Tk, int64_t H, int64_t B, int head_dim, size_t* counter_bytes) {
+    const int64_t parts = Tq <= 0 || Tk <= 0 || H <= 0 || B <= 0 ? 0 : prompt_attention_parts(Tq, Tk, H, B);
+    if (counter_bytes != nullptr) *counter_bytes = prompt_attention_counter_bytes(parts);
+    return prompt_attention_partial_bytes(parts, head_dim);
 }
 
 int cb_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides6, void* out, int64_t Tq, int64_t Tk,
@@ -159,8 +168,9 @@ int cb_prompt_attention(const void* q, const void* k, const void* v, const int64
         CB_REQUIRE(used <= 1 || (strides6[i] > 0 && strides6[i] % 8 == 0 && strides6[i] < (1ll << 38)),
                    "%s: strides must be positive multiples of 8 elements", who);
     }
-    CB_REQUIRE(counters != nullptr && counter_bytes >= prompt_attention_counter_bytes() && partial != nullptr && aligned16(partial) &&
-                   partial_bytes >= prompt_attention_partial_bytes(head_dim),
+    const int64_t parts = prompt_attention_parts(Tq, Tk, H, B);
+    CB_REQUIRE(counters != nullptr && counter_bytes >= prompt_attention_counter_bytes(parts) && partial != nullptr && aligned16(partial) &&
+                   partial_bytes >= prompt_attention_partial_bytes(parts, head_dim),
                "%s: scratch is missing or too small (cb_prompt_attention_scratch)", who);
     const int64_t out_bytes = 2 * Tq * H * head_dim;
     CB_REQUIRE(!meets(out, out_bytes, q, head_dim, Tq, strides6[0], H, strides6[1]) && !meets(out, out_bytes, k, head_dim, Tk, strides6[2], Hkv, strides6[3]) &&

@@ -67,6 +67,7 @@ struct PromptParams {
     float scale_log2;                                 // |scale| * log2(e), above 0
     int negate;                                       // the scale is negative: the products with q are negated
     int causal;
+    int most_rounds;                                  // that the scratch is made for
     // Where the line of work is cut inside a (head, tile), the pieces leave (O, m, l) in `partial`, two slots for a part of the line, and the last to
     // finish joins them.  counters: 8 for a part (that of the first piece; one for each softmax warp), zero between calls.
     float* partial;
@@ -258,7 +259,7 @@ __device__ __forceinline__ bool walk_begin(const PromptParams& P, int lane, Walk
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
-    const int rounds = (int)min(max(div64(U, (int64_t)gridDim.x * kRoundUnits), (int64_t)1), (int64_t)kMaxRounds);
+    const int rounds = (int)min(max(div64(U, (int64_t)gridDim.x * kRoundUnits), (int64_t)1), (int64_t)P.most_rounds);
     const int64_t nc = min((int64_t)gridDim.x * rounds, U);
     if ((int64_t)blockIdx.x >= nc) return false;
     const int64_t share = nc == 0 ? 0 : div64(U, nc), extra = U - share * nc;
@@ -912,14 +913,22 @@ int launch_prompt_t(const CUtensorMap (&maps)[3], const PromptParams& P, int gri
 
 }  // namespace
 
-size_t prompt_attention_partial_bytes(int head_dim) {
-    const int sms = sm_count_current();
-    return sms <= 0 ? 0 : (size_t)sms * kMaxRounds * 2 * kTileQ * (head_dim + 2) * sizeof(float);
+// Rounds that a call of these sizes may take: by the units that its sequences have at most (tiles, and key tiles of each), one CTA to an SM.
+static int prompt_rounds(int64_t Tq, int64_t Tk, int64_t H, int64_t B, int sms) {
+    const int64_t tiles = Tq / kTileQ + std::min(B, Tq), each = kOpen + (Tk + kTileK - 1) / kTileK;
+    const int64_t enough = (int64_t)sms * kRoundUnits * kMaxRounds;          // H < 2^20, tiles and each < 2^31: the products are looked at one by one
+    const int64_t per_head = tiles > enough / each ? enough : tiles * each;
+    const int64_t units = per_head > enough / H ? enough : per_head * H;
+    return (int)std::min<int64_t>(std::max<int64_t>(units / ((int64_t)sms * kRoundUnits), 1), kMaxRounds);
 }
-size_t prompt_attention_counter_bytes() {
+int64_t prompt_attention_most_parts() { return (int64_t)std::max(sm_count_current(), 0) * kMaxRounds; }
+// Parts of the line, each of which may leave two pieces in scratch.  Up to kTileK keys a tile is one key tile, and never cut.
+int64_t prompt_attention_parts(int64_t Tq, int64_t Tk, int64_t H, int64_t B) {
     const int sms = sm_count_current();
-    return sms <= 0 ? 0 : (size_t)sms * kMaxRounds * 8 * sizeof(int);
+    return sms <= 0 || Tk <= kTileK ? 0 : (int64_t)sms * prompt_rounds(Tq, Tk, H, B, sms);
 }
+size_t prompt_attention_partial_bytes(int64_t parts, int head_dim) { return (size_t)parts * 2 * kTileQ * (head_dim + 2) * sizeof(float); }
+size_t prompt_attention_counter_bytes(int64_t parts) { return (size_t)parts * 8 * sizeof(int); }
 
 // Arguments are checked by the caller.  strides: {q token, q head, k token, k head, v token, v head} in elements.
 int launch_prompt_attention(const void* q, const void* k, const void* v, const int64_t* strides, void* out, int64_t Tq, int64_t Tk,
@@ -953,6 +962,7 @@ int launch_prompt_attention(const void* q, const void* k, const void* v, const i
     P.scale_log2 = scale == 0.f ? 1e-45f : fabsf(scale) * 1.4426950408889634f;
     P.negate = scale < 0.f ? 1 : 0;
     P.causal = causal ? 1 : 0;
+    P.most_rounds = prompt_rounds(Tq, Tk, H, B, sms);
     P.counters = counters; P.partial = partial;
     const int grid = sms;
     const bool bf = dtype == CB_BF16;

@@ -464,3 +464,60 @@ def test_a_value_that_is_not_finite_behind_very_many_keys(d, dtype):
         want, tol = reference(q[a:a + 128], k[:a + 128], clean[:a + 128], [0, 128], [0, a + 128])
         seen = ~hit[a:a + 128]
         assert ((got[a:a + 128].double() - want).abs() <= tol)[seen].all()
+
+
+@pytest.mark.gpu
+def test_scratch_is_of_the_calls_size():
+    """None for up to 128 keys, one round's for a few thousand tokens, all of it for long prompts; never more than what suffices for every call."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    lib = _C._lib
+    lib.cb_prompt_attention_scratch.argtypes, lib.cb_prompt_attention_scratch.restype = [ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_size_t
+
+    def need(tq, tk, h, b, d=128):
+        c = ctypes.c_size_t(99)
+        return lib.cb_prompt_attention_scratch_for(tq, tk, h, b, d, c), c.value
+
+    c = ctypes.c_size_t(0)
+    most = lib.cb_prompt_attention_scratch(128, c), c.value
+    assert need(37, 37, 32, 1) == need(128, 128, 64, 5) == need(5, 0, 4, 1) == (0, 0)
+    assert need(2000, 2000, 32, 1) == (most[0] // 4, most[1] // 4) and need(16384, 16384, 32, 1) == most
+    sizes = [need(1 << a, 1 << b, h, s) for a in (0, 8, 14, 29) for b in (0, 8, 14, 29) for h in (1, 40, (1 << 20) - 1) for s in (1, 9, 1 << 24)]
+    assert all(n <= most[0] and k <= most[1] for n, k in sizes)
+    x = rand(300, 4, 128, torch.float16, 1)
+    s = torch.cuda.Stream()
+    _C._attention_eager.pop((torch.cuda.current_device(), s.cuda_stream), None)      # torch hands streams out again
+    with torch.cuda.stream(s):
+        ck.prompt_attention(x[:100], x[:100], x[:100], i32([0, 37, 100]))
+        have = _C._attention_eager[(torch.cuda.current_device(), s.cuda_stream)]
+        assert have[1].numel() < 1024
+        want = ck.prompt_attention(x, x, x, i32([0, 300]))
+        assert _C._attention_eager[(torch.cuda.current_device(), s.cuda_stream)][1].numel() == most[0] // 4
+    torch.cuda.synchronize()
+    check(want, reference(x, x, x, [0, 300], [0, 300]))
+
+
+@pytest.mark.gpu
+def test_captures_of_many_prompts_leave_counters_for_others():
+    """Three captures of forty calls each need twice what was prepared: the eager calls between them, a warm-up's, make up for it."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    n = 6000
+    x, cu = rand(n, 40, 64, torch.float16, 1), i32([0, n])
+    k = x[:, :1].contiguous()
+    want = ck.prompt_attention(x, k, k, cu)
+    slab, graphs = _C._attention_slab[torch.cuda.current_device()], []
+    for _ in range(3):
+        assert torch.equal(ck.prompt_attention(x, k, k, cu), want)
+        g, before = torch.cuda.CUDAGraph(), slab[1]
+        assert before <= slab[0].numel() // 2
+        with torch.cuda.graph(g):
+            outs = [ck.prompt_attention(x, k, k, cu)]
+            for _ in range(39):
+                outs = [ck.prompt_attention(x, k, k, cu, out=outs[0])]
+        used = slab[1] - before
+        assert used > 0
+        graphs.append((g, outs))
+    for g, outs in graphs * 2:
+        g.replay()
+        assert torch.equal(outs[0], want)
