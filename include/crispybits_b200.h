@@ -354,7 +354,7 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * k token, k head, v token, v head} in elements, multiples of 8 and positive (that of a dimension of one entry is not used);
  * out [Tq, H, head_dim] contiguous, 16-byte aligned, outside the memory from the first to the last value of q, k and v.  Sequence s has queries cu_q[s] .. cu_q[s + 1] - 1 and keys cu_k[s] ..
  * cu_k[s + 1] - 1 (device memory; bounds outside the tensors are cut to them).  Head h reads key head h / (H / Hkv).  head_dim 64 or 128,
- * dtype CB_F16 or CB_BF16.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
+ * dtype CB_F16 or CB_BF16; at most 2^22 sequences.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
  * behind a query's last one do not touch it, infinities and NaN among them; a value of v that is not finite makes the
  * same value of the queries that see it inf or NaN.
  * The work is cut into equal parts for the SMs, whatever the lengths are; where a cut falls inside a tile, its parts meet in scratch and are joined in

@@ -157,7 +157,9 @@ int cb_prompt_attention(const void* q, const void* k, const void* v, const int64
     CB_REQUIRE(dtype == CB_F16 || dtype == CB_BF16, "%s: dtype must be fp16 or bf16", who);
     CB_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128 (got %d)", who, head_dim);
     CB_REQUIRE(Tq >= 0 && Tk >= 0 && Tq < (1ll << 30) && Tk < (1ll << 30), "%s: too many tokens", who);
-    CB_REQUIRE(H >= 0 && Hkv >= 0 && H < (1 << 20) && Hkv < (1 << 20) && B >= 0 && B < (1ll << 30), "%s: heads or sequences out of range", who);
+    CB_REQUIRE(H >= 0 && Hkv >= 0 && H < (1 << 20) && Hkv < (1 << 20) && B >= 0, "%s: heads or sequences out of range", who);
+    // every CTA walks over the bounds of all sequences, a microsecond for 32 of them, while its other warps wait with a limit of a second
+    CB_REQUIRE(B <= (1ll << 22), "%s: more than 2^22 sequences", who);
     CB_REQUIRE(std::isfinite(scale), "%s: scale must be finite", who);
     if (Tq == 0 || H == 0 || B == 0) return CB_OK;
     CB_REQUIRE(Hkv > 0 && H % Hkv == 0, "%s: H must be a multiple of Hkv", who);

@@ -521,3 +521,32 @@ def test_captures_of_many_prompts_leave_counters_for_others():
     for g, outs in graphs * 2:
         g.replay()
         assert torch.equal(outs[0], want)
+
+
+def test_more_sequences_than_the_walk_can_take_are_refused():
+    from crispybits_kernels import _C
+    lib, s6 = _C._lib, (ctypes.c_int64 * 6)(*[128] * 6)
+    assert lib.cb_prompt_attention(256, 256, 256, s6, 256, 4, 4, 2, 2, 64, 1, 256, 256, (1 << 22) + 1, 1.0, 1, 256, 1 << 20, 256, 1 << 40, 0) == 1
+    assert b"sequences" in lib.cb_last_error()
+
+
+@pytest.mark.gpu
+def test_as_many_sequences_as_there_may_be():
+    """2^22 sequences, most of them empty: the walk over their bounds stays far inside the others' waits."""
+    import crispybits_kernels as ck
+    from crispybits_kernels import _C
+    B, n = 1 << 22, 700
+    q, k, v = rand(n, 2, 64, torch.float16, 1), rand(n, 1, 64, torch.float16, 2), rand(n, 1, 64, torch.float16, 3)
+    cu = torch.zeros(B + 1, dtype=torch.int32)
+    cu[100:], cu[B // 2:], cu[B:] = 300, 301, n
+    _C.decode_status()
+    t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    dev = cu.to(DEV)
+    t0.record()
+    got = ck.prompt_attention(q, k, v, dev)
+    t1.record()
+    torch.cuda.synchronize()
+    assert _C.decode_status() == 0
+    print("ms", t0.elapsed_time(t1))
+    want = [0, 300, 301, n]
+    check(got, reference(q, k, v, want, want))
