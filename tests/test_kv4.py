@@ -965,3 +965,40 @@ def test_calls_of_different_needs_share_scratch_without_making_it_anew():
             assert have[0].numel() >= B * heads
     torch.cuda.synchronize()
     assert kept[0] == kept[1] == kept[2]
+
+
+# ------------------------------------------------------------------------------------------------ GPU: each schedule against the definition
+def schedule(lens, heads, rows):
+    """How kv4_attention shares out the work: ("aligned" parts that end with their segments, or "equal" ones that cut them), and whether short segments
+    go to single warps."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    segs = heads * (-(-rows // (16 if rows > 8 else 8)))
+    blocks, total = segs * sum(-(-n // 16) for n in lens), len(lens) * segs
+    if 4 * total <= sms and not (16 * total > sms and blocks > 16 * sms):
+        return "aligned", False
+    return "equal", 4 * total > sms and total >= sms
+
+
+def mixed(count, pattern):
+    return [pattern[i % len(pattern)] for i in range(count)]
+
+
+SCHEDULES = [(mixed(5, [1000, 0, 3, 700, 64]), 2, 1, 1, ("aligned", False)), (mixed(20, [900, 1, 333, 0, 64, 1000, 17, 500]), 4, 1, 4, ("equal", False)),
+             (mixed(25, [129, 700, 0, 1, 40]), 4, 2, 2, ("equal", False)), (mixed(40, [100, 1, 129, 0, 2000, 128]), 4, 1, 1, ("equal", True)),
+             (mixed(70, [5, 2000, 130, 100]), 3, 3, 4, ("equal", True)), ([1500, 1600, 1700, 1540, 1499, 2100, 1800, 1650], 4, 1, 2, ("equal", False)),
+             ([4000, 3900], 6, 2, 3, ("equal", False)), ([3000] * 37, 1, 1, 9, ("equal", False))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,heads,T,group,kind", SCHEDULES)
+@pytest.mark.parametrize("d,gs,dtype", [(64, 32, torch.bfloat16), (128, 64, torch.float16)])
+def test_each_schedule_matches_the_definition(lens, heads, T, group, kind, d, gs, dtype):
+    """Parts joined across cuts, single warps and cut segments in one launch, the device's own change from aligned to equal parts."""
+    import crispybits_kernels as ck
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert schedule(lens, heads, T * group) == kind
+    f = Filled(lens, heads, d, gs, 16, dtype, seed=len(lens))
+    q = rand_q(len(lens), T, heads * group, d, dtype)
+    got = ck.kv4_attention(q, f.cache, f.table, f.lengths)
+    check(got, f.reference(q))
+    assert torch.equal(got, ck.kv4_attention(q, f.cache, f.table, f.lengths))

@@ -550,3 +550,32 @@ def test_as_many_sequences_as_there_may_be():
     print("ms", t0.elapsed_time(t1))
     want = [0, 300, 301, n]
     check(got, reference(q, k, v, want, want))
+
+
+def rounds(lens, keys, heads, causal):
+    """In how many rounds a call goes through its work: by units, key tiles of each tile of 256 queries and three more."""
+    units = 0
+    for lq, lk in zip(lens, keys):
+        for r in range(0, lq, 256):
+            seen = [min(lk, r + x + min(lq - r - x, 128) + lk - lq) if causal else lk for x in (0, 128) if lq > r + x]
+            units += 3 + max(max(0, -(-n // 128)) for n in seen)
+    return min(max(units * heads // (100 * torch.cuda.get_device_properties(0).multi_processor_count), 1), 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens,past,heads,d,dtype,causal,want", [([8192, 300, 1, 5000], [0] * 4, 24, 64, torch.float16, True, 2),
+                                                                ([4000, 0, 8000], [3000, 500, 2000], 24, 128, torch.bfloat16, True, 3),
+                                                                ([3000, 2000], [9000, 6000], 48, 64, torch.bfloat16, False, 4),
+                                                                ([700] * 60, [1500] * 60, 8, 128, torch.float16, True, 1)])
+def test_work_in_several_rounds(lens, past, heads, d, dtype, causal, want):
+    """Work of more than two rounds: a CTA comes back for other parts, with scratch and counters of their own.  Some heads against their definition."""
+    import crispybits_kernels as ck
+    keys = [n + p for n, p in zip(lens, past)]
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert rounds(lens, keys, heads, causal) == want
+    cq, ckv = offsets(lens), offsets(keys)
+    q, k, v = rand(cq[-1], heads, d, dtype, 1), rand(ckv[-1], heads // 4, d, dtype, 2), rand(ckv[-1], heads // 4, d, dtype, 3)
+    got = ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal)
+    assert torch.equal(got, ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal))
+    for h in (0, 1, heads // 2 - 1, heads // 2, heads - 2, heads - 1):
+        check(got[:, h:h + 1], reference(q[:, h:h + 1], k[:, h // 4:h // 4 + 1], v[:, h // 4:h // 4 + 1], cq, ckv, causal=causal))
