@@ -932,7 +932,7 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     const int tile = attn_tile_rows(P.R);
     P.row_tiles = (P.R + tile - 1) / tile;
     P.q_sign = scale < 0.f ? -1.f : scale > 0.f ? 1.f : 0.f;
-    P.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f;         // a scale of 0 weighs all keys alike: queries of 0 do
+    P.scale_log2 = scale == 0.f ? 1.f : std::min(fabsf(scale) * 1.4426950408889634f, FLT_MAX);         // a scale of 0 weighs all keys alike: queries of 0 do
     P.zero = 0u;
     {   // with 2^s >= d > 2^(s - 1), m = ceil(2^(31 + s) / d) < 2^32 is off by less than 1, n * m / 2^(31 + s) by less than n / 2^(31 + s) < 1 / d
         const uint32_t d = (uint32_t)P.c.blocks_per_page;

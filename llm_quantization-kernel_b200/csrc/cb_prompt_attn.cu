@@ -32,6 +32,7 @@
 // Every wait is bounded; a wait that runs out raises a flag in shared memory and the status word, every role leaves its
 // loops, TMEM is released, and the kernel returns.
 #include <algorithm>
+#include <cfloat>
 
 #include "cb_common.cuh"
 #include "cb_f32x2.cuh"
@@ -959,7 +960,7 @@ int launch_prompt_attention(const void* q, const void* k, const void* v, const i
     P.q_tok = strides[0]; P.q_head = strides[1]; P.k_tok = strides[2]; P.k_head = strides[3]; P.v_tok = strides[4]; P.v_head = strides[5];
     P.Tq = (int)Tq; P.Tk = (int)Tk; P.H = (int)H; P.group = (int)(H / Hkv); P.B = (int)B;
     // a scale of 0 weighs all keys alike: the smallest float does (0 itself would make NaN of the -inf that stands for an unseen key)
-    P.scale_log2 = scale == 0.f ? 1e-45f : fabsf(scale) * 1.4426950408889634f;
+    P.scale_log2 = scale == 0.f ? 1e-45f : std::min(fabsf(scale) * 1.4426950408889634f, FLT_MAX);
     P.negate = scale < 0.f ? 1 : 0;
     P.causal = causal ? 1 : 0;
     P.most_rounds = prompt_rounds(Tq, Tk, H, B, sms);

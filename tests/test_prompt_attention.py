@@ -579,3 +579,12 @@ def test_work_in_several_rounds(lens, past, heads, d, dtype, causal, want):
     assert torch.equal(got, ck.prompt_attention(q, k, v, i32(cq), i32(ckv), causal=causal))
     for h in (0, 1, heads // 2 - 1, heads // 2, heads - 2, heads - 1):
         check(got[:, h:h + 1], reference(q[:, h:h + 1], k[:, h // 4:h // 4 + 1], v[:, h // 4:h // 4 + 1], cq, ckv, causal=causal))
+
+
+@pytest.mark.gpu
+def test_the_largest_scales():
+    """3e38 is finite, and so is what queries of zeros make of it."""
+    import crispybits_kernels as ck
+    q, k, v = torch.zeros(200, 2, 64, dtype=torch.bfloat16, device=DEV), rand(200, 1, 64, torch.bfloat16, 2), rand(200, 1, 64, torch.bfloat16, 3)
+    for scale in (3e38, -3e38):
+        check(ck.prompt_attention(q, k, v, i32([0, 200]), scale=scale), reference(q, k, v, [0, 200], [0, 200], 0.0))
