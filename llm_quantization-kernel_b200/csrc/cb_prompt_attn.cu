@@ -346,6 +346,23 @@ template <typename T> __device__ __forceinline__ void dot8(const uint4& a, const
     }
 }
 
+// Is there a value that is not finite among keys [from, end) of the step?  The warp looks together, D / 32 columns to a lane.
+template <typename T, int D>
+__device__ __forceinline__ bool any_not_finite(const PromptParams& P, int lane, int head, int64_t k_first, int from, int end) {
+    const T* val = reinterpret_cast<const T*>(P.v) + k_first * P.v_tok + (head / P.group) * P.v_head + lane * (D / 32);
+    bool found = false;
+#pragma unroll 8
+    for (int key = from; key < end; ++key) {
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(val + key * P.v_tok);
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+            const float2 f = unpack2<T>(at[i]);
+            found = found || !(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY);
+        }
+    }
+    return __any_sync(0xffffffffu, found);
+}
+
 // One row, as this warp has just stored it: finished at `out` (O times inv), or O itself at `part` (column c at part[c * kSub]).  If a key of the row's key
 // tiles that the row does not see holds a value that is not finite in a column that came out as NaN, the column's sum over the keys that the row
 // does see is formed again: keys [0, limit) of the step.  The warp does this together, a key to a lane for the weights, D / 32 columns to a lane for the
@@ -408,6 +425,10 @@ __device__ __forceinline__ void mend(const PromptParams& P, int lane, int head, 
                 for (int c = 0; c < kV; ++c) v[c] = fmaf(pi, x[c], v[c]);
             }
         if ((key0 & 4095) == 0 && lane == 0) atomicAdd(beat, 1);
+        bool open = false;                                        // NaN stays: the row may see one itself
+#pragma unroll
+        for (int c = 0; c < kV; ++c) open = open || (((spoilt >> c) & 1u) && v[c] == v[c]);
+        if (!__any_sync(0xffffffffu, open)) break;
     }
 #pragma unroll
     for (int i = 0; i < kV; ++i)
@@ -799,7 +820,10 @@ prompt_attention_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_c
                 float s0, s1;
                 unpair(add2(sums[0], sums[1]), s0, s1);
                 __syncwarp();                                     // other lanes have stored this row
-                for (unsigned left = __ballot_sync(0xffffffffu, !(fabsf(s0 + s1) < INFINITY) && live && !blind && l == l); left != 0u; left &= left - 1u) {
+                unsigned left = __ballot_sync(0xffffffffu, !(fabsf(s0 + s1) < INFINITY) && live && !blind && l == l);
+                // (that the rows see such values themselves is the commoner case)
+                if (left != 0u && !any_not_finite<T, D>(P, lane, w.head, w.k_first, __shfl_sync(0xffffffffu, limit, __ffs(left) - 1), min(n * kTileK, w.lk))) left = 0u;
+                for (; left != 0u; left &= left - 1u) {
                     const int of = __ffs(left) - 1, at = w.row0 + x * kSub + quad * 32 + of;      // the row of another lane
                     const float f = __shfl_sync(0xffffffffu, factor, of), m = __shfl_sync(0xffffffffu, m_ref, of), i = __shfl_sync(0xffffffffu, inv, of);
                     const int see = __shfl_sync(0xffffffffu, limit, of);

@@ -588,3 +588,19 @@ def test_the_largest_scales():
     q, k, v = torch.zeros(200, 2, 64, dtype=torch.bfloat16, device=DEV), rand(200, 1, 64, torch.bfloat16, 2), rand(200, 1, 64, torch.bfloat16, 3)
     for scale in (3e38, -3e38):
         check(ck.prompt_attention(q, k, v, i32([0, 200]), scale=scale), reference(q, k, v, [0, 200], [0, 200], 0.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_values_that_are_all_not_finite(bad):
+    """A column of v that is not finite throughout: every query sees one, and nothing has to be found out at length."""
+    import crispybits_kernels as ck
+    n = 4000
+    q, k, v = rand(n, 4, 64, torch.float16, 1), rand(n, 2, 64, torch.float16, 2), rand(n, 2, 64, torch.float16, 3)
+    want, tol = reference(q, k, v, [0, n], [0, n])
+    v[:, 0, 5] = bad
+    v[0, 1] = bad
+    got = ck.prompt_attention(q, k, v, i32([0, n]))
+    hit = torch.zeros(4, 64, dtype=torch.bool, device=DEV)
+    hit[:2, 5] = hit[2:] = True
+    assert (~torch.isfinite(got) == hit).all() and ((got.double() - want).abs() <= tol)[:, ~hit].all()
