@@ -798,7 +798,7 @@ def _zero_attention_counters(index: int):
     for one: it may hide another."""
     torch.cuda.synchronize(index)
     with _attention_lock, _on_device(torch.device("cuda", index)):
-        kept = [have[0] for (dev, _), have in _attention_eager.items() if dev == index]
+        kept = [have[0] for (dev, _), have in list(_attention_eager.items()) if dev == index]
         slabs = [slab[0] for slab in _attention_slab.values()] + _attention_spent
         for counters in kept + [slab for slab in slabs if slab.get_device() == index]:
             counters.zero_()

@@ -100,23 +100,25 @@ class StackCache:
         self.page_table = torch.arange(batch * pages, dtype=torch.int32, device=stack.device).view(batch, pages)
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=stack.device)      # cached tokens of each sequence
         self.seen = torch.zeros_like(self.lengths)                                     # of the running step: its own tokens too
-        self._longest, self._at, self._replayed = 0, None, False      # the largest of `lengths`, and the version of them that it was read from
+        self._longest, self._at, self._replayed = 0, None, False      # the largest of `lengths`, and what they were when it was known
 
     def longest(self) -> int:
         """Tokens of the longest sequence.  The lengths are read from the device only where they may have changed behind the eager calls that
         advance them: by hand, or by replays of a captured step."""
-        version = None if self.lengths.is_inference() else self.lengths._version
-        if version is None or version != self._at or self._replayed:
-            self._longest, self._at = max(self.lengths.tolist(), default=0), version
+        if self._at is None or self._at != self._version() or self._replayed:
+            self._longest, self._at = max(self.lengths.tolist(), default=0), self._version()
         return self._longest
+
+    def _version(self):
+        return None if self.lengths.is_inference() else (self.lengths.data_ptr(), self.lengths._version)
 
     def advance(self, longest: int):
         """`seen` becomes `lengths`; `longest` of them, from an eager call."""
         self.lengths.copy_(self.seen)
         if self.lengths.is_cuda and torch.cuda.is_current_stream_capturing():
             self._replayed = True
-        elif not self.lengths.is_inference():
-            self._longest, self._at = longest, self.lengths._version
+        else:
+            self._longest, self._at = longest, self._version()
 
 
 class DecodeStack:
