@@ -337,7 +337,7 @@ int cb_kv4_read(const cb_kv4_cache* cache, void* k, void* v, int64_t n_tokens, c
 
 /* Attention of the newest T tokens of each of B sequences over the cache: out[b, j] = softmax(scale * q[b, j] K^T) V over the first
  * lengths[b] - T + 1 + j cached tokens of sequence b; head h reads key head h / (H / kv_heads).  A row that sees
- * nothing is 0.  scale is finite (this and prompt attention).  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
+ * nothing is 0; one with a score that is NaN, by a query or a key that is not finite, is NaN.  scale is finite (this and prompt attention).  Lengths below 0 count as 0, lengths beyond the table as the table's capacity.  q: rows of head_dim contiguous values, 16-byte aligned;
  * strides3 = {b, t, h} in elements, multiples of 8; out [B, T, H, head_dim] contiguous, sharing no memory with q.  Tokens on a page whose number
  * lies outside the cache are left out and set the status word (3001).  counters: cb_kv4_attention_counters() int32, zeroed ONCE,
  * left zero by every call that ends well (cb_decode_status); partial: cb_kv4_attention_partial_bytes() bytes, 16-byte aligned, of any content.  Calls that may overlap on
@@ -356,7 +356,9 @@ size_t cb_kv4_attention_partial_bytes(int64_t T, int64_t H, int64_t kv_heads, in
  * cu_k[s + 1] - 1 (device memory; bounds outside the tensors are cut to them).  Head h reads key head h / (H / Hkv).  head_dim 64 or 128,
  * dtype CB_F16 or CB_BF16; at most 2^22 sequences.  A query that sees no key gives 0; rows of no sequence are left as they were.  Keys and values
  * behind a query's last one do not touch it, infinities and NaN among them; a value of v that is not finite makes the
- * same value of the queries that see it inf or NaN.
+ * same value of the queries that see it inf or NaN, and a query that has a score of NaN or +inf, or none above -inf, is NaN.
+ * (Both attentions add up weights times values, weights of up to 2^8, in fp32 before they divide: with n keys, values beyond 2^120 / n may overflow.  Scores of
+ * 2^24 or more, times log2(e), are told apart by steps of 1.)
  * The work is cut into equal parts for the SMs, whatever the lengths are; where a cut falls inside a tile, its parts meet in scratch and are joined in
  * order, so that the result is the same from call to call.  cb_prompt_attention_scratch gives the bytes of `partial` (16-byte aligned, of any
  * content) that suffice for every call and, in *counter_bytes, of `counters` (zeroed ONCE, left zero by every call that ends well).  Calls that may overlap on the GPU need their own. */

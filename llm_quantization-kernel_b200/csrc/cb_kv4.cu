@@ -11,9 +11,9 @@
 // block that the call fills in part (a decode step's token, the ends of a prompt) is written value by value.  A thread
 // owns 8 consecutive values of a row (token, head, K or V).
 //
-// Measured: 13584 tokens of 8 prompts, 32 heads, D = 128, are written in 122 us (4.7 TB/s; bound by the arithmetic of a value: minimum and maximum,
-// quotient, check for ties) and 54193 tokens of 8 heads read back in 49.4 us (5.8 TB/s, near a copy's rate).  A decode step's append takes
-// 2.8 us, little more than an empty launch.
+// Measured: 13584 tokens of 8 prompts, 32 heads, D = 128, are written in 79 us (3.6 TB/s; bfloat16, which meets more ties, 101 us), bound by the arithmetic of
+// a value: issue slots are 73 % busy, DRAM 40 %.  54193 tokens of 8 heads are read back in 49.4 us (5.8 TB/s, near a copy's rate).  A decode step's append takes
+// 3.4 us, little more than an empty launch.
 #include <algorithm>
 
 #include "cb_f32x2.cuh"
@@ -239,7 +239,7 @@ template <int D> struct Place {
 };
 
 template <typename T, int D, int GS>
-__global__ void __launch_bounds__(kThreads, 4)              // 64 registers; with three CTAs to an SM the prompts above take 136 us for 125
+__global__ void __launch_bounds__(kThreads, 4)              // 64 registers; with three CTAs to an SM writing and reading 13584 tokens takes 136 us for 125
 kv4_append_kernel(const RowParams P) {
     using L = KvLayout<D, GS>;
     constexpr int kTpr = Place<D>::kTpr, kPer = Place<D>::kPer, kBatch = 4;       // kBatch: loads in flight
@@ -387,8 +387,8 @@ int launch_kv4_rows(bool append, const cb_kv4_cache* c, const void* k_in, const 
     if (strides != nullptr) { P.k_tok = strides[0]; P.k_head = strides[1]; P.v_tok = strides[2]; P.v_head = strides[3]; }
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
-    // few blocks: one head to a CTA, so that a decode step spreads over the SMs; many: up to eight, for fewer look-ups and more loads in flight (the
-    // prompts and histories above, one head to a CTA: 276 and 88.5 us)
+    // few blocks: one head to a CTA, so that a decode step spreads over the SMs; many: up to eight, for fewer look-ups and more loads in flight (13584 tokens
+    // written and read 122 us, one head to a CTA 276; 54193 read 49 and 88.5)
     const int64_t items = items_of(n_tokens, n_seqs, P.per_seq, cu != nullptr);
     int hp = 1;
     while (hp < kMaxHeads && items * ((c->kv_heads + 2 * hp - 1) / (2 * hp)) >= 4 * sms) hp *= 2;

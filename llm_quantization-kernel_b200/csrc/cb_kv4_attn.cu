@@ -28,10 +28,12 @@
 // (max, sum, output) in scratch and the CTA that arrives last adds them in order of position: the result does not
 // depend on timing.
 //
-// Measured (D = 128, groups of 64): one sequence of 131071 tokens, 64 heads over 8, in 42.2 us, 3.6 TB/s or 0.55 of a copy's rate; sixteen of them
-// in 483, 0.77.  The steady state runs at about 0.83 of that rate (the stages of unpacking, products and softmax share the issue slots of three warps on
-// each scheduler); the rest is the chain of a launch, 12 us long: lengths, schedule, look-ups, first copies, the warps' meeting, the join.  24 sequences of
-// 0 to 8192 tokens, 32 heads over 8: 27.1 us (2.1 TB/s), one of 777, 32 heads: 9.8 us, of which that chain is most.
+// Measured (D = 128, groups of 64): one sequence of 131071 tokens, 64 heads over 8, in 42.7 us, 3.5 TB/s or 0.55 of a copy's rate; sixteen of them
+// in 479, 0.78.  The steady state runs at about 0.83 of that rate (the stages of unpacking, products and softmax share the issue slots of three warps on
+// each scheduler, which are half busy; a warp's next instruction waits for the one before most of the rest); the rest is the chain of a launch, 12 us long:
+// lengths, schedule, look-ups, first copies, the warps' meeting, the join.  16 sequences of 4000 tokens, 32 key heads of one query head: 84 us, 3.5 TB/s.  Of
+// caches that the L2 still holds: 24 sequences of 0 to 8192 tokens, 32 heads over 8, 25.4 us, one of 777, 32 heads, 10.1 us, of which that chain is most.
+// At D = 128 and groups of 32 the compiler spills 42 bytes (tiles of 16 rows: 82), elsewhere nothing.
 #include <algorithm>
 #include <cfloat>
 
@@ -179,9 +181,10 @@ constexpr float kLag = 8.f;
 // step of 1 or more in fp32 anyway.
 constexpr float kLargeScore = 16777216.f;
 
-// What a segment costs besides its blocks (query rows, the warps' meeting, the join), in blocks.  24 sequences of up to 8192 tokens with 8 key
-// heads take 27.1 us with it, 27.3 with 48, 32.3 with 96 and 37.7 with 8; 12 short ones with 12 heads 15.8, 15.9, 16.0 and 28.7; one long
-// sequence is indifferent.
+// What a segment costs besides its blocks (query rows, the warps' meeting, the join), in blocks.  With 8, 32, 48, 64 and 96 of them: 32 sequences of up to
+// 4000 tokens, 32 key heads, take 177, 115, 96, 86 and 89 us; 24 of up to 8192, 8 key heads, 48, 29, 28, 30 and 32; 12 short ones with 12 heads
+// 36, 19.9, 18.1, 18.3 and 18.3; 8 of 4000 with 32 rows to a key head 40.8, 40.5, 39.8, 40.5 and 39.5; 32 of 4000 at D = 64 and groups of 32
+// 36.5, 36.2, 36.0, 35.4 and 35.4.
 constexpr int kOpen = 64;
 
 // Blocks of a CTA up to which parts end with their segment although a tenth of the CTAs or more may then be idle.
@@ -231,7 +234,7 @@ kv4_attention_kernel(const AttnParams P) {
     };
     uint32_t U = all_units();
     // With few CTAs to a segment those that are left over stay idle: only where that costs little beside the rest (32 segments of 131071 tokens on 148
-    // SMs: 4 CTAs each, 144 us, cut into equal parts 130; 32 segments of 777 tokens: 9.8 and 10.3).
+    // SMs: 4 CTAs each, 145 us, cut into equal parts 129; 32 segments of 777 tokens: 10.1 and 10.7).
     if (aligned && 16 * B * segs > (int)gridDim.x && U > kAlignedBlocks * gridDim.x) {
         aligned = false;
         U = all_units();
@@ -905,7 +908,7 @@ int launch_attn_t(const AttnParams& P, int sms, cudaStream_t stream) {
 
 }  // namespace
 
-// Query rows of a tile: 8, or 16 where a key head has more than 8.  (4 to 8 rows in tiles of 16: 38.7 us for 27.1, 73.1 for 42.2.)
+// Query rows of a tile: 8, or 16 where a key head has more than 8.  (4 rows in tiles of 16: 37.9 us for 30.0, 8 rows 63.9 for 42.2.)
 static int attn_tile_rows(int64_t rows) { return rows > 8 ? 16 : 8; }
 
 int64_t kv4_attention_segments(int64_t B, int64_t rows, int64_t kv_heads) {
@@ -945,10 +948,10 @@ int launch_kv4_attention(const cb_kv4_cache* c, const void* q, const int64_t* q_
     const int sms = sm_count_current();
     if (sms <= 0) return CB_ERR_CUDA;
     // Few segments: parts that end with their segment, so that each CTA goes through the chain of copy, product and join once (8 segments of
-    // 131071 tokens: 42.2 us, cut into equal parts 43.6); the parts are then up to a quarter longer.  Many: equal parts.
+    // 131071 tokens: 42.2 us, cut into equal parts 43.4); the parts are then up to a quarter longer.  Many: equal parts.
     P.aligned = 4 * B * c->kv_heads * P.row_tiles <= sms;
-    // Segments enough to fill the SMs: the short ones (up to 128 tokens) one to a warp (512 segments of 100 tokens: 13.2 us, by whole CTAs
-    // 23.9; where few are that short: 27.1 and 28.6).
+    // Segments enough to fill the SMs: the short ones (up to 128 tokens) one to a warp (512 segments of 100 tokens: 13.5 us, by whole CTAs
+    // 23.6; where a fifth are that short, 192 segments of up to 8192: 30.0 and 27.5).
     P.solo = !P.aligned && B * c->kv_heads * P.row_tiles >= sms ? 8 : 0;
     const bool bf = c->dtype == CB_BF16;
 #define CB_KV4_NT(d, gs, nt) (bf ? launch_attn_t<__nv_bfloat16, d, gs, nt>(P, sms, stream) : launch_attn_t<__half, d, gs, nt>(P, sms, stream))

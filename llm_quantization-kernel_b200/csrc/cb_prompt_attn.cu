@@ -9,7 +9,8 @@
 // The two sub-tiles alternate: while the softmax warps of one work on its scores, the tensor cores run the other's products.
 // A thread of the softmax warps owns a row (a TMEM lane), so maxima and sums need no exchange.  The reference m is moved only
 // when the maximum has grown by more than 2^8 (then O and l are rescaled), which makes rescaling rare: p stays below 256, and its 16-bit
-// rounding is relative.  p is rounded to the inputs' type; the sum l takes the unrounded p.
+// rounding is relative.  p is rounded to the inputs' type, which is what the product with V takes (error of the whole output against 64 bits: bf16 2.0e-3
+// where its own rounding is 1.6e-3, fp16 2.2e-4 to 2.5e-4 and 2.0e-4); the sum l takes the unrounded p.
 //
 // TMEM map (512 columns): S0/P0 [0, 128), S1/P1 [128, 256), O0 [256, 256 + D), O1 [384, 384 + D).
 // Warps: 0-3 softmax and epilogue of sub-tile 0, 4-7 of sub-tile 1, 8 TMA, 9 MMA, 10 the walk through
@@ -23,11 +24,14 @@
 // What bounds it at D = 128: 4 * 128 * 128 * D operations of a sub-tile and key tile are 1024 clocks of the tensor cores, and
 // its 128 * 128 exponentials are 1024 clocks of the special-function units; at D = 64 these are twice the products' time.  So the softmax warps may not
 // lose issue slots: packed fp32 arithmetic, a row to a thread, nothing unrolled that runs once a tile.
-//   16384 tokens, 32 heads, D = 128, causal, bf16:            1.69 to 1.73 ms, 1270 to 1300 TFLOP/s (the GPU at its power limit)
-//   12 prompts of 1 to 4096 tokens, 32 heads over 8, D = 128: 258 us, 930 TFLOP/s of what the pairs need; tiles on the diagonal and at prompts'
-//                                                              ends, and a tile's opening and epilogue (kOpen), are the rest
-//   16384 tokens, 16 heads, D = 64, causal, fp16:             768 us, 720 TFLOP/s
-//   one prompt of 37 tokens, 32 heads:                        10 us: launch, tensor maps, TMEM, one pass through the roles
+//   16384 tokens, 32 heads, D = 128, causal, bf16:            1.72 to 1.81 ms in a replayed graph, 1220 to 1280 TFLOP/s; 2.0 ms, 1100 TFLOP/s, in calls that
+//                                                              follow one another on new inputs: the GPU is at its power limit, and runs differ by as much
+//   12 prompts of 1 to 4096 tokens, 32 heads over 8, D = 128: 262 us (calls: 301), 920 TFLOP/s of what the pairs need; tiles on the diagonal and at
+//                                                              prompts' ends, and a tile's opening and epilogue (kOpen), are the rest
+//   4 prompts of 4096, 32 heads over 8, D = 128, not causal:  0.89 ms, 1230 TFLOP/s
+//   16384 tokens, 16 heads, D = 64, causal, fp16:             840 to 920 us, 600 to 655 TFLOP/s
+//   one prompt of 37 tokens, 32 heads:                        10 us (calls: 15): launch, tensor maps, TMEM, one pass through the roles
+// The compiler spills 76 to 88 bytes of a softmax thread's registers at 168 a thread at launch.
 //
 // Every wait is bounded; a wait that runs out raises a flag in shared memory and the status word, every role leaves its
 // loops, TMEM is released, and the kernel returns.
@@ -42,7 +46,7 @@ namespace {
 
 constexpr int kSub = 128, kTileQ = 2 * kSub, kTileK = 128;
 constexpr int kOpen = 3;                              // what a CTA spends on a (tile, head) besides its products, in key tiles (the 12 prompts with 1: 272 us)
-// A round is kRoundUnits units for a CTA, or more: 16384 tokens, 32 heads take 1.69 to 1.73 ms in four rounds, 1.81 in one, whose keys do not stay in the L2.
+// A round is kRoundUnits units for a CTA, or more: 16384 tokens, 32 heads took 1.69 to 1.73 ms in four rounds, 1.81 in one, whose keys do not stay in the L2.
 // Work of less than two such rounds is one round: each cut tile costs a join.
 constexpr int kRoundUnits = 100, kMaxRounds = 4;
 constexpr int kTmaWarp = 8, kMmaWarp = 9, kWalkWarp = 10, kFixWarp = 11, kThreads = 384;
