@@ -112,7 +112,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor, le
 
     q: [B, H, head_dim], one token of each sequence, or [B, T, H, head_dim], the T newest; any strides.  H is a multiple of the
     cache's heads, and query head h reads key head h // (H // kv_heads).  `lengths` [B]: cached tokens of each sequence, q's own
-    among them; token j of T sees the first lengths - T + 1 + j.  A row that sees nothing (lengths 0) is 0.  scale: finite, default head_dim ** -0.5.
+    among them; token j of T sees the first lengths - T + 1 + j.  A row that sees nothing (lengths 0) is 0, one with a score
+    that is NaN is NaN.  scale: finite, default head_dim ** -0.5.
     T may be any, but the cache is read once for each 16 rows (T * H / kv_heads of them) of a key head: for long pieces of
     a prompt, read the history back and use prompt attention."""
     return _C().kv4_attention(q, cache, page_table, lengths, cache.head_dim ** -0.5 if scale is None else float(scale))
@@ -127,7 +128,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     reads key head h // (H // Hkv)); any strides, rows that are not contiguous or not 16-byte aligned are copied first.
     `cu_seqlens` int32 [B + 1]: the first query of each sequence and the end of the last; `cu_seqlens_k` the same for the keys where
     they differ: a piece of a prompt attends to what came before it and to itself.  causal: query r of Lq sees the first
-    Lk - Lq + r + 1 keys.  A query that sees none gives 0.  Rows of no sequence are left as they are in `out` (and are
+    Lk - Lq + r + 1 keys.  A query that sees none gives 0, one with a score of NaN or +inf, or none above -inf, NaN.  Rows of no sequence are left as they are in `out` (and are
     undefined without it; it shares no memory with q, k and v).  scale: finite, default head_dim ** -0.5.  Keys and values that a query does not see do not
     touch it, infinities and NaN among them.  Scratch for tiles that are cut between SMs (on 148 SMs at head_dim 128 158 MB for long prompts, 39 MB for
     a few thousand tokens, none for up to 128) is kept for each stream that calls this eagerly, and comes from the graph's pool in a capture."""
